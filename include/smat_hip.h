@@ -506,6 +506,110 @@ int smat_decode_step(int dtype, const void* phi_t, const void* psi_t, const void
                      int64_t q_sb, int64_t k_sb, int64_t v_sb, void* stream);
 
 /*
+ * smat_decode_step with requests at their own positions: sequence s (of
+ * request s / (nb / requests)) takes row type (step + ahead[request]) mod B.
+ * ahead: (requests) int32 on the device, entries >= 0 (a negative one counts
+ * as 0), or NULL for smat_decode_step's one position.  No counterpart in the
+ * reference, whose decoder steps in lockstep (src/smat/attention.py:496-528).
+ */
+int smat_decode_step_at(int dtype, const void* phi_t, const void* psi_t, const void* vb_t,
+                        const float* S_in, float* S_out, const float* U, float* out,
+                        float* o_full, const int32_t* ahead, int requests, int nb, int B, int r,
+                        int p, int64_t step, int64_t q_sb, int64_t k_sb, int64_t v_sb,
+                        void* stream);
+
+/*
+ * Drafted trees over the decoder's cache, no counterpart in the reference.
+ * Node j at level l (roots at level 0) of a tree of M <= 64 nodes:
+ *   N_j = Phi_j (S + U[(step + ahead + l) mod B]) + sum_a (Phi_j . Psi_a) Vb_a
+ * over j's ancestors a and j itself; out_j = N_j[:p-1] / N_j[p-1]: what
+ * decode steps along j's path give.  smat_tree_state forms
+ *   S_out = S + sum_a Psi_a Vb_a^T
+ * over the path that ends in nodes[request] (a value outside [0, M): none)
+ * and, with ahead not NULL, adds the path's length to ahead[request].
+ * Phi, Psi: (nb, M, r), Vb: (nb, M, p) of dtype; S: (nb, r, p), U: (nb, B, r,
+ * p), out: (nb, M, p-1) fp32 contiguous; nb is a multiple of trees and of
+ * requests (heads innermost).  Tables of each tree: anc (trees, M), bit a of
+ * word j set when a is j or an ancestor of j (0: an unused node, whose out row
+ * is zero); order (trees, M) the used nodes by level, then the unused ones;
+ * lstart (trees, M + 1) the first of each level in order, at and past the
+ * tree's last level the count of used nodes.  Entries are trusted.
+ */
+int smat_tree_step(int dtype, const void* phi, const void* psi, const void* vb, const float* S,
+                   const float* U, float* out, const int64_t* anc, const int32_t* order,
+                   const int32_t* lstart, const int32_t* ahead, int nb, int trees, int requests,
+                   int M, int levels, int B, int r, int p, int64_t step, int64_t q_sb,
+                   int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st,
+                   void* stream);
+int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, float* S_out,
+                    const int64_t* anc, const int32_t* nodes, int32_t* ahead, int nb, int trees,
+                    int requests, int M, int r, int p, int64_t k_sb, int64_t k_st, int64_t v_sb,
+                    int64_t v_st, void* stream);
+
+/*
+ * The gated delta rule, no counterpart in the reference's path (its language
+ * models take it from another library; the decayed scan above is the same
+ * state without the erase term):
+ *   S_t = a_t S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - a_t S_{t-1}^T k_t),
+ *   o_t = scale S_t^T q_t,  a_t = exp(logA_t)
+ * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides, nbk dividing nb
+ * (value sequence s reads key sequence s / (nb / nbk)); logA, beta: (nb, T)
+ * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256.
+ * Segments: chunks (nch, 2) = first token, tokens (<= 64); runs (nruns, 3) =
+ * first chunk, end chunk, segment, every segment's runs together and in order,
+ * an empty segment with one empty run; segrun (nseg + 1) the first run of each
+ * segment.  Entries are trusted.  All three NULL: one segment, chunks of 64,
+ * runs of K chunks, nch = ceil(T / 64), nruns = max(1, ceil(nch / K)).
+ * With more runs than segments the sequences are also split along T.
+ * smat_delta_run_chunks: the run length that fills the GPU (longest: the
+ * chunks of the longest segment).
+ * state: (nseg, nb, r, p) fp32 entering each segment (NULL: zero); state_out
+ * the same leaving it (may be NULL; not state itself).
+ * Training: save_s (nb, nch, R, P) and save_u (nb, nch, 64, P) fp32, R and P
+ * being r and p rounded up to 32, receive the states entering chunks and U.
+ * workspace: smat_delta_workspace_bytes(..., backward) bytes, 256-byte aligned.
+ */
+int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p);
+int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg, int nruns,
+                                   int r, int p, int backward);
+int smat_delta_scan(int dtype, const void* q, const void* k, const void* v, const float* logA,
+                    const float* beta, const float* state, void* out, float* state_out,
+                    float* save_s, float* save_u, const int32_t* chunks, const int32_t* runs,
+                    const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch, int nruns,
+                    int K, int r, int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
+                    int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st,
+                    int64_t b_sb, int64_t b_st, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+
+/*
+ * Its gradient: dout (nb, T, p) of dtype with strides and dstate_out (the
+ * gradient of state_out, or NULL) -> dq, dk (nbk, T, r), dv (nb, T, p) of
+ * dtype, dlogA, dbeta (nb, T) fp32, all contiguous, and dstate (nseg, nb, r,
+ * p) fp32 or NULL.  Tokens no segment holds are left as they were.
+ */
+int smat_delta_scan_backward(int dtype, const void* q, const void* k, const void* v,
+                             const float* logA, const float* beta, const void* dout,
+                             const float* dstate_out, const float* save_s, const float* save_u,
+                             void* dq, void* dk, void* dv, float* dlogA, float* dbeta,
+                             float* dstate, const int32_t* chunks, const int32_t* runs,
+                             const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch,
+                             int nruns, int K, int r, int p, float scale, int64_t q_sb,
+                             int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb,
+                             int64_t v_st, int64_t a_sb, int64_t a_st, int64_t b_sb,
+                             int64_t b_st, int64_t d_sb, int64_t d_st, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/*
+ * One token of it: S_out from S_in (both (nb, r, p) fp32 contiguous; they may
+ * be the same buffer) and out (nb, p) of dtype, contiguous.  q, k: (nbk, r),
+ * v: (nb, p), logA, beta: (nb) fp32, with batch strides.
+ */
+int smat_delta_step(int dtype, const void* q, const void* k, const void* v, const float* logA,
+                    const float* beta, const float* S_in, float* S_out, void* out, int nb,
+                    int nbk, int r, int p, float scale, int64_t q_sb, int64_t k_sb, int64_t v_sb,
+                    int64_t a_sb, int64_t b_sb, void* stream);
+
+/*
  * Unpooled long-range sums  U_h = sum_{j in cols_h} Psi_{n_P+j}^T Vb_{n_P+j}
  * (fp32, U: (nb, B, r, p) contiguous), one row type per list: cols (B, kappa)
  * int32 landmark columns, row h holding its counts[h] columns first.

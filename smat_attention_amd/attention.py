@@ -34,7 +34,10 @@ from typing import Callable, Dict, Optional
 import numpy as np
 import torch
 
+from .kernels import hip_delta as _delta
 from .kernels import hip_fwd as _hip
+from .kernels.hip_delta import Segments
+from .kernels.hip_fwd import DraftTree
 from .mask import MaskSpec
 
 __all__ = [
@@ -43,6 +46,7 @@ __all__ = [
     "apply_incidence",
     "query_by_type", "zeta_transform", "walsh_incidence", "direct_long_range",
     "smat_attention", "smat_attention_fused", "dense_masked_kernel_attention", "SmatDecoder",
+    "DraftTree", "Segments", "gated_delta_scan", "gated_delta_step", "GatedDeltaDecoder",
     "have_triton", "have_hip",
 ]
 
@@ -423,6 +427,52 @@ def _decayed_forward(Ph, Ps, Vv, la, n: int, C: int):
     out = _hip.chunk_local_decay(Ph.reshape(nb, nc, C, r), Ps.reshape(nb, nc, C, r),
                                  Vv.reshape(nb, nc, C, p), Sin, L)
     return out.reshape(nb, Tp, p), L, Sin
+
+
+def gated_delta_scan(Q, K, V, logA, beta, *, scale: float = 1.0, state=None,
+                     segments: Optional[Segments] = None, return_state: bool = False):
+    """The gated delta rule over whole sequences::
+
+        S_t = a_t S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - a_t S_{t-1}^T k_t),
+        o_t = scale S_t^T q_t,           a_t = exp(logA_t)
+
+    the decayed scan's state with an erase term: what the state holds under ``k_t`` is
+    replaced by ``v_t`` in the proportion ``beta_t`` before it is read.  It has no counterpart
+    in the reference's path, whose language models take it from another library.
+
+    ``Q, K (nbk, T, r)`` and ``V (nb, T, p)`` in one of bf16, fp16 and fp32, ``logA, beta
+    (nb, T)`` in fp32 (16-bit ones are taken to fp32 first); ``nbk`` divides ``nb`` and value
+    sequence s reads key sequence ``s // (nb // nbk)`` (value heads innermost).  Any strides
+    with contiguous columns are read in place, so packed ``(tokens, heads, columns)`` tensors
+    come as their transposed views.  r <= 128, p <= 256; the values of a chunk of 64 tokens
+    meet in products, so inputs are expected to be finite (``logA = -inf`` counts as a decay to
+    zero).  A token with ``beta = 0, logA = 0`` leaves the state as it is: padding.
+
+    ``segments`` (:class:`Segments`) packs sequences of any lengths along T; each starts from
+    its own state.  ``state`` fp32 ``(nb, r, p)``, with segments ``(segments, nb, r, p)``
+    (zero if None), is the state entering; ``return_state`` returns ``(o, state_out)``, else
+    ``o (nb, T, p)`` in the inputs' type.  Chunked: each chunk of 64 is a triangular system
+    solved once, and only the products through the state run along T; few long sequences are
+    also split along T.  Differentiable in Q, K, V, logA, beta and state.
+    """
+    who = "gated_delta_scan"
+    _delta.check_scan(who, Q, K, V, logA, beta, state, segments)
+    if _wants_grad(Q, K, V, logA, beta, state):
+        o, s_out = _delta.GatedDeltaFunction.apply(Q, K, V, logA, beta, state, float(scale),
+                                                   segments, return_state)
+    else:
+        o, s_out = _delta.scan(Q, K, V, logA, beta, state, scale, segments, return_state,
+                               False)[:2]
+    return (o, s_out) if return_state else o
+
+
+def gated_delta_step(q, k, v, logA, beta, state, *, scale: float = 1.0, out=None,
+                     out_state=None):
+    """One token of :func:`gated_delta_scan` for a batch of sequences: ``q, k (nbk, r)``,
+    ``v (nb, p)``, ``logA, beta (nb,)``, ``state (nb, r, p)`` fp32.  The new state goes to
+    ``out_state``, or replaces ``state`` if that is None; returns ``o (nb, p)`` in v's type.
+    One launch, for serving: no gradients."""
+    return _delta.step(q, k, v, logA, beta, state, float(scale), out, out_state)
 
 
 def pool_profiles(Psi, Vb, spec: MaskSpec, acc_dtype=None, backend: str = "auto"):
@@ -821,6 +871,35 @@ class SmatDecoder:
                    torch.empty(nb, r, p, device=dev, dtype=torch.float32)]
         self._cur = 0
         self.i = 0
+        self.ahead = None
+
+    @classmethod
+    def from_cache(cls, U, S, i: int = 0, *, ahead=None, spec: Optional[MaskSpec] = None):
+        """A decoder over tables that a program already holds (a cache that was saved, moved
+        or cut out of a larger batch): the type table ``U (nb, B, r, p)``, the running state
+        ``S (nb, r, p)``, both contiguous fp32, the tokens ``i`` taken since the prefix, and
+        the requests' positions past it (``ahead``, see :meth:`commit`).  ``S`` becomes one of
+        the decoder's two state buffers."""
+        who = "SmatDecoder.from_cache"
+        _hip._on_gpu(who, U, S)
+        if S.dim() != 3:
+            raise ValueError(f"{who}: S must be (nb, r, p), got {tuple(S.shape)}")
+        nb, r, p = S.shape
+        _hip._shape(who, "U", U, (nb, None, r, p))
+        if not (U.is_contiguous() and S.is_contiguous() and U.dtype == S.dtype == torch.float32):
+            raise ValueError(f"{who}: U and S must be contiguous fp32")
+        if U.device != S.device:
+            raise ValueError(f"{who}: U is on {U.device}, S on {S.device}")
+        if U.shape[1] < 1 or p < 2 or i < 0:
+            raise ValueError(f"{who}: need a row type, p >= 2 and i >= 0")
+        if ahead is not None:
+            _hip._check_requests(who, "ahead", ahead, nb, S.device)
+        self = cls.__new__(cls)
+        self.spec, self.acc = spec, torch.float32
+        self.nb, self.r, self.p = nb, r, p
+        self.U, self._S, self._cur = U, [S, torch.empty_like(S)], 0
+        self.i, self.ahead = int(i), ahead
+        return self
 
     @property
     def S(self) -> torch.Tensor:
@@ -848,10 +927,41 @@ class SmatDecoder:
     def step(self, Phi_t, Psi_t, Vb_t, *, out=None):
         """One token.  ``Phi_t, Psi_t: (nb, r)``, ``Vb_t: (nb, p)``; returns fp32 ``(nb, p-1)``."""
         S_in, S_out = self._S[self._cur], self._S[1 - self._cur]
-        o = _hip.decode_step(Phi_t, Psi_t, Vb_t, S_in, S_out, self.U, self.i, out=out)
+        o = _hip.decode_step(Phi_t, Psi_t, Vb_t, S_in, S_out, self.U, self.i, out=out,
+                             ahead=self.ahead)
         self._cur = 1 - self._cur
         self.i += 1
         return o
+
+    def tree_step(self, Phi, Psi, Vb, tree: DraftTree, *, out=None):
+        """Every node of drafted trees read against the cache, which stays as it is: row j is
+        what :meth:`step` would return for node j after steps through its ancestors.
+        ``Phi, Psi (nb, M, r)``, ``Vb (nb, M, p)`` are the M nodes' rows in the tree's order;
+        returns fp32 ``(nb, M, p-1)``, zero at unused nodes.  One launch."""
+        return _hip.tree_step(Phi, Psi, Vb, tree, self.S, self.U, self.i, ahead=self.ahead,
+                              out=out)
+
+    def tree_state(self, Psi, Vb, tree: DraftTree, nodes, *, out=None) -> torch.Tensor:
+        """The state that accepting ``nodes`` would leave: ``S + sum psi vb^T`` over the path
+        from the root to each request's accepted node.  ``nodes`` int32 on the device, one
+        entry a request (heads innermost); an entry outside [0, M) accepts nothing."""
+        if out is None:
+            out = torch.empty_like(self.S)
+        return _hip.tree_state(Psi, Vb, tree, nodes, self.S, out)
+
+    def commit(self, Psi, Vb, tree: DraftTree, nodes) -> None:
+        """Take each request's accepted path into its state and move its position by the
+        path's length.  Requests may accept different numbers of tokens: from the first commit
+        on, ``ahead`` (int32, on the device) holds how far each is past the step counter
+        ``i``, and :meth:`step` and :meth:`tree_step` read it there."""
+        if self.ahead is None:
+            _hip._check_requests("SmatDecoder.commit", "nodes", nodes, self.nb, self.S.device)
+            ahead = torch.zeros_like(nodes)
+        else:
+            ahead = self.ahead
+        _hip.tree_state(Psi, Vb, tree, nodes, self.S, self._S[1 - self._cur], ahead=ahead)
+        self.ahead = ahead
+        self._cur = 1 - self._cur
 
     def cache_words(self) -> int:
         return int(self.S.numel() + self.U.numel())
@@ -859,3 +969,33 @@ class SmatDecoder:
     @staticmethod
     def kv_cache_words(nb: int, T: int, d_v: int) -> int:
         return int(nb * 2 * T * d_v)
+
+
+class GatedDeltaDecoder:
+    """A gated delta layer's state in serving: a prompt in chunks, then token by token.
+
+    ``state`` fp32 ``(nb, r, p)`` is taken over and updated in place (zero it for a new
+    sequence, copy it to branch).  The arguments of the calls are :func:`gated_delta_scan`'s
+    and :func:`gated_delta_step`'s."""
+
+    def __init__(self, state: torch.Tensor, *, scale: float = 1.0):
+        who = "GatedDeltaDecoder"
+        _hip._on_gpu(who, state)
+        if state.dim() != 3 or state.dtype != torch.float32 or not state.is_contiguous():
+            raise ValueError(f"{who}: the state must be contiguous fp32 (nb, r, p)")
+        self.S, self.scale = state, float(scale)
+
+    @torch.no_grad()
+    def prefill(self, Q, K, V, logA, beta) -> torch.Tensor:
+        """Any number of tokens at once; returns ``o (nb, T, p)``."""
+        o, S = gated_delta_scan(Q, K, V, logA, beta, scale=self.scale, state=self.S,
+                                return_state=True)
+        self.S.copy_(S)
+        return o
+
+    def step(self, q, k, v, logA, beta, *, out=None) -> torch.Tensor:
+        """One token; returns ``o (nb, p)``."""
+        return gated_delta_step(q, k, v, logA, beta, self.S, scale=self.scale, out=out)
+
+    def cache_words(self) -> int:
+        return int(self.S.numel())

@@ -27,8 +27,8 @@ template <typename In, int kCols>
 __global__ __launch_bounds__(dc::kThreads) void decode_step_kernel(
     const In* __restrict__ phi, const In* __restrict__ psi, const In* __restrict__ vb,
     const float* __restrict__ S_in, float* __restrict__ S_out, const float* __restrict__ U,
-    float* __restrict__ out, float* __restrict__ o_full, int B, int r, int p, int64_t step,
-    int64_t q_sb, int64_t k_sb, int64_t v_sb) {
+    float* __restrict__ out, float* __restrict__ o_full, const int32_t* __restrict__ ahead,
+    int per, int B, int r, int p, int64_t step, int64_t q_sb, int64_t k_sb, int64_t v_sb) {
   using namespace dc;
   constexpr int kParts = kThreads / kCols;                 // feature partitions
   constexpr int kRows = (kMaxR + kParts - 1) / kParts;     // rows per thread
@@ -39,7 +39,9 @@ __global__ __launch_bounds__(dc::kThreads) void decode_step_kernel(
   const int sp = blockIdx.y, nsplit = gridDim.y;
   const int tid = threadIdx.x;
   const int cl = tid % kCols, part = tid / kCols;
-  const int h = (int)(step % B);
+  int64_t at = step;
+  if (ahead) at += max(0, ahead[b / per]);                 // this request's own position
+  const int h = (int)(at % B);
   const int cw = (p - 1 + nsplit - 1) / nsplit;            // value columns per workgroup
   const int cbeg = sp * cw;
   const int ncw = max(0, min(p - 1, cbeg + cw) - cbeg);    // this one's (ncw < kCols)
@@ -119,9 +121,9 @@ static int decode_split(int nb) {
 
 template <typename In>
 static int launch_decode(const void* phi, const void* psi, const void* vb, const float* S_in,
-                         float* S_out, const float* U, float* out, float* o_full, int nb, int B,
-                         int r, int p, int64_t step, int64_t q_sb, int64_t k_sb, int64_t v_sb,
-                         hipStream_t stream) {
+                         float* S_out, const float* U, float* out, float* o_full,
+                         const int32_t* ahead, int per, int nb, int B, int r, int p, int64_t step,
+                         int64_t q_sb, int64_t k_sb, int64_t v_sb, hipStream_t stream) {
   const int ns = decode_split(nb);
   const dim3 grid((unsigned)nb, (unsigned)ns);
   // local columns: ceil((p - 1) / ns) value columns and the normaliser, with
@@ -129,46 +131,67 @@ static int launch_decode(const void* phi, const void* psi, const void* vb, const
   if (ns == 1)
     hipLaunchKernelGGL((decode_step_kernel<In, 144>), grid, dim3(dc::kThreads), 0, stream,
                        (const In*)phi, (const In*)psi, (const In*)vb, S_in, S_out, U, out, o_full,
-                       B, r, p, step, q_sb, k_sb, v_sb);
+                       ahead, per, B, r, p, step, q_sb, k_sb, v_sb);
   else if (ns == 2)
     hipLaunchKernelGGL((decode_step_kernel<In, 80>), grid, dim3(dc::kThreads), 0, stream,
                        (const In*)phi, (const In*)psi, (const In*)vb, S_in, S_out, U, out, o_full,
-                       B, r, p, step, q_sb, k_sb, v_sb);
+                       ahead, per, B, r, p, step, q_sb, k_sb, v_sb);
   else
     hipLaunchKernelGGL((decode_step_kernel<In, 48>), grid, dim3(dc::kThreads), 0, stream,
                        (const In*)phi, (const In*)psi, (const In*)vb, S_in, S_out, U, out, o_full,
-                       B, r, p, step, q_sb, k_sb, v_sb);
+                       ahead, per, B, r, p, step, q_sb, k_sb, v_sb);
   return launch_status("smat_decode_step");
 }
 
 }  // namespace smat
 
+static int decode(const char* who, int dtype, const void* phi_t, const void* psi_t,
+                  const void* vb_t, const float* S_in, float* S_out, const float* U, float* out,
+                  float* o_full, const int32_t* ahead, int requests, int nb, int B, int r, int p,
+                  int64_t step, int64_t q_sb, int64_t k_sb, int64_t v_sb, void* stream) {
+  using namespace smat;
+  clear_error();
+  SMAT_REQUIRE(phi_t && psi_t && vb_t && S_in && S_out && U && out, SMAT_EINVAL,
+               "%s: null pointer", who);
+  SMAT_REQUIRE(S_in != S_out, SMAT_EINVAL, "%s: S_in and S_out must differ", who);
+  SMAT_REQUIRE(nb >= 0 && B >= 1 && step >= 0 && p >= 2, SMAT_EINVAL,
+               "%s: bad sizes (B=%d p=%d step=%lld)", who, B, p, (long long)step);
+  SMAT_REQUIRE(r >= 1 && r <= kMaxR && p <= kMaxP, SMAT_EUNSUPPORTED,
+               "%s: r=%d p=%d beyond r<=%d, p<=%d", who, r, p, kMaxR, kMaxP);
+  SMAT_REQUIRE(requests >= 1 && nb % requests == 0, SMAT_EINVAL,
+               "%s: %d requests must divide nb=%d", who, requests, nb);
+  if (nb == 0) return SMAT_OK;
+  hipStream_t st = (hipStream_t)stream;
+  const int per = nb / requests;
+  switch (dtype) {
+    case SMAT_BF16:
+      return launch_decode<bf16>(phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full, ahead, per, nb,
+                                 B, r, p, step, q_sb, k_sb, v_sb, st);
+    case SMAT_F16:
+      return launch_decode<f16>(phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full, ahead, per, nb,
+                                B, r, p, step, q_sb, k_sb, v_sb, st);
+    case SMAT_F32:
+      return launch_decode<float>(phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full, ahead, per, nb,
+                                  B, r, p, step, q_sb, k_sb, v_sb, st);
+  }
+  set_error("%s: unknown dtype %d", who, dtype);
+  return SMAT_EINVAL;
+}
+
 extern "C" int smat_decode_step(int dtype, const void* phi_t, const void* psi_t, const void* vb_t,
                                 const float* S_in, float* S_out, const float* U, float* out,
                                 float* o_full, int nb, int B, int r, int p, int64_t step,
                                 int64_t q_sb, int64_t k_sb, int64_t v_sb, void* stream) {
-  using namespace smat;
-  clear_error();
-  SMAT_REQUIRE(phi_t && psi_t && vb_t && S_in && S_out && U && out, SMAT_EINVAL,
-               "smat_decode_step: null pointer");
-  SMAT_REQUIRE(S_in != S_out, SMAT_EINVAL, "smat_decode_step: S_in and S_out must differ");
-  SMAT_REQUIRE(nb >= 0 && B >= 1 && step >= 0 && p >= 2, SMAT_EINVAL,
-               "smat_decode_step: bad sizes (B=%d p=%d step=%lld)", B, p, (long long)step);
-  SMAT_REQUIRE(r >= 1 && r <= kMaxR && p <= kMaxP, SMAT_EUNSUPPORTED,
-               "smat_decode_step: r=%d p=%d beyond r<=%d, p<=%d", r, p, kMaxR, kMaxP);
-  if (nb == 0) return SMAT_OK;
-  hipStream_t st = (hipStream_t)stream;
-  switch (dtype) {
-    case SMAT_BF16:
-      return launch_decode<bf16>(phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full, nb, B, r, p,
-                                 step, q_sb, k_sb, v_sb, st);
-    case SMAT_F16:
-      return launch_decode<f16>(phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full, nb, B, r, p,
-                                step, q_sb, k_sb, v_sb, st);
-    case SMAT_F32:
-      return launch_decode<float>(phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full, nb, B, r, p,
-                                  step, q_sb, k_sb, v_sb, st);
-  }
-  set_error("smat_decode_step: unknown dtype %d", dtype);
-  return SMAT_EINVAL;
+  return decode("smat_decode_step", dtype, phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full,
+                nullptr, 1, nb, B, r, p, step, q_sb, k_sb, v_sb, stream);
+}
+
+extern "C" int smat_decode_step_at(int dtype, const void* phi_t, const void* psi_t,
+                                   const void* vb_t, const float* S_in, float* S_out,
+                                   const float* U, float* out, float* o_full,
+                                   const int32_t* ahead, int requests, int nb, int B, int r,
+                                   int p, int64_t step, int64_t q_sb, int64_t k_sb, int64_t v_sb,
+                                   void* stream) {
+  return decode("smat_decode_step_at", dtype, phi_t, psi_t, vb_t, S_in, S_out, U, out, o_full,
+                ahead, requests, nb, B, r, p, step, q_sb, k_sb, v_sb, stream);
 }

@@ -1,0 +1,373 @@
+// The gated delta rule over whole sequences (gated_delta_scan): the mathematics, the
+// operand splits and the fragment layout are in delta_common.hpp, the state-free
+// part of a chunk in delta_prep.hpp.
+//
+// delta_chain_kernel walks the chunks.  The columns of the state do not mix, so a
+// wave takes 16 of them with all r rows in registers (fp32) and needs nothing of
+// any other wave: K S and Q S from the state, U = T b (V - e K S), O, and the new
+// state, each product's result tiles being the next one's operand as they lie.
+//
+// One wave walks a whole segment where sequences and columns give enough waves.
+// Where they do not, segments are cut into runs: a first pass takes every run from
+// the zero state for its end state E and from the identity for its transition M
+// (its columns are more columns of the same recurrence, with V = 0), a kernel
+// carries the states across the runs, S <- M S + E, and the second pass takes every
+// run from its own state.
+#include "delta_prep.hpp"
+
+namespace smat {
+namespace dl {
+
+struct ChainIO {
+  const void* v;
+  void* o;
+  const float* start;     // state entering run i of sequence s: start + (i nb + s) r p; or null
+  float* end;             // state leaving it, same layout; or null
+  float* trans;           // first pass: M of run i, (i nb + s) R R row-major (R = 32 RB); or null
+  float *save_s, *save_u; // training: states entering chunks, and U, rows padded to p32; or null
+  int ptiles;             // value tiles of 16 columns (tiles behind them are M's)
+  bool vvec, ovec;
+};
+
+template <typename In, int RB, bool OUT>
+__global__ __launch_bounds__(256) void delta_chain_kernel(Geo g, Ops o, ChainIO io, int tiles) {
+  constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid, R = 32 * RB;
+  constexpr int KB = 4 * RB * kFrag, TB = kTri * kFrag;
+  const int ct = blockIdx.x * (blockDim.x >> 6) + wave_id();
+  if (ct >= tiles) return;
+  const int run = blockIdx.y, s = blockIdx.z;
+  const int m = lane_id() & 15, gq = lane_id() >> 4;
+  int c0, c1, seg;
+  run_of(g, run, c0, c1, seg);
+  const bool values = ct < io.ptiles;              // else columns of the transition
+  const int col = 16 * (values ? ct : ct - io.ptiles) + m;
+  const int64_t ks = key_of(g, s);
+  const int64_t rp = (int64_t)g.r * g.p, sn = (int64_t)run * g.nb + s;
+  const int ld = (g.p + 31) / 32 * 32;
+
+  f32x4 S[2 * RB];
+#pragma unroll
+  for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = 16 * mt + 4 * gq + i;
+      if (!values)
+        S[mt][i] = a == col ? 1.f : 0.f;
+      else
+        S[mt][i] = (io.start && a < g.r && col < g.p) ? io.start[sn * rp + (int64_t)a * g.p + col]
+                                                      : 0.f;
+    }
+  const In* vs = (const In*)io.v + s * g.v_sb + col;
+  const bool vlive = values && col < g.p;
+
+  for (int c = c0; c < c1; ++c) {
+    int t0, len;
+    chunk_of(g, c, t0, len);
+    const int64_t sc = (int64_t)s * g.nch + c;
+    const bf16* kr = o.kr + (ks * g.nch + c) * (int64_t)NT * KB;
+    const bf16* kt = o.kt + (ks * g.nch + c) * (int64_t)NT * KB;
+    const bf16* tm = o.tm + sc * NI * TB;
+    const float* vec = o.vec + sc * kVec;
+
+    f32x4 x[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 16 * mt + 4 * gq + i;
+        x[mt][i] = (vlive && t < len) ? to_f32(vs[(int64_t)(t0 + t) * g.v_st]) : 0.f;
+      }
+    if (OUT && io.save_s) {
+      float* Sp = io.save_s + sc * R * ld;
+#pragma unroll
+      for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Sp[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = S[mt][i];
+    }
+    Frag<NI> sb[RB];
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
+    // b (V - e K S)
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      f32x4 a = zero4();
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb)
+        a = mul(a, load_frag<NT>(kr + (mt * RB + kb) * kFrag, KB), sb[kb]);
+      const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
+      const f32x4 b = *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[mt][i] = b[i] * (x[mt][i] - e[i] * a[i]);
+    }
+    f32x4 ot[4];
+    if (OUT) {
+      const bf16* qr = o.qr + (ks * g.nch + c) * (int64_t)NT * KB;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {             // columns in registers, token in the lane
+        ot[mt] = zero4();
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb)
+          ot[mt] = mul(ot[mt], lead<NO>(sb[kb]), load_frag<NT>(qr + (mt * RB + kb) * kFrag, KB));
+        ot[mt] *= g.scale * vec[16 * mt + m];
+      }
+    }
+    Frag<NI> f[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {               // U, in place of x
+      x[mt] = zero4();
+#pragma unroll
+      for (int kb = 0; kb <= mt / 2; ++kb)
+        x[mt] = mul(x[mt], load_frag<NI>(tm + tri(mt, kb) * kFrag, TB), f[kb]);
+    }
+    if (OUT) {
+      if (io.save_u) {
+        float* Up = io.save_u + sc * C * ld;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) Up[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = x[mt][i];
+      }
+      Frag<NO> fo[2];
+      const bf16* pm = o.pm + sc * NO * TB;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NO>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int kb = 0; kb <= mt / 2; ++kb)
+          ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pm + tri(mt, kb) * kFrag, TB));
+        const int t = 16 * mt + m, oc = 16 * ct + 4 * gq;
+        if (t < len)
+          store4((In*)io.o + ((int64_t)s * g.T + t0 + t) * g.p + oc, ot[mt], g.p - oc, io.ovec);
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+      x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+    const float aC = vec[3 * C];
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt) {
+      S[mt] *= aC;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        S[mt] = mul(S[mt], load_frag<NT>(kt + (mt * 2 + kb) * kFrag, KB), f[kb]);
+    }
+  }
+  if (values ? io.end != nullptr : io.trans != nullptr) {
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = 16 * mt + 4 * gq + i;
+        if (!values)
+          io.trans[(sn * R + a) * R + col] = S[mt][i];
+        else if (a < g.r && col < g.p)
+          io.end[sn * rp + (int64_t)a * g.p + col] = S[mt][i];
+      }
+  }
+}
+
+// The states across the runs of a segment: entering run i (start), S <- M_i S + E_i,
+// and out of the last (final).  A wave a (sequence, segment, 16 columns); `rev`
+// walks the runs backwards (the gradient's direction).
+template <int RB>
+__global__ __launch_bounds__(64) void delta_carry_kernel(Geo g, const float* __restrict__ init,
+                                                         const float* __restrict__ E,
+                                                         const float* __restrict__ M,
+                                                         float* __restrict__ start,
+                                                         float* __restrict__ fin, bool rev) {
+  constexpr int R = 32 * RB, NI = kMid;
+  const int m = lane_id() & 15, gq = lane_id() >> 4;
+  const int col = 16 * blockIdx.x + m, seg = blockIdx.y, s = blockIdx.z;
+  const int64_t rp = (int64_t)g.r * g.p;
+  const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
+  f32x4 S[2 * RB];
+  auto each = [&](auto fn) {
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = 16 * mt + 4 * gq + i;
+        if (a < g.r && col < g.p) fn(mt, i, (int64_t)a * g.p + col);
+      }
+  };
+#pragma unroll
+  for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = zero4();
+  const int64_t ss = ((int64_t)seg * g.nb + s) * rp;
+  if (init) each([&](int mt, int i, int64_t off) { S[mt][i] = init[ss + off]; });
+  for (int n = r0; n < r1; ++n) {
+    const int run = rev ? r0 + r1 - 1 - n : n;
+    const int64_t sn = (int64_t)run * g.nb + s;
+    each([&](int mt, int i, int64_t off) { start[sn * rp + off] = S[mt][i]; });
+    Frag<NI> sb[RB];
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = zero4();
+    each([&](int mt, int i, int64_t off) { S[mt][i] = E[sn * rp + off]; });
+    const float* Mr = M + sn * R * R + (int64_t)m * R + 4 * gq;
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) {
+        const float* p = Mr + (int64_t)16 * mt * R + 32 * kb;
+        S[mt] = mul(S[mt],
+                    split<NI>(*reinterpret_cast<const f32x4*>(p),
+                              *reinterpret_cast<const f32x4*>(p + 16)), sb[kb]);
+      }
+  }
+  if (fin) each([&](int mt, int i, int64_t off) { fin[ss + off] = S[mt][i]; });
+}
+
+
+int check_geo(const char* who, int dtype, const Geo& g) {
+  SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
+               "%s: unknown dtype %d", who, dtype);
+  SMAT_REQUIRE(g.nb >= 0 && g.nbk >= 1 && g.T >= 0 && g.nseg >= 1 && g.nch >= 0, SMAT_EINVAL,
+               "%s: bad sizes (nb=%d nbk=%d T=%d nseg=%d nch=%d)", who, g.nb, g.nbk, g.T, g.nseg,
+               g.nch);
+  SMAT_REQUIRE(g.nb % g.nbk == 0, SMAT_EINVAL, "%s: nbk=%d does not divide nb=%d", who, g.nbk,
+               g.nb);
+  SMAT_REQUIRE(g.r >= 1 && g.r <= kMaxR && g.p >= 1 && g.p <= kMaxP, SMAT_EUNSUPPORTED,
+               "%s: r=%d p=%d beyond r<=%d, p<=%d", who, g.r, g.p, kMaxR, kMaxP);
+  SMAT_REQUIRE(g.nb <= 65535 && g.nruns <= 65535 && g.nseg <= 65535, SMAT_EUNSUPPORTED,
+               "%s: nb=%d, %d segments and %d runs must stay within 65535", who, g.nb, g.nseg,
+               g.nruns);
+  if (g.chunks || g.runs || g.segrun) {
+    SMAT_REQUIRE(g.chunks && g.runs && g.segrun && g.nruns >= g.nseg, SMAT_EINVAL,
+                 "%s: segments need the chunk, run and segment tables", who);
+  } else {
+    SMAT_REQUIRE(g.nseg == 1 && g.nch == (g.T + C - 1) / C, SMAT_EINVAL,
+                 "%s: %d chunks for T=%d", who, g.nch, g.T);
+    SMAT_REQUIRE(g.K >= 1 && g.nruns == (g.nch > 0 ? (g.nch + g.K - 1) / g.K : 1), SMAT_EINVAL,
+                 "%s: %d runs of %d chunks for %d chunks", who, g.nruns, g.K, g.nch);
+  }
+  return SMAT_OK;
+}
+
+template <int RB>
+static void carry_kernel(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
+                         hipStream_t st) {
+  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3((g.p + 15) / 16, g.nseg, g.nb), dim3(64), 0, st,
+                     g, init, c.E, c.M, c.start, fin, rev);
+}
+
+int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
+                 hipStream_t st) {
+  switch (rblocks(g.r)) {
+    case 1: carry_kernel<1>(g, init, c, fin, rev, st); break;
+    case 2: carry_kernel<2>(g, init, c, fin, rev, st); break;
+    case 3: carry_kernel<3>(g, init, c, fin, rev, st); break;
+    default: carry_kernel<4>(g, init, c, fin, rev, st); break;
+  }
+  return launch_status("smat_delta_scan: carry");
+}
+
+template <typename In, int RB, bool OUT>
+static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipStream_t st) {
+  const int W = tiles < 4 ? tiles : 4;
+  hipLaunchKernelGGL((delta_chain_kernel<In, RB, OUT>), dim3((tiles + W - 1) / W, g.nruns, g.nb),
+                     dim3(64 * W), 0, st, g, o, io, tiles);
+}
+
+template <typename In, int RB>
+static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v,
+                const float* logA, const float* beta, const float* state, void* out,
+                float* state_out, float* save_s, float* save_u, void* ws, hipStream_t st) {
+  constexpr int eb = sizeof(In);
+  Arena ar{(char*)ws};
+  const Ops o = take_ops(ar, dtype, g.nb, g.nbk, g.nch, g.r, false);
+  const bool qvec = vec4_ok(q, g.q_sb, g.q_st, eb), kvec = vec4_ok(k, g.k_sb, g.k_st, eb);
+  if (g.nch > 0)
+    hipLaunchKernelGGL((delta_prep_kernel<In, RB, false>), dim3(g.nch, g.nb), dim3(256), 0, st, q,
+                       k, logA, beta, g, o, qvec, kvec);
+  ChainIO io = {};
+  io.v = v;
+  io.o = out;
+  io.start = state;
+  io.end = state_out;
+  io.ovec = vec4_ok(out, 0, g.p, eb);
+  io.ptiles = (g.p + 15) / 16;
+  if (g.nruns > g.nseg) {
+    const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);
+    ChainIO first = io;
+    first.o = nullptr;
+    first.start = nullptr;
+    first.end = c.E;
+    first.trans = c.M;
+    chain<In, RB, false>(g, o, first, io.ptiles + 2 * RB, st);
+    const int rc = launch_carry(g, state, c, state_out, false, st);
+    if (rc) return rc;
+    io.start = c.start;
+    io.end = nullptr;
+  }
+  io.save_s = save_s;
+  io.save_u = save_u;
+  if (save_s) io.ptiles = p32(g.p) / 16;
+  chain<In, RB, true>(g, o, io, io.ptiles, st);
+  return launch_status("smat_delta_scan");
+}
+
+}  // namespace dl
+}  // namespace smat
+
+extern "C" int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p) {
+  // waves that whole segments give, were they all as long as the longest
+  const int64_t work = (int64_t)nb * ((p + 15) / 16) * nch;       // chunk steps
+  if (longest < 32 || work >= (int64_t)512 * longest) return longest > 0 ? longest : 1;
+  const int64_t K = (work + 1023) / 1024;
+  return (int)(K < 8 ? 8 : K < longest ? K : longest);
+}
+
+extern "C" int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg,
+                                              int nruns, int r, int p, int backward) {
+  using namespace smat::dl;
+  Arena ar{nullptr};
+  take_ops(ar, dtype, nb, nbk, nch, r, backward != 0);
+  if (nruns > nseg) take_carry(ar, nb, nruns, r, p);
+  if (backward) {
+    ar.take<float>((int64_t)nb * nch * 32 * rblocks(r) * p32(p));   // dS' of every chunk
+    ar.take<float>((int64_t)nb * nch * C * p32(p));                 // Z
+  }
+  return ar.used;
+}
+
+extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const void* v,
+                               const float* logA, const float* beta, const float* state, void* out,
+                               float* state_out, float* save_s, float* save_u,
+                               const int32_t* chunks, const int32_t* runs, const int32_t* segrun,
+                               int nb, int nbk, int T, int nseg, int nch, int nruns, int K, int r,
+                               int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
+                               int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb,
+                               int64_t a_st, int64_t b_sb, int64_t b_st, void* workspace,
+                               int64_t workspace_bytes, void* stream) {
+  using namespace smat;
+  using namespace smat::dl;
+  clear_error();
+  const char* who = "smat_delta_scan";
+  const Geo g = {chunks, runs, segrun, nb, nbk, T, nseg, nch, nruns, K, r, p, scale,
+                 q_sb, q_st, k_sb, k_st, v_sb, v_st, a_sb, a_st, b_sb, b_st};
+  const int rc = check_geo(who, dtype, g);
+  if (rc) return rc;
+  if (nb == 0) return SMAT_OK;
+  SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && out), SMAT_EINVAL, "%s: null pointer",
+               who);
+  SMAT_REQUIRE(!save_s == !save_u, SMAT_EINVAL, "%s: save_s and save_u go together", who);
+  SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
+  const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 0);
+  SMAT_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
+                   ((uintptr_t)workspace & 255) == 0,
+               SMAT_EINVAL, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who,
+               (long long)workspace_bytes, (long long)need);
+  hipStream_t st = (hipStream_t)stream;
+  auto go = [&](auto in, auto rb) {
+    typedef decltype(in) In;
+    return scan<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, v, logA, beta,
+                                         state, out, state_out, save_s, save_u, workspace, st);
+  };
+  return dispatch(dtype, r, go);
+}

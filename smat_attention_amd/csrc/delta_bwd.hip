@@ -1,0 +1,492 @@
+// The gradient of the gated delta rule over whole sequences.  With the notation of
+// delta_common.hpp, the gradient dO of the output and dS' of the state leaving a
+// chunk:
+//
+//   dU = P^T dO + w K dS'            Z = T^T dU              dV = b Z
+//   dS = exp(L_C) dS' + Q^T (scale e dO) - K^T (e b Z)
+//   G  = D . (scale dO U^T) (j <= i)     N = -D . (Z U^T) (j < i)
+//   dQ = scale e dO S^T + G K
+//   y  = N K - e Z S^T                   dK = b y + w U dS'^T + G^T Q + (b N)^T K
+//   db_i = Z_i.V_i + k_i.y_i
+//   dlogA_t = sum_{i >= t} (q_i.dQ_i + b_i k_i.y_i - k_i.(dK_i - b_i y_i)) + <dS', S'>
+//
+// (L_i enters as q_i e^{L_i}, as the e^{L_i} of the reading k_i and as the e^{-L_i}
+// of the writing one, and everything behind the chunk as e^{L_C} in S'.)
+//
+// Two kernels after the chunks' operands: delta_rchain_kernel walks the chunks
+// backwards through dS as the forward's chain walks them through S (16 columns a
+// wave, no exchange), storing dS' and Z of every chunk; delta_grad_kernel, one
+// workgroup a (key sequence, chunk), forms the rest for the group's value heads one
+// after another, so the gradients of a shared key head are sums in registers, in
+// the heads' order.
+#include "delta_prep.hpp"
+
+namespace smat {
+namespace dl {
+
+struct RChainIO {
+  const void* dout;       // (nb, T, p), strides d_sb, d_st
+  int64_t d_sb, d_st;
+  const float* start;     // dS behind run i of sequence s: start + (i nb + s) r p; or null
+  float* end;             // dS before it, same layout; or null
+  float* trans;           // first pass: the run's transition; or null
+  float *save_d, *z;      // dS' of every chunk (R x p32) and Z (64 x p32)
+  void* dv;               // (nb, T, p) contiguous
+  int ptiles;
+};
+
+template <typename In, int RB, bool OUT>
+__global__ __launch_bounds__(256) void delta_rchain_kernel(Geo g, Ops o, RChainIO io, int tiles) {
+  constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB;
+  constexpr int KB = 4 * RB * kFrag, TB = kTri * kFrag;
+  const int ct = blockIdx.x * (blockDim.x >> 6) + wave_id();
+  if (ct >= tiles) return;
+  const int run = blockIdx.y, s = blockIdx.z;
+  const int m = lane_id() & 15, gq = lane_id() >> 4;
+  int c0, c1, seg;
+  run_of(g, run, c0, c1, seg);
+  const bool values = ct < io.ptiles;
+  const int col = 16 * (values ? ct : ct - io.ptiles) + m;
+  const int64_t ks = key_of(g, s);
+  const int64_t rp = (int64_t)g.r * g.p, sn = (int64_t)run * g.nb + s;
+  const int ld = (g.p + 31) / 32 * 32;
+
+  f32x4 S[2 * RB];                                 // dS
+#pragma unroll
+  for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = 16 * mt + 4 * gq + i;
+      if (!values)
+        S[mt][i] = a == col ? 1.f : 0.f;
+      else
+        S[mt][i] = (io.start && a < g.r && col < g.p) ? io.start[sn * rp + (int64_t)a * g.p + col]
+                                                      : 0.f;
+    }
+  const In* ds = (const In*)io.dout + s * io.d_sb + col;
+  const bool dlive = values && col < g.p;
+
+  for (int c = c1 - 1; c >= c0; --c) {
+    int t0, len;
+    chunk_of(g, c, t0, len);
+    const int64_t sc = (int64_t)s * g.nch + c;
+    const int64_t kc = (ks * g.nch + c) * (int64_t)NT * KB;
+    const float* vec = o.vec + sc * kVec;
+    f32x4 d[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 16 * mt + 4 * gq + i;
+        d[mt][i] = (dlive && t < len) ? to_f32(ds[(int64_t)(t0 + t) * io.d_st]) : 0.f;
+      }
+    if (OUT) {
+      float* Sp = io.save_d + sc * R * ld;
+#pragma unroll
+      for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Sp[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = S[mt][i];
+    }
+    f32x4 x[4];                                    // dU
+    {
+      Frag<NI> sb[RB];
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        x[mt] = zero4();
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb)
+          x[mt] = mul(x[mt], load_frag<NT>(o.kr + kc + (mt * RB + kb) * kFrag, KB), sb[kb]);
+        x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
+      }
+    }
+    if (values) {
+      Frag<NT> df[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int kb = mt / 2; kb < 2; ++kb)
+          x[mt] = mul(x[mt], load_frag<NI>(o.pt + (sc * NI * kTri + tri_t(mt, kb)) * kFrag, TB),
+                      df[kb]);
+    }
+    Frag<NI> f[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {               // Z
+      x[mt] = zero4();
+#pragma unroll
+      for (int kb = mt / 2; kb < 2; ++kb)
+        x[mt] = mul(x[mt], load_frag<NI>(o.tt + (sc * NI * kTri + tri_t(mt, kb)) * kFrag, TB),
+                    f[kb]);
+    }
+    if (OUT) {
+      float* Zp = io.z + sc * C * ld;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) Zp[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = x[mt][i];
+    }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
+      x[mt] *= *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);     // b Z
+      if (OUT && dlive) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = 16 * mt + 4 * gq + i;
+          if (t < len)
+            ((In*)io.dv)[((int64_t)s * g.T + t0 + t) * g.p + col] = from_f32<In>(x[mt][i]);
+        }
+      }
+      x[mt] *= -e;
+      d[mt] *= g.scale * e;
+    }
+    const float aC = vec[3 * C];
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt) S[mt] *= aC;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        S[mt] = mul(S[mt], load_frag<NT>(o.kt + kc + (mt * 2 + kb) * kFrag, KB), f[kb]);
+    if (values) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
+#pragma unroll
+      for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          S[mt] = mul(S[mt], load_frag<NT>(o.qt + kc + (mt * 2 + kb) * kFrag, KB), f[kb]);
+    }
+  }
+  if (values ? io.end != nullptr : io.trans != nullptr) {
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = 16 * mt + 4 * gq + i;
+        if (!values)
+          io.trans[(sn * R + a) * R + col] = S[mt][i];
+        else if (a < g.r && col < g.p)
+          io.end[sn * rp + (int64_t)a * g.p + col] = S[mt][i];
+      }
+  }
+}
+
+struct GradIO {
+  const void *q, *k, *v, *dout;
+  const float *logA, *beta;
+  int64_t d_sb, d_st;
+  const float *save_s, *save_u, *save_d, *z;
+  void *dq, *dk;          // (nbk, T, r) contiguous
+  float *dlogA, *dbeta;   // (nb, T) contiguous
+  bool qvec, kvec, vvec, dvec, ovec;
+};
+
+// Eight consecutive fp32 values as terms.
+template <int N> __device__ __forceinline__ Frag<N> split8(const float* p) {
+  return split<N>(*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4));
+}
+__device__ __forceinline__ float dot4(const f32x4& a, const f32x4& b) {
+  return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
+}
+// Sum over the four lane groups (lanes m, m + 16, m + 32, m + 48).
+__device__ __forceinline__ float sum_groups(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+template <typename In, int RB>
+__global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io) {
+  constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB;
+  constexpr int KB = 4 * RB * kFrag;
+  __shared__ __align__(16) float G[C * kLd], N[C * kLd];
+  __shared__ double Ls[C];
+  __shared__ float bs[C], dLs[C], inter[C], pair[2][4];
+  const int c = blockIdx.x, ks = blockIdx.y, group = g.nb / g.nbk;
+  const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
+  const int tok = 16 * w + m, ld = (g.p + 31) / 32 * 32;
+  int t0, len;
+  chunk_of(g, c, t0, len);
+  const bool live = tok < len;
+  const int64_t row = t0 + (live ? tok : 0);
+  const int64_t kc = ((int64_t)ks * g.nch + c) * NT * KB;
+  const In* qrow = (const In*)io.q + ks * g.q_sb + row * g.q_st;
+  const In* krow = (const In*)io.k + ks * g.k_sb + row * g.k_st;
+
+  // token in the lane, features 16 rt + 4 gq + i in registers, throughout
+  f32x4 dQ[2 * RB], dK[2 * RB];
+#pragma unroll
+  for (int rt = 0; rt < 2 * RB; ++rt) dQ[rt] = dK[rt] = zero4();
+
+  for (int h = 0; h < group; ++h) {
+    const int s = ks * group + h;
+    const int64_t sc = (int64_t)s * g.nch + c;
+    const float *Sp = io.save_s + sc * R * ld, *Dp = io.save_d + sc * R * ld;
+    const float *Up = io.save_u + sc * C * ld, *Zp = io.z + sc * C * ld;
+    const float* vec = o.vec + sc * kVec;
+    const In* drow = (const In*)io.dout + s * io.d_sb + row * io.d_st;
+    const In* vrow = (const In*)io.v + s * g.v_sb + row * g.v_st;
+    chunk_decays(g, io.logA, io.beta, s, t0, len, Ls, bs);
+
+    f32x4 a[2 * RB], y[2 * RB], kw[2 * RB], gp[4], np[4];
+#pragma unroll
+    for (int rt = 0; rt < 2 * RB; ++rt) a[rt] = y[rt] = kw[rt] = zero4();
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) gp[jt] = np[jt] = zero4();
+    float zv = 0.f, dots = 0.f;
+    for (int pb = 0; pb < ld; pb += 32) {
+      const int pc = pb + 8 * gq;
+      f32x4 d0 = zero4(), d1 = zero4(), v0 = zero4(), v1 = zero4();
+      if (live) {
+        d0 = load4(drow + pc, g.p - pc, io.dvec);
+        d1 = load4(drow + pc + 4, g.p - pc - 4, io.dvec);
+        v0 = load4(vrow + pc, g.p - pc, io.vvec);
+        v1 = load4(vrow + pc + 4, g.p - pc - 4, io.vvec);
+      }
+      const Frag<NT> df = split<NT>(d0, d1);
+      const f32x4 z0 = *reinterpret_cast<const f32x4*>(Zp + (int64_t)tok * ld + pc);
+      const f32x4 z1 = *reinterpret_cast<const f32x4*>(Zp + (int64_t)tok * ld + pc + 4);
+      zv += dot4(z0, v0) + dot4(z1, v1);
+      const Frag<NI> zf = split<NI>(z0, z1);
+      const Frag<NI> uf = split8<NI>(Up + (int64_t)tok * ld + pc);
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt)
+        if (jt <= w) {                             // column j in the lane, rows i in registers
+          const Frag<NI> uj = split8<NI>(Up + (int64_t)(16 * jt + m) * ld + pc);
+          gp[jt] = mul(gp[jt], df, uj);
+          np[jt] = mul(np[jt], zf, uj);
+        }
+#pragma unroll
+      for (int rt = 0; rt < 2 * RB; ++rt) {
+        const int64_t at = (int64_t)(16 * rt + m) * ld + pc;
+        const f32x4 s0 = *reinterpret_cast<const f32x4*>(Sp + at);
+        const f32x4 s1 = *reinterpret_cast<const f32x4*>(Sp + at + 4);
+        const f32x4 e0 = *reinterpret_cast<const f32x4*>(Dp + at);
+        const f32x4 e1 = *reinterpret_cast<const f32x4*>(Dp + at + 4);
+        if ((rt & 3) == w) dots += dot4(s0, e0) + dot4(s1, e1);
+        const Frag<NI> sf = split<NI>(s0, s1), ef = split<NI>(e0, e1);
+        a[rt] = mul(a[rt], sf, df);
+        y[rt] = mul(y[rt], sf, zf);
+        kw[rt] = mul(kw[rt], ef, uf);
+      }
+    }
+    zv = sum_groups(zv);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) dots += __shfl_xor(dots, d);
+    if (lane_id() == 0) pair[h & 1][w] = dots;       // wave 0 may still read the last head's
+    __syncthreads();                               // Ls and bs, pair; G and N free
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ti = 16 * w + 4 * gq + i, j = 16 * jt + m;
+        const float D = j <= ti ? expf((float)(Ls[ti] - Ls[j])) : 0.f;
+        G[ti * kLd + j] = j <= ti ? g.scale * (D * gp[jt][i]) : 0.f;
+        N[ti * kLd + j] = j < ti ? -(D * np[jt][i]) : 0.f;
+      }
+    __syncthreads();
+    const float e = vec[tok], wt = vec[C + tok], b = vec[2 * C + tok];
+    float kint = 0.f;
+#pragma unroll
+    for (int rt = 0; rt < 2 * RB; ++rt) {
+      a[rt] *= g.scale * e;
+      y[rt] *= -e;
+      kw[rt] *= wt;
+    }
+#pragma unroll
+    for (int rt = 0; rt < 2 * RB; ++rt) {
+      const int f0 = 16 * rt + 4 * gq;
+      kint += live ? dot4(load4(krow + f0, g.r - f0, io.kvec), kw[rt]) : 0.f;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int j0 = 32 * kb + 4 * gq;
+      if (kb <= w / 2) {                           // rows i = tok, over j
+        const float *Gr = G + tok * kLd + j0, *Nr = N + tok * kLd + j0;
+        const Frag<NI> gf = split<NI>(*reinterpret_cast<const f32x4*>(Gr),
+                                      *reinterpret_cast<const f32x4*>(Gr + 16));
+        const Frag<NI> nf = split<NI>(*reinterpret_cast<const f32x4*>(Nr),
+                                      *reinterpret_cast<const f32x4*>(Nr + 16));
+#pragma unroll
+        for (int rt = 0; rt < 2 * RB; ++rt) {
+          const Frag<NT> kf = load_frag<NT>(o.kt + kc + (rt * 2 + kb) * kFrag, KB);
+          a[rt] = mul(a[rt], kf, gf);
+          y[rt] = mul(y[rt], kf, nf);
+        }
+      }
+      if (kb >= w / 2) {                           // columns j = tok, over i
+        f32x4 gx[2], nx[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int ti = j0 + 16 * t + i;
+            gx[t][i] = G[ti * kLd + tok];
+            nx[t][i] = bs[ti] * N[ti * kLd + tok];
+          }
+        const Frag<NI> gf = split<NI>(gx[0], gx[1]), nf = split<NI>(nx[0], nx[1]);
+#pragma unroll
+        for (int rt = 0; rt < 2 * RB; ++rt) {
+          kw[rt] = mul(kw[rt], load_frag<NT>(o.qt + kc + (rt * 2 + kb) * kFrag, KB), gf);
+          kw[rt] = mul(kw[rt], load_frag<NT>(o.kt + kc + (rt * 2 + kb) * kFrag, KB), nf);
+        }
+      }
+    }
+    float qd = 0.f, ky = 0.f, kk = 0.f;
+#pragma unroll
+    for (int rt = 0; rt < 2 * RB; ++rt) {
+      const int f0 = 16 * rt + 4 * gq;
+      const f32x4 kv = live ? load4(krow + f0, g.r - f0, io.kvec) : zero4();
+      const f32x4 qv = live ? load4(qrow + f0, g.r - f0, io.qvec) : zero4();
+      qd += dot4(qv, a[rt]);
+      ky += dot4(kv, y[rt]);
+      kk += dot4(kv, kw[rt]);
+      dQ[rt] += a[rt];
+      dK[rt] += b * y[rt] + kw[rt];
+    }
+    qd = sum_groups(qd);
+    ky = sum_groups(ky);
+    kk = sum_groups(kk);
+    kint = sum_groups(kint);
+    if (gq == 0) {
+      dLs[tok] = qd + b * ky - kk;
+      inter[tok] = kint;
+      if (live) io.dbeta[(int64_t)s * g.T + t0 + tok] = zv + ky;
+    }
+    __syncthreads();
+    if (w == 0) {
+      const int t = lane_id();
+      float x = dLs[t], sum = inter[t];
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const float up = __shfl_down(x, d);
+        if (t + d < 64) x += up;
+        sum += __shfl_xor(sum, d);
+      }
+      const float* pr = pair[h & 1];
+      sum += vec[3 * C] * (pr[0] + pr[1] + pr[2] + pr[3]);           // <dS', S'>
+      if (t < len) io.dlogA[(int64_t)s * g.T + t0 + t] = x + sum;
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int rt = 0; rt < 2 * RB; ++rt) {
+    const int f0 = 16 * rt + 4 * gq;
+    const int64_t at = ((int64_t)ks * g.T + row) * g.r + f0;
+    store4((In*)io.dq + at, dQ[rt], g.r - f0, io.ovec);
+    store4((In*)io.dk + at, dK[rt], g.r - f0, io.ovec);
+  }
+}
+
+template <typename In, int RB, bool OUT>
+static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hipStream_t st) {
+  const int W = tiles < 4 ? tiles : 4;
+  hipLaunchKernelGGL((delta_rchain_kernel<In, RB, OUT>), dim3((tiles + W - 1) / W, g.nruns, g.nb),
+                     dim3(64 * W), 0, st, g, o, io, tiles);
+}
+
+template <typename In, int RB>
+static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr, void* dv,
+                    const float* dstate_out, float* dstate, void* ws, hipStream_t st) {
+  constexpr int eb = sizeof(In);
+  Arena ar{(char*)ws};
+  const Ops o = take_ops(ar, dtype, g.nb, g.nbk, g.nch, g.r, true);
+  gr.qvec = vec4_ok(q, g.q_sb, g.q_st, eb);
+  gr.kvec = vec4_ok(k, g.k_sb, g.k_st, eb);
+  gr.vvec = vec4_ok(gr.v, g.v_sb, g.v_st, eb);
+  gr.dvec = vec4_ok(gr.dout, gr.d_sb, gr.d_st, eb);
+  gr.ovec = vec4_ok(gr.dq, 0, g.r, eb) && vec4_ok(gr.dk, 0, g.r, eb);
+  if (g.nch > 0)
+    hipLaunchKernelGGL((delta_prep_kernel<In, RB, true>), dim3(g.nch, g.nb), dim3(256), 0, st, q,
+                       k, gr.logA, gr.beta, g, o, gr.qvec, gr.kvec);
+  RChainIO io = {};
+  io.dout = gr.dout;
+  io.d_sb = gr.d_sb;
+  io.d_st = gr.d_st;
+  io.dv = dv;
+  io.start = dstate_out;
+  io.end = dstate;
+  io.ptiles = (g.p + 15) / 16;
+  if (g.nruns > g.nseg) {
+    const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);
+    RChainIO first = io;
+    first.start = nullptr;
+    first.end = c.E;
+    first.trans = c.M;
+    rchain<In, RB, false>(g, o, first, io.ptiles + 2 * RB, st);
+    const int rc = launch_carry(g, dstate_out, c, dstate, true, st);
+    if (rc) return rc;
+    io.start = c.start;
+    io.end = nullptr;
+  }
+  float* save_d = ar.take<float>((int64_t)g.nb * g.nch * 32 * RB * p32(g.p));
+  float* z = ar.take<float>((int64_t)g.nb * g.nch * C * p32(g.p));
+  io.save_d = save_d;
+  io.z = z;
+  io.ptiles = p32(g.p) / 16;
+  rchain<In, RB, true>(g, o, io, io.ptiles, st);
+  gr.save_d = save_d;
+  gr.z = z;
+  if (g.nch > 0)
+    hipLaunchKernelGGL((delta_grad_kernel<In, RB>), dim3(g.nch, g.nbk), dim3(256), 0, st, g, o,
+                       gr);
+  return launch_status("smat_delta_scan_backward");
+}
+
+}  // namespace dl
+}  // namespace smat
+
+extern "C" int smat_delta_scan_backward(
+    int dtype, const void* q, const void* k, const void* v, const float* logA, const float* beta,
+    const void* dout, const float* dstate_out, const float* save_s, const float* save_u, void* dq,
+    void* dk, void* dv, float* dlogA, float* dbeta, float* dstate, const int32_t* chunks,
+    const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch,
+    int nruns, int K, int r, int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
+    int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st, int64_t b_sb,
+    int64_t b_st, int64_t d_sb, int64_t d_st, void* workspace, int64_t workspace_bytes,
+    void* stream) {
+  using namespace smat;
+  using namespace smat::dl;
+  clear_error();
+  const char* who = "smat_delta_scan_backward";
+  const Geo g = {chunks, runs, segrun, nb, nbk, T, nseg, nch, nruns, K, r, p, scale,
+                 q_sb, q_st, k_sb, k_st, v_sb, v_st, a_sb, a_st, b_sb, b_st};
+  const int rc = check_geo(who, dtype, g);
+  if (rc) return rc;
+  if (nb == 0) return SMAT_OK;
+  SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && dout && save_s && save_u && dq && dk &&
+                            dv && dlogA && dbeta),
+               SMAT_EINVAL, "%s: null pointer", who);
+  const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 1);
+  SMAT_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
+                   ((uintptr_t)workspace & 255) == 0,
+               SMAT_EINVAL, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who,
+               (long long)workspace_bytes, (long long)need);
+  GradIO gr = {};
+  gr.q = q;
+  gr.k = k;
+  gr.v = v;
+  gr.dout = dout;
+  gr.logA = logA;
+  gr.beta = beta;
+  gr.d_sb = d_sb;
+  gr.d_st = d_st;
+  gr.save_s = save_s;
+  gr.save_u = save_u;
+  gr.dq = dq;
+  gr.dk = dk;
+  gr.dlogA = dlogA;
+  gr.dbeta = dbeta;
+  return dispatch(dtype, r, [&](auto in, auto rb) {
+    typedef decltype(in) In;
+    return backward<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, gr, dv,
+                                             dstate_out, dstate, workspace, (hipStream_t)stream);
+  });
+}

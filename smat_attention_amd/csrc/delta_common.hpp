@@ -1,0 +1,272 @@
+// The gated delta rule's chunked form (delta.hip, delta_bwd.hip): sizes, operand
+// splits, and the layout of a chunk's operands in the workspace.
+//
+//   S_t = a_t S_{t-1} + k_t u_t^T,   u_t = b_t (v_t - a_t S_{t-1}^T k_t),
+//   o_t = scale S_t^T q_t,           a_t = exp(logA_t).
+//
+// Over a chunk of C = 64 tokens entered with state S, with L the running sum of
+// logA inside it, e_i = exp(L_i), w_i = exp(L_C - L_i) and D_ij = exp(L_i - L_j):
+//
+//   (I + A) U = b (V - e K S),   A_ij = b_i D_ij k_i.k_j  (j < i)
+//   O  = scale e Q S + P U,      P_ij = scale D_ij q_i.k_j  (j <= i)
+//   S' = exp(L_C) S + (w K)^T U
+//
+// T = (I + A)^{-1}, P and the row factors do not depend on S, so one kernel forms
+// them for every chunk at once; what remains along the sequence is the chain of
+// products through S.
+//
+// Operands.  Every product runs on v_mfma_f32_16x16x32_bf16.  A value held in
+// fewer than its own bits is a sum of bf16 terms: bf16 inputs are one term, fp16
+// inputs two (exact: 11 bits), fp32 inputs and everything that is computed in fp32
+// on the way to a state or a gradient three (24 bits), so that states and the fp32
+// gradients have fp32's accuracy.  What ends in a 16-bit output alone (Q S, P U)
+// takes two terms, 2^-17 of the value and 2^8 finer than the output's rounding.  A
+// product keeps the terms whose orders sum below the larger count.  (fp32 MFMA
+// needs 16 times the cycles of one bf16 product, these forms three to six.)
+//
+// Contraction slots.  A 16x16 result has its column in lane & 15 and rows 4g + i
+// (g = lane >> 4) in registers.  Slot (g, j) of a 32-long contraction stands for
+// index 4g + j (j < 4) or 16 + 4g + j - 4: then two stacked result tiles are an
+// operand of the next product as they lie in registers, and the chain needs no
+// exchange between lanes.  All operands in the workspace are stored in that order,
+// one 16 x 32 fragment in 1 KB, lane by lane.
+#pragma once
+
+#include <type_traits>
+
+#include "smat_host.hpp"
+
+namespace smat {
+namespace dl {
+
+constexpr int C = 64;              // tokens a chunk
+constexpr int kFrag = 512;         // elements a 16 x 32 fragment
+constexpr int kVec = 256;          // floats a chunk: e[64], w[64], b[64], exp(L_C), unused
+constexpr int kTri = 6;            // fragments of a 64 x 64 triangle
+constexpr int kMaxR = 128, kMaxP = 256;
+
+template <typename In> struct Terms;
+template <> struct Terms<bf16> { static constexpr int in = 1, out = 2; };
+template <> struct Terms<f16> { static constexpr int in = 2, out = 2; };
+template <> struct Terms<float> { static constexpr int in = 3, out = 3; };
+constexpr int kMid = 3;            // terms of what is computed in fp32
+
+template <int N> struct Frag { bf16x8 t[N]; };
+
+// Eight fp32 values as N bf16 terms each.
+template <int N>
+__device__ __forceinline__ Frag<N> split(const f32x4& a, const f32x4& b) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  Frag<N> f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    f32x2 v = q < 2 ? f32x2{a[2 * q], a[2 * q + 1]} : f32x2{b[2 * q - 4], b[2 * q - 3]};
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const bf16x2 h = __builtin_convertvector(v, bf16x2);
+      f.t[n][2 * q] = h[0];
+      f.t[n][2 * q + 1] = h[1];
+      if (n + 1 < N) {
+        const unsigned u = __builtin_bit_cast(unsigned, h);
+        v[0] -= __uint_as_float(u << 16);
+        v[1] -= __uint_as_float(u & 0xffff0000u);
+      }
+    }
+  }
+  return f;
+}
+
+template <int N> __device__ __forceinline__ Frag<N> zero_frag() {
+  return split<N>(zero4(), zero4());
+}
+
+// The leading N terms.
+template <int N, int M> __device__ __forceinline__ Frag<N> lead(const Frag<M>& f) {
+  static_assert(N <= M, "");
+  Frag<N> g;
+#pragma unroll
+  for (int n = 0; n < N; ++n) g.t[n] = f.t[n];
+  return g;
+}
+
+// c += a b over the terms of order below max(NA, NB), small ones first.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mul(f32x4 c, const Frag<NA>& a, const Frag<NB>& b) {
+  constexpr int M = NA > NB ? NA : NB;
+#pragma unroll
+  for (int o = M - 1; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (o - i >= 0 && o - i < NB) c = mma(c, a.t[i], b.t[o - i]);
+  return c;
+}
+
+// Terms of a stored fragment: term n lies `ts` elements behind term n - 1.
+template <int N>
+__device__ __forceinline__ Frag<N> load_frag(const bf16* p, int64_t ts) {
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    f.t[n] = *reinterpret_cast<const bf16x8*>(p + n * ts + lane_id() * 8);
+  return f;
+}
+template <int N>
+__device__ __forceinline__ void store_frag(bf16* p, int64_t ts, const Frag<N>& f) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) *reinterpret_cast<bf16x8*>(p + n * ts + lane_id() * 8) = f.t[n];
+}
+
+// Fragment of a lower triangle's row tile mt, contraction block kb (kb <= mt / 2),
+// and of its transpose (kb >= mt / 2).
+__device__ __forceinline__ constexpr int tri(int mt, int kb) {
+  return mt < 2 ? mt : 2 * mt - 2 + kb;
+}
+__device__ __forceinline__ constexpr int tri_t(int mt, int kb) {
+  return mt < 2 ? 2 * mt + kb : mt + 2;
+}
+
+// Four consecutive elements; those at and past nv are zero.
+template <typename In>
+__device__ __forceinline__ f32x4 load4(const In* p, int nv, bool vec) {
+  f32x4 x = zero4();
+  if (vec && nv >= 4) {
+    typedef In In4 __attribute__((ext_vector_type(4)));
+    const In4 v = *reinterpret_cast<const In4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_f32(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < nv) x[i] = to_f32(p[i]);
+  }
+  return x;
+}
+template <typename In>
+__device__ __forceinline__ void store4(In* p, const f32x4& x, int nv, bool vec) {
+  if (vec && nv >= 4) {
+    typedef In In4 __attribute__((ext_vector_type(4)));
+    In4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = from_f32<In>(x[i]);
+    *reinterpret_cast<In4*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < nv) p[i] = from_f32<In>(x[i]);
+  }
+}
+
+// Whether groups of four elements of rows at p may be read at once.
+inline bool vec4_ok(const void* p, int64_t sb, int64_t st, int eb) {
+  return (reinterpret_cast<uintptr_t>(p) % (4 * eb)) == 0 && sb % 4 == 0 && st % 4 == 0;
+}
+
+// One call's geometry.  Chunks and runs (consecutive chunks of one segment that one
+// wave walks) come from tables when the sequences are segmented, else from
+// arithmetic: chunk c is tokens [64 c, 64 c + 64), run g chunks [g K, g K + K).
+struct Geo {
+  const int32_t* chunks;   // (nch, 2): first token, tokens; or null
+  const int32_t* runs;     // (nruns, 3): first chunk, end chunk, segment; or null
+  const int32_t* segrun;   // (nseg + 1): first run of each segment; or null
+  int nb, nbk, T, nseg, nch, nruns, K, r, p;
+  float scale;
+  int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st, a_sb, a_st, b_sb, b_st;
+};
+__device__ __forceinline__ void chunk_of(const Geo& g, int c, int& t0, int& len) {
+  if (g.chunks) {
+    t0 = g.chunks[2 * c];
+    len = g.chunks[2 * c + 1];
+  } else {
+    t0 = c * C;
+    len = min(C, g.T - t0);
+  }
+}
+__device__ __forceinline__ void run_of(const Geo& g, int i, int& c0, int& c1, int& seg) {
+  if (g.runs) {
+    c0 = g.runs[3 * i];
+    c1 = g.runs[3 * i + 1];
+    seg = g.runs[3 * i + 2];
+  } else {
+    c0 = i * g.K;
+    c1 = min(c0 + g.K, g.nch);
+    seg = 0;
+  }
+}
+
+// The chunks' operands in the workspace.
+struct Ops {
+  bf16 *kr, *kt, *qr, *qt;  // rows of K and Q (contraction over r), and transposed (over tokens)
+  bf16 *tm, *pm;            // T and P by rows
+  bf16 *tt, *pt;            // transposed
+  float* vec;
+};
+
+__device__ __forceinline__ int64_t key_of(const Geo& g, int s) { return s / (g.nb / g.nbk); }
+
+// Hands out 256-byte aligned pieces of a workspace; with no base it only counts.
+struct Arena {
+  char* base;
+  int64_t used = 0;
+  template <typename T> T* take(int64_t n) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += (n * (int64_t)sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+inline int rblocks(int r) { return (r + 31) / 32; }
+inline int p32(int p) { return (p + 31) / 32 * 32; }
+inline int in_terms(int dtype) { return dtype == SMAT_BF16 ? 1 : dtype == SMAT_F16 ? 2 : 3; }
+inline int out_terms(int dtype) { return dtype == SMAT_F32 ? 3 : 2; }
+
+inline Ops take_ops(Arena& ar, int dtype, int64_t nb, int64_t nbk, int64_t nch, int r, bool bwd) {
+  const int64_t rows = nbk * nch * in_terms(dtype) * 4 * rblocks(r) * kFrag;
+  const int64_t tris = nb * nch * kTri * kFrag;
+  Ops o = {};
+  o.kr = ar.take<bf16>(rows);
+  o.kt = ar.take<bf16>(rows);
+  (bwd ? o.qt : o.qr) = ar.take<bf16>(rows);
+  (bwd ? o.tt : o.tm) = ar.take<bf16>(tris * kMid);
+  (bwd ? o.pt : o.pm) = ar.take<bf16>(tris * (bwd ? kMid : out_terms(dtype)));
+  o.vec = ar.take<float>(nb * nch * kVec);
+  return o;
+}
+
+// What the runs' states take: E, the states entering runs, and M.
+struct Carry {
+  float *E, *start, *M;
+};
+inline Carry take_carry(Arena& ar, int64_t nb, int64_t nruns, int r, int p) {
+  const int64_t R = 32 * rblocks(r);
+  Carry c;
+  c.E = ar.take<float>(nruns * nb * r * p);
+  c.start = ar.take<float>(nruns * nb * r * p);
+  c.M = ar.take<float>(nruns * nb * R * R);
+  return c;
+}
+
+// fn(In(), integral_constant of the 32-row blocks of r).
+template <typename F>
+inline int dispatch(int dtype, int r, F fn) {
+  auto rows = [&](auto in) {
+    switch (rblocks(r)) {
+      case 1: return fn(in, std::integral_constant<int, 1>());
+      case 2: return fn(in, std::integral_constant<int, 2>());
+      case 3: return fn(in, std::integral_constant<int, 3>());
+      default: return fn(in, std::integral_constant<int, 4>());
+    }
+  };
+  if (dtype == SMAT_BF16) return rows(bf16());
+  if (dtype == SMAT_F16) return rows(f16());
+  return rows(float());
+}
+
+// The checks that the forward and the backward share.
+int check_geo(const char* who, int dtype, const Geo& g);
+// Launches the runs' carry (both directions).
+int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
+                 hipStream_t st);
+
+}  // namespace dl
+}  // namespace smat

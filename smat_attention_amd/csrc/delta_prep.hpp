@@ -1,0 +1,286 @@
+// The state-free part of every chunk: fragments of K and Q, T = (I + A)^{-1}, P, and
+// the row factors (delta_common.hpp).  One workgroup of four waves a (value
+// sequence, chunk); wave w owns token rows 16 w .. 16 w + 15.
+//
+// T.  Wave w inverts diagonal block w by substitution (a lane a column, 120 steps
+// in registers against broadcast LDS rows); the blocks below follow from
+// [[X, 0], [Y, Z]]^{-1} = [[X', 0], [-Z' Y X', Z']] at 16 and at 32, on fp32 MFMA:
+// substitution's accuracy without its 64-step chain.
+// L is summed and subtracted in fp64, so that a decay that has cost the chunk
+// hundreds of nats leaves the differences of later tokens exact; logA below -1e5
+// (a = 0 many times over) counts as -1e5, which keeps -inf - -inf out.
+#pragma once
+
+#include "delta_common.hpp"
+
+namespace smat {
+namespace dl {
+
+constexpr int kLd = 68;            // floats a row of the 64 x 64 LDS tiles
+
+// acc += A B for 16 x 16 fp32 blocks, A row-major in LDS, B as a result tile in
+// registers (row 4g + i in element i): instruction i contracts rows 4g + i.
+__device__ __forceinline__ f32x4 mm16(f32x4 acc, const float* A, const f32x4& B) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(A + (lane_id() & 15) * kLd + 4 * (lane_id() >> 4));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], B[i], acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ f32x4 tile_of(const float* B) {
+  f32x4 b;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b[i] = B[(4 * (lane_id() >> 4) + i) * kLd + (lane_id() & 15)];
+  return b;
+}
+__device__ __forceinline__ void put_tile(float* B, const f32x4& b, float s) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) B[(4 * (lane_id() >> 4) + i) * kLd + (lane_id() & 15)] = s * b[i];
+}
+
+// Am (strictly lower, zero elsewhere) -> Tm = (I + Am)^{-1}, lower tiles only.
+// Called by four waves; ends with a barrier.
+__device__ __forceinline__ void unit_lower_inverse(const float* Am, float* Tm) {
+  const int w = wave_id(), lane = lane_id(), c = lane & 15;
+  auto at = [](const float* M, int a, int b) { return M + (16 * a) * kLd + 16 * b; };
+  {
+    const float* A = at(Am, w, w);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = (i == c) ? 1.f : 0.f;
+#pragma unroll
+      for (int j4 = 0; j4 < (i + 3) / 4; ++j4) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(A + i * kLd + 4 * j4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * j4 + j < i) s -= a[j] * x[4 * j4 + j];
+      }
+      x[i] = s;
+    }
+    if (lane < 16) {
+      float* Tw = Tm + (16 * w) * kLd + 16 * w;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) Tw[i * kLd + c] = x[i];
+    }
+  }
+  __syncthreads();
+  if (w < 2) {                                     // blocks (1, 0) and (3, 2)
+    const int a = 2 * w + 1, b = 2 * w;
+    f32x4 y = mm16(zero4(), at(Am, a, b), tile_of(at(Tm, b, b)));
+    y = mm16(zero4(), at(Tm, a, a), y);
+    put_tile(Tm + (16 * a) * kLd + 16 * b, y, -1.f);
+  }
+  __syncthreads();
+  {                                                // rows 2, 3 x columns 0, 1
+    const int a = 2 + (w >> 1), b = w & 1;
+    f32x4 y2 = zero4(), y3 = zero4(), t;
+    const f32x4 t1 = tile_of(at(Tm, 1, b));
+    y2 = mm16(y2, at(Am, 2, 1), t1);
+    if (a == 3) y3 = mm16(y3, at(Am, 3, 1), t1);
+    if (b == 0) {
+      const f32x4 t0 = tile_of(at(Tm, 0, 0));
+      y2 = mm16(y2, at(Am, 2, 0), t0);
+      if (a == 3) y3 = mm16(y3, at(Am, 3, 0), t0);
+    }
+    t = mm16(zero4(), at(Tm, a, 2), y2);
+    if (a == 3) t = mm16(t, at(Tm, 3, 3), y3);
+    put_tile(Tm + (16 * a) * kLd + 16 * b, t, -1.f);
+  }
+  __syncthreads();
+}
+
+// Running sum of the chunk's logA in fp64 into Ls (wave 0), beta into bs.  Tokens
+// past the chunk's end count as logA = 0, beta = 0.
+__device__ __forceinline__ void chunk_decays(const Geo& g, const float* logA, const float* beta,
+                                             int s, int t0, int len, double* Ls, float* bs) {
+  const int t = threadIdx.x;
+  if (t < C) {
+    const bool ok = t < len;
+    double x = 0.0;
+    if (ok) {
+      const float a = logA[s * g.a_sb + (int64_t)(t0 + t) * g.a_st];
+      x = a < -1e5f ? -1e5 : (double)a;          // NaN stays NaN
+    }
+    bs[t] = ok ? beta[s * g.b_sb + (int64_t)(t0 + t) * g.b_st] : 0.f;
+#pragma unroll
+    for (int d = 1; d < C; d <<= 1) {
+      const double y = __shfl_up(x, d);
+      if (t >= d) x += y;
+    }
+    Ls[t] = x;
+  }
+}
+
+// The eight values (slots of contraction block kb) of token row m as terms.
+template <typename In, int N>
+__device__ __forceinline__ Frag<N> row_frag(const In* row, bool ok, int c0, int r, bool vec) {
+  const f32x4 a = ok ? load4(row + c0, r - c0, vec) : zero4();
+  const f32x4 b = ok ? load4(row + c0 + 16, r - c0 - 16, vec) : zero4();
+  return split<N>(a, b);
+}
+
+// Fragment of the transpose from row fragments in LDS (one term): rows 16 mt + ..
+// of the feature axis, tokens of block kb.
+template <int RB>
+__device__ __forceinline__ bf16x8 transposed(const bf16* rows, int mt, int kb) {
+  const int lane = lane_id(), col = 16 * mt + (lane & 15), g = lane >> 4;
+  // feature col sits in contraction block col / 32, slot (gc, jc)
+  const int kc = col >> 5, c5 = col & 31, gc = (c5 & 15) >> 2, jc = (c5 & 3) + (c5 & 16 ? 4 : 0);
+  bf16x8 f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int tt = 2 * kb + (j >> 2), m = 4 * g + (j & 3);      // token 16 tt + m
+    f[j] = rows[(tt * RB + kc) * kFrag + (gc * 16 + m) * 8 + jc];
+  }
+  return f;
+}
+
+template <typename In, int RB, bool BWD>
+__global__ __launch_bounds__(256) void delta_prep_kernel(
+    const In* __restrict__ q, const In* __restrict__ k, const float* __restrict__ logA,
+    const float* __restrict__ beta, Geo g, Ops o, bool qvec, bool kvec) {
+  constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid;
+  constexpr int KB = 4 * RB * kFrag;               // elements of one term of a chunk's rows
+  __shared__ __align__(16) bf16 rows[NT * KB];
+  __shared__ __align__(16) float Am[C * kLd], Tm[C * kLd];
+  __shared__ double Ls[C];
+  __shared__ float bs[C];
+  const int c = blockIdx.x, s = blockIdx.y;
+  const int w = wave_id(), lane = lane_id(), m = lane & 15, gq = lane >> 4;
+  int t0, len;
+  chunk_of(g, c, t0, len);
+  const int64_t ks = key_of(g, s);
+  const bool first = s % (g.nb / g.nbk) == 0;      // this workgroup stores K's and Q's fragments
+  chunk_decays(g, logA, beta, s, t0, len, Ls, bs);
+
+  const int tok = 16 * w + m;
+  const bool live = tok < len;
+  const In* krow = k + ks * g.k_sb + (int64_t)(t0 + (live ? tok : 0)) * g.k_st;
+  const In* qrow = q + ks * g.q_sb + (int64_t)(t0 + (live ? tok : 0)) * g.q_st;
+  const int64_t kc = (ks * g.nch + c) * (int64_t)NT * KB, sc = (int64_t)s * g.nch + c;
+  Frag<NT> kf[RB], qf[RB];
+#pragma unroll
+  for (int kb = 0; kb < RB; ++kb) {
+    kf[kb] = row_frag<In, NT>(krow, live, 32 * kb + 4 * gq, g.r, kvec);
+    qf[kb] = row_frag<In, NT>(qrow, live, 32 * kb + 4 * gq, g.r, qvec);
+    store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, kf[kb]);
+    if (first) {
+      store_frag<NT>(o.kr + kc + (w * RB + kb) * kFrag, KB, kf[kb]);
+      if (!BWD) store_frag<NT>(o.qr + kc + (w * RB + kb) * kFrag, KB, qf[kb]);
+    }
+  }
+  __syncthreads();
+  if (first) {
+#pragma unroll
+    for (int f = w; f < 4 * RB; f += 4)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+        *reinterpret_cast<bf16x8*>(o.kt + kc + n * KB + f * kFrag + lane * 8) =
+            transposed<RB>(rows + n * KB, f >> 1, f & 1);
+  }
+  // A = b D K K^T below the diagonal: column j in the lane, rows 16 w + 4 gq + i
+  f32x4 pacc[4];
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt) {
+    f32x4 a = zero4();
+    pacc[jt] = zero4();
+    if (jt <= w) {
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) {
+        const Frag<NT> kj = load_frag<NT>(rows + (jt * RB + kb) * kFrag, KB);
+        a = mul(a, kf[kb], kj);
+        if (!BWD) pacc[jt] = mul(pacc[jt], kj, qf[kb]);   // token i in the lane, rows j
+      }
+    }
+    const int j = 16 * jt + m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int ti = 16 * w + 4 * gq + i;
+      Am[ti * kLd + j] = j < ti ? bs[ti] * (expf((float)(Ls[ti] - Ls[j])) * a[i]) : 0.f;
+    }
+  }
+  if (!BWD) {
+    // P by rows: lane holds token i = 16 w + m, tile jt's rows j = 16 jt + 4 gq + i
+    const double Li = Ls[tok];
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = 16 * jt + 4 * gq + i;
+        pacc[jt][i] = j <= tok ? g.scale * (expf((float)(Li - Ls[j])) * pacc[jt][i]) : 0.f;
+      }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+      if (kb <= w / 2)
+        store_frag<NO>(o.pm + (sc * NO * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
+                       split<NO>(pacc[2 * kb], pacc[2 * kb + 1]));
+  }
+  __syncthreads();                                 // Am whole; rows free
+  if (BWD) {
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, qf[kb]);
+  }
+  unit_lower_inverse(Am, Tm);
+  if (BWD) {
+    // Q transposed, and P^T: lane holds token j = 16 w + m, rows i = 16 it + 4 gq + ..
+    if (first) {
+#pragma unroll
+      for (int f = w; f < 4 * RB; f += 4)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<bf16x8*>(o.qt + kc + n * KB + f * kFrag + lane * 8) =
+              transposed<RB>(rows + n * KB, f >> 1, f & 1);
+    }
+    const double Lj = Ls[tok];
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      if (it >= w) {
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb)
+          pacc[it] = mul(pacc[it], load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ti = 16 * it + 4 * gq + i;
+        pacc[it][i] = tok <= ti ? g.scale * (expf((float)(Ls[ti] - Lj)) * pacc[it][i]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+      if (kb >= w / 2) {
+        store_frag<NI>(o.pt + (sc * NI * kTri + tri_t(w, kb)) * kFrag, kTri * kFrag,
+                       split<NI>(pacc[2 * kb], pacc[2 * kb + 1]));
+        f32x4 x[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int ti = 32 * kb + 16 * h + 4 * gq + i;
+            x[h][i] = ti >= 16 * w ? Tm[ti * kLd + tok] : 0.f;
+          }
+        store_frag<NI>(o.tt + (sc * NI * kTri + tri_t(w, kb)) * kFrag, kTri * kFrag,
+                       split<NI>(x[0], x[1]));
+      }
+  } else {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+      if (kb <= w / 2) {
+        const float* row = Tm + tok * kLd + 32 * kb + 4 * gq;
+        const f32x4 x0 = *reinterpret_cast<const f32x4*>(row);
+        const f32x4 x1 = 2 * kb + 1 <= w ? *reinterpret_cast<const f32x4*>(row + 16) : zero4();
+        store_frag<NI>(o.tm + (sc * NI * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
+                       split<NI>(x0, x1));
+      }
+  }
+  if (threadIdx.x < C) {
+    const int t = threadIdx.x;
+    float* v = o.vec + sc * kVec;
+    v[t] = expf((float)Ls[t]);
+    v[C + t] = expf((float)(Ls[C - 1] - Ls[t]));
+    v[2 * C + t] = bs[t];
+    if (t == 0) v[3 * C] = expf((float)Ls[C - 1]);
+  }
+}
+
+}  // namespace dl
+}  // namespace smat

@@ -1,0 +1,281 @@
+// Drafted trees over the decoder's cache (SmatDecoder.tree_step / tree_state): the
+// tokens of a tree are read against the cache of one prefix, each node seeing the
+// prefix, its ancestors and itself.  For node j at level l (a root is at level 0)
+//
+//   N_j = phi_j (S + U[(i + l) mod B]) + sum_a (phi_j . psi_a) vb_a,  out_j = N_j[:-1] / N_j[-1]
+//
+// over the ancestors a of j and j itself: what step-by-step decoding of j's path
+// gives, with S read once and each level's type row U_h once.
+//
+// Bound by reading the tables (r p fp32 a level and sequence).  A wave owns 15 value
+// columns and the normaliser's, so its division needs no other wave; it adds S and
+// U_h in registers and multiplies the level's nodes by the sum on bf16 MFMA in three
+// terms (fp32's 24 bits; two for the features in fp16, three in fp32).  The scores
+// phi_j . psi_a are formed once a workgroup; their product with vb runs over the
+// ancestors alone on the vector units, so a value of another branch, infinite or NaN,
+// never meets a zero.
+#include "delta_common.hpp"
+
+namespace smat {
+namespace tr {
+
+using dl::Frag;
+using dl::load4;
+using dl::mul;
+using dl::split;
+
+constexpr int kMaxNodes = 64;
+constexpr int kMaxWaves = 5;       // half of the ceil(143 / 15) column tiles
+
+struct Args {
+  const int64_t* anc;      // (trees, M): bit a of word j: a is j or an ancestor of j
+  const int32_t* order;    // (trees, M): nodes by level, unused ones last
+  const int32_t* lstart;   // (trees, M + 1): first of each level in order
+  const int32_t* ahead;    // (requests): tokens past `step`; or null
+  int nb, trees, requests, M, levels, B, r, p;
+  int64_t step;
+  int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st;
+};
+
+template <typename In, int RB>
+__global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
+    const In* __restrict__ phi, const In* __restrict__ psi, const In* __restrict__ vb,
+    const float* __restrict__ S, const float* __restrict__ U, float* __restrict__ out, Args g,
+    int tiles, bool qvec, bool kvec) {
+  constexpr int NT = dl::Terms<In>::in;
+  __shared__ __align__(16) float sc[16][kMaxNodes + 4];
+  const int s = blockIdx.x, W = blockDim.x >> 6;
+  const int m = lane_id() & 15, gq = lane_id() >> 4;
+  const int tile = blockIdx.y * W + wave_id();     // may lie past the last: computes, never stores
+  const int tree = g.trees == 1 ? 0 : s / (g.nb / g.trees);
+  const int64_t* anc = g.anc + (int64_t)tree * g.M;
+  const int32_t* order = g.order + (int64_t)tree * g.M;
+  const int32_t* lstart = g.lstart + (int64_t)tree * (g.M + 1);
+  const int nval = g.p - 1;
+  const int v0 = tile * 15;                        // value columns v0 .. v0 + 14, then p - 1
+  const bool mine = m < 15 && v0 + m < nval;
+  const int col = mine ? v0 + m : nval;
+  const int64_t at = g.step + (g.ahead ? max(0, g.ahead[s / (g.nb / g.requests)]) : 0);
+
+  const float* Sb = S + (int64_t)s * g.r * g.p + col;
+  f32x4 St[2 * RB];
+#pragma unroll
+  for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = 16 * mt + 4 * gq + i;
+      St[mt][i] = a < g.r ? Sb[(int64_t)a * g.p] : 0.f;
+    }
+  for (int l = blockIdx.z; l < g.levels; l += gridDim.z) {
+    const int n0 = lstart[l], n1 = lstart[l + 1];
+    if (n0 >= n1) break;                           // this tree has fewer levels (uniform)
+    const int64_t h = (at + l) % g.B;
+    const float* Ub = U + ((int64_t)s * g.B + h) * g.r * g.p + col;
+    Frag<3> tb[RB];
+    {
+      f32x4 t[2 * RB];
+#pragma unroll
+      for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int a = 16 * mt + 4 * gq + i;
+          t[mt][i] = a < g.r ? Ub[(int64_t)a * g.p] : 0.f;
+        }
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb)
+        tb[kb] = split<3>(St[2 * kb] + t[2 * kb], St[2 * kb + 1] + t[2 * kb + 1]);
+    }
+    for (int n = n0; n < n1; n += 16) {
+      const int node = order[min(n + m, n1 - 1)];
+      uint64_t mask = (uint64_t)anc[node];
+      uint64_t all = mask;                         // ancestors of any node of this tile
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) all |= __shfl_xor((unsigned long long)all, d);
+      const In* row = phi + (int64_t)s * g.q_sb + (int64_t)node * g.q_st;
+      Frag<NT> pf[RB];
+      f32x4 acc = zero4();
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) {
+        const int c = 32 * kb + 4 * gq;
+        pf[kb] = split<NT>(load4(row + c, g.r - c, qvec), load4(row + c + 16, g.r - c - 16, qvec));
+        acc = mul(acc, pf[kb], tb[kb]);            // column in the lane, nodes 4 gq + i
+      }
+      __syncthreads();                             // the last tile's scores are read
+      for (int a0 = 16 * wave_id(); a0 < g.M; a0 += 16 * W) {
+        if (((all >> a0) & 0xffff) == 0) continue; // uniform over the wave
+        const int a = min(a0 + m, g.M - 1);
+        const In* kr = psi + (int64_t)s * g.k_sb + (int64_t)a * g.k_st;
+        f32x4 x = zero4();
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb) {
+          const int c = 32 * kb + 4 * gq;
+          x = mul(x, split<NT>(load4(kr + c, g.r - c, kvec), load4(kr + c + 16, g.r - c - 16, kvec)),
+                  pf[kb]);                         // node in the lane, a in registers
+        }
+        *reinterpret_cast<f32x4*>(&sc[m][a0 + 4 * gq]) = x;
+      }
+      __syncthreads();
+      uint64_t mine4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine4[i] = __shfl((unsigned long long)mask, 4 * gq + i);
+      for (uint64_t left = all; left; left &= left - 1) {
+        const int a = __ffsll((unsigned long long)left) - 1;
+        const float x = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)a * g.v_st + col]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          acc[i] = (mine4[i] >> a) & 1 ? acc[i] + sc[4 * gq + i][a] * x : acc[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float den = __shfl(acc[i], gq * 16 + 15);
+        const int j = n + 4 * gq + i;
+        if (mine && j < n1) out[((int64_t)s * g.M + order[j]) * nval + col] = acc[i] / den;
+      }
+    }
+  }
+  if (blockIdx.z == 0 && mine)                     // unused nodes read nothing and give zeros
+    for (int j = lstart[g.levels] + gq; j < g.M; j += 4)
+      out[((int64_t)s * g.M + order[j]) * nval + col] = 0.f;
+}
+
+// S' = S + sum of psi_a vb_a^T over the accepted path of each request, ancestors in
+// order, sixteen at a time through LDS; `ahead` moves by the path's length.
+constexpr int kElems = 8;          // elements of S a thread
+
+template <typename In>
+__global__ __launch_bounds__(256) void tree_state_kernel(
+    const In* __restrict__ psi, const In* __restrict__ vb, const float* __restrict__ S,
+    float* __restrict__ So, const int32_t* __restrict__ nodes, int32_t* ahead, Args g) {
+  __shared__ float sp[16][128], sv[16][144];
+  const int s = blockIdx.x, tid = threadIdx.x;
+  const int per = g.nb / g.requests, req = s / per;
+  const int tree = g.trees == 1 ? 0 : s / (g.nb / g.trees);
+  const int node = nodes[req];
+  const uint64_t path =
+      node >= 0 && node < g.M ? (uint64_t)g.anc[(int64_t)tree * g.M + node] : 0;
+  const int rp = g.r * g.p;
+  const int64_t base = (int64_t)s * rp;
+  float x[kElems];
+  int row[kElems], col[kElems];
+#pragma unroll
+  for (int j = 0; j < kElems; ++j) {
+    const int e = (blockIdx.y * kElems + j) * 256 + tid;
+    row[j] = min(e, rp - 1) / g.p;
+    col[j] = min(e, rp - 1) - row[j] * g.p;
+    x[j] = S[base + min(e, rp - 1)];
+  }
+  uint64_t left = path;
+  while (left) {
+    int n = 0;
+    for (; left && n < 16; left &= left - 1, ++n) {
+      const int a = __ffsll((unsigned long long)left) - 1;
+      if (tid < g.r) sp[n][tid] = to_f32(psi[(int64_t)s * g.k_sb + (int64_t)a * g.k_st + tid]);
+      if (tid < g.p) sv[n][tid] = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)a * g.v_st + tid]);
+    }
+    __syncthreads();
+    for (int i = 0; i < n; ++i)
+#pragma unroll
+      for (int j = 0; j < kElems; ++j) x[j] += sp[i][row[j]] * sv[i][col[j]];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int j = 0; j < kElems; ++j) {
+    const int e = (blockIdx.y * kElems + j) * 256 + tid;
+    if (e < rp) So[base + e] = x[j];
+  }
+  if (ahead && blockIdx.y == 0 && tid == 0 && s % per == 0)
+    ahead[req] += __popcll((unsigned long long)path);
+}
+
+static int check(const char* who, int dtype, const Args& g) {
+  SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
+               "%s: unknown dtype %d", who, dtype);
+  SMAT_REQUIRE(g.nb >= 0 && g.trees >= 1 && g.requests >= 1 && g.nb % g.trees == 0 &&
+                   g.nb % g.requests == 0,
+               SMAT_EINVAL, "%s: %d trees and %d requests must divide nb=%d", who, g.trees,
+               g.requests, g.nb);
+  SMAT_REQUIRE(g.M >= 1 && g.M <= kMaxNodes, SMAT_EUNSUPPORTED, "%s: %d nodes, at most %d", who,
+               g.M, kMaxNodes);
+  SMAT_REQUIRE(g.r >= 1 && g.r <= kMaxR && g.p >= 2 && g.p <= kMaxP, SMAT_EUNSUPPORTED,
+               "%s: r=%d p=%d beyond r<=%d, 2<=p<=%d", who, g.r, g.p, kMaxR, kMaxP);
+  return SMAT_OK;
+}
+
+}  // namespace tr
+}  // namespace smat
+
+extern "C" int smat_tree_step(int dtype, const void* phi, const void* psi, const void* vb,
+                              const float* S, const float* U, float* out, const int64_t* anc,
+                              const int32_t* order, const int32_t* lstart, const int32_t* ahead,
+                              int nb, int trees, int requests, int M, int levels, int B, int r,
+                              int p, int64_t step, int64_t q_sb, int64_t q_st, int64_t k_sb,
+                              int64_t k_st, int64_t v_sb, int64_t v_st, void* stream) {
+  using namespace smat;
+  using namespace smat::tr;
+  clear_error();
+  const char* who = "smat_tree_step";
+  const Args g = {anc, order, lstart, ahead, nb, trees, requests, M, levels, B, r, p, step,
+                  q_sb, q_st, k_sb, k_st, v_sb, v_st};
+  const int rc = check(who, dtype, g);
+  if (rc) return rc;
+  SMAT_REQUIRE(levels >= 0 && levels <= M && B >= 1 && step >= 0, SMAT_EINVAL,
+               "%s: bad sizes (levels=%d B=%d step=%lld)", who, levels, B, (long long)step);
+  if (nb == 0) return SMAT_OK;
+  SMAT_REQUIRE(phi && psi && vb && S && U && out && anc && order && lstart, SMAT_EINVAL,
+               "%s: null pointer", who);
+  const int tiles = (p - 1 + 14) / 15;
+  // a wave walks every level with S in registers while the sequences fill the GPU;
+  // else levels and columns are spread over workgroups
+  const bool few = nb < 256;
+  const int W = few ? (tiles + 2) / 3 : (tiles + 1) / 2;
+  int z = few ? (256 * 4 + nb * tiles - 1) / (nb * tiles) : 1;
+  z = z < 1 ? 1 : z > levels ? (levels > 0 ? levels : 1) : z;
+  return dl::dispatch(dtype, r, [&](auto in, auto rb) {
+    typedef decltype(in) In;
+    constexpr int eb = sizeof(In);
+    hipLaunchKernelGGL((tree_step_kernel<In, decltype(rb)::value>),
+                       dim3(nb, (tiles + W - 1) / W, z), dim3(64 * W), 0, (hipStream_t)stream,
+                       (const In*)phi, (const In*)psi, (const In*)vb, S, U, out, g, tiles,
+                       dl::vec4_ok(phi, q_sb, q_st, eb), dl::vec4_ok(psi, k_sb, k_st, eb));
+    return launch_status(who);
+  });
+}
+
+extern "C" int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S,
+                               float* S_out, const int64_t* anc, const int32_t* nodes,
+                               int32_t* ahead, int nb, int trees, int requests, int M, int r,
+                               int p, int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st,
+                               void* stream) {
+  using namespace smat;
+  using namespace smat::tr;
+  clear_error();
+  const char* who = "smat_tree_state";
+  Args g = {};
+  g.anc = anc;
+  g.nb = nb;
+  g.trees = trees;
+  g.requests = requests;
+  g.M = M;
+  g.r = r;
+  g.p = p;
+  g.k_sb = k_sb;
+  g.k_st = k_st;
+  g.v_sb = v_sb;
+  g.v_st = v_st;
+  const int rc = check(who, dtype, g);
+  if (rc) return rc;
+  if (nb == 0) return SMAT_OK;
+  SMAT_REQUIRE(psi && vb && S && S_out && anc && nodes, SMAT_EINVAL, "%s: null pointer", who);
+  SMAT_REQUIRE(S != S_out, SMAT_EINVAL, "%s: S and S_out must differ", who);
+  const dim3 grid(nb, (r * p + 256 * kElems - 1) / (256 * kElems));
+  hipStream_t st = (hipStream_t)stream;
+  auto go = [&](auto in) {
+    typedef decltype(in) In;
+    hipLaunchKernelGGL(tree_state_kernel<In>, grid, dim3(256), 0, st, (const In*)psi,
+                       (const In*)vb, S, S_out, nodes, ahead, g);
+    return launch_status(who);
+  };
+  if (dtype == SMAT_BF16) return go(bf16());
+  if (dtype == SMAT_F16) return go(f16());
+  return go(float());
+}

@@ -123,6 +123,23 @@ SIGNATURES = {
     "smat_incidence_complement": (_i, [_p, _p, _i, _i, _i, _i64, _p]),
     "smat_decode_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i64,
                               _i64, _i64, _i64, _p]),
+    "smat_decode_step_at": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i64,
+                                 _i64, _i64, _i64, _p]),
+    "smat_tree_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i,
+                            _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
+    "smat_tree_state": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i64, _i64,
+                             _i64, _i64, _p]),
+    "smat_delta_run_chunks": (_i, [_i, _i, _i, _i, _i]),
+    "smat_delta_workspace_bytes": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "smat_delta_scan": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i,
+                             _i, _i, _i, _i, _i, _i, _f, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                             _i64, _i64, _i64, _p, _i64, _p]),
+    "smat_delta_scan_backward": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                                      _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i64,
+                                      _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                                      _i64, _p, _i64, _p]),
+    "smat_delta_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _i64, _i64,
+                             _i64, _i64, _i64, _p]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,308 @@
+"""The gated delta rule's kernels (csrc/delta*.hip) behind their Python checks.
+
+``scan`` runs a whole-sequence forward, ``scan_backward`` its gradient, ``step`` one
+token; :class:`GatedDeltaFunction` ties the first two into autograd.  As in
+:mod:`.hip_fwd`, inputs are borrowed, outputs and workspaces come from torch's caching
+allocator, work goes to torch's current stream of the inputs' device, and every failure
+raises.  :mod:`smat_attention_amd.attention` has the public entry points.
+"""
+from __future__ import annotations
+
+from contextlib import nullcontext
+
+import numpy as np
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import call, ptr, stream_of
+from .hip_fwd import _code, _on_gpu, _rows3, _shape
+
+CHUNK = 64
+MAX_R, MAX_P = 128, 256
+
+
+def on_device(t: torch.Tensor):
+    """Launches go to ``t``'s device, whichever is the current one."""
+    if t.get_device() == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def same_device(who: str, ref: torch.Tensor, *ts) -> None:
+    _on_gpu(who, ref, *ts)
+    for t in ts:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{who}: tensors on {ref.device} and {t.device}")
+
+
+class Segments:
+    """Packed sequences: ``offsets`` = 0, ..., T are the borders of the segments along the
+    token axis (as many as the list has entries, less one; empty ones are allowed).  Checked
+    and staged on ``device`` once; a program keeps it as long as its batch keeps the layout.
+    """
+
+    def __init__(self, offsets, device):
+        off = np.asarray(offsets.cpu() if isinstance(offsets, torch.Tensor) else offsets)
+        if off.ndim != 1 or off.size < 2 or off.dtype.kind not in "iu":
+            raise ValueError("Segments: offsets must be a list of at least two integers")
+        off = off.astype(np.int64)
+        if off[0] != 0 or np.any(np.diff(off) < 0):
+            raise ValueError("Segments: offsets must start at 0 and not decrease")
+        if off[-1] >= 2 ** 31:
+            raise ValueError("Segments: at most 2^31 - 1 tokens")
+        self.offsets = [int(x) for x in off]
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        counts = -(-np.diff(off) // CHUNK)                       # chunks of each segment
+        first = np.concatenate([[0], np.cumsum(counts)])
+        seg = np.repeat(np.arange(len(counts)), counts)
+        t0 = off[:-1][seg] + (np.arange(first[-1]) - first[:-1][seg]) * CHUNK
+        rows = np.stack([t0, np.minimum(CHUNK, off[1:][seg] - t0)], 1).astype(np.int32)
+        self._first, self._counts = first, counts
+        # one row at least, so that the table's address says that there is one
+        self.chunks = torch.from_numpy(rows if len(rows) else
+                                       np.zeros((1, 2), np.int32)).to(self.device)
+        self.nch, self.longest = int(first[-1]), int(counts.max())
+        self._runs = {}
+
+    def __len__(self):
+        return len(self.offsets) - 1
+
+    @property
+    def T(self):
+        return self.offsets[-1]
+
+    def runs(self, K: int):
+        """``(runs, segrun)`` on the device for runs of ``K`` chunks; staged at the first call
+        with that K (outside a graph capture)."""
+        if K not in self._runs:
+            rows, segrun = [], [0]
+            for s, n in enumerate(self._counts):
+                c0 = int(self._first[s])
+                for a in range(0, max(int(n), 1), K):
+                    rows.append((c0 + a, c0 + min(a + K, int(n)), s))
+                segrun.append(len(rows))
+            self._runs[K] = tuple(torch.tensor(x, dtype=torch.int32).to(self.device)
+                                  for x in (rows, segrun))
+        return self._runs[K]
+
+
+class _Plan:
+    """One call's geometry: its sizes and table addresses in the C entry points' order."""
+
+    def __init__(self, who, Q, V, segments):
+        self.nbk, self.T, self.r = Q.shape
+        self.nb, _, self.p = V.shape
+        if segments is None:
+            self.nseg, self.nch = 1, -(-self.T // CHUNK)
+        else:
+            if segments.T != self.T:
+                raise ValueError(f"{who}: segments end at {segments.T}, the inputs at {self.T}")
+            if segments.device != Q.device:
+                raise ValueError(f"{who}: segments are on {segments.device}, the inputs on "
+                                 f"{Q.device}")
+            self.nseg, self.nch = len(segments), segments.nch
+        longest = self.nch if segments is None else segments.longest
+        self.K = _lib.query("smat_delta_run_chunks", self.nb, self.nch, longest, self.r, self.p)
+        if segments is None:
+            self.tables = (None, None, None)
+            self.nruns = max(1, -(-self.nch // self.K))
+        else:
+            runs, segrun = segments.runs(self.K)
+            self.tables = (segments.chunks.data_ptr(), runs.data_ptr(), segrun.data_ptr())
+            self.nruns = runs.shape[0]
+        self.R, self.P = -(-self.r // 32) * 32, -(-self.p // 32) * 32
+
+    def sizes(self, scale):
+        return (*self.tables, self.nb, max(self.nbk, 1), self.T, self.nseg, self.nch, self.nruns, self.K,
+                self.r, self.p, float(scale))
+
+    def workspace(self, code, backward, device):
+        n = _lib.query("smat_delta_workspace_bytes", code, self.nb, self.nbk, self.nch, self.nseg,
+                       self.nruns, self.r, self.p, backward)
+        return torch.empty(max(n, 1), device=device, dtype=torch.uint8), n
+
+
+def check_scan(who, Q, K, V, logA, beta, state, segments):
+    """The argument checks of the whole-sequence form."""
+    if Q.dim() != 3 or V.dim() != 3:
+        raise ValueError(f"{who}: Q, K and V must be (sequences, T, columns)")
+    same_device(who, Q, K, V, logA, beta, state)
+    nbk, T, r = Q.shape
+    nb, _, p = V.shape
+    _shape(who, "K", K, (nbk, T, r))
+    _shape(who, "V", V, (nb, T, p))
+    _shape(who, "logA", logA, (nb, T))
+    _shape(who, "beta", beta, (nb, T))
+    if (nbk == 0) != (nb == 0) or (nbk and nb % nbk):
+        raise ValueError(f"{who}: {nbk} key sequences do not divide {nb} value sequences")
+    _check_types(who, Q, K, V, logA, beta, state)
+    _check_widths(who, r, p)
+    if state is not None:
+        _shape(who, "state", state, (nb, r, p) if segments is None else
+               (len(segments), nb, r, p))
+
+
+def _check_types(who, Q, K, V, logA, beta, state):
+    _code(Q, who)
+    if K.dtype != Q.dtype or V.dtype != Q.dtype:
+        raise TypeError(f"{who}: Q, K and V must share a dtype, got {Q.dtype}, {K.dtype} and "
+                        f"{V.dtype}")
+    for name, t in (("logA", logA), ("beta", beta)):
+        if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise TypeError(f"{who}: {name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if state is not None and state.dtype != torch.float32:
+        raise TypeError(f"{who}: the state is held in float32, got {state.dtype}")
+
+
+def _check_widths(who, r, p):
+    if not (1 <= r <= MAX_R and 1 <= p <= MAX_P):
+        raise ValueError(f"{who}: key size {r} and value size {p} must lie in 1..{MAX_R} and "
+                         f"1..{MAX_P}")
+
+
+def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bool):
+    """``(o, state_out or None, save_s, save_u, inputs)``: the forward over checked arguments;
+    ``inputs`` are the tensors that the kernels read (rows with unit column stride, fp32
+    gates)."""
+    who = "gated_delta_scan"
+    plan = _Plan(who, Q, V, segments)
+    code, dev = _code(Q, who), Q.device
+    (Q, q_sb, q_st), (K, k_sb, k_st), (V, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
+    logA, beta = logA.float(), beta.float()
+    o = torch.empty(plan.nb, plan.T, plan.p, device=dev, dtype=V.dtype)
+    lead = () if segments is None else (plan.nseg,)
+    s_out = (torch.empty(*lead, plan.nb, plan.r, plan.p, device=dev, dtype=torch.float32)
+             if want_state else None)
+    save_s = save_u = None
+    if save:
+        save_s = torch.empty(plan.nb, plan.nch, plan.R, plan.P, device=dev)
+        save_u = torch.empty(plan.nb, plan.nch, CHUNK, plan.P, device=dev)
+    ws, n = plan.workspace(code, 0, dev)
+    if state is not None:
+        state = state.contiguous()
+    with on_device(Q):
+        call("smat_delta_scan", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(), logA.data_ptr(),
+             beta.data_ptr(), ptr(state), o.data_ptr(), ptr(s_out), ptr(save_s) or None,
+             ptr(save_u) or None, *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st,
+             *logA.stride(), *beta.stride(), ws.data_ptr(), n, stream_of(Q))
+    return o, s_out, save_s, save_u, (Q, K, V, logA, beta)
+
+
+def scan_backward(inputs, save_s, save_u, dO, dS, scale, segments, want_dstate: bool):
+    """``(dQ, dK, dV, dlogA, dbeta, dstate or None)`` of one forward."""
+    who = "gated_delta_scan"
+    Q, K, V, logA, beta = inputs
+    plan = _Plan(who, Q, V, segments)
+    code, dev = _code(Q, who), Q.device
+    (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
+    dO, d_sb, d_st = _rows3(dO)
+    dQ = torch.empty(plan.nbk, plan.T, plan.r, device=dev, dtype=Q.dtype)
+    dK = torch.empty_like(dQ)
+    dV = torch.empty(plan.nb, plan.T, plan.p, device=dev, dtype=V.dtype)
+    dlogA = torch.empty(plan.nb, plan.T, device=dev, dtype=torch.float32)
+    dbeta = torch.empty_like(dlogA)
+    lead = () if segments is None else (plan.nseg,)
+    dstate = (torch.empty(*lead, plan.nb, plan.r, plan.p, device=dev, dtype=torch.float32)
+              if want_dstate else None)
+    ws, n = plan.workspace(code, 1, dev)
+    if dS is not None:
+        dS = dS.contiguous()
+    with on_device(Q):
+        call("smat_delta_scan_backward", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
+             logA.data_ptr(), beta.data_ptr(), dO.data_ptr(), ptr(dS), save_s.data_ptr(),
+             save_u.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlogA.data_ptr(),
+             dbeta.data_ptr(), ptr(dstate), *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb,
+             v_st, *logA.stride(), *beta.stride(), d_sb, d_st, ws.data_ptr(), n, stream_of(Q))
+    return dQ, dK, dV, dlogA, dbeta, dstate
+
+
+class GatedDeltaFunction(torch.autograd.Function):
+    """The whole-sequence form with gradients of Q, K, V, logA, beta and the state.
+
+    The forward keeps, besides its inputs, the state entering every chunk of 64 tokens and
+    the chunk's ``U`` in fp32; the backward forms the chunks' other operands again."""
+
+    @staticmethod
+    def forward(ctx, Q, K, V, logA, beta, state, scale, segments, want_state):
+        o, s_out, save_s, save_u, inputs = scan(
+            Q.detach(), K.detach(), V.detach(), logA.detach(), beta.detach(),
+            None if state is None else state.detach(), scale, segments, want_state, True)
+        ctx.save_for_backward(*inputs, save_s, save_u)
+        ctx.meta = (scale, segments, logA.dtype, beta.dtype)
+        ctx.set_materialize_grads(False)
+        return o, s_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dO, dS):
+        *inputs, save_s, save_u = ctx.saved_tensors
+        scale, segments, a_type, b_type = ctx.meta
+        if dO is None and dS is None:
+            return (None,) * 9
+        if dO is None:
+            V = inputs[2]
+            dO = torch.zeros(V.shape, device=V.device, dtype=V.dtype)
+        dQ, dK, dV, dlogA, dbeta, dstate = scan_backward(
+            inputs, save_s, save_u, dO.to(inputs[2].dtype), dS, scale, segments,
+            ctx.needs_input_grad[5])
+        return (dQ, dK, dV, dlogA.to(a_type), dbeta.to(b_type), dstate, None, None, None)
+
+
+def step(q, k, v, logA, beta, state, scale, out, out_state):
+    """One token (the checks are in place and the helpers that word the errors are called only
+    when one fails: a step is a launch of a few microseconds)."""
+    who = "gated_delta_step"
+    if q.dim() != 2 or v.dim() != 2 or state.dim() != 3:
+        raise ValueError(f"{who}: q, k and v must be (sequences, columns), the state "
+                         f"(sequences, r, p)")
+    nbk, r = q.shape
+    nb, p = v.shape
+    dev, dt = state.device, q.dtype
+    if out_state is None:
+        out_state = state
+    if out is None:
+        out = torch.empty(nb, p, device=dev, dtype=v.dtype)
+    if not (q.is_cuda and dev == q.device == k.device == v.device == logA.device == beta.device
+            == out.device == out_state.device):
+        same_device(who, q, k, v, logA, beta, state, out, out_state)
+    rows = (nb, r, p)
+    if not (k.shape == q.shape and logA.shape == beta.shape == (nb,) and state.shape == rows
+            and out_state.shape == rows and out.shape == v.shape):
+        _shape(who, "k", k, (nbk, r))
+        _shape(who, "logA", logA, (nb,))
+        _shape(who, "beta", beta, (nb,))
+        _shape(who, "state", state, rows)
+        _shape(who, "out_state", out_state, rows)
+        _shape(who, "out", out, (nb, p))
+    if (nbk == 0) != (nb == 0) or (nbk and nb % nbk):
+        raise ValueError(f"{who}: {nbk} key sequences do not divide {nb} value sequences")
+    f32 = torch.float32
+    if not (k.dtype == v.dtype == dt and logA.dtype == beta.dtype == state.dtype == f32):
+        _check_types(who, q, k, v, logA, beta, state)
+        logA, beta = logA.float(), beta.float()
+    if out.dtype != dt or out_state.dtype != f32:
+        raise TypeError(f"{who}: out must be {dt} and out_state float32, got {out.dtype} and "
+                        f"{out_state.dtype}")
+    if not (state.is_contiguous() and out_state.is_contiguous() and out.is_contiguous()):
+        raise ValueError(f"{who}: state, out_state and out must be contiguous")
+    if r > MAX_R or p > MAX_P or r < 1 or p < 1:
+        _check_widths(who, r, p)
+    if out_state is not state and out_state.data_ptr() != state.data_ptr():
+        lo, hi = sorted((state.data_ptr(), out_state.data_ptr()))
+        if hi < lo + state.numel() * 4:
+            raise ValueError(f"{who}: out_state must be state itself or lie apart from it")
+    (q_sb, q_s1), (k_sb, k_s1), (v_sb, v_s1) = q.stride(), k.stride(), v.stride()
+    if not ((q_s1 == 1 or r == 1) and (k_s1 == 1 or r == 1) and (v_s1 == 1 or p == 1)):
+        raise ValueError(f"{who}: rows of q, k and v must be contiguous")
+    args = (_code(q, who), q.data_ptr(), k.data_ptr(), v.data_ptr(), logA.data_ptr(),
+            beta.data_ptr(), state.data_ptr(), out_state.data_ptr(), out.data_ptr(), nb,
+            max(nbk, 1), r, p, scale, q_sb, k_sb, v_sb, logA.stride(0), beta.stride(0))
+    if dev.index == torch.cuda.current_device():
+        call("smat_delta_step", *args, stream_of(q))
+    else:
+        with torch.cuda.device(dev):
+            call("smat_delta_step", *args, stream_of(q))
+    return out

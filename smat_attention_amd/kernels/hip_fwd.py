@@ -19,6 +19,7 @@ from __future__ import annotations
 
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -32,7 +33,7 @@ __all__ = [
     "available", "chunk_local", "incidence", "pool_ok", "pool", "incidence_plane",
     "chunk_states", "segment_scan", "causal_scan", "query", "normalise", "forward",
     "forward_workspace_bytes", "decode_step", "validate_table", "direct", "zeta", "walsh",
-    "incidence_complement",
+    "incidence_complement", "DraftTree", "tree_step", "tree_state",
     "HipKernelError", "HipUnavailable", "MAX_R", "MAX_P", "MAX_C",
 ]
 
@@ -599,8 +600,11 @@ def forward_fused(W, kind: str, Q, K, V, h, idx, deg: int, *, n: int, n_P: int, 
     return out
 
 
-def decode_step(Phi_t, Psi_t, Vb_t, S_in, S_out, U, step: int, *, out=None, o_full=None):
-    """One decode step for a batch; returns fp32 ``(nb, p-1)`` and writes ``S_out``."""
+def decode_step(Phi_t, Psi_t, Vb_t, S_in, S_out, U, step: int, *, out=None, o_full=None,
+                ahead=None):
+    """One decode step for a batch; returns fp32 ``(nb, p-1)`` and writes ``S_out``.
+    ``ahead`` (int32, one entry a request, heads innermost): the requests' own positions past
+    ``step``."""
     who = "decode_step"
     if not (Phi_t.is_cuda and Psi_t.is_cuda and Vb_t.is_cuda and S_in.is_cuda
             and S_out.is_cuda and U.is_cuda):
@@ -644,7 +648,142 @@ def decode_step(Phi_t, Psi_t, Vb_t, S_in, S_out, U, step: int, *, out=None, o_fu
     if o_full is not None and (o_full.shape != (nb, P) or o_full.dtype != torch.float32
                                or not o_full.is_contiguous()):
         raise ValueError(f"{who}: o_full must be contiguous fp32 {(nb, P)}")
+    if ahead is not None:
+        _check_requests(who, "ahead", ahead, nb, U.device)
+        call("smat_decode_step_at", code, Phi_t.data_ptr(), Psi_t.data_ptr(), Vb_t.data_ptr(),
+             S_in.data_ptr(), S_out.data_ptr(), U.data_ptr(), out.data_ptr(), ptr(o_full),
+             ahead.data_ptr(), ahead.numel(), nb, B, R, P, int(step), q_sb, k_sb, v_sb,
+             stream_of(U))
+        return out
     call("smat_decode_step", code, Phi_t.data_ptr(), Psi_t.data_ptr(), Vb_t.data_ptr(),
          S_in.data_ptr(), S_out.data_ptr(), U.data_ptr(), out.data_ptr(), ptr(o_full), nb, B, R,
          P, int(step), q_sb, k_sb, v_sb, stream_of(U))
     return out
+
+
+# ---------------------------------------------------------------------------
+# drafted trees over the decode cache
+# ---------------------------------------------------------------------------
+
+MAX_NODES = 64
+
+
+def _check_requests(who: str, name: str, t: torch.Tensor, nb: int, device) -> None:
+    """One int32 entry a request, requests dividing the sequences."""
+    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{who}: {name} must be a contiguous int32 vector on {device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.numel() < 1 or nb % t.numel():
+        raise ValueError(f"{who}: {t.numel()} entries of {name} do not divide {nb} sequences")
+
+
+class DraftTree:
+    """The trees of one verification pass.  ``parents`` is a list of node parents (-1: a root,
+    a child of the prefix; -2: an unused node), shared by every sequence, or one list per
+    request; a parent comes before its children.  At most 64 nodes.  Checked and staged on
+    ``device`` once."""
+
+    def __init__(self, parents, device):
+        par = np.asarray(parents.cpu() if isinstance(parents, torch.Tensor) else parents)
+        if par.ndim == 1:
+            par = par[None]
+        if par.ndim != 2 or par.size == 0 or par.dtype.kind not in "iu":
+            raise ValueError("DraftTree: parents must be a list of integers, or one list of the "
+                             "same length a request")
+        trees, M = par.shape
+        if M > MAX_NODES:
+            raise ValueError(f"DraftTree: {M} nodes, at most {MAX_NODES}")
+        anc = np.zeros((trees, M), np.uint64)
+        level = np.full((trees, M), -1, np.int64)
+        for t in range(trees):
+            for j, a in enumerate(int(x) for x in par[t]):
+                if a == -2:
+                    continue
+                if not -1 <= a < j or (a >= 0 and level[t, a] < 0):
+                    raise ValueError(f"DraftTree: node {j} of tree {t} has parent {a}; a parent "
+                                     f"is -1 or an earlier used node")
+                level[t, j] = 0 if a < 0 else level[t, a] + 1
+                anc[t, j] = (anc[t, a] if a >= 0 else np.uint64(0)) | np.uint64(1 << j)
+        key = np.where(level < 0, M, level)
+        order = np.argsort(key, axis=1, kind="stable")
+        lstart = np.stack([np.searchsorted(np.sort(k), np.arange(M + 1)) for k in key])
+        self.parents, self.trees, self.nodes = par, trees, M
+        self.levels = int(level.max()) + 1
+        self.level = level
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.anc = torch.from_numpy(anc.view(np.int64)).to(self.device)
+        self.order = torch.from_numpy(order.astype(np.int32)).to(self.device)
+        self.lstart = torch.from_numpy(lstart.astype(np.int32)).to(self.device)
+
+
+def _tree_inputs(who, tree, nb, R, P, device, **rows):
+    """Check the drafted rows (nb, M, columns) and return each as (tensor, strides)."""
+    if tree.device != device:
+        raise ValueError(f"{who}: the tree is on {tree.device}, the cache on {device}")
+    if nb % tree.trees:
+        raise ValueError(f"{who}: {tree.trees} trees do not divide {nb} sequences")
+    ref = next(iter(rows.values()))
+    got = []
+    for name, t in rows.items():
+        _shape(who, name, t, (nb, tree.nodes, P if name == "Vb" else R))
+        if t.device != device:
+            raise ValueError(f"{who}: {name} is on {t.device}, the cache on {device}")
+        _same_dtype(who, ref, **{name: t})
+        got += _rows3(t)
+    _code(ref, who)
+    return got
+
+
+def tree_step(Phi, Psi, Vb, tree: DraftTree, S, U, step: int, *, ahead=None, out=None):
+    """Every node of the drafted trees read against the cache: fp32 ``(nb, M, p-1)``."""
+    who = "tree_step"
+    _on_gpu(who, S, U)
+    nb, R, P = S.shape
+    _shape(who, "U", U, (nb, None, R, P))
+    Phi, q_sb, q_st, Psi, k_sb, k_st, Vb, v_sb, v_st = _tree_inputs(
+        who, tree, nb, R, P, S.device, Phi=Phi, Psi=Psi, Vb=Vb)
+    if ahead is not None:
+        _check_requests(who, "ahead", ahead, nb, S.device)
+    want = (nb, tree.nodes, P - 1)
+    if out is None:
+        out = torch.empty(want, device=S.device, dtype=torch.float32)
+    elif out.shape != want or out.dtype != torch.float32 or not out.is_contiguous() \
+            or out.device != S.device:
+        raise ValueError(f"{who}: out must be contiguous fp32 {want} on {S.device}")
+    if not (S.is_contiguous() and U.is_contiguous() and S.dtype == U.dtype == torch.float32):
+        raise ValueError(f"{who}: S and U must be contiguous fp32")
+    with torch.cuda.device(S.device):
+        call("smat_tree_step", _code(Phi, who), Phi.data_ptr(), Psi.data_ptr(), Vb.data_ptr(),
+             S.data_ptr(), U.data_ptr(), out.data_ptr(), tree.anc.data_ptr(),
+             tree.order.data_ptr(), tree.lstart.data_ptr(), ptr(ahead) or None, nb, tree.trees,
+             ahead.numel() if ahead is not None else 1, tree.nodes, tree.levels, U.shape[1], R, P,
+             int(step), q_sb, q_st, k_sb, k_st, v_sb, v_st, stream_of(S))
+    return out
+
+
+def tree_state(Psi, Vb, tree: DraftTree, nodes, S, S_out, *, ahead=None):
+    """``S_out = S`` with each request's accepted path added; moves ``ahead`` by its length."""
+    who = "tree_state"
+    _on_gpu(who, S, S_out)
+    nb, R, P = S.shape
+    _shape(who, "S_out", S_out, (nb, R, P))
+    Psi, k_sb, k_st, Vb, v_sb, v_st = _tree_inputs(who, tree, nb, R, P, S.device, Psi=Psi, Vb=Vb)
+    _check_requests(who, "nodes", nodes, nb, S.device)
+    if ahead is not None:
+        _check_requests(who, "ahead", ahead, nb, S.device)
+        if ahead.numel() != nodes.numel():
+            raise ValueError(f"{who}: {nodes.numel()} accepted nodes for {ahead.numel()} requests")
+    if tree.trees not in (1, nodes.numel()):
+        raise ValueError(f"{who}: {nodes.numel()} accepted nodes for {tree.trees} trees")
+    if not (S.is_contiguous() and S_out.is_contiguous() and S.dtype == S_out.dtype
+            == torch.float32 and S_out.device == S.device):
+        raise ValueError(f"{who}: S and S_out must be contiguous fp32 on one device")
+    if abs(S.data_ptr() - S_out.data_ptr()) < S.numel() * 4:
+        raise ValueError(f"{who}: S and S_out must be distinct buffers")
+    with torch.cuda.device(S.device):
+        call("smat_tree_state", _code(Psi, who), Psi.data_ptr(), Vb.data_ptr(), S.data_ptr(),
+             S_out.data_ptr(), tree.anc.data_ptr(), nodes.data_ptr(), ptr(ahead) or None, nb,
+             tree.trees, nodes.numel(), tree.nodes, R, P, k_sb, k_st, v_sb, v_st, stream_of(S))
+    return S_out
