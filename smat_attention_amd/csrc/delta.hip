@@ -5,7 +5,10 @@
 // delta_chain_kernel walks the chunks.  The columns of the state do not mix, so a
 // wave takes 16 of them with all r rows in registers (fp32) and needs nothing of
 // any other wave: K S and Q S from the state, U = T b (V - e K S), O, and the new
-// state, each product's result tiles being the next one's operand as they lie.
+// state, each product's result tiles being the next one's operand as they lie.  The
+// waves of a workgroup share the chunk's operands in LDS, copied there two phases
+// ahead of their use: while K S, Q S and T run, the chunk's P and the next K land;
+// while P U and K^T U run, the next Q and T.
 //
 // One wave walks a whole segment where sequences and columns give enough waves.
 // Where they do not, segments are cut into runs: a first pass takes every run from
@@ -29,12 +32,29 @@ struct ChainIO {
   bool vvec, ovec;
 };
 
+// Bytes of LDS: KD buffers of K and the factors, T; and Q and P with the outputs.
+template <typename In, int RB, bool OUT> constexpr int chain_lds(int KD) {
+  constexpr int NT = Terms<In>::in, NO = Terms<In>::out;
+  return KD * (2 * NT * tile_elems(RB) + kVec * 4) +
+         2 * (kTri * kFrag * kMid + (OUT ? NT * tile_elems(RB) + kTri * kFrag * NO : 0));
+}
+// fp32 tiles of more than 64 features fit once only: their next K is copied between
+// the chunks.
+template <typename In, int RB, bool OUT> constexpr int chain_bufs() {
+  return chain_lds<In, RB, OUT>(2) <= kMaxLds ? 2 : 1;
+}
+
 template <typename In, int RB, bool OUT>
-__global__ __launch_bounds__(256) void delta_chain_kernel(Geo g, Ops o, ChainIO io, int tiles) {
+__global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO io, int tiles) {
   constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid, R = 32 * RB;
-  constexpr int KB = 4 * RB * kFrag, TB = kTri * kFrag;
-  const int ct = blockIdx.x * (blockDim.x >> 6) + wave_id();
-  if (ct >= tiles) return;
+  constexpr int TL = NT * tile_elems(RB), TB = kTri * kFrag;
+  constexpr int KD = chain_bufs<In, RB, OUT>();
+  extern __shared__ __align__(1024) bf16 lds[];
+  bf16 *kl = lds, *tl = lds + KD * TL, *ql = tl + NI * TB, *pl = ql + (OUT ? TL : 0);
+  float* vl = reinterpret_cast<float*>(pl + (OUT ? NO * TB : 0));
+  const int w = uniform_wave(), W = blockDim.x >> 6;
+  const int ct = blockIdx.x * W + w;
+  const bool on = ct < tiles;                      // else: copies and barriers only
   const int run = blockIdx.y, s = blockIdx.z;
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
@@ -57,106 +77,151 @@ __global__ __launch_bounds__(256) void delta_chain_kernel(Geo g, Ops o, ChainIO 
         S[mt][i] = (io.start && a < g.r && col < g.p) ? io.start[sn * rp + (int64_t)a * g.p + col]
                                                       : 0.f;
     }
-  const In* vs = (const In*)io.v + s * g.v_sb + col;
+  const In* vs = (const In*)io.v + s * g.v_sb;
+  const int64_t voff = 4 * gq * g.v_st + col;
+  const int soff = 4 * gq * ld + col;              // in rows of ld floats
   const bool vlive = values && col < g.p;
+  In v[16];
+  auto load_v = [&](int t0, int len) {
+    const int64_t off = fresh(voff);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int t = 16 * (j >> 2) + (j & 3);
+      v[j] = vlive && t + 4 * gq < len ? (vs + (int64_t)(t0 + t) * g.v_st)[off] : from_f32<In>(0.f);
+    }
+  };
+  auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
+  auto stage_k = [&](int c, int t0, int len, int buf) {
+    stage_tile<RB, NT>(kl + buf * TL, o.k, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
+    stage(vl + buf * kVec, vec_of(c), 1, (w + 1) % W, W);
+  };
+  auto stage_qt = [&](int c, int t0, int len) {
+    stage(tl, o.tm + ((int64_t)s * g.nch + c) * NI * TB, NI * kTri, w, W);
+    if (OUT) stage_tile<RB, NT>(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
+  };
 
+  int t0 = 0, len = 0, t1 = 0, len1 = 0;
+  if (c0 < c1) {
+    chunk_of(g, c0, t0, len);
+    load_v(t0, len);
+    stage_k(c0, t0, len, 0);
+    stage_qt(c0, t0, len);
+  }
   for (int c = c0; c < c1; ++c) {
-    int t0, len;
-    chunk_of(g, c, t0, len);
+    const int buf = KD == 2 ? (c - c0) & 1 : 0;
+    const bool more = c + 1 < c1;
     const int64_t sc = (int64_t)s * g.nch + c;
-    const bf16* kr = o.kr + (ks * g.nch + c) * (int64_t)NT * KB;
-    const bf16* kt = o.kt + (ks * g.nch + c) * (int64_t)NT * KB;
-    const bf16* tm = o.tm + sc * NI * TB;
-    const float* vec = o.vec + sc * kVec;
-
+    const bf16* kt = kl + buf * TL;
+    const float* vec = vl + buf * kVec;
+    if (more) chunk_of(g, c + 1, t1, len1);
+    wait_vmcnt<0>();
+    lds_barrier();
+    // ---- K, Q, T and the factors of chunk c are in LDS
     f32x4 x[4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+    for (int j = 0; j < 16; ++j) x[j >> 2][j & 3] = to_f32(v[j]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * mt + 4 * gq + i;
-        x[mt][i] = (vlive && t < len) ? to_f32(vs[(int64_t)(t0 + t) * g.v_st]) : 0.f;
-      }
-    if (OUT && io.save_s) {
-      float* Sp = io.save_s + sc * R * ld;
-#pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) Sp[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = S[mt][i];
-    }
-    Frag<NI> sb[RB];
-#pragma unroll
-    for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-    // b (V - e K S)
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      f32x4 a = zero4();
-#pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
-        a = mul(a, load_frag<NT>(kr + (mt * RB + kb) * kFrag, KB), sb[kb]);
-      const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
-      const f32x4 b = *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[mt][i] = b[i] * (x[mt][i] - e[i] * a[i]);
-    }
+    for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(x[mt]));   // their wait is here
+    if (OUT) stage(pl, o.pm + sc * NO * TB, NO * kTri, w, W);
+    if (KD == 2 && more) stage_k(c + 1, t1, len1, 1 - buf);
+
     f32x4 ot[4];
-    if (OUT) {
-      const bf16* qr = o.qr + (ks * g.nch + c) * (int64_t)NT * KB;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {             // columns in registers, token in the lane
-        ot[mt] = zero4();
-#pragma unroll
-        for (int kb = 0; kb < RB; ++kb)
-          ot[mt] = mul(ot[mt], lead<NO>(sb[kb]), load_frag<NT>(qr + (mt * RB + kb) * kFrag, KB));
-        ot[mt] *= g.scale * vec[16 * mt + m];
-      }
-    }
     Frag<NI> f[2];
+    if (on) {
+      if (OUT && io.save_s) {
+        const int off = fresh(soff);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {               // U, in place of x
-      x[mt] = zero4();
-#pragma unroll
-      for (int kb = 0; kb <= mt / 2; ++kb)
-        x[mt] = mul(x[mt], load_frag<NI>(tm + tri(mt, kb) * kFrag, TB), f[kb]);
-    }
-    if (OUT) {
-      if (io.save_u) {
-        float* Up = io.save_u + sc * C * ld;
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) Up[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = x[mt][i];
+        for (int mt = 0; mt < 2 * RB; ++mt)
+          put_rows(io.save_s + (sc * R + 16 * mt) * ld, off, ld, S[mt]);
       }
-      Frag<NO> fo[2];
-      const bf16* pm = o.pm + sc * NO * TB;
+      Frag<NI> sb[RB];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NO>(x[2 * kb], x[2 * kb + 1]);
+      for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
+      __builtin_amdgcn_sched_barrier(0);           // keeps a stage's operands from piling up
+      // b (V - e K S)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
+        f32x4 a = zero4();
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb) a = mul(a, rows_of<RB, NT>(kt, mt, kb), sb[kb]);
+        const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[mt][i] = b[i] * (x[mt][i] - e[i] * a[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (OUT) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {           // columns in registers, token in the lane
+          ot[mt] = zero4();
+#pragma unroll
+          for (int kb = 0; kb < RB; ++kb)
+            ot[mt] = mul(ot[mt], lead<NO>(sb[kb]), rows_of<RB, NT>(ql, mt, kb));
+          ot[mt] *= g.scale * vec[16 * mt + m];
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {             // U, in place of x
+        x[mt] = zero4();
 #pragma unroll
         for (int kb = 0; kb <= mt / 2; ++kb)
-          ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pm + tri(mt, kb) * kFrag, TB));
-        const int t = 16 * mt + m, oc = 16 * ct + 4 * gq;
-        if (t < len)
-          store4((In*)io.o + ((int64_t)s * g.T + t0 + t) * g.p + oc, ot[mt], g.p - oc, io.ovec);
+          x[mt] = mul(x[mt], load_frag<NI>(tl + tri(mt, kb) * kFrag, TB), f[kb]);
       }
     }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
-      x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-    const float aC = vec[3 * C];
-#pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt) {
-      S[mt] *= aC;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        S[mt] = mul(S[mt], load_frag<NT>(kt + (mt * 2 + kb) * kFrag, KB), f[kb]);
+    wait_vmcnt<0>();
+    lds_barrier();
+    // ---- P of chunk c and the next K are in LDS; Q and T are free
+    if (more) {
+      load_v(t1, len1);
+      stage_qt(c + 1, t1, len1);
     }
+    if (on) {
+      if (OUT) {
+        if (io.save_u) {
+          const int off = fresh(soff);
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt)
+            put_rows(io.save_u + (sc * C + 16 * mt) * ld, off, ld, x[mt]);
+        }
+        Frag<NO> fo[2];
+        const int ooff = fresh(m * g.p + 4 * gq);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NO>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+          for (int kb = 0; kb <= mt / 2; ++kb)
+            ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pl + tri(mt, kb) * kFrag, TB));
+          if (16 * mt + m < len)
+            store4((In*)io.o + ((int64_t)s * g.T + t0 + 16 * mt) * g.p + 16 * ct + ooff, ot[mt],
+                   g.p - 16 * ct - 4 * gq, io.ovec);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+        x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+      const float aC = vec[3 * C];
+#pragma unroll
+      for (int mt = 0; mt < 2 * RB; ++mt) {
+        S[mt] *= aC;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb), f[kb]);
+      }
+    }
+    if (KD == 1 && more) {
+      lds_barrier();                               // K is read
+      stage_k(c + 1, t1, len1, 0);
+    }
+    t0 = t1;
+    len = len1;
   }
+  if (!on) return;
   if (values ? io.end != nullptr : io.trans != nullptr) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
@@ -267,11 +332,16 @@ int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bo
   return launch_status("smat_delta_scan: carry");
 }
 
+// Two workgroups of four waves a CU where their LDS allows, else one of eight.
 template <typename In, int RB, bool OUT>
 static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipStream_t st) {
-  const int W = tiles < 4 ? tiles : 4;
-  hipLaunchKernelGGL((delta_chain_kernel<In, RB, OUT>), dim3((tiles + W - 1) / W, g.nruns, g.nb),
-                     dim3(64 * W), 0, st, g, o, io, tiles);
+  constexpr int lds = chain_lds<In, RB, OUT>(chain_bufs<In, RB, OUT>());
+  static_assert(lds <= kMaxLds, "");
+  const int most = 2 * lds <= kMaxLds ? 4 : 8;
+  const int n = (tiles + most - 1) / most, W = (tiles + n - 1) / n;
+  auto kern = delta_chain_kernel<In, RB, OUT>;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL(kern, dim3(n, g.nruns, g.nb), dim3(64 * W), lds, st, g, o, io, tiles);
 }
 
 template <typename In, int RB>
@@ -280,7 +350,7 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
                 float* state_out, float* save_s, float* save_u, void* ws, hipStream_t st) {
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
-  const Ops o = take_ops(ar, dtype, g.nb, g.nbk, g.nch, g.r, false);
+  const Ops o = place_ops(ar, dtype, g, q, k, false);
   const bool qvec = vec4_ok(q, g.q_sb, g.q_st, eb), kvec = vec4_ok(k, g.k_sb, g.k_st, eb);
   if (g.nch > 0)
     hipLaunchKernelGGL((delta_prep_kernel<In, RB, false>), dim3(g.nch, g.nb), dim3(256), 0, st, q,
@@ -327,7 +397,7 @@ extern "C" int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nc
                                               int nruns, int r, int p, int backward) {
   using namespace smat::dl;
   Arena ar{nullptr};
-  take_ops(ar, dtype, nb, nbk, nch, r, backward != 0);
+  take_ops(ar, dtype, nb, nbk, nch, r, backward != 0, false);
   if (nruns > nseg) take_carry(ar, nb, nruns, r, p);
   if (backward) {
     ar.take<float>((int64_t)nb * nch * 32 * rblocks(r) * p32(p));   // dS' of every chunk

@@ -15,7 +15,7 @@
 //
 // Two kernels after the chunks' operands: delta_rchain_kernel walks the chunks
 // backwards through dS as the forward's chain walks them through S (16 columns a
-// wave, no exchange), storing dS' and Z of every chunk; delta_grad_kernel, one
+// wave, operands shared in LDS), storing dS' and Z of every chunk; delta_grad_kernel, one
 // workgroup a (key sequence, chunk), forms the rest for the group's value heads one
 // after another, so the gradients of a shared key head are sums in registers, in
 // the heads' order.
@@ -35,12 +35,27 @@ struct RChainIO {
   int ptiles;
 };
 
+// Bytes of LDS: KD buffers of K and the factors, Q, T^T and P^T.
+template <typename In, int RB> constexpr int rchain_lds(int KD) {
+  constexpr int NT = Terms<In>::in;
+  return KD * (2 * NT * tile_elems(RB) + kVec * 4) +
+         2 * (NT * tile_elems(RB) + 2 * kTri * kFrag * kMid);
+}
+template <typename In, int RB> constexpr int rchain_bufs() {
+  return rchain_lds<In, RB>(2) <= kMaxLds ? 2 : 1;
+}
+
 template <typename In, int RB, bool OUT>
-__global__ __launch_bounds__(256) void delta_rchain_kernel(Geo g, Ops o, RChainIO io, int tiles) {
+__global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainIO io, int tiles) {
   constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB;
-  constexpr int KB = 4 * RB * kFrag, TB = kTri * kFrag;
-  const int ct = blockIdx.x * (blockDim.x >> 6) + wave_id();
-  if (ct >= tiles) return;
+  constexpr int TL = NT * tile_elems(RB), TB = kTri * kFrag;
+  constexpr int KD = rchain_bufs<In, RB>();
+  extern __shared__ __align__(1024) bf16 lds[];
+  bf16 *kl = lds, *ql = lds + KD * TL, *tl = ql + TL, *pl = tl + NI * TB;
+  float* vl = reinterpret_cast<float*>(pl + NI * TB);
+  const int w = uniform_wave(), W = blockDim.x >> 6;
+  const int ct = blockIdx.x * W + w;
+  const bool on = ct < tiles;                      // else: copies and barriers only
   const int run = blockIdx.y, s = blockIdx.z;
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
@@ -63,108 +78,153 @@ __global__ __launch_bounds__(256) void delta_rchain_kernel(Geo g, Ops o, RChainI
         S[mt][i] = (io.start && a < g.r && col < g.p) ? io.start[sn * rp + (int64_t)a * g.p + col]
                                                       : 0.f;
     }
-  const In* ds = (const In*)io.dout + s * io.d_sb + col;
+  const In* ds = (const In*)io.dout + s * io.d_sb;
+  const int64_t doff = 4 * gq * io.d_st + col;
+  const int soff = 4 * gq * ld + col;              // in rows of ld floats
   const bool dlive = values && col < g.p;
-
-  for (int c = c1 - 1; c >= c0; --c) {
-    int t0, len;
-    chunk_of(g, c, t0, len);
+  In dv[16];
+  auto load_d = [&](int t0, int len) {
+    const int64_t off = fresh(doff);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int t = 16 * (j >> 2) + (j & 3);
+      dv[j] =
+          dlive && t + 4 * gq < len ? (ds + (int64_t)(t0 + t) * io.d_st)[off] : from_f32<In>(0.f);
+    }
+  };
+  auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
+  auto stage_k = [&](int c, int t0, int len, int buf) {
+    stage_tile<RB, NT>(kl + buf * TL, o.k, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
+    stage(vl + buf * kVec, vec_of(c), 1, (w + 1) % W, W);
+  };
+  auto stage_tp = [&](int c) {
     const int64_t sc = (int64_t)s * g.nch + c;
-    const int64_t kc = (ks * g.nch + c) * (int64_t)NT * KB;
-    const float* vec = o.vec + sc * kVec;
-    f32x4 d[4];
+    stage(tl, o.tt + sc * NI * TB, NI * kTri, w, W);
+    stage(pl, o.pt + sc * NI * TB, NI * kTri, w, W);
+  };
+
+  int t0 = 0, len = 0, t1 = 0, len1 = 0;
+  if (c0 < c1) {
+    chunk_of(g, c1 - 1, t0, len);
+    load_d(t0, len);
+    stage_k(c1 - 1, t0, len, 0);
+    stage_tp(c1 - 1);
+  }
+  for (int c = c1 - 1; c >= c0; --c) {
+    const int buf = KD == 2 ? (c1 - 1 - c) & 1 : 0;
+    const bool more = c > c0;
+    const int64_t sc = (int64_t)s * g.nch + c;
+    const bf16* kt = kl + buf * TL;
+    const float* vec = vl + buf * kVec;
+    if (more) chunk_of(g, c - 1, t1, len1);
+    wait_vmcnt<0>();
+    lds_barrier();
+    // ---- K, T^T, P^T and the factors of chunk c are in LDS
+    f32x4 d[4], x[4];
+    Frag<NT> df[2];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+    for (int j = 0; j < 16; ++j) d[j >> 2][j & 3] = to_f32(dv[j]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 16 * mt + 4 * gq + i;
-        d[mt][i] = (dlive && t < len) ? to_f32(ds[(int64_t)(t0 + t) * io.d_st]) : 0.f;
+    for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(d[mt]));   // their wait is here
+    stage_tile<RB, NT>(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
+    if (KD == 2 && more) stage_k(c - 1, t1, len1, 1 - buf);
+    if (on) {
+      if (OUT) {
+        const int off = fresh(soff);
+#pragma unroll
+        for (int mt = 0; mt < 2 * RB; ++mt)
+          put_rows(io.save_d + (sc * R + 16 * mt) * ld, off, ld, S[mt]);
       }
-    if (OUT) {
-      float* Sp = io.save_d + sc * R * ld;
+      Frag<NI> f[2];
+      {
+        Frag<NI> sb[RB];
 #pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt)
+        for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
+        __builtin_amdgcn_sched_barrier(0);         // keeps a stage's operands from piling up
 #pragma unroll
-        for (int i = 0; i < 4; ++i) Sp[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = S[mt][i];
-    }
-    f32x4 x[4];                                    // dU
-    {
-      Frag<NI> sb[RB];
+        for (int mt = 0; mt < 4; ++mt) {           // dU
+          x[mt] = zero4();
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        x[mt] = zero4();
-#pragma unroll
-        for (int kb = 0; kb < RB; ++kb)
-          x[mt] = mul(x[mt], load_frag<NT>(o.kr + kc + (mt * RB + kb) * kFrag, KB), sb[kb]);
-        x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
-      }
-    }
-    if (values) {
-      Frag<NT> df[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int kb = mt / 2; kb < 2; ++kb)
-          x[mt] = mul(x[mt], load_frag<NI>(o.pt + (sc * NI * kTri + tri_t(mt, kb)) * kFrag, TB),
-                      df[kb]);
-    }
-    Frag<NI> f[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {               // Z
-      x[mt] = zero4();
-#pragma unroll
-      for (int kb = mt / 2; kb < 2; ++kb)
-        x[mt] = mul(x[mt], load_frag<NI>(o.tt + (sc * NI * kTri + tri_t(mt, kb)) * kFrag, TB),
-                    f[kb]);
-    }
-    if (OUT) {
-      float* Zp = io.z + sc * C * ld;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) Zp[(int64_t)(16 * mt + 4 * gq + i) * ld + col] = x[mt][i];
-    }
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
-      x[mt] *= *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);     // b Z
-      if (OUT && dlive) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int t = 16 * mt + 4 * gq + i;
-          if (t < len)
-            ((In*)io.dv)[((int64_t)s * g.T + t0 + t) * g.p + col] = from_f32<In>(x[mt][i]);
+          for (int kb = 0; kb < RB; ++kb) x[mt] = mul(x[mt], rows_of<RB, NT>(kt, mt, kb), sb[kb]);
+          x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
         }
       }
-      x[mt] *= -e;
-      d[mt] *= g.scale * e;
+      __builtin_amdgcn_sched_barrier(0);
+      if (values) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+          for (int kb = mt / 2; kb < 2; ++kb)
+            x[mt] = mul(x[mt], load_frag<NI>(pl + tri_t(mt, kb) * kFrag, TB), df[kb]);
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {             // Z
+        x[mt] = zero4();
+#pragma unroll
+        for (int kb = mt / 2; kb < 2; ++kb)
+          x[mt] = mul(x[mt], load_frag<NI>(tl + tri_t(mt, kb) * kFrag, TB), f[kb]);
+      }
     }
-    const float aC = vec[3 * C];
-#pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt) S[mt] *= aC;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-#pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        S[mt] = mul(S[mt], load_frag<NT>(o.kt + kc + (mt * 2 + kb) * kFrag, KB), f[kb]);
-    if (values) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
-#pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-          S[mt] = mul(S[mt], load_frag<NT>(o.qt + kc + (mt * 2 + kb) * kFrag, KB), f[kb]);
+    wait_vmcnt<0>();
+    lds_barrier();
+    // ---- Q of chunk c and the next K are in LDS; T^T and P^T are free
+    if (more) {
+      load_d(t1, len1);
+      stage_tp(c - 1);
     }
+    if (on) {
+      if (OUT) {
+        const int off = fresh(soff);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) put_rows(io.z + (sc * C + 16 * mt) * ld, off, ld, x[mt]);
+      }
+      const int voff = fresh(4 * gq * g.p + col);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
+        x[mt] *= *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);     // b Z
+        if (OUT && dlive) {
+          In* row = (In*)io.dv + ((int64_t)s * g.T + t0 + 16 * mt) * g.p;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * mt + 4 * gq + i < len) (row + (int64_t)i * g.p)[voff] = from_f32<In>(x[mt][i]);
+        }
+        x[mt] *= -e;
+        d[mt] *= g.scale * e;
+      }
+      const float aC = vec[3 * C];
+      Frag<NI> f[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int mt = 0; mt < 2 * RB; ++mt) {
+        S[mt] *= aC;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb), f[kb]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      if (values) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
+#pragma unroll
+        for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(ql, mt, kb), f[kb]);
+      }
+    }
+    if (KD == 1 && more) {
+      lds_barrier();                               // K is read
+      stage_k(c - 1, t1, len1, 0);
+    }
+    t0 = t1;
+    len = len1;
   }
+  if (!on) return;
   if (values ? io.end != nullptr : io.trans != nullptr) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
@@ -204,9 +264,10 @@ __device__ __forceinline__ float sum_groups(float x) {
 
 template <typename In, int RB>
 __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io) {
-  constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB;
-  constexpr int KB = 4 * RB * kFrag;
-  __shared__ __align__(16) float G[C * kLd], N[C * kLd];
+  constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB, TL = NT * tile_elems(RB);
+  extern __shared__ __align__(1024) bf16 lds[];
+  bf16 *kl = lds, *ql = lds + TL;
+  float *G = reinterpret_cast<float*>(ql + TL), *N = G + C * kLd;
   __shared__ double Ls[C];
   __shared__ float bs[C], dLs[C], inter[C], pair[2][4];
   const int c = blockIdx.x, ks = blockIdx.y, group = g.nb / g.nbk;
@@ -216,7 +277,12 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
   chunk_of(g, c, t0, len);
   const bool live = tok < len;
   const int64_t row = t0 + (live ? tok : 0);
-  const int64_t kc = ((int64_t)ks * g.nch + c) * NT * KB;
+  {
+    const float* vec = o.vec + ((int64_t)ks * group * g.nch + c) * kVec;
+    stage_tile<RB, NT>(kl, o.k, ks, g.nch, c, t0, len, g.r, vec, uniform_wave(), 4);
+    stage_tile<RB, NT>(ql, o.q, ks, g.nch, c, t0, len, g.r, vec, uniform_wave(), 4);
+    wait_vmcnt<0>();                               // the first barrier below publishes them
+  }
   const In* qrow = (const In*)io.q + ks * g.q_sb + row * g.q_st;
   const In* krow = (const In*)io.k + ks * g.k_sb + row * g.k_st;
 
@@ -316,7 +382,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
                                       *reinterpret_cast<const f32x4*>(Nr + 16));
 #pragma unroll
         for (int rt = 0; rt < 2 * RB; ++rt) {
-          const Frag<NT> kf = load_frag<NT>(o.kt + kc + (rt * 2 + kb) * kFrag, KB);
+          const Frag<NT> kf = cols_of<RB, NT>(kl, rt, kb);
           a[rt] = mul(a[rt], kf, gf);
           y[rt] = mul(y[rt], kf, nf);
         }
@@ -334,8 +400,8 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
         const Frag<NI> gf = split<NI>(gx[0], gx[1]), nf = split<NI>(nx[0], nx[1]);
 #pragma unroll
         for (int rt = 0; rt < 2 * RB; ++rt) {
-          kw[rt] = mul(kw[rt], load_frag<NT>(o.qt + kc + (rt * 2 + kb) * kFrag, KB), gf);
-          kw[rt] = mul(kw[rt], load_frag<NT>(o.kt + kc + (rt * 2 + kb) * kFrag, KB), nf);
+          kw[rt] = mul(kw[rt], cols_of<RB, NT>(ql, rt, kb), gf);
+          kw[rt] = mul(kw[rt], cols_of<RB, NT>(kl, rt, kb), nf);
         }
       }
     }
@@ -387,9 +453,13 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
 
 template <typename In, int RB, bool OUT>
 static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hipStream_t st) {
-  const int W = tiles < 4 ? tiles : 4;
-  hipLaunchKernelGGL((delta_rchain_kernel<In, RB, OUT>), dim3((tiles + W - 1) / W, g.nruns, g.nb),
-                     dim3(64 * W), 0, st, g, o, io, tiles);
+  constexpr int lds = rchain_lds<In, RB>(rchain_bufs<In, RB>());
+  static_assert(lds <= kMaxLds, "");
+  const int most = 2 * lds <= kMaxLds ? 4 : 8;
+  const int n = (tiles + most - 1) / most, W = (tiles + n - 1) / n;
+  auto kern = delta_rchain_kernel<In, RB, OUT>;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL(kern, dim3(n, g.nruns, g.nb), dim3(64 * W), lds, st, g, o, io, tiles);
 }
 
 template <typename In, int RB>
@@ -397,7 +467,7 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
                     const float* dstate_out, float* dstate, void* ws, hipStream_t st) {
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
-  const Ops o = take_ops(ar, dtype, g.nb, g.nbk, g.nch, g.r, true);
+  const Ops o = place_ops(ar, dtype, g, q, k, true);
   gr.qvec = vec4_ok(q, g.q_sb, g.q_st, eb);
   gr.kvec = vec4_ok(k, g.k_sb, g.k_st, eb);
   gr.vvec = vec4_ok(gr.v, g.v_sb, g.v_st, eb);
@@ -434,9 +504,13 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   rchain<In, RB, true>(g, o, io, io.ptiles, st);
   gr.save_d = save_d;
   gr.z = z;
-  if (g.nch > 0)
-    hipLaunchKernelGGL((delta_grad_kernel<In, RB>), dim3(g.nch, g.nbk), dim3(256), 0, st, g, o,
-                       gr);
+  if (g.nch > 0) {
+    constexpr int lds = 4 * Terms<In>::in * tile_elems(RB) + 8 * C * kLd;
+    static_assert(lds + 2048 <= kMaxLds, "");
+    auto kern = delta_grad_kernel<In, RB>;
+    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL(kern, dim3(g.nch, g.nbk), dim3(256), lds, st, g, o, gr);
+  }
   return launch_status("smat_delta_scan_backward");
 }
 

@@ -28,8 +28,17 @@
 // (g = lane >> 4) in registers.  Slot (g, j) of a 32-long contraction stands for
 // index 4g + j (j < 4) or 16 + 4g + j - 4: then two stacked result tiles are an
 // operand of the next product as they lie in registers, and the chain needs no
-// exchange between lanes.  All operands in the workspace are stored in that order,
-// one 16 x 32 fragment in 1 KB, lane by lane.
+// exchange between lanes.  T and P are stored as fragments in that order, 16 x 32
+// in 1 KB, lane by lane.
+//
+// K and Q are read both by rows (contraction over features) and transposed (over
+// tokens).  Both reads come from one LDS tile of 64 rows: 8-byte reads of a row's
+// slots, and transposing reads.  The tile's rows hold RS 16-byte chunks, chunk k of
+// row t at k ^ swz(t), which keeps both reads free of bank conflicts (64 banks;
+// 32 lanes a phase: 16 rows x 16 bytes one way, 8 rows x 32 bytes the other).
+// Tiles are copied to LDS by the DMA path straight from the caller's rows where
+// those are bf16 in 16-byte groups; otherwise delta_prep_kernel writes them to the
+// workspace, a tile a term, padded and swizzled.
 #pragma once
 
 #include <type_traits>
@@ -41,7 +50,8 @@ namespace dl {
 
 constexpr int C = 64;              // tokens a chunk
 constexpr int kFrag = 512;         // elements a 16 x 32 fragment
-constexpr int kVec = 256;          // floats a chunk: e[64], w[64], b[64], exp(L_C), unused
+constexpr int kVec = 256;          // floats a chunk: e[64], w[64], b[64], exp(L_C), zeros
+constexpr int kZero = 3 * C + 4;   // where 16 bytes of zeros lie in it
 constexpr int kTri = 6;            // fragments of a 64 x 64 triangle
 constexpr int kMaxR = 128, kMaxP = 256;
 
@@ -126,6 +136,108 @@ __device__ __forceinline__ constexpr int tri_t(int mt, int kb) {
   return mt < 2 ? 2 * mt + kb : mt + 2;
 }
 
+// 16-byte chunks a tile row, and elements a tile.
+constexpr int row_chunks(int RB) { return RB == 1 ? 4 : RB == 2 ? 8 : 16; }
+constexpr int tile_elems(int RB) { return C * row_chunks(RB) * 8; }
+template <int RS> __device__ __forceinline__ int swz(int t) {
+  if (RS == 16) return (((t & 7) << 1) | ((t >> 3) & 1)) ^ (t & 8);
+  if (RS == 8) return (t & 6) | ((t >> 3) & 1);
+  return ((t >> 1) & 2) | ((t >> 3) & 1);
+}
+
+// Row fragment: token 16 mt + (lane & 15), feature slots of block kb.
+template <int RB, int N>
+__device__ __forceinline__ Frag<N> rows_of(const bf16* tile, int mt, int kb) {
+  constexpr int RS = row_chunks(RB);
+  const int m = lane_id() & 15, g = lane_id() >> 4;
+  const int k0 = (4 * kb + (g >> 1)) ^ swz<RS>(m), k1 = (4 * kb + 2 + (g >> 1)) ^ swz<RS>(m);
+  const bf16* p = tile + (16 * mt + m) * RS * 8 + 4 * (g & 1);
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const bf16x4 a = *reinterpret_cast<const bf16x4*>(p + n * tile_elems(RB) + k0 * 8);
+    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p + n * tile_elems(RB) + k1 * 8);
+    f.t[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// Transposed fragment: feature 16 mt + (lane & 15), token slots of block kb.  Lane
+// 4 e + q of each sixteen addresses token 16 (2 kb + h) + 4 g + e, features 4 q .. + 3.
+template <int RB, int N>
+__device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb) {
+  typedef short short4v __attribute__((ext_vector_type(4)));
+  constexpr int RS = row_chunks(RB);
+  const int r16 = lane_id() & 15, row = 4 * (lane_id() >> 4) + (r16 >> 2);
+  const int k = (2 * mt + ((r16 & 3) >> 1)) ^ swz<RS>(row);
+  const bf16* p = tile + ((32 * kb + row) * RS + k) * 8 + 4 * (r16 & 1);
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    bf16x4 h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bf16* a = p + n * tile_elems(RB) + i * 16 * RS * 8;
+      h[i] = __builtin_bit_cast(
+          bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                      (__attribute__((address_space(3))) short4v*)(uint32_t)(uintptr_t)a));
+    }
+    f.t[n] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// Where a key sequence's tiles come from.
+struct TileSrc {
+  const bf16* ws;          // tiles (nbk, nch, terms); or null
+  const bf16* raw;         // the caller's rows, strides sb, st
+  int64_t sb, st;
+};
+
+// A lane's offset that the compiler takes for new: addresses built from it inside a
+// loop are formed there, not kept in registers across it.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+__device__ __forceinline__ int64_t fresh(int64_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+// A result tile's column in fp32 rows: p is the wave's (uniform) row 0, off the
+// lane's 4 gq ld + column, rows ld apart.
+__device__ __forceinline__ void put_rows(float* p, int off, int ld, const f32x4& x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) (p + (int64_t)i * ld)[off] = x[i];
+}
+__device__ __forceinline__ int uniform_wave() {
+  return __builtin_amdgcn_readfirstlane(wave_id());
+}
+
+// Copies of 1 KB a wave into LDS, spread over W waves; they land by the next
+// wait_vmcnt<0>() and barrier.
+__device__ __forceinline__ void stage(void* dst, const void* src, int kb, int w, int W) {
+  for (int u = w; u < kb; u += W)
+    lds_dma16<true>((const char*)src + u * 1024 + lane_id() * 16, (char*)dst + u * 1024);
+}
+template <int RB, int N>
+__device__ __forceinline__ void stage_tile(bf16* dst, const TileSrc& src, int64_t ks, int64_t nch,
+                                           int c, int t0, int len, int r, const float* vec, int w,
+                                           int W) {
+  constexpr int RS = row_chunks(RB);
+  if (N > 1 || src.ws) {
+    stage(dst, src.ws + (ks * nch + c) * (int64_t)N * tile_elems(RB), N * RS, w, W);
+  } else {
+    const bf16* base = src.raw + ks * src.sb + (int64_t)t0 * src.st;
+    for (int u = w; u < RS; u += W) {
+      const int l = u * 64 + lane_id(), t = l / RS, k = (l % RS) ^ swz<RS>(t);
+      const void* p = t < len && 8 * k < r ? (const void*)(base + (int64_t)t * src.st + 8 * k)
+                                           : (const void*)(vec + kZero);
+      lds_dma16<true>(p, dst + u * 512);
+    }
+  }
+}
+
 // Four consecutive elements; those at and past nv are zero.
 template <typename In>
 __device__ __forceinline__ f32x4 load4(const In* p, int nv, bool vec) {
@@ -194,9 +306,10 @@ __device__ __forceinline__ void run_of(const Geo& g, int i, int& c0, int& c1, in
   }
 }
 
-// The chunks' operands in the workspace.
+// The chunks' operands.
 struct Ops {
-  bf16 *kr, *kt, *qr, *qt;  // rows of K and Q (contraction over r), and transposed (over tokens)
+  TileSrc k, q;
+  bf16 *kw, *qw;            // the tiles' place in the workspace; or null
   bf16 *tm, *pm;            // T and P by rows
   bf16 *tt, *pt;            // transposed
   float* vec;
@@ -215,21 +328,45 @@ struct Arena {
   }
 };
 
+constexpr int kMaxLds = 160 * 1024;
+
 inline int rblocks(int r) { return (r + 31) / 32; }
 inline int p32(int p) { return (p + 31) / 32 * 32; }
 inline int in_terms(int dtype) { return dtype == SMAT_BF16 ? 1 : dtype == SMAT_F16 ? 2 : 3; }
 inline int out_terms(int dtype) { return dtype == SMAT_F32 ? 3 : 2; }
 
-inline Ops take_ops(Arena& ar, int dtype, int64_t nb, int64_t nbk, int64_t nch, int r, bool bwd) {
-  const int64_t rows = nbk * nch * in_terms(dtype) * 4 * rblocks(r) * kFrag;
+// Whether rows can be copied as they are: bf16 in aligned groups of eight.
+inline bool raw_ok(int dtype, const void* p, int64_t sb, int64_t st, int r) {
+  return dtype == SMAT_BF16 && r % 8 == 0 && rows_vec8_ok(p, sb, st);
+}
+
+// raw: no tiles in the workspace.
+inline Ops take_ops(Arena& ar, int dtype, int64_t nb, int64_t nbk, int64_t nch, int r, bool bwd,
+                    bool raw) {
+  const int64_t tiles = nbk * nch * in_terms(dtype) * tile_elems(rblocks(r));
   const int64_t tris = nb * nch * kTri * kFrag;
   Ops o = {};
-  o.kr = ar.take<bf16>(rows);
-  o.kt = ar.take<bf16>(rows);
-  (bwd ? o.qt : o.qr) = ar.take<bf16>(rows);
+  if (!raw) {
+    o.kw = ar.take<bf16>(tiles);
+    o.qw = ar.take<bf16>(tiles);
+    o.k.ws = o.kw;
+    o.q.ws = o.qw;
+  }
   (bwd ? o.tt : o.tm) = ar.take<bf16>(tris * kMid);
   (bwd ? o.pt : o.pm) = ar.take<bf16>(tris * (bwd ? kMid : out_terms(dtype)));
   o.vec = ar.take<float>(nb * nch * kVec);
+  return o;
+}
+
+inline Ops place_ops(Arena& ar, int dtype, const Geo& g, const void* q, const void* k, bool bwd) {
+  const bool raw = raw_ok(dtype, q, g.q_sb, g.q_st, g.r) && raw_ok(dtype, k, g.k_sb, g.k_st, g.r);
+  Ops o = take_ops(ar, dtype, g.nb, g.nbk, g.nch, g.r, bwd, raw);
+  o.k.raw = (const bf16*)k;
+  o.k.sb = g.k_sb;
+  o.k.st = g.k_st;
+  o.q.raw = (const bf16*)q;
+  o.q.sb = g.q_sb;
+  o.q.st = g.q_st;
   return o;
 }
 

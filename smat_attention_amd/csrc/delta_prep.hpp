@@ -1,5 +1,6 @@
-// The state-free part of every chunk: fragments of K and Q, T = (I + A)^{-1}, P, and
-// the row factors (delta_common.hpp).  One workgroup of four waves a (value
+// The state-free part of every chunk: T = (I + A)^{-1}, P and the row factors, and
+// the tiles of K and Q where the caller's rows are not copied as they are
+// (delta_common.hpp).  One workgroup of four waves a (value
 // sequence, chunk); wave w owns token rows 16 w .. 16 w + 15.
 //
 // T.  Wave w inverts diagonal block w by substitution (a lane a column, 120 steps
@@ -119,20 +120,21 @@ __device__ __forceinline__ Frag<N> row_frag(const In* row, bool ok, int c0, int 
   return split<N>(a, b);
 }
 
-// Fragment of the transpose from row fragments in LDS (one term): rows 16 mt + ..
-// of the feature axis, tokens of block kb.
-template <int RB>
-__device__ __forceinline__ bf16x8 transposed(const bf16* rows, int mt, int kb) {
-  const int lane = lane_id(), col = 16 * mt + (lane & 15), g = lane >> 4;
-  // feature col sits in contraction block col / 32, slot (gc, jc)
-  const int kc = col >> 5, c5 = col & 31, gc = (c5 & 15) >> 2, jc = (c5 & 3) + (c5 & 16 ? 4 : 0);
-  bf16x8 f;
+// A token's slots of contraction block kb into its row of a tile (a tile a term).
+template <int RB, int N>
+__device__ __forceinline__ void store_row(bf16* tile, int t, int kb, const Frag<N>& f) {
+  constexpr int RS = row_chunks(RB);
+  const int g = lane_id() >> 4;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int tt = 2 * kb + (j >> 2), m = 4 * g + (j & 3);      // token 16 tt + m
-    f[j] = rows[(tt * RB + kc) * kFrag + (gc * 16 + m) * 8 + jc];
-  }
-  return f;
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = (4 * kb + 2 * h + (g >> 1)) ^ swz<RS>(t);
+      bf16* p = tile + n * tile_elems(RB) + (t * RS + k) * 8 + 4 * (g & 1);
+      *reinterpret_cast<bf16x4*>(p) =
+          h ? __builtin_shufflevector(f.t[n], f.t[n], 4, 5, 6, 7)
+            : __builtin_shufflevector(f.t[n], f.t[n], 0, 1, 2, 3);
+    }
 }
 
 template <typename In, int RB, bool BWD>
@@ -146,38 +148,30 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
   __shared__ double Ls[C];
   __shared__ float bs[C];
   const int c = blockIdx.x, s = blockIdx.y;
-  const int w = wave_id(), lane = lane_id(), m = lane & 15, gq = lane >> 4;
+  const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
   int t0, len;
   chunk_of(g, c, t0, len);
   const int64_t ks = key_of(g, s);
-  const bool first = s % (g.nb / g.nbk) == 0;      // this workgroup stores K's and Q's fragments
+  const bool tiles = o.kw && s % (g.nb / g.nbk) == 0;   // this workgroup stores K's and Q's tiles
   chunk_decays(g, logA, beta, s, t0, len, Ls, bs);
 
   const int tok = 16 * w + m;
   const bool live = tok < len;
   const In* krow = k + ks * g.k_sb + (int64_t)(t0 + (live ? tok : 0)) * g.k_st;
   const In* qrow = q + ks * g.q_sb + (int64_t)(t0 + (live ? tok : 0)) * g.q_st;
-  const int64_t kc = (ks * g.nch + c) * (int64_t)NT * KB, sc = (int64_t)s * g.nch + c;
+  const int64_t kc = (ks * g.nch + c) * (int64_t)NT * tile_elems(RB), sc = (int64_t)s * g.nch + c;
   Frag<NT> kf[RB], qf[RB];
 #pragma unroll
   for (int kb = 0; kb < RB; ++kb) {
     kf[kb] = row_frag<In, NT>(krow, live, 32 * kb + 4 * gq, g.r, kvec);
     qf[kb] = row_frag<In, NT>(qrow, live, 32 * kb + 4 * gq, g.r, qvec);
     store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, kf[kb]);
-    if (first) {
-      store_frag<NT>(o.kr + kc + (w * RB + kb) * kFrag, KB, kf[kb]);
-      if (!BWD) store_frag<NT>(o.qr + kc + (w * RB + kb) * kFrag, KB, qf[kb]);
+    if (tiles) {
+      store_row<RB, NT>(o.kw + kc, tok, kb, kf[kb]);
+      store_row<RB, NT>(o.qw + kc, tok, kb, qf[kb]);
     }
   }
   __syncthreads();
-  if (first) {
-#pragma unroll
-    for (int f = w; f < 4 * RB; f += 4)
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-        *reinterpret_cast<bf16x8*>(o.kt + kc + n * KB + f * kFrag + lane * 8) =
-            transposed<RB>(rows + n * KB, f >> 1, f & 1);
-  }
   // A = b D K K^T below the diagonal: column j in the lane, rows 16 w + 4 gq + i
   f32x4 pacc[4];
 #pragma unroll
@@ -222,15 +216,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
   }
   unit_lower_inverse(Am, Tm);
   if (BWD) {
-    // Q transposed, and P^T: lane holds token j = 16 w + m, rows i = 16 it + 4 gq + ..
-    if (first) {
-#pragma unroll
-      for (int f = w; f < 4 * RB; f += 4)
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-          *reinterpret_cast<bf16x8*>(o.qt + kc + n * KB + f * kFrag + lane * 8) =
-              transposed<RB>(rows + n * KB, f >> 1, f & 1);
-    }
+    // P^T: lane holds token j = 16 w + m, rows i = 16 it + 4 gq + ..
     const double Lj = Ls[tok];
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
@@ -278,7 +264,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
     v[t] = expf((float)Ls[t]);
     v[C + t] = expf((float)(Ls[C - 1] - Ls[t]));
     v[2 * C + t] = bs[t];
-    if (t == 0) v[3 * C] = expf((float)Ls[C - 1]);
+    v[3 * C + t] = t == 0 ? expf((float)Ls[C - 1]) : 0.f;
   }
 }
 

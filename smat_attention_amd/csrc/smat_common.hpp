@@ -302,7 +302,8 @@ template <bool UNTRACKED>
 __device__ __forceinline__ void lds_dma16(const void* src, void* dst) {
   typedef __attribute__((address_space(3))) char lds_char;
   if constexpr (UNTRACKED) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(size_t)(lds_char*)(dst));
+    // (a generic LDS address carries the LDS offset in its low half)
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
     uint32_t keep;
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\t"
