@@ -29,7 +29,7 @@ struct ChainIO {
   float* trans;           // first pass: M of run i, (i nb + s) R R row-major (R = 32 RB); or null
   float *save_s, *save_u; // training: states entering chunks, and U, rows padded to p32; or null
   int ptiles;             // value tiles of 16 columns (tiles behind them are M's)
-  bool vvec, ovec;
+  bool narrow, ovec;      // v's rows lie within 32-bit offsets; out in groups of four
 };
 
 // Bytes of LDS: KD buffers of K and the factors, T; and Q and P with the outputs.
@@ -44,15 +44,22 @@ template <typename In, int RB, bool OUT> constexpr int chain_bufs() {
   return chain_lds<In, RB, OUT>(2) <= kMaxLds ? 2 : 1;
 }
 
+// Two workgroups of four waves a CU where their LDS allows, else one of eight.
+template <typename In, int RB, bool OUT> constexpr int chain_waves() {
+  return 2 * chain_lds<In, RB, OUT>(chain_bufs<In, RB, OUT>()) <= kMaxLds ? 4 : 8;
+}
+
 template <typename In, int RB, bool OUT>
-__global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO io, int tiles) {
+__global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_chain_kernel(
+    Geo g, Ops o, ChainIO io, int tiles) {
   constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid, R = 32 * RB;
   constexpr int TL = NT * tile_elems(RB), TB = kTri * kFrag;
   constexpr int KD = chain_bufs<In, RB, OUT>();
   extern __shared__ __align__(1024) bf16 lds[];
   bf16 *kl = lds, *tl = lds + KD * TL, *ql = tl + NI * TB, *pl = ql + (OUT ? TL : 0);
   float* vl = reinterpret_cast<float*>(pl + (OUT ? NO * TB : 0));
-  const int w = uniform_wave(), W = blockDim.x >> 6;
+  constexpr int W = chain_waves<In, RB, OUT>();
+  const int w = uniform_wave();
   const int ct = blockIdx.x * W + w;
   const bool on = ct < tiles;                      // else: copies and barriers only
   const int run = blockIdx.y, s = blockIdx.z;
@@ -78,26 +85,22 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
                                                       : 0.f;
     }
   const In* vs = (const In*)io.v + s * g.v_sb;
-  const int64_t voff = 4 * gq * g.v_st + col;
-  const int soff = 4 * gq * ld + col;              // in rows of ld floats
+  const uint32_t soff = (4 * gq * ld + col) * 4;    // in fp32 rows of ld
   const bool vlive = values && col < g.p;
+  const bool any = on && values && 16 * ct < g.p;
   In v[16];
   auto load_v = [&](int t0, int len) {
-    const int64_t off = fresh(voff);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int t = 16 * (j >> 2) + (j & 3);
-      v[j] = vlive && t + 4 * gq < len ? (vs + (int64_t)(t0 + t) * g.v_st)[off] : from_f32<In>(0.f);
-    }
+    load_column(v, vs, g.v_st, io.narrow, t0, len, col, vlive, any);
   };
+  const TileStage<RB, NT, W> kstage(o.k, g.r, w), qstage(o.q, g.r, w);
   auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
   auto stage_k = [&](int c, int t0, int len, int buf) {
-    stage_tile<RB, NT>(kl + buf * TL, o.k, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
-    stage(vl + buf * kVec, vec_of(c), 1, (w + 1) % W, W);
+    kstage(kl + buf * TL, o.k, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
+    stage<1, W>(vl + buf * kVec, vec_of(c), W - 1 - w);
   };
   auto stage_qt = [&](int c, int t0, int len) {
-    stage(tl, o.tm + ((int64_t)s * g.nch + c) * NI * TB, NI * kTri, w, W);
-    if (OUT) stage_tile<RB, NT>(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
+    stage<NI * kTri, W>(tl, o.tm + ((int64_t)s * g.nch + c) * NI * TB, w);
+    if (OUT) qstage(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
   };
 
   int t0 = 0, len = 0, t1 = 0, len1 = 0;
@@ -118,26 +121,24 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
     lds_barrier();
     // ---- K, Q, T and the factors of chunk c are in LDS
     f32x4 x[4];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) x[j >> 2][j & 3] = to_f32(v[j]);
+    column_values(x, v, vlive);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(x[mt]));   // their wait is here
-    if (OUT) stage(pl, o.pm + sc * NO * TB, NO * kTri, w, W);
+    if (OUT) stage<NO * kTri, W>(pl, o.pm + sc * NO * TB, w);
     if (KD == 2 && more) stage_k(c + 1, t1, len1, 1 - buf);
 
     f32x4 ot[4];
     Frag<NI> f[2];
     if (on) {
       if (OUT && io.save_s) {
-        const int off = fresh(soff);
 #pragma unroll
         for (int mt = 0; mt < 2 * RB; ++mt)
-          put_rows(io.save_s + (sc * R + 16 * mt) * ld, off, ld, S[mt]);
+          put_rows(io.save_s + (sc * R + 16 * mt) * ld, soff, ld, S[mt]);
       }
       Frag<NI> sb[RB];
 #pragma unroll
       for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-      __builtin_amdgcn_sched_barrier(0);           // keeps a stage's operands from piling up
+      narrow_schedule<RB>();
       // b (V - e K S)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[mt][i] = b[i] * (x[mt][i] - e[i] * a[i]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      narrow_schedule<RB>();
       if (OUT) {
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {           // columns in registers, token in the lane
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
           ot[mt] *= g.scale * vec[16 * mt + m];
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      narrow_schedule<RB>();
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
@@ -181,13 +182,13 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
     if (on) {
       if (OUT) {
         if (io.save_u) {
-          const int off = fresh(soff);
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt)
-            put_rows(io.save_u + (sc * C + 16 * mt) * ld, off, ld, x[mt]);
+            put_rows(io.save_u + (sc * C + 16 * mt) * ld, soff, ld, x[mt]);
         }
         Frag<NO> fo[2];
-        const int ooff = fresh(m * g.p + 4 * gq);
+        const uint32_t ooff = (m * g.p + 4 * gq) * sizeof(In);
+        const int left = g.p - 16 * ct - 4 * gq;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NO>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
@@ -195,12 +196,13 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
 #pragma unroll
           for (int kb = 0; kb <= mt / 2; ++kb)
             ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pl + tri(mt, kb) * kFrag, TB));
-          if (16 * mt + m < len)
-            store4((In*)io.o + ((int64_t)s * g.T + t0 + 16 * mt) * g.p + 16 * ct + ooff, ot[mt],
-                   g.p - 16 * ct - 4 * gq, io.ovec);
+          In* row = (In*)io.o + ((int64_t)s * g.T + t0 + 16 * mt) * g.p + 16 * ct;
+          if (16 * mt + m < len && left > 0)
+            store4(reinterpret_cast<In*>(reinterpret_cast<char*>(row) + ooff), ot[mt],
+                   io.ovec ? 4 : left, io.ovec);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      narrow_schedule<RB>();
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
         x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
@@ -237,57 +239,86 @@ __global__ __launch_bounds__(512) void delta_chain_kernel(Geo g, Ops o, ChainIO 
 }
 
 // The states across the runs of a segment: entering run i (start), S <- M_i S + E_i,
-// and out of the last (final).  A wave a (sequence, segment, 16 columns); `rev`
-// walks the runs backwards (the gradient's direction).
+// and out of the last (fin).  A wave 16 columns, four waves a workgroup; `rev` walks
+// the runs backwards (the gradient's direction).  A step waits on the last one, so
+// what does not depend on it is done ahead: the next M and E are loaded while a step
+// computes, and the waves split M into terms once, in LDS, for each other.
 template <int RB>
-__global__ __launch_bounds__(64) void delta_carry_kernel(Geo g, const float* __restrict__ init,
-                                                         const float* __restrict__ E,
-                                                         const float* __restrict__ M,
-                                                         float* __restrict__ start,
-                                                         float* __restrict__ fin, bool rev) {
-  constexpr int R = 32 * RB, NI = kMid;
-  const int m = lane_id() & 15, gq = lane_id() >> 4;
-  const int col = 16 * blockIdx.x + m, seg = blockIdx.y, s = blockIdx.z;
+__global__ __launch_bounds__(256) void delta_carry_kernel(Geo g, const float* __restrict__ init,
+                                                          const float* __restrict__ E,
+                                                          const float* __restrict__ M,
+                                                          float* __restrict__ start,
+                                                          float* __restrict__ fin, bool rev) {
+  constexpr int R = 32 * RB, NI = kMid, NF = 2 * RB * RB, PER = (NF + 3) / 4;
+  extern __shared__ __align__(1024) bf16 lds[];    // NF fragments, a plane a term
+  const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
+  const int col = 16 * (4 * blockIdx.x + w) + m, seg = blockIdx.y, s = blockIdx.z;
   const int64_t rp = (int64_t)g.r * g.p;
   const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
-  f32x4 S[2 * RB];
-  auto each = [&](auto fn) {
+  const bool live = col < g.p;
+  auto at = [&](int n) { return (int64_t)(rev ? r0 + r1 - 1 - n : n) * g.nb + s; };
+  auto load_cols = [&](f32x4* x, const float* p) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int a = 16 * mt + 4 * gq + i;
-        if (a < g.r && col < g.p) fn(mt, i, (int64_t)a * g.p + col);
+        x[mt][i] = live && a < g.r ? p[(int64_t)a * g.p + col] : 0.f;
       }
+  };
+  auto store_cols = [&](float* p, const f32x4* x) {
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = 16 * mt + 4 * gq + i;
+        if (live && a < g.r) p[(int64_t)a * g.p + col] = x[mt][i];
+      }
+  };
+  f32x4 S[2 * RB], e[2 * RB], x[PER][2];
+  auto load_m = [&](int n) {
+    const float* p = M + at(n) * R * R + (int64_t)m * R + 4 * gq;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int f = min(u * 4 + w, NF - 1), mt = f / RB, kb = f % RB;
+      const float* q = p + (int64_t)16 * mt * R + 32 * kb;
+      x[u][0] = *reinterpret_cast<const f32x4*>(q);
+      x[u][1] = *reinterpret_cast<const f32x4*>(q + 16);
+    }
   };
 #pragma unroll
   for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = zero4();
   const int64_t ss = ((int64_t)seg * g.nb + s) * rp;
-  if (init) each([&](int mt, int i, int64_t off) { S[mt][i] = init[ss + off]; });
+  if (init) load_cols(S, init + ss);
+  if (r0 < r1) {
+    load_m(r0);
+    load_cols(e, E + at(r0) * rp);
+  }
   for (int n = r0; n < r1; ++n) {
-    const int run = rev ? r0 + r1 - 1 - n : n;
-    const int64_t sn = (int64_t)run * g.nb + s;
-    each([&](int mt, int i, int64_t off) { start[sn * rp + off] = S[mt][i]; });
+    __syncthreads();                               // the last step's fragments are read
+#pragma unroll
+    for (int u = 0; u < PER; ++u)
+      if (u * 4 + w < NF)
+        store_frag<NI>(lds + (u * 4 + w) * kFrag, NF * kFrag, split<NI>(x[u][0], x[u][1]));
+    store_cols(start + at(n) * rp, S);
     Frag<NI> sb[RB];
 #pragma unroll
     for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
 #pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = zero4();
-    each([&](int mt, int i, int64_t off) { S[mt][i] = E[sn * rp + off]; });
-    const float* Mr = M + sn * R * R + (int64_t)m * R + 4 * gq;
+    for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = e[mt];
+    if (n + 1 < r1) {
+      load_m(n + 1);
+      load_cols(e, E + at(n + 1) * rp);
+    }
+    lds_barrier();
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) {
-        const float* p = Mr + (int64_t)16 * mt * R + 32 * kb;
-        S[mt] = mul(S[mt],
-                    split<NI>(*reinterpret_cast<const f32x4*>(p),
-                              *reinterpret_cast<const f32x4*>(p + 16)), sb[kb]);
-      }
+      for (int kb = 0; kb < RB; ++kb)
+        S[mt] = mul(S[mt], load_frag<NI>(lds + (mt * RB + kb) * kFrag, NF * kFrag), sb[kb]);
   }
-  if (fin) each([&](int mt, int i, int64_t off) { fin[ss + off] = S[mt][i]; });
+  if (fin) store_cols(fin + ss, S);
 }
-
 
 int check_geo(const char* who, int dtype, const Geo& g) {
   SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
@@ -317,8 +348,11 @@ int check_geo(const char* who, int dtype, const Geo& g) {
 template <int RB>
 static void carry_kernel(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
                          hipStream_t st) {
-  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3((g.p + 15) / 16, g.nseg, g.nb), dim3(64), 0, st,
-                     g, init, c.E, c.M, c.start, fin, rev);
+  constexpr int lds = 2 * RB * RB * kMid * kFrag * 2;
+  auto kern = delta_carry_kernel<RB>;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  hipLaunchKernelGGL(kern, dim3((g.p + 63) / 64, g.nseg, g.nb), dim3(256), lds, st, g, init, c.E,
+                     c.M, c.start, fin, rev);
 }
 
 int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
@@ -332,16 +366,15 @@ int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bo
   return launch_status("smat_delta_scan: carry");
 }
 
-// Two workgroups of four waves a CU where their LDS allows, else one of eight.
 template <typename In, int RB, bool OUT>
 static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipStream_t st) {
   constexpr int lds = chain_lds<In, RB, OUT>(chain_bufs<In, RB, OUT>());
+  constexpr int W = chain_waves<In, RB, OUT>();
   static_assert(lds <= kMaxLds, "");
-  const int most = 2 * lds <= kMaxLds ? 4 : 8;
-  const int n = (tiles + most - 1) / most, W = (tiles + n - 1) / n;
   auto kern = delta_chain_kernel<In, RB, OUT>;
   (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL(kern, dim3(n, g.nruns, g.nb), dim3(64 * W), lds, st, g, o, io, tiles);
+  hipLaunchKernelGGL(kern, dim3((tiles + W - 1) / W, g.nruns, g.nb), dim3(64 * W), lds, st, g, o,
+                     io, tiles);
 }
 
 template <typename In, int RB>
@@ -361,6 +394,7 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
   io.start = state;
   io.end = state_out;
   io.ovec = vec4_ok(out, 0, g.p, eb);
+  io.narrow = narrow_stride(g.v_st);
   io.ptiles = (g.p + 15) / 16;
   if (g.nruns > g.nseg) {
     const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);

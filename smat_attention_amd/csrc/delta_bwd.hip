@@ -15,9 +15,9 @@
 //
 // Two kernels after the chunks' operands: delta_rchain_kernel walks the chunks
 // backwards through dS as the forward's chain walks them through S (16 columns a
-// wave, operands shared in LDS), storing dS' and Z of every chunk; delta_grad_kernel, one
-// workgroup a (key sequence, chunk), forms the rest for the group's value heads one
-// after another, so the gradients of a shared key head are sums in registers, in
+// wave, operands shared in LDS), storing dS' and Z of every chunk; delta_grad_kernel,
+// one workgroup a (key sequence, chunk), forms the rest for the group's value heads
+// one after another, so the gradients of a shared key head are sums in registers, in
 // the heads' order.
 #include "delta_prep.hpp"
 
@@ -33,6 +33,7 @@ struct RChainIO {
   float *save_d, *z;      // dS' of every chunk (R x p32) and Z (64 x p32)
   void* dv;               // (nb, T, p) contiguous
   int ptiles;
+  bool narrow;            // dout's rows lie within 32-bit offsets
 };
 
 // Bytes of LDS: KD buffers of K and the factors, Q, T^T and P^T.
@@ -45,15 +46,21 @@ template <typename In, int RB> constexpr int rchain_bufs() {
   return rchain_lds<In, RB>(2) <= kMaxLds ? 2 : 1;
 }
 
+template <typename In, int RB> constexpr int rchain_waves() {
+  return 2 * rchain_lds<In, RB>(rchain_bufs<In, RB>()) <= kMaxLds ? 4 : 8;
+}
+
 template <typename In, int RB, bool OUT>
-__global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainIO io, int tiles) {
+__global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain_kernel(
+    Geo g, Ops o, RChainIO io, int tiles) {
   constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB;
   constexpr int TL = NT * tile_elems(RB), TB = kTri * kFrag;
   constexpr int KD = rchain_bufs<In, RB>();
   extern __shared__ __align__(1024) bf16 lds[];
   bf16 *kl = lds, *ql = lds + KD * TL, *tl = ql + TL, *pl = tl + NI * TB;
   float* vl = reinterpret_cast<float*>(pl + NI * TB);
-  const int w = uniform_wave(), W = blockDim.x >> 6;
+  constexpr int W = rchain_waves<In, RB>();
+  const int w = uniform_wave();
   const int ct = blockIdx.x * W + w;
   const bool on = ct < tiles;                      // else: copies and barriers only
   const int run = blockIdx.y, s = blockIdx.z;
@@ -79,28 +86,23 @@ __global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainI
                                                       : 0.f;
     }
   const In* ds = (const In*)io.dout + s * io.d_sb;
-  const int64_t doff = 4 * gq * io.d_st + col;
-  const int soff = 4 * gq * ld + col;              // in rows of ld floats
+  const uint32_t soff = (4 * gq * ld + col) * 4;    // in fp32 rows of ld
   const bool dlive = values && col < g.p;
+  const bool any = on && values && 16 * ct < g.p;
   In dv[16];
   auto load_d = [&](int t0, int len) {
-    const int64_t off = fresh(doff);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int t = 16 * (j >> 2) + (j & 3);
-      dv[j] =
-          dlive && t + 4 * gq < len ? (ds + (int64_t)(t0 + t) * io.d_st)[off] : from_f32<In>(0.f);
-    }
+    load_column(dv, ds, io.d_st, io.narrow, t0, len, col, dlive, any);
   };
+  const TileStage<RB, NT, W> kstage(o.k, g.r, w), qstage(o.q, g.r, w);
   auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
   auto stage_k = [&](int c, int t0, int len, int buf) {
-    stage_tile<RB, NT>(kl + buf * TL, o.k, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
-    stage(vl + buf * kVec, vec_of(c), 1, (w + 1) % W, W);
+    kstage(kl + buf * TL, o.k, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
+    stage<1, W>(vl + buf * kVec, vec_of(c), W - 1 - w);
   };
   auto stage_tp = [&](int c) {
     const int64_t sc = (int64_t)s * g.nch + c;
-    stage(tl, o.tt + sc * NI * TB, NI * kTri, w, W);
-    stage(pl, o.pt + sc * NI * TB, NI * kTri, w, W);
+    stage<NI * kTri, W>(tl, o.tt + sc * NI * TB, w);
+    stage<NI * kTri, W>(pl, o.pt + sc * NI * TB, w);
   };
 
   int t0 = 0, len = 0, t1 = 0, len1 = 0;
@@ -122,25 +124,23 @@ __global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainI
     // ---- K, T^T, P^T and the factors of chunk c are in LDS
     f32x4 d[4], x[4];
     Frag<NT> df[2];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) d[j >> 2][j & 3] = to_f32(dv[j]);
+    column_values(d, dv, dlive);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(d[mt]));   // their wait is here
-    stage_tile<RB, NT>(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w, W);
+    qstage(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
     if (KD == 2 && more) stage_k(c - 1, t1, len1, 1 - buf);
     if (on) {
       if (OUT) {
-        const int off = fresh(soff);
 #pragma unroll
         for (int mt = 0; mt < 2 * RB; ++mt)
-          put_rows(io.save_d + (sc * R + 16 * mt) * ld, off, ld, S[mt]);
+          put_rows(io.save_d + (sc * R + 16 * mt) * ld, soff, ld, S[mt]);
       }
       Frag<NI> f[2];
       {
         Frag<NI> sb[RB];
 #pragma unroll
         for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-        __builtin_amdgcn_sched_barrier(0);         // keeps a stage's operands from piling up
+        narrow_schedule<RB>();
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {           // dU
           x[mt] = zero4();
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainI
           x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      narrow_schedule<RB>();
       if (values) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
@@ -178,11 +178,10 @@ __global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainI
     }
     if (on) {
       if (OUT) {
-        const int off = fresh(soff);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) put_rows(io.z + (sc * C + 16 * mt) * ld, off, ld, x[mt]);
+        for (int mt = 0; mt < 4; ++mt) put_rows(io.z + (sc * C + 16 * mt) * ld, soff, ld, x[mt]);
       }
-      const int voff = fresh(4 * gq * g.p + col);
+      const uint32_t voff = (4 * gq * g.p + col) * sizeof(In);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
@@ -191,7 +190,9 @@ __global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainI
           In* row = (In*)io.dv + ((int64_t)s * g.T + t0 + 16 * mt) * g.p;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (16 * mt + 4 * gq + i < len) (row + (int64_t)i * g.p)[voff] = from_f32<In>(x[mt][i]);
+            if (len == C || 16 * mt + 4 * gq + i < len)
+              *reinterpret_cast<In*>(reinterpret_cast<char*>(row + (int64_t)i * g.p) + voff) =
+                  from_f32<In>(x[mt][i]);
         }
         x[mt] *= -e;
         d[mt] *= g.scale * e;
@@ -200,14 +201,14 @@ __global__ __launch_bounds__(512) void delta_rchain_kernel(Geo g, Ops o, RChainI
       Frag<NI> f[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-      __builtin_amdgcn_sched_barrier(0);
+      narrow_schedule<RB>();
 #pragma unroll
       for (int mt = 0; mt < 2 * RB; ++mt) {
         S[mt] *= aC;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb), f[kb]);
       }
-      __builtin_amdgcn_sched_barrier(0);
+      narrow_schedule<RB>();
       if (values) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
@@ -249,10 +250,6 @@ struct GradIO {
   bool qvec, kvec, vvec, dvec, ovec;
 };
 
-// Eight consecutive fp32 values as terms.
-template <int N> __device__ __forceinline__ Frag<N> split8(const float* p) {
-  return split<N>(*reinterpret_cast<const f32x4*>(p), *reinterpret_cast<const f32x4*>(p + 4));
-}
 __device__ __forceinline__ float dot4(const f32x4& a, const f32x4& b) {
   return a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3];
 }
@@ -261,133 +258,190 @@ __device__ __forceinline__ float sum_groups(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
 }
+// Eight consecutive elements; those at and past nv are zero.  vec: groups of four.
+template <typename In>
+__device__ __forceinline__ void load8f(f32x4* x, const In* p, int nv, bool vec) {
+  x[0] = load4(p, nv, vec);
+  x[1] = load4(p + 4, nv - 4, vec);
+}
 
+// Feature tiles are shared by H waves a token tile: two for more than 64 features, to
+// keep the sums of a wave within half of its SIMD's registers.
+constexpr int grad_split(int RB) { return RB >= 3 ? 2 : 1; }
+constexpr int most(int a, int b) { return a > b ? a : b; }
+// K's and Q's tiles beside the fragments, or, where that is too much (fp32 of more than
+// 64 features), behind G and N once the fragments are read, for each head anew.
+template <typename In, int RB> constexpr bool grad_late() {
+  return 4 * Terms<In>::in * tile_elems(RB) + (4 * RB + 8) * kMid * kFrag * 2 + 8192 > kMaxLds;
+}
+template <typename In, int RB> constexpr int grad_lds() {
+  const int frags = (4 * RB + 8) * kMid * kFrag * 2, gn = 8 * C * kLd;
+  const int tiles = 4 * Terms<In>::in * tile_elems(RB);
+  return grad_late<In, RB>() ? most(frags, gn + tiles) : tiles + most(frags, gn);
+}
+
+// Wave (token tile tt, half hf).  The products over the value columns take S, dS', U and
+// Z in steps of 32 columns, split into terms once, by the wave that loaded them, and
+// shared as fragments in LDS; the next step's are loaded while one computes.  G and N
+// then take the fragments' place.
 template <typename In, int RB>
-__global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io) {
+__global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo g, Ops o,
+                                                                              GradIO io) {
   constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB, TL = NT * tile_elems(RB);
+  constexpr int H = grad_split(RB), W = 4 * H, RT = 2 * RB / H;   // feature tiles a wave
+  constexpr int FS = 0, FD = 2 * RB, FU = 4 * RB, FZ = FU + 4, NF = FZ + 4, FP = NF * kFrag;
   extern __shared__ __align__(1024) bf16 lds[];
-  bf16 *kl = lds, *ql = lds + TL;
-  float *G = reinterpret_cast<float*>(ql + TL), *N = G + C * kLd;
+  constexpr bool LATE = grad_late<In, RB>();
+  bf16 *kl = lds + (LATE ? 4 * C * kLd : 0), *ql = kl + TL, *fr = LATE ? lds : ql + TL;
+  float *G = reinterpret_cast<float*>(fr), *N = G + C * kLd;
   __shared__ double Ls[C];
-  __shared__ float bs[C], dLs[C], inter[C], pair[2][4];
+  __shared__ float bs[C], zvs[C], pair[W], sums[H][4][C];
   const int c = blockIdx.x, ks = blockIdx.y, group = g.nb / g.nbk;
-  const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
-  const int tok = 16 * w + m, ld = (g.p + 31) / 32 * 32;
+  const int w = uniform_wave(), tt = w & 3, hf = w >> 2;
+  const int m = lane_id() & 15, gq = lane_id() >> 4;
+  const int tok = 16 * tt + m, ld = (g.p + 31) / 32 * 32, rt0 = hf * RT;
   int t0, len;
   chunk_of(g, c, t0, len);
   const bool live = tok < len;
   const int64_t row = t0 + (live ? tok : 0);
-  {
+  auto stage_tiles = [&]() {
     const float* vec = o.vec + ((int64_t)ks * group * g.nch + c) * kVec;
-    stage_tile<RB, NT>(kl, o.k, ks, g.nch, c, t0, len, g.r, vec, uniform_wave(), 4);
-    stage_tile<RB, NT>(ql, o.q, ks, g.nch, c, t0, len, g.r, vec, uniform_wave(), 4);
-    wait_vmcnt<0>();                               // the first barrier below publishes them
-  }
+    TileStage<RB, NT, W>(o.k, g.r, w)(kl, o.k, ks, g.nch, c, t0, len, g.r, vec, w);
+    TileStage<RB, NT, W>(o.q, g.r, w)(ql, o.q, ks, g.nch, c, t0, len, g.r, vec, w);
+  };
+  if (!LATE) stage_tiles();
   const In* qrow = (const In*)io.q + ks * g.q_sb + row * g.q_st;
   const In* krow = (const In*)io.k + ks * g.k_sb + row * g.k_st;
 
   // token in the lane, features 16 rt + 4 gq + i in registers, throughout
-  f32x4 dQ[2 * RB], dK[2 * RB];
+  f32x4 dQ[RT], dK[RT];
 #pragma unroll
-  for (int rt = 0; rt < 2 * RB; ++rt) dQ[rt] = dK[rt] = zero4();
+  for (int rt = 0; rt < RT; ++rt) dQ[rt] = dK[rt] = zero4();
 
   for (int h = 0; h < group; ++h) {
     const int s = ks * group + h;
     const int64_t sc = (int64_t)s * g.nch + c;
-    const float *Sp = io.save_s + sc * R * ld, *Dp = io.save_d + sc * R * ld;
-    const float *Up = io.save_u + sc * C * ld, *Zp = io.z + sc * C * ld;
     const float* vec = o.vec + sc * kVec;
     const In* drow = (const In*)io.dout + s * io.d_sb + row * io.d_st;
     const In* vrow = (const In*)io.v + s * g.v_sb + row * g.v_st;
+    // this wave's loads of a step: tile w of S and dS' (while there is one), and rows of
+    // U (waves of half 0) and Z (waves of the last half)
+    const bool pairs = w < 2 * RB, has_u = hf == 0, has_z = hf == H - 1;
+    const int64_t lane_row = (int64_t)m * ld + 8 * gq;
+    const float* Sp = io.save_s + (sc * R + 16 * w) * ld + lane_row;
+    const float* Dp = io.save_d + (sc * R + 16 * w) * ld + lane_row;
+    const float* Up = io.save_u + (sc * C + 16 * tt) * ld + lane_row;
+    const float* Zp = io.z + (sc * C + 16 * tt) * ld + lane_row;
+    f32x4 sx[2], ex[2], ux[2], zx[2], dx[2], vx[2];
+    auto get = [&](f32x4* x, const float* p) {
+      x[0] = *reinterpret_cast<const f32x4*>(p);
+      x[1] = *reinterpret_cast<const f32x4*>(p + 4);
+    };
+    auto load_step = [&](int pb) {
+      if (pairs) {
+        get(sx, Sp + pb);
+        get(ex, Dp + pb);
+      }
+      if (has_u) get(ux, Up + pb);
+      if (has_z) get(zx, Zp + pb);
+      const int pc = pb + 8 * gq;
+      load8f(dx, drow + pc, live ? g.p - pc : 0, io.dvec);
+      if (has_z) load8f(vx, vrow + pc, live ? g.p - pc : 0, io.vvec);
+    };
+    load_step(0);
+    __syncthreads();                               // the last head's LDS is read
     chunk_decays(g, io.logA, io.beta, s, t0, len, Ls, bs);
 
-    f32x4 a[2 * RB], y[2 * RB], kw[2 * RB], gp[4], np[4];
+    f32x4 a[RT], y[RT], kw[RT], gp[4], np[4];
 #pragma unroll
-    for (int rt = 0; rt < 2 * RB; ++rt) a[rt] = y[rt] = kw[rt] = zero4();
+    for (int rt = 0; rt < RT; ++rt) a[rt] = y[rt] = kw[rt] = zero4();
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) gp[jt] = np[jt] = zero4();
     float zv = 0.f, dots = 0.f;
     for (int pb = 0; pb < ld; pb += 32) {
-      const int pc = pb + 8 * gq;
-      f32x4 d0 = zero4(), d1 = zero4(), v0 = zero4(), v1 = zero4();
-      if (live) {
-        d0 = load4(drow + pc, g.p - pc, io.dvec);
-        d1 = load4(drow + pc + 4, g.p - pc - 4, io.dvec);
-        v0 = load4(vrow + pc, g.p - pc, io.vvec);
-        v1 = load4(vrow + pc + 4, g.p - pc - 4, io.vvec);
+      if (pairs) {
+        dots += dot4(sx[0], ex[0]) + dot4(sx[1], ex[1]);
+        store_frag<NI>(fr + (FS + w) * kFrag, FP, split<NI>(sx[0], sx[1]));
+        store_frag<NI>(fr + (FD + w) * kFrag, FP, split<NI>(ex[0], ex[1]));
       }
-      const Frag<NT> df = split<NT>(d0, d1);
-      const f32x4 z0 = *reinterpret_cast<const f32x4*>(Zp + (int64_t)tok * ld + pc);
-      const f32x4 z1 = *reinterpret_cast<const f32x4*>(Zp + (int64_t)tok * ld + pc + 4);
-      zv += dot4(z0, v0) + dot4(z1, v1);
-      const Frag<NI> zf = split<NI>(z0, z1);
-      const Frag<NI> uf = split8<NI>(Up + (int64_t)tok * ld + pc);
+      if (has_u) store_frag<NI>(fr + (FU + tt) * kFrag, FP, split<NI>(ux[0], ux[1]));
+      if (has_z) {
+        zv += dot4(zx[0], vx[0]) + dot4(zx[1], vx[1]);
+        store_frag<NI>(fr + (FZ + tt) * kFrag, FP, split<NI>(zx[0], zx[1]));
+      }
+      const Frag<NT> df = split<NT>(dx[0], dx[1]);
+      __syncthreads();
+      if (pb + 32 < ld) load_step(pb + 32);
+      {
+        const Frag<NI> zf = load_frag<NI>(fr + (FZ + tt) * kFrag, FP);
+        const Frag<NI> uf = load_frag<NI>(fr + (FU + tt) * kFrag, FP);
 #pragma unroll
-      for (int jt = 0; jt < 4; ++jt)
-        if (jt <= w) {                             // column j in the lane, rows i in registers
-          const Frag<NI> uj = split8<NI>(Up + (int64_t)(16 * jt + m) * ld + pc);
-          gp[jt] = mul(gp[jt], df, uj);
-          np[jt] = mul(np[jt], zf, uj);
+        for (int rt = 0; rt < RT; ++rt) {
+          const Frag<NI> sf = load_frag<NI>(fr + (FS + rt0 + rt) * kFrag, FP);
+          a[rt] = mul(a[rt], sf, df);
+          y[rt] = mul(y[rt], sf, zf);
+          kw[rt] = mul(kw[rt], load_frag<NI>(fr + (FD + rt0 + rt) * kFrag, FP), uf);
         }
 #pragma unroll
-      for (int rt = 0; rt < 2 * RB; ++rt) {
-        const int64_t at = (int64_t)(16 * rt + m) * ld + pc;
-        const f32x4 s0 = *reinterpret_cast<const f32x4*>(Sp + at);
-        const f32x4 s1 = *reinterpret_cast<const f32x4*>(Sp + at + 4);
-        const f32x4 e0 = *reinterpret_cast<const f32x4*>(Dp + at);
-        const f32x4 e1 = *reinterpret_cast<const f32x4*>(Dp + at + 4);
-        if ((rt & 3) == w) dots += dot4(s0, e0) + dot4(s1, e1);
-        const Frag<NI> sf = split<NI>(s0, s1), ef = split<NI>(e0, e1);
-        a[rt] = mul(a[rt], sf, df);
-        y[rt] = mul(y[rt], sf, zf);
-        kw[rt] = mul(kw[rt], ef, uf);
+        for (int jt = 0; jt < 4; ++jt)
+          if (jt <= tt) {                          // column j in the lane, rows i in registers
+            const Frag<NI> uj = load_frag<NI>(fr + (FU + jt) * kFrag, FP);
+            if (has_u) gp[jt] = mul(gp[jt], df, uj);
+            if (has_z) np[jt] = mul(np[jt], zf, uj);
+          }
       }
+      lds_barrier();                               // the fragments are read
     }
-    zv = sum_groups(zv);
+    if (LATE) stage_tiles();
+    if (pairs) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) dots += __shfl_xor(dots, d);
-    if (lane_id() == 0) pair[h & 1][w] = dots;       // wave 0 may still read the last head's
-    __syncthreads();                               // Ls and bs, pair; G and N free
+      for (int d = 1; d < 64; d <<= 1) dots += __shfl_xor(dots, d);
+    }
+    if (lane_id() == 0) pair[w] = dots;
+    if (has_z) {
+      zv = sum_groups(zv);
+      if (gq == 0) zvs[tok] = zv;
+    }
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int ti = 16 * w + 4 * gq + i, j = 16 * jt + m;
-        const float D = j <= ti ? expf((float)(Ls[ti] - Ls[j])) : 0.f;
-        G[ti * kLd + j] = j <= ti ? g.scale * (D * gp[jt][i]) : 0.f;
-        N[ti * kLd + j] = j < ti ? -(D * np[jt][i]) : 0.f;
+        const int ti = 16 * tt + 4 * gq + i, j = 16 * jt + m;
+        const float D = jt <= tt && j <= ti ? decay(Ls[ti] - Ls[j]) : 0.f;
+        if (has_u) G[ti * kLd + j] = j <= ti ? g.scale * (D * gp[jt][i]) : 0.f;
+        if (has_z) N[ti * kLd + j] = j < ti ? -(D * np[jt][i]) : 0.f;
       }
+    if (LATE || h == 0) wait_vmcnt<0>();           // K's and Q's tiles
     __syncthreads();
-    const float e = vec[tok], wt = vec[C + tok], b = vec[2 * C + tok];
-    float kint = 0.f;
+    const float e = vec[tok], wt = vec[C + tok], b = bs[tok];
+    f32x4 kv[RT];
+    float qd = 0.f, ky = 0.f, kk = 0.f, kint = 0.f;
 #pragma unroll
-    for (int rt = 0; rt < 2 * RB; ++rt) {
+    for (int rt = 0; rt < RT; ++rt) {
+      const int f0 = 16 * (rt0 + rt) + 4 * gq;
+      kv[rt] = load4(krow + f0, live ? g.r - f0 : 0, io.kvec);
       a[rt] *= g.scale * e;
       y[rt] *= -e;
       kw[rt] *= wt;
-    }
-#pragma unroll
-    for (int rt = 0; rt < 2 * RB; ++rt) {
-      const int f0 = 16 * rt + 4 * gq;
-      kint += live ? dot4(load4(krow + f0, g.r - f0, io.kvec), kw[rt]) : 0.f;
+      kint += dot4(kv[rt], kw[rt]);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const int j0 = 32 * kb + 4 * gq;
-      if (kb <= w / 2) {                           // rows i = tok, over j
+      if (kb <= tt / 2) {                          // rows i = tok, over j
         const float *Gr = G + tok * kLd + j0, *Nr = N + tok * kLd + j0;
         const Frag<NI> gf = split<NI>(*reinterpret_cast<const f32x4*>(Gr),
                                       *reinterpret_cast<const f32x4*>(Gr + 16));
         const Frag<NI> nf = split<NI>(*reinterpret_cast<const f32x4*>(Nr),
                                       *reinterpret_cast<const f32x4*>(Nr + 16));
 #pragma unroll
-        for (int rt = 0; rt < 2 * RB; ++rt) {
-          const Frag<NT> kf = cols_of<RB, NT>(kl, rt, kb);
+        for (int rt = 0; rt < RT; ++rt) {
+          const Frag<NT> kf = cols_of<RB, NT>(kl, rt0 + rt, kb);
           a[rt] = mul(a[rt], kf, gf);
           y[rt] = mul(y[rt], kf, nf);
         }
       }
-      if (kb >= w / 2) {                           // columns j = tok, over i
+      if (kb >= tt / 2) {                          // columns j = tok, over i
         f32x4 gx[2], nx[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -399,21 +453,18 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
           }
         const Frag<NI> gf = split<NI>(gx[0], gx[1]), nf = split<NI>(nx[0], nx[1]);
 #pragma unroll
-        for (int rt = 0; rt < 2 * RB; ++rt) {
-          kw[rt] = mul(kw[rt], cols_of<RB, NT>(ql, rt, kb), gf);
-          kw[rt] = mul(kw[rt], cols_of<RB, NT>(kl, rt, kb), nf);
+        for (int rt = 0; rt < RT; ++rt) {
+          kw[rt] = mul(kw[rt], cols_of<RB, NT>(ql, rt0 + rt, kb), gf);
+          kw[rt] = mul(kw[rt], cols_of<RB, NT>(kl, rt0 + rt, kb), nf);
         }
       }
     }
-    float qd = 0.f, ky = 0.f, kk = 0.f;
 #pragma unroll
-    for (int rt = 0; rt < 2 * RB; ++rt) {
-      const int f0 = 16 * rt + 4 * gq;
-      const f32x4 kv = live ? load4(krow + f0, g.r - f0, io.kvec) : zero4();
-      const f32x4 qv = live ? load4(qrow + f0, g.r - f0, io.qvec) : zero4();
-      qd += dot4(qv, a[rt]);
-      ky += dot4(kv, y[rt]);
-      kk += dot4(kv, kw[rt]);
+    for (int rt = 0; rt < RT; ++rt) {
+      const int f0 = 16 * (rt0 + rt) + 4 * gq;
+      qd += dot4(load4(qrow + f0, live ? g.r - f0 : 0, io.qvec), a[rt]);
+      ky += dot4(kv[rt], y[rt]);
+      kk += dot4(kv[rt], kw[rt]);
       dQ[rt] += a[rt];
       dK[rt] += b * y[rt] + kw[rt];
     }
@@ -422,29 +473,37 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
     kk = sum_groups(kk);
     kint = sum_groups(kint);
     if (gq == 0) {
-      dLs[tok] = qd + b * ky - kk;
-      inter[tok] = kint;
-      if (live) io.dbeta[(int64_t)s * g.T + t0 + tok] = zv + ky;
+      sums[hf][0][tok] = qd;
+      sums[hf][1][tok] = ky;
+      sums[hf][2][tok] = kk;
+      sums[hf][3][tok] = kint;
     }
     __syncthreads();
     if (w == 0) {
       const int t = lane_id();
-      float x = dLs[t], sum = inter[t];
+      float v4[4];
+#pragma unroll
+      for (int n = 0; n < 4; ++n) v4[n] = H == 2 ? sums[0][n][t] + sums[H - 1][n][t] : sums[0][n][t];
+      float x = v4[0] + bs[t] * v4[1] - v4[2], sum = v4[3], ds = 0.f;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const float up = __shfl_down(x, d);
         if (t + d < 64) x += up;
         sum += __shfl_xor(sum, d);
       }
-      const float* pr = pair[h & 1];
-      sum += vec[3 * C] * (pr[0] + pr[1] + pr[2] + pr[3]);           // <dS', S'>
-      if (t < len) io.dlogA[(int64_t)s * g.T + t0 + t] = x + sum;
+#pragma unroll
+      for (int n = 0; n < W; ++n) ds += pair[n];
+      sum += vec[3 * C] * ds;                      // <dS', S'>
+      if (t < len) {
+        io.dlogA[(int64_t)s * g.T + t0 + t] = x + sum;
+        io.dbeta[(int64_t)s * g.T + t0 + t] = zvs[t] + v4[1];
+      }
     }
   }
   if (!live) return;
 #pragma unroll
-  for (int rt = 0; rt < 2 * RB; ++rt) {
-    const int f0 = 16 * rt + 4 * gq;
+  for (int rt = 0; rt < RT; ++rt) {
+    const int f0 = 16 * (rt0 + rt) + 4 * gq;
     const int64_t at = ((int64_t)ks * g.T + row) * g.r + f0;
     store4((In*)io.dq + at, dQ[rt], g.r - f0, io.ovec);
     store4((In*)io.dk + at, dK[rt], g.r - f0, io.ovec);
@@ -453,13 +512,12 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Geo g, Ops o, GradIO io
 
 template <typename In, int RB, bool OUT>
 static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hipStream_t st) {
-  constexpr int lds = rchain_lds<In, RB>(rchain_bufs<In, RB>());
+  constexpr int lds = rchain_lds<In, RB>(rchain_bufs<In, RB>()), W = rchain_waves<In, RB>();
   static_assert(lds <= kMaxLds, "");
-  const int most = 2 * lds <= kMaxLds ? 4 : 8;
-  const int n = (tiles + most - 1) / most, W = (tiles + n - 1) / n;
   auto kern = delta_rchain_kernel<In, RB, OUT>;
   (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL(kern, dim3(n, g.nruns, g.nb), dim3(64 * W), lds, st, g, o, io, tiles);
+  hipLaunchKernelGGL(kern, dim3((tiles + W - 1) / W, g.nruns, g.nb), dim3(64 * W), lds, st, g, o,
+                     io, tiles);
 }
 
 template <typename In, int RB>
@@ -481,6 +539,7 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   io.d_sb = gr.d_sb;
   io.d_st = gr.d_st;
   io.dv = dv;
+  io.narrow = narrow_stride(gr.d_st);
   io.start = dstate_out;
   io.end = dstate;
   io.ptiles = (g.p + 15) / 16;
@@ -505,11 +564,11 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   gr.save_d = save_d;
   gr.z = z;
   if (g.nch > 0) {
-    constexpr int lds = 4 * Terms<In>::in * tile_elems(RB) + 8 * C * kLd;
-    static_assert(lds + 2048 <= kMaxLds, "");
+    constexpr int lds = grad_lds<In, RB>();
+    static_assert(lds + 4096 <= kMaxLds, "");
     auto kern = delta_grad_kernel<In, RB>;
     (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    hipLaunchKernelGGL(kern, dim3(g.nch, g.nbk), dim3(256), lds, st, g, o, gr);
+    hipLaunchKernelGGL(kern, dim3(g.nch, g.nbk), dim3(256 * grad_split(RB)), lds, st, g, o, gr);
   }
   return launch_status("smat_delta_scan_backward");
 }

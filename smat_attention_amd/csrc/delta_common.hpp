@@ -151,7 +151,11 @@ __device__ __forceinline__ Frag<N> rows_of(const bf16* tile, int mt, int kb) {
   constexpr int RS = row_chunks(RB);
   const int m = lane_id() & 15, g = lane_id() >> 4;
   const int k0 = (4 * kb + (g >> 1)) ^ swz<RS>(m), k1 = (4 * kb + 2 + (g >> 1)) ^ swz<RS>(m);
-  const bf16* p = tile + (16 * mt + m) * RS * 8 + 4 * (g & 1);
+  int at = (16 * mt + m) * RS * 8 + 4 * (g & 1);
+  // odd row tiles take an address the compiler cannot relate to the even ones': fused
+  // into ds_read2st64_b64 the pair would be read at half the rate
+  if (mt & 1) asm("" : "+v"(at));
+  const bf16* p = tile + at;
   Frag<N> f;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
@@ -180,7 +184,7 @@ __device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb) {
       const bf16* a = p + n * tile_elems(RB) + i * 16 * RS * 8;
       h[i] = __builtin_bit_cast(
           bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                      (__attribute__((address_space(3))) short4v*)(uint32_t)(uintptr_t)a));
+                      (__attribute__((address_space(3))) short4v*)(uintptr_t)(uint32_t)(uintptr_t)a));
     }
     f.t[n] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
@@ -194,41 +198,74 @@ struct TileSrc {
   int64_t sb, st;
 };
 
-// A lane's offset that the compiler takes for new: addresses built from it inside a
-// loop are formed there, not kept in registers across it.
-__device__ __forceinline__ int fresh(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-__device__ __forceinline__ int64_t fresh(int64_t x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-// A result tile's column in fp32 rows: p is the wave's (uniform) row 0, off the
-// lane's 4 gq ld + column, rows ld apart.
-__device__ __forceinline__ void put_rows(float* p, int off, int ld, const f32x4& x) {
+// A result tile's rows of fp32: p is the wave's row 0 (uniform), off the lane's bytes
+// to row 4 gq and its column, rows ld floats apart.
+__device__ __forceinline__ void put_rows(float* p, uint32_t off, int ld, const f32x4& x) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) (p + (int64_t)i * ld)[off] = x[i];
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<float*>(reinterpret_cast<char*>(p + (int64_t)i * ld) + off) = x[i];
 }
 __device__ __forceinline__ int uniform_wave() {
   return __builtin_amdgcn_readfirstlane(wave_id());
 }
 
-// Copies of 1 KB a wave into LDS, spread over W waves; they land by the next
-// wait_vmcnt<0>() and barrier.
-__device__ __forceinline__ void stage(void* dst, const void* src, int kb, int w, int W) {
-  for (int u = w; u < kb; u += W)
-    lds_dma16<true>((const char*)src + u * 1024 + lane_id() * 16, (char*)dst + u * 1024);
+// One copy of 16 bytes a lane into LDS, as lds_dma16<true>, from a uniform address
+// and a lane's byte offset: no vector address arithmetic.
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, const void* dst) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
+  uint32_t keep;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(keep)
+      : "v"(off), "s"(base), "s"(m0)
+      : "memory");
 }
-template <int RB, int N>
-__device__ __forceinline__ void stage_tile(bf16* dst, const TileSrc& src, int64_t ks, int64_t nch,
-                                           int c, int t0, int len, int r, const float* vec, int w,
-                                           int W) {
-  constexpr int RS = row_chunks(RB);
-  if (N > 1 || src.ws) {
-    stage(dst, src.ws + (ks * nch + c) * (int64_t)N * tile_elems(RB), N * RS, w, W);
-  } else {
+
+// Copies of 1 KB a wave into LDS, spread over W waves (w is this one, uniform); they
+// land by the next wait_vmcnt<0>() and barrier.
+template <int KB, int W>
+__device__ __forceinline__ void stage(void* dst, const void* src, int w) {
+#pragma unroll
+  for (int u = 0; u < (KB + W - 1) / W; ++u)
+    if (KB % W == 0 || u * W + w < KB)
+      dma16((const char*)src + (u * W + w) * 1024, lane_id() * 16, (char*)dst + (u * W + w) * 1024);
+}
+
+// Between the products of a wide state, where more operands in flight than the next
+// product needs would cost spills.
+template <int RB> __device__ __forceinline__ void narrow_schedule() {
+  if constexpr (RB >= 3) __builtin_amdgcn_sched_barrier(0);
+}
+
+// A key sequence's tile of chunk c.  Wave w's copies are rows 16 W / .. apart, whole
+// turns of the swizzle, so one lane offset serves all of a full chunk's.
+template <int RB, int N, int W> struct TileStage {
+  static constexpr int RS = row_chunks(RB), RPU = 64 / RS;      // rows a copy
+  static_assert((RPU * W) % 16 == 0, "");
+  uint32_t off;
+  bool fast;               // full rows, and offsets within 32 bits
+
+  __device__ __forceinline__ TileStage(const TileSrc& src, int r, int w) {
+    const int t = w * RPU + lane_id() / RS, k = (lane_id() % RS) ^ swz<RS>(t);
+    fast = N == 1 && r == 8 * RS && src.st >= 0 && src.st < (1 << 24);
+    off = fast ? (uint32_t)((t * src.st + 8 * k) * 2) : 0;
+  }
+  __device__ __forceinline__ void operator()(bf16* dst, const TileSrc& src, int64_t ks,
+                                             int64_t nch, int c, int t0, int len, int r,
+                                             const float* vec, int w) const {
+    if (N > 1 || src.ws) {
+      stage<N * RS, W>(dst, src.ws + (ks * nch + c) * (int64_t)N * tile_elems(RB), w);
+      return;
+    }
     const bf16* base = src.raw + ks * src.sb + (int64_t)t0 * src.st;
+    if (fast && len == C) {
+#pragma unroll
+      for (int u = 0; u < (RS + W - 1) / W; ++u)
+        if (RS % W == 0 || u * W + w < RS)
+          dma16(base + (int64_t)(u * W * RPU) * src.st, off, dst + (u * W + w) * 512);
+      return;
+    }
     for (int u = w; u < RS; u += W) {
       const int l = u * 64 + lane_id(), t = l / RS, k = (l % RS) ^ swz<RS>(t);
       const void* p = t < len && 8 * k < r ? (const void*)(base + (int64_t)t * src.st + 8 * k)
@@ -236,7 +273,42 @@ __device__ __forceinline__ void stage_tile(bf16* dst, const TileSrc& src, int64_
       lds_dma16<true>(p, dst + u * 512);
     }
   }
+};
+
+// A chunk's 64 values of a column in result-tile order: element j is token
+// 16 (j >> 2) + 4 gq + (j & 3).  Absent tokens, and all if !live, are zero.
+template <typename In>
+__device__ __forceinline__ void load_column(In* v, const In* rows, int64_t st, bool narrow,
+                                            int64_t t0, int len, int col, bool live, bool any) {
+  const int gq = lane_id() >> 4;
+  if (!any) {                                      // uniform: nothing here for the whole wave
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = from_f32<In>(0.f);
+    return;
+  }
+  const In* p = rows + t0 * st;
+  if (narrow && len == C) {
+    const uint32_t off = (uint32_t)((4 * gq * (uint32_t)st + (live ? col : 0)) * sizeof(In));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      v[j] = *reinterpret_cast<const In*>(reinterpret_cast<const char*>(p) + off);
+      p += (j & 3) == 3 ? 13 * st : st;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int t = 16 * (j >> 2) + 4 * gq + (j & 3);
+      v[j] = live && t < len ? p[(int64_t)t * st + col] : from_f32<In>(0.f);
+    }
+  }
 }
+// (a dead lane of a live wave read column 0)
+template <typename In>
+__device__ __forceinline__ void column_values(f32x4* x, const In* v, bool live) {
+#pragma unroll
+  for (int j = 0; j < 16; ++j) x[j >> 2][j & 3] = live ? to_f32(v[j]) : 0.f;
+}
+inline bool narrow_stride(int64_t st) { return st >= 0 && st < (1 << 24); }
 
 // Four consecutive elements; those at and past nv are zero.
 template <typename In>

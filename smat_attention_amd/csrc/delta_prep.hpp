@@ -90,8 +90,8 @@ __device__ __forceinline__ void unit_lower_inverse(const float* Am, float* Tm) {
   __syncthreads();
 }
 
-// Running sum of the chunk's logA in fp64 into Ls (wave 0), beta into bs.  Tokens
-// past the chunk's end count as logA = 0, beta = 0.
+// Running sum of the chunk's logA in fp64, in units of log 2, into Ls (wave 0), beta
+// into bs.  Tokens past the chunk's end count as logA = 0, beta = 0.
 __device__ __forceinline__ void chunk_decays(const Geo& g, const float* logA, const float* beta,
                                              int s, int t0, int len, double* Ls, float* bs) {
   const int t = threadIdx.x;
@@ -100,7 +100,7 @@ __device__ __forceinline__ void chunk_decays(const Geo& g, const float* logA, co
     double x = 0.0;
     if (ok) {
       const float a = logA[s * g.a_sb + (int64_t)(t0 + t) * g.a_st];
-      x = a < -1e5f ? -1e5 : (double)a;          // NaN stays NaN
+      x = (a < -1e5f ? -1e5 : (double)a) * 1.4426950408889634;   // NaN stays NaN
     }
     bs[t] = ok ? beta[s * g.b_sb + (int64_t)(t0 + t) * g.b_st] : 0.f;
 #pragma unroll
@@ -111,13 +111,37 @@ __device__ __forceinline__ void chunk_decays(const Geo& g, const float* logA, co
     Ls[t] = x;
   }
 }
+// 2^x of a difference of them: v_exp_f32, within an ulp and zero below 2^-126.
+__device__ __forceinline__ float decay(double x) { return __builtin_amdgcn_exp2f((float)x); }
 
-// The eight values (slots of contraction block kb) of token row m as terms.
+// The eight values (slots of contraction block kb) of token row m as terms.  Rows that
+// are read whole (a full bf16 chunk of 32 RB features) skip the checks.
 template <typename In, int N>
 __device__ __forceinline__ Frag<N> row_frag(const In* row, bool ok, int c0, int r, bool vec) {
   const f32x4 a = ok ? load4(row + c0, r - c0, vec) : zero4();
   const f32x4 b = ok ? load4(row + c0 + 16, r - c0 - 16, vec) : zero4();
   return split<N>(a, b);
+}
+__device__ __forceinline__ Frag<1> whole_frag(const bf16* row, int c0) {
+  const bf16x4 a = *reinterpret_cast<const bf16x4*>(row + c0);
+  const bf16x4 b = *reinterpret_cast<const bf16x4*>(row + c0 + 16);
+  Frag<1> f;
+  f.t[0] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  return f;
+}
+template <typename In, int RB, int N>
+__device__ __forceinline__ void row_frags(Frag<N>* f, const In* row, bool ok, int r, bool vec,
+                                          int len) {
+  const int gq = lane_id() >> 4;
+  if constexpr (__is_same(In, bf16)) {
+    if (vec && len == C && r == 32 * RB) {
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) f[kb] = whole_frag(row, 32 * kb + 4 * gq);
+      return;
+    }
+  }
+#pragma unroll
+  for (int kb = 0; kb < RB; ++kb) f[kb] = row_frag<In, N>(row, ok, 32 * kb + 4 * gq, r, vec);
 }
 
 // A token's slots of contraction block kb into its row of a tile (a tile a term).
@@ -137,134 +161,153 @@ __device__ __forceinline__ void store_row(bf16* tile, int t, int kb, const Frag<
     }
 }
 
+// LDS: the row fragments of K (BWD: then of Q), with T's tile in their place once they
+// are read, and A's tile.
+template <typename In, int RB, bool BWD> constexpr int prep_rows() {
+  constexpr int rows = Terms<In>::in * 4 * RB * kFrag * 2;
+  return BWD || rows < C * kLd * 4 ? (BWD ? rows + C * kLd * 4 : C * kLd * 4) : rows;
+}
+
 template <typename In, int RB, bool BWD>
 __global__ __launch_bounds__(256) void delta_prep_kernel(
     const In* __restrict__ q, const In* __restrict__ k, const float* __restrict__ logA,
     const float* __restrict__ beta, Geo g, Ops o, bool qvec, bool kvec) {
   constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid;
   constexpr int KB = 4 * RB * kFrag;               // elements of one term of a chunk's rows
-  __shared__ __align__(16) bf16 rows[NT * KB];
-  __shared__ __align__(16) float Am[C * kLd], Tm[C * kLd];
+  __shared__ __align__(16) char mem[prep_rows<In, RB, BWD>()];
+  __shared__ __align__(16) float Am[C * kLd];
   __shared__ double Ls[C];
   __shared__ float bs[C];
+  bf16* rows = reinterpret_cast<bf16*>(mem);
+  float* Tm = reinterpret_cast<float*>(mem + (BWD ? NT * KB * 2 : 0));
   const int c = blockIdx.x, s = blockIdx.y;
-  const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
+  const int w = uniform_wave(), m = lane_id() & 15, gq = lane_id() >> 4;
   int t0, len;
   chunk_of(g, c, t0, len);
   const int64_t ks = key_of(g, s);
   const bool tiles = o.kw && s % (g.nb / g.nbk) == 0;   // this workgroup stores K's and Q's tiles
-  chunk_decays(g, logA, beta, s, t0, len, Ls, bs);
-
   const int tok = 16 * w + m;
   const bool live = tok < len;
   const In* krow = k + ks * g.k_sb + (int64_t)(t0 + (live ? tok : 0)) * g.k_st;
   const In* qrow = q + ks * g.q_sb + (int64_t)(t0 + (live ? tok : 0)) * g.q_st;
   const int64_t kc = (ks * g.nch + c) * (int64_t)NT * tile_elems(RB), sc = (int64_t)s * g.nch + c;
   Frag<NT> kf[RB], qf[RB];
+  row_frags<In, RB, NT>(kf, krow, live, g.r, kvec, len);
+  row_frags<In, RB, NT>(qf, qrow, live, g.r, qvec, len);
+  chunk_decays(g, logA, beta, s, t0, len, Ls, bs);
 #pragma unroll
-  for (int kb = 0; kb < RB; ++kb) {
-    kf[kb] = row_frag<In, NT>(krow, live, 32 * kb + 4 * gq, g.r, kvec);
-    qf[kb] = row_frag<In, NT>(qrow, live, 32 * kb + 4 * gq, g.r, qvec);
-    store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, kf[kb]);
-    if (tiles) {
+  for (int kb = 0; kb < RB; ++kb) store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, kf[kb]);
+  if (tiles) {
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) {
       store_row<RB, NT>(o.kw + kc, tok, kb, kf[kb]);
       store_row<RB, NT>(o.qw + kc, tok, kb, qf[kb]);
     }
   }
   __syncthreads();
-  // A = b D K K^T below the diagonal: column j in the lane, rows 16 w + 4 gq + i
+  const double Lt = Ls[tok];
   f32x4 pacc[4];
 #pragma unroll
-  for (int jt = 0; jt < 4; ++jt) {
-    f32x4 a = zero4();
-    pacc[jt] = zero4();
-    if (jt <= w) {
-#pragma unroll
-      for (int kb = 0; kb < RB; ++kb) {
-        const Frag<NT> kj = load_frag<NT>(rows + (jt * RB + kb) * kFrag, KB);
-        a = mul(a, kf[kb], kj);
-        if (!BWD) pacc[jt] = mul(pacc[jt], kj, qf[kb]);   // token i in the lane, rows j
-      }
-    }
-    const int j = 16 * jt + m;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int ti = 16 * w + 4 * gq + i;
-      Am[ti * kLd + j] = j < ti ? bs[ti] * (expf((float)(Ls[ti] - Ls[j])) * a[i]) : 0.f;
-    }
-  }
+  for (int t = 0; t < 4; ++t) pacc[t] = zero4();
   if (!BWD) {
-    // P by rows: lane holds token i = 16 w + m, tile jt's rows j = 16 jt + 4 gq + i
-    const double Li = Ls[tok];
+    // token i = 16 w + m in the lane, tile jt's rows j = 16 jt + 4 gq + i in registers: A
+    // below the diagonal (row i of it in vectors) and P by rows from one set of decays
+    const float b = bs[tok];
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt)
+      if (jt <= w) {
+        f32x4 a = zero4(), P = zero4();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = 16 * jt + 4 * gq + i;
-        pacc[jt][i] = j <= tok ? g.scale * (expf((float)(Li - Ls[j])) * pacc[jt][i]) : 0.f;
+        for (int kb = 0; kb < RB; ++kb) {
+          const Frag<NT> kj = load_frag<NT>(rows + (jt * RB + kb) * kFrag, KB);
+          a = mul(a, kj, kf[kb]);
+          P = mul(P, kj, qf[kb]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = 16 * jt + 4 * gq + i;
+          const float D = decay(Lt - Ls[j]);
+          a[i] = j < tok ? b * (D * a[i]) : 0.f;
+          pacc[jt][i] = j <= tok ? g.scale * (D * P[i]) : 0.f;
+        }
+        *reinterpret_cast<f32x4*>(Am + tok * kLd + 16 * jt + 4 * gq) = a;
       }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
       if (kb <= w / 2)
         store_frag<NO>(o.pm + (sc * NO * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
                        split<NO>(pacc[2 * kb], pacc[2 * kb + 1]));
-  }
-  __syncthreads();                                 // Am whole; rows free
-  if (BWD) {
+    __syncthreads();                               // Am whole; the rows are read
+  } else {
+    // token j = 16 w + m in the lane, rows i = 16 it + 4 gq + .. in registers: the same
+    // decays serve column j of A and of P, whose queries come through LDS
+    f32x4 D[4];
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+      if (it >= w) {
+        f32x4 a = zero4();
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb)
+          a = mul(a, load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int ti = 16 * it + 4 * gq + i;
+          D[it][i] = tok <= ti ? decay(Ls[ti] - Lt) : 0.f;
+          Am[ti * kLd + tok] = tok < ti ? bs[ti] * (D[it][i] * a[i]) : 0.f;
+        }
+      }
+    __syncthreads();                               // Am whole; K's rows are read
 #pragma unroll
     for (int kb = 0; kb < RB; ++kb) store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, qf[kb]);
-  }
-  unit_lower_inverse(Am, Tm);
-  if (BWD) {
-    // P^T: lane holds token j = 16 w + m, rows i = 16 it + 4 gq + ..
-    const double Lj = Ls[tok];
+    __syncthreads();
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
+    for (int it = 0; it < 4; ++it)
       if (it >= w) {
 #pragma unroll
         for (int kb = 0; kb < RB; ++kb)
           pacc[it] = mul(pacc[it], load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
-      }
+        // selected, not multiplied: a query that is not finite stays in its own row
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ti = 16 * it + 4 * gq + i;
-        pacc[it][i] = tok <= ti ? g.scale * (expf((float)(Ls[ti] - Lj)) * pacc[it][i]) : 0.f;
+        for (int i = 0; i < 4; ++i)
+          pacc[it][i] = tok <= 16 * it + 4 * gq + i ? g.scale * (D[it][i] * pacc[it][i]) : 0.f;
       }
-    }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
-      if (kb >= w / 2) {
+      if (kb >= w / 2)
         store_frag<NI>(o.pt + (sc * NI * kTri + tri_t(w, kb)) * kFrag, kTri * kFrag,
                        split<NI>(pacc[2 * kb], pacc[2 * kb + 1]));
-        f32x4 x[2];
+  }
+  unit_lower_inverse(Am, Tm);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+  for (int kb = 0; kb < 2; ++kb) {
+    if (BWD && kb >= w / 2) {
+      f32x4 x[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int ti = 32 * kb + 16 * h + 4 * gq + i;
-            x[h][i] = ti >= 16 * w ? Tm[ti * kLd + tok] : 0.f;
-          }
-        store_frag<NI>(o.tt + (sc * NI * kTri + tri_t(w, kb)) * kFrag, kTri * kFrag,
-                       split<NI>(x[0], x[1]));
-      }
-  } else {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-      if (kb <= w / 2) {
-        const float* row = Tm + tok * kLd + 32 * kb + 4 * gq;
-        const f32x4 x0 = *reinterpret_cast<const f32x4*>(row);
-        const f32x4 x1 = 2 * kb + 1 <= w ? *reinterpret_cast<const f32x4*>(row + 16) : zero4();
-        store_frag<NI>(o.tm + (sc * NI * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
-                       split<NI>(x0, x1));
-      }
+        for (int i = 0; i < 4; ++i) {
+          const int ti = 32 * kb + 16 * h + 4 * gq + i;
+          x[h][i] = ti >= 16 * w ? Tm[ti * kLd + tok] : 0.f;
+        }
+      store_frag<NI>(o.tt + (sc * NI * kTri + tri_t(w, kb)) * kFrag, kTri * kFrag,
+                     split<NI>(x[0], x[1]));
+    }
+    if (!BWD && kb <= w / 2) {
+      const float* row = Tm + tok * kLd + 32 * kb + 4 * gq;
+      const f32x4 x0 = *reinterpret_cast<const f32x4*>(row);
+      const f32x4 x1 = 2 * kb + 1 <= w ? *reinterpret_cast<const f32x4*>(row + 16) : zero4();
+      store_frag<NI>(o.tm + (sc * NI * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
+                     split<NI>(x0, x1));
+    }
   }
   if (threadIdx.x < C) {
     const int t = threadIdx.x;
     float* v = o.vec + sc * kVec;
-    v[t] = expf((float)Ls[t]);
-    v[C + t] = expf((float)(Ls[C - 1] - Ls[t]));
+    const double Lc = Ls[C - 1];
+    v[t] = decay(Ls[t]);
+    v[C + t] = decay(Lc - Ls[t]);
     v[2 * C + t] = bs[t];
-    v[3 * C + t] = t == 0 ? expf((float)Ls[C - 1]) : 0.f;
+    v[3 * C + t] = t == 0 ? decay(Lc) : 0.f;
   }
 }
 
