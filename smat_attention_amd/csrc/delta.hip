@@ -25,8 +25,9 @@ struct ChainIO {
   const void* v;
   void* o;
   const float* start;     // state entering run i of sequence s: start + (i nb + s) r p; or null
-  float* end;             // state leaving it, same layout; or null
-  float* trans;           // first pass: M of run i, (i nb + s) R R row-major (R = 32 RB); or null
+  float* end;             // first pass: the state leaving it, same layout
+  float* trans;           // first pass: M of run i, (i nb + s) R R row-major (R = 32 RB)
+  float* fin;             // state leaving segment j: fin + (j nb + s) r p; or null
   float *save_s, *save_u; // training: states entering chunks, and U, rows padded to p32; or null
   int ptiles;             // value tiles of 16 columns (tiles behind them are M's)
   bool narrow, ovec;      // v's rows lie within 32-bit offsets; out in groups of four
@@ -65,7 +66,9 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
   const int run = blockIdx.y, s = blockIdx.z;
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
-  run_of(g, run, c0, c1, seg);
+  bool head, tail;
+  run_of(g, run, c0, c1, seg, head, tail);
+  if (!OUT && tail) return;                        // nothing is carried past a segment's last run
   const bool values = ct < io.ptiles;              // else columns of the transition
   const int col = 16 * (values ? ct : ct - io.ptiles) + m;
   const int64_t ks = key_of(g, s);
@@ -110,12 +113,16 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     stage_k(c0, t0, len, 0);
     stage_qt(c0, t0, len);
   }
+  Frag<NI> sb[RB];                                 // S as the next products' operand
+#pragma unroll
+  for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
   for (int c = c0; c < c1; ++c) {
     const int buf = KD == 2 ? (c - c0) & 1 : 0;
     const bool more = c + 1 < c1;
     const int64_t sc = (int64_t)s * g.nch + c;
     const bf16* kt = kl + buf * TL;
     const float* vec = vl + buf * kVec;
+    const int lane = fresh_lane(), fm = lane & 15, f4 = 4 * (lane >> 4);
     if (more) chunk_of(g, c + 1, t1, len1);
     wait_vmcnt<0>();
     lds_barrier();
@@ -135,33 +142,26 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
         for (int mt = 0; mt < 2 * RB; ++mt)
           put_rows(io.save_s + (sc * R + 16 * mt) * ld, soff, ld, S[mt]);
       }
-      Frag<NI> sb[RB];
+      // K S, and Q S transposed (columns in registers, token in the lane)
+      f32x4 ks4[4];
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-      narrow_schedule<RB>();
+      for (int mt = 0; mt < 4; ++mt) ks4[mt] = ot[mt] = zero4();
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb)
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          ks4[mt] = mul(ks4[mt], rows_of<RB, NT>(kt, mt, kb, lane), sb[kb]);
+          if (OUT) ot[mt] = mul(ot[mt], lead<NO>(sb[kb]), rows_of<RB, NT>(ql, mt, kb, lane));
+        }
       // b (V - e K S)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        f32x4 a = zero4();
+        const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + f4);
+        const f32x4 b = *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + f4);
 #pragma unroll
-        for (int kb = 0; kb < RB; ++kb) a = mul(a, rows_of<RB, NT>(kt, mt, kb), sb[kb]);
-        const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
-        const f32x4 b = *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[mt][i] = b[i] * (x[mt][i] - e[i] * a[i]);
+        for (int i = 0; i < 4; ++i) x[mt][i] = b[i] * (x[mt][i] - e[i] * ks4[mt][i]);
+        if (OUT) ot[mt] *= g.scale * vec[16 * mt + fm];
       }
-      narrow_schedule<RB>();
-      if (OUT) {
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {           // columns in registers, token in the lane
-          ot[mt] = zero4();
-#pragma unroll
-          for (int kb = 0; kb < RB; ++kb)
-            ot[mt] = mul(ot[mt], lead<NO>(sb[kb]), rows_of<RB, NT>(ql, mt, kb));
-          ot[mt] *= g.scale * vec[16 * mt + m];
-        }
-      }
-      narrow_schedule<RB>();
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
@@ -169,7 +169,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
         x[mt] = zero4();
 #pragma unroll
         for (int kb = 0; kb <= mt / 2; ++kb)
-          x[mt] = mul(x[mt], load_frag<NI>(tl + tri(mt, kb) * kFrag, TB), f[kb]);
+          x[mt] = mul(x[mt], load_frag<NI>(tl + tri(mt, kb) * kFrag, TB, lane), f[kb]);
       }
     }
     wait_vmcnt<0>();
@@ -180,40 +180,45 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
       stage_qt(c + 1, t1, len1);
     }
     if (on) {
-      if (OUT) {
-        if (io.save_u) {
+      if (OUT && io.save_u) {
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt)
-            put_rows(io.save_u + (sc * C + 16 * mt) * ld, soff, ld, x[mt]);
-        }
-        Frag<NO> fo[2];
-        const uint32_t ooff = (m * g.p + 4 * gq) * sizeof(In);
-        const int left = g.p - 16 * ct - 4 * gq;
+        for (int mt = 0; mt < 4; ++mt)
+          put_rows(io.save_u + (sc * C + 16 * mt) * ld, soff, ld, x[mt]);
+      }
+      Frag<NO> fo[2];
+      if (OUT) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NO>(x[2 * kb], x[2 * kb + 1]);
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+        x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + f4);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+      if (OUT) {
+        const uint32_t ooff = (fm * g.p + f4) * sizeof(In);
+        const int left = g.p - 16 * ct - f4;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
 #pragma unroll
           for (int kb = 0; kb <= mt / 2; ++kb)
-            ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pl + tri(mt, kb) * kFrag, TB));
+            ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pl + tri(mt, kb) * kFrag, TB, lane));
           In* row = (In*)io.o + ((int64_t)s * g.T + t0 + 16 * mt) * g.p + 16 * ct;
-          if (16 * mt + m < len && left > 0)
+          if (16 * mt + fm < len && left > 0)
             store4(reinterpret_cast<In*>(reinterpret_cast<char*>(row) + ooff), ot[mt],
                    io.ovec ? 4 : left, io.ovec);
         }
       }
-      narrow_schedule<RB>();
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-        x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
       const float aC = vec[3 * C];
 #pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt) {
-        S[mt] *= aC;
+      for (int sk = 0; sk < RB; ++sk) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb), f[kb]);
+        for (int mt = 2 * sk; mt < 2 * sk + 2; ++mt) {
+          S[mt] *= aC;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb, lane), f[kb]);
+        }
+        sb[sk] = split<NI>(S[2 * sk], S[2 * sk + 1]);
       }
     }
     if (KD == 1 && more) {
@@ -224,7 +229,9 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     len = len1;
   }
   if (!on) return;
-  if (values ? io.end != nullptr : io.trans != nullptr) {
+  float* out = OUT ? (io.fin && tail ? io.fin + ((int64_t)seg * g.nb + s) * rp : nullptr)
+                   : io.end + sn * rp;
+  if (values ? out != nullptr : true) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
@@ -233,22 +240,21 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
         if (!values)
           io.trans[(sn * R + a) * R + col] = S[mt][i];
         else if (a < g.r && col < g.p)
-          io.end[sn * rp + (int64_t)a * g.p + col] = S[mt][i];
+          out[(int64_t)a * g.p + col] = S[mt][i];
       }
   }
 }
 
-// The states across the runs of a segment: entering run i (start), S <- M_i S + E_i,
-// and out of the last (fin).  A wave 16 columns, four waves a workgroup; `rev` walks
-// the runs backwards (the gradient's direction).  A step waits on the last one, so
+// The states entering the runs of a segment (start): S <- M_i S + E_i past each but
+// the last.  A wave 16 columns, four waves a workgroup; `rev` walks the runs
+// backwards (the gradient's direction).  A step waits on the last one, so
 // what does not depend on it is done ahead: the next M and E are loaded while a step
 // computes, and the waves split M into terms once, in LDS, for each other.
 template <int RB>
 __global__ __launch_bounds__(256) void delta_carry_kernel(Geo g, const float* __restrict__ init,
                                                           const float* __restrict__ E,
                                                           const float* __restrict__ M,
-                                                          float* __restrict__ start,
-                                                          float* __restrict__ fin, bool rev) {
+                                                          float* __restrict__ start, bool rev) {
   constexpr int R = 32 * RB, NI = kMid, NF = 2 * RB * RB, PER = (NF + 3) / 4;
   extern __shared__ __align__(1024) bf16 lds[];    // NF fragments, a plane a term
   const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
@@ -290,11 +296,11 @@ __global__ __launch_bounds__(256) void delta_carry_kernel(Geo g, const float* __
   for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = zero4();
   const int64_t ss = ((int64_t)seg * g.nb + s) * rp;
   if (init) load_cols(S, init + ss);
-  if (r0 < r1) {
+  if (r0 + 1 < r1) {
     load_m(r0);
     load_cols(e, E + at(r0) * rp);
   }
-  for (int n = r0; n < r1; ++n) {
+  for (int n = r0; n + 1 < r1; ++n) {
     __syncthreads();                               // the last step's fragments are read
 #pragma unroll
     for (int u = 0; u < PER; ++u)
@@ -306,7 +312,7 @@ __global__ __launch_bounds__(256) void delta_carry_kernel(Geo g, const float* __
     for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = e[mt];
-    if (n + 1 < r1) {
+    if (n + 2 < r1) {
       load_m(n + 1);
       load_cols(e, E + at(n + 1) * rp);
     }
@@ -317,7 +323,7 @@ __global__ __launch_bounds__(256) void delta_carry_kernel(Geo g, const float* __
       for (int kb = 0; kb < RB; ++kb)
         S[mt] = mul(S[mt], load_frag<NI>(lds + (mt * RB + kb) * kFrag, NF * kFrag), sb[kb]);
   }
-  if (fin) store_cols(fin + ss, S);
+  if (r0 < r1) store_cols(start + at(r1 - 1) * rp, S);
 }
 
 int check_geo(const char* who, int dtype, const Geo& g) {
@@ -346,22 +352,21 @@ int check_geo(const char* who, int dtype, const Geo& g) {
 }
 
 template <int RB>
-static void carry_kernel(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
+static void carry_kernel(const Geo& g, const float* init, const Carry& c, bool rev,
                          hipStream_t st) {
   constexpr int lds = 2 * RB * RB * kMid * kFrag * 2;
   auto kern = delta_carry_kernel<RB>;
   (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   hipLaunchKernelGGL(kern, dim3((g.p + 63) / 64, g.nseg, g.nb), dim3(256), lds, st, g, init, c.E,
-                     c.M, c.start, fin, rev);
+                     c.M, c.start, rev);
 }
 
-int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
-                 hipStream_t st) {
+int launch_carry(const Geo& g, const float* init, const Carry& c, bool rev, hipStream_t st) {
   switch (rblocks(g.r)) {
-    case 1: carry_kernel<1>(g, init, c, fin, rev, st); break;
-    case 2: carry_kernel<2>(g, init, c, fin, rev, st); break;
-    case 3: carry_kernel<3>(g, init, c, fin, rev, st); break;
-    default: carry_kernel<4>(g, init, c, fin, rev, st); break;
+    case 1: carry_kernel<1>(g, init, c, rev, st); break;
+    case 2: carry_kernel<2>(g, init, c, rev, st); break;
+    case 3: carry_kernel<3>(g, init, c, rev, st); break;
+    default: carry_kernel<4>(g, init, c, rev, st); break;
   }
   return launch_status("smat_delta_scan: carry");
 }
@@ -392,7 +397,7 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
   io.v = v;
   io.o = out;
   io.start = state;
-  io.end = state_out;
+  io.fin = state_out;
   io.ovec = vec4_ok(out, 0, g.p, eb);
   io.narrow = narrow_stride(g.v_st);
   io.ptiles = (g.p + 15) / 16;
@@ -404,10 +409,9 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
     first.end = c.E;
     first.trans = c.M;
     chain<In, RB, false>(g, o, first, io.ptiles + 2 * RB, st);
-    const int rc = launch_carry(g, state, c, state_out, false, st);
+    const int rc = launch_carry(g, state, c, false, st);
     if (rc) return rc;
     io.start = c.start;
-    io.end = nullptr;
   }
   io.save_s = save_s;
   io.save_u = save_u;
@@ -422,8 +426,8 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 extern "C" int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p) {
   // waves that whole segments give, were they all as long as the longest
   const int64_t work = (int64_t)nb * ((p + 15) / 16) * nch;       // chunk steps
-  if (longest < 32 || work >= (int64_t)512 * longest) return longest > 0 ? longest : 1;
-  const int64_t K = (work + 1023) / 1024;
+  if (longest < 32 || work >= (int64_t)1024 * longest) return longest > 0 ? longest : 1;
+  const int64_t K = (work + 2047) / 2048;
   return (int)(K < 8 ? 8 : K < longest ? K : longest);
 }
 

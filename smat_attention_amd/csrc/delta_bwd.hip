@@ -28,8 +28,9 @@ struct RChainIO {
   const void* dout;       // (nb, T, p), strides d_sb, d_st
   int64_t d_sb, d_st;
   const float* start;     // dS behind run i of sequence s: start + (i nb + s) r p; or null
-  float* end;             // dS before it, same layout; or null
-  float* trans;           // first pass: the run's transition; or null
+  float* end;             // first pass: dS before it, same layout
+  float* trans;           // first pass: the run's transition
+  float* fin;             // dS before segment j: fin + (j nb + s) r p; or null
   float *save_d, *z;      // dS' of every chunk (R x p32) and Z (64 x p32)
   void* dv;               // (nb, T, p) contiguous
   int ptiles;
@@ -66,7 +67,9 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
   const int run = blockIdx.y, s = blockIdx.z;
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
-  run_of(g, run, c0, c1, seg);
+  bool head, tail;
+  run_of(g, run, c0, c1, seg, head, tail);
+  if (!OUT && head) return;                        // nothing is carried past a segment's first run
   const bool values = ct < io.ptiles;
   const int col = 16 * (values ? ct : ct - io.ptiles) + m;
   const int64_t ks = key_of(g, s);
@@ -112,52 +115,52 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
     stage_k(c1 - 1, t0, len, 0);
     stage_tp(c1 - 1);
   }
+  Frag<NI> sb[RB];                                 // dS as the next products' operand
+#pragma unroll
+  for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
   for (int c = c1 - 1; c >= c0; --c) {
     const int buf = KD == 2 ? (c1 - 1 - c) & 1 : 0;
     const bool more = c > c0;
     const int64_t sc = (int64_t)s * g.nch + c;
     const bf16* kt = kl + buf * TL;
     const float* vec = vl + buf * kVec;
+    const int lane = fresh_lane(), f4 = 4 * (lane >> 4);
     if (more) chunk_of(g, c - 1, t1, len1);
     wait_vmcnt<0>();
     lds_barrier();
     // ---- K, T^T, P^T and the factors of chunk c are in LDS
     f32x4 d[4], x[4];
-    Frag<NT> df[2];
     column_values(d, dv, dlive);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(d[mt]));   // their wait is here
     qstage(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
     if (KD == 2 && more) stage_k(c - 1, t1, len1, 1 - buf);
+    Frag<NI> f[2];
     if (on) {
       if (OUT) {
 #pragma unroll
         for (int mt = 0; mt < 2 * RB; ++mt)
           put_rows(io.save_d + (sc * R + 16 * mt) * ld, soff, ld, S[mt]);
       }
-      Frag<NI> f[2];
-      {
-        Frag<NI> sb[RB];
 #pragma unroll
-        for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-        narrow_schedule<RB>();
+      for (int mt = 0; mt < 4; ++mt) x[mt] = zero4();                // dU
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {           // dU
-          x[mt] = zero4();
+      for (int kb = 0; kb < RB; ++kb)
 #pragma unroll
-          for (int kb = 0; kb < RB; ++kb) x[mt] = mul(x[mt], rows_of<RB, NT>(kt, mt, kb), sb[kb]);
-          x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + 4 * gq);
-        }
-      }
-      narrow_schedule<RB>();
+        for (int mt = 0; mt < 4; ++mt)
+          x[mt] = mul(x[mt], rows_of<RB, NT>(kt, mt, kb, lane), sb[kb]);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+        x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + f4);
       if (values) {
+        Frag<NT> df[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
           for (int kb = mt / 2; kb < 2; ++kb)
-            x[mt] = mul(x[mt], load_frag<NI>(pl + tri_t(mt, kb) * kFrag, TB), df[kb]);
+            x[mt] = mul(x[mt], load_frag<NI>(pl + tri_t(mt, kb) * kFrag, TB, lane), df[kb]);
       }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
@@ -166,7 +169,7 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
         x[mt] = zero4();
 #pragma unroll
         for (int kb = mt / 2; kb < 2; ++kb)
-          x[mt] = mul(x[mt], load_frag<NI>(tl + tri_t(mt, kb) * kFrag, TB), f[kb]);
+          x[mt] = mul(x[mt], load_frag<NI>(tl + tri_t(mt, kb) * kFrag, TB, lane), f[kb]);
       }
     }
     wait_vmcnt<0>();
@@ -181,16 +184,17 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) put_rows(io.z + (sc * C + 16 * mt) * ld, soff, ld, x[mt]);
       }
-      const uint32_t voff = (4 * gq * g.p + col) * sizeof(In);
+      const uint32_t voff = (f4 * g.p + col) * sizeof(In);
+      Frag<NI> fd[2];
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + 4 * gq);
-        x[mt] *= *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + 4 * gq);     // b Z
+        const f32x4 e = *reinterpret_cast<const f32x4*>(vec + 16 * mt + f4);
+        x[mt] *= *reinterpret_cast<const f32x4*>(vec + 2 * C + 16 * mt + f4);     // b Z
         if (OUT && dlive) {
           In* row = (In*)io.dv + ((int64_t)s * g.T + t0 + 16 * mt) * g.p;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (len == C || 16 * mt + 4 * gq + i < len)
+            if (len == C || 16 * mt + f4 + i < len)
               *reinterpret_cast<In*>(reinterpret_cast<char*>(row + (int64_t)i * g.p) + voff) =
                   from_f32<In>(x[mt][i]);
         }
@@ -198,24 +202,26 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
         d[mt] *= g.scale * e;
       }
       const float aC = vec[3 * C];
-      Frag<NI> f[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-      narrow_schedule<RB>();
-#pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt) {
-        S[mt] *= aC;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb), f[kb]);
-      }
-      narrow_schedule<RB>();
       if (values) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
+        for (int kb = 0; kb < 2; ++kb) fd[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
+      }
 #pragma unroll
-        for (int mt = 0; mt < 2 * RB; ++mt)
+      for (int sk = 0; sk < RB; ++sk) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(ql, mt, kb), f[kb]);
+        for (int mt = 2 * sk; mt < 2 * sk + 2; ++mt) {
+          S[mt] *= aC;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb, lane), f[kb]);
+          if (values) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+              S[mt] = mul(S[mt], cols_of<RB, NT>(ql, mt, kb, lane), fd[kb]);
+          }
+        }
+        sb[sk] = split<NI>(S[2 * sk], S[2 * sk + 1]);
       }
     }
     if (KD == 1 && more) {
@@ -226,7 +232,9 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
     len = len1;
   }
   if (!on) return;
-  if (values ? io.end != nullptr : io.trans != nullptr) {
+  float* out = OUT ? (io.fin && head ? io.fin + ((int64_t)seg * g.nb + s) * rp : nullptr)
+                   : io.end + sn * rp;
+  if (values ? out != nullptr : true) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
@@ -235,19 +243,19 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
         if (!values)
           io.trans[(sn * R + a) * R + col] = S[mt][i];
         else if (a < g.r && col < g.p)
-          io.end[sn * rp + (int64_t)a * g.p + col] = S[mt][i];
+          out[(int64_t)a * g.p + col] = S[mt][i];
       }
   }
 }
 
 struct GradIO {
-  const void *q, *k, *v, *dout;
+  const void *v, *dout;
   const float *logA, *beta;
   int64_t d_sb, d_st;
   const float *save_s, *save_u, *save_d, *z;
   void *dq, *dk;          // (nbk, T, r) contiguous
   float *dlogA, *dbeta;   // (nb, T) contiguous
-  bool qvec, kvec, vvec, dvec, ovec;
+  bool vvec, dvec, ovec;
 };
 
 __device__ __forceinline__ float dot4(const f32x4& a, const f32x4& b) {
@@ -284,7 +292,12 @@ template <typename In, int RB> constexpr int grad_lds() {
 // Z in steps of 32 columns, split into terms once, by the wave that loaded them, and
 // shared as fragments in LDS; the next step's are loaded while one computes.  G and N
 // then take the fragments' place.
-template <typename In, int RB>
+// Keeps the operands of one group of products from being fetched during another's: the
+// sums take most registers.
+__device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0); }
+
+// SHARED: key heads shared by value heads, whose sums take registers of their own.
+template <typename In, int RB, bool SHARED>
 __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo g, Ops o,
                                                                               GradIO io) {
   constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB, TL = NT * tile_elems(RB);
@@ -296,29 +309,38 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
   float *G = reinterpret_cast<float*>(fr), *N = G + C * kLd;
   __shared__ double Ls[C];
   __shared__ float bs[C], zvs[C], pair[W], sums[H][4][C];
-  const int c = blockIdx.x, ks = blockIdx.y, group = g.nb / g.nbk;
+  const int c = blockIdx.x, ks = blockIdx.y, group = SHARED ? g.nb / g.nbk : 1;
   const int w = uniform_wave(), tt = w & 3, hf = w >> 2;
-  const int m = lane_id() & 15, gq = lane_id() >> 4;
-  const int tok = 16 * tt + m, ld = (g.p + 31) / 32 * 32, rt0 = hf * RT;
+  const int ld = (g.p + 31) / 32 * 32, rt0 = hf * RT;
   int t0, len;
   chunk_of(g, c, t0, len);
-  const bool live = tok < len;
-  const int64_t row = t0 + (live ? tok : 0);
   auto stage_tiles = [&]() {
     const float* vec = o.vec + ((int64_t)ks * group * g.nch + c) * kVec;
     TileStage<RB, NT, W>(o.k, g.r, w)(kl, o.k, ks, g.nch, c, t0, len, g.r, vec, w);
     TileStage<RB, NT, W>(o.q, g.r, w)(ql, o.q, ks, g.nch, c, t0, len, g.r, vec, w);
   };
   if (!LATE) stage_tiles();
-  const In* qrow = (const In*)io.q + ks * g.q_sb + row * g.q_st;
-  const In* krow = (const In*)io.k + ks * g.k_sb + row * g.k_st;
-
   // token in the lane, features 16 rt + 4 gq + i in registers, throughout
-  f32x4 dQ[RT], dK[RT];
+  f32x4 dQ[SHARED ? RT : 1], dK[SHARED ? RT : 1];
+  if (SHARED) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) dQ[rt] = dK[rt] = zero4();
+    for (int rt = 0; rt < RT; ++rt) dQ[rt] = dK[rt] = zero4();
+  }
+  auto put = [&](int tok, int rt, const f32x4& q, const f32x4& k) {
+    const int f0 = 16 * (rt0 + rt) + 4 * (lane_id() >> 4);
+    const int64_t at = ((int64_t)ks * g.T + t0 + tok) * g.r + f0;
+    store4((In*)io.dq + at, q, g.r - f0, io.ovec);
+    store4((In*)io.dk + at, k, g.r - f0, io.ovec);
+  };
 
   for (int h = 0; h < group; ++h) {
+    // the lane's place, new to the compiler in every pass: what is built from it would
+    // otherwise be kept in registers across the heads
+    int lane = lane_id();
+    asm("" : "+v"(lane));
+    const int m = lane & 15, gq = lane >> 4, tok = 16 * tt + m;
+    const bool live = tok < len;
+    const int64_t row = t0 + (live ? tok : 0);
     const int s = ks * group + h;
     const int64_t sc = (int64_t)s * g.nch + c;
     const float* vec = o.vec + sc * kVec;
@@ -382,6 +404,7 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
           y[rt] = mul(y[rt], sf, zf);
           kw[rt] = mul(kw[rt], load_frag<NI>(fr + (FD + rt0 + rt) * kFrag, FP), uf);
         }
+        hold();
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt)
           if (jt <= tt) {                          // column j in the lane, rows i in registers
@@ -414,20 +437,18 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
     if (LATE || h == 0) wait_vmcnt<0>();           // K's and Q's tiles
     __syncthreads();
     const float e = vec[tok], wt = vec[C + tok], b = bs[tok];
-    f32x4 kv[RT];
     float qd = 0.f, ky = 0.f, kk = 0.f, kint = 0.f;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int f0 = 16 * (rt0 + rt) + 4 * gq;
-      kv[rt] = load4(krow + f0, live ? g.r - f0 : 0, io.kvec);
       a[rt] *= g.scale * e;
       y[rt] *= -e;
       kw[rt] *= wt;
-      kint += dot4(kv[rt], kw[rt]);
+      kint += dot4(tile_values<RB, NT>(kl, tok, 16 * (rt0 + rt) + 4 * gq), kw[rt]);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       const int j0 = 32 * kb + 4 * gq;
+      hold();
       if (kb <= tt / 2) {                          // rows i = tok, over j
         const float *Gr = G + tok * kLd + j0, *Nr = N + tok * kLd + j0;
         const Frag<NI> gf = split<NI>(*reinterpret_cast<const f32x4*>(Gr),
@@ -441,6 +462,7 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
           y[rt] = mul(y[rt], kf, nf);
         }
       }
+      hold();
       if (kb >= tt / 2) {                          // columns j = tok, over i
         f32x4 gx[2], nx[2];
 #pragma unroll
@@ -459,15 +481,22 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
         }
       }
     }
+    hold();
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int f0 = 16 * (rt0 + rt) + 4 * gq;
-      qd += dot4(load4(qrow + f0, live ? g.r - f0 : 0, io.qvec), a[rt]);
-      ky += dot4(kv[rt], y[rt]);
-      kk += dot4(kv[rt], kw[rt]);
-      dQ[rt] += a[rt];
-      dK[rt] += b * y[rt] + kw[rt];
+      const f32x4 kv = tile_values<RB, NT>(kl, tok, 16 * (rt0 + rt) + 4 * gq);
+      qd += dot4(tile_values<RB, NT>(ql, tok, 16 * (rt0 + rt) + 4 * gq), a[rt]);
+      ky += dot4(kv, y[rt]);
+      kk += dot4(kv, kw[rt]);
+      const f32x4 dk = b * y[rt] + kw[rt];
+      if constexpr (SHARED) {
+        dQ[rt] += a[rt];
+        dK[rt] += dk;
+      } else if (live) {
+        put(tok, rt, a[rt], dk);
+      }
     }
+    hold();
     qd = sum_groups(qd);
     ky = sum_groups(ky);
     kk = sum_groups(kk);
@@ -500,13 +529,10 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
       }
     }
   }
-  if (!live) return;
+  const int tok = 16 * tt + (lane_id() & 15);
+  if (SHARED && tok < len) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int f0 = 16 * (rt0 + rt) + 4 * gq;
-    const int64_t at = ((int64_t)ks * g.T + row) * g.r + f0;
-    store4((In*)io.dq + at, dQ[rt], g.r - f0, io.ovec);
-    store4((In*)io.dk + at, dK[rt], g.r - f0, io.ovec);
+    for (int rt = 0; rt < RT; ++rt) put(tok, rt, dQ[rt], dK[rt]);
   }
 }
 
@@ -526,14 +552,13 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
   const Ops o = place_ops(ar, dtype, g, q, k, true);
-  gr.qvec = vec4_ok(q, g.q_sb, g.q_st, eb);
-  gr.kvec = vec4_ok(k, g.k_sb, g.k_st, eb);
+  const bool qvec = vec4_ok(q, g.q_sb, g.q_st, eb), kvec = vec4_ok(k, g.k_sb, g.k_st, eb);
   gr.vvec = vec4_ok(gr.v, g.v_sb, g.v_st, eb);
   gr.dvec = vec4_ok(gr.dout, gr.d_sb, gr.d_st, eb);
   gr.ovec = vec4_ok(gr.dq, 0, g.r, eb) && vec4_ok(gr.dk, 0, g.r, eb);
   if (g.nch > 0)
     hipLaunchKernelGGL((delta_prep_kernel<In, RB, true>), dim3(g.nch, g.nb), dim3(256), 0, st, q,
-                       k, gr.logA, gr.beta, g, o, gr.qvec, gr.kvec);
+                       k, gr.logA, gr.beta, g, o, qvec, kvec);
   RChainIO io = {};
   io.dout = gr.dout;
   io.d_sb = gr.d_sb;
@@ -541,7 +566,7 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   io.dv = dv;
   io.narrow = narrow_stride(gr.d_st);
   io.start = dstate_out;
-  io.end = dstate;
+  io.fin = dstate;
   io.ptiles = (g.p + 15) / 16;
   if (g.nruns > g.nseg) {
     const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);
@@ -550,10 +575,9 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
     first.end = c.E;
     first.trans = c.M;
     rchain<In, RB, false>(g, o, first, io.ptiles + 2 * RB, st);
-    const int rc = launch_carry(g, dstate_out, c, dstate, true, st);
+    const int rc = launch_carry(g, dstate_out, c, true, st);
     if (rc) return rc;
     io.start = c.start;
-    io.end = nullptr;
   }
   float* save_d = ar.take<float>((int64_t)g.nb * g.nch * 32 * RB * p32(g.p));
   float* z = ar.take<float>((int64_t)g.nb * g.nch * C * p32(g.p));
@@ -566,7 +590,7 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   if (g.nch > 0) {
     constexpr int lds = grad_lds<In, RB>();
     static_assert(lds + 4096 <= kMaxLds, "");
-    auto kern = delta_grad_kernel<In, RB>;
+    auto kern = g.nb > g.nbk ? delta_grad_kernel<In, RB, true> : delta_grad_kernel<In, RB, false>;
     (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL(kern, dim3(g.nch, g.nbk), dim3(256 * grad_split(RB)), lds, st, g, o, gr);
   }
@@ -603,8 +627,6 @@ extern "C" int smat_delta_scan_backward(
                SMAT_EINVAL, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who,
                (long long)workspace_bytes, (long long)need);
   GradIO gr = {};
-  gr.q = q;
-  gr.k = k;
   gr.v = v;
   gr.dout = dout;
   gr.logA = logA;

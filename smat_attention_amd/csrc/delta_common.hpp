@@ -114,11 +114,10 @@ __device__ __forceinline__ f32x4 mul(f32x4 c, const Frag<NA>& a, const Frag<NB>&
 
 // Terms of a stored fragment: term n lies `ts` elements behind term n - 1.
 template <int N>
-__device__ __forceinline__ Frag<N> load_frag(const bf16* p, int64_t ts) {
+__device__ __forceinline__ Frag<N> load_frag(const bf16* p, int64_t ts, int lane = lane_id()) {
   Frag<N> f;
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-    f.t[n] = *reinterpret_cast<const bf16x8*>(p + n * ts + lane_id() * 8);
+  for (int n = 0; n < N; ++n) f.t[n] = *reinterpret_cast<const bf16x8*>(p + n * ts + lane * 8);
   return f;
 }
 template <int N>
@@ -147,9 +146,10 @@ template <int RS> __device__ __forceinline__ int swz(int t) {
 
 // Row fragment: token 16 mt + (lane & 15), feature slots of block kb.
 template <int RB, int N>
-__device__ __forceinline__ Frag<N> rows_of(const bf16* tile, int mt, int kb) {
+__device__ __forceinline__ Frag<N> rows_of(const bf16* tile, int mt, int kb,
+                                           int lane = lane_id()) {
   constexpr int RS = row_chunks(RB);
-  const int m = lane_id() & 15, g = lane_id() >> 4;
+  const int m = lane & 15, g = lane >> 4;
   const int k0 = (4 * kb + (g >> 1)) ^ swz<RS>(m), k1 = (4 * kb + 2 + (g >> 1)) ^ swz<RS>(m);
   int at = (16 * mt + m) * RS * 8 + 4 * (g & 1);
   // odd row tiles take an address the compiler cannot relate to the even ones': fused
@@ -169,10 +169,11 @@ __device__ __forceinline__ Frag<N> rows_of(const bf16* tile, int mt, int kb) {
 // Transposed fragment: feature 16 mt + (lane & 15), token slots of block kb.  Lane
 // 4 e + q of each sixteen addresses token 16 (2 kb + h) + 4 g + e, features 4 q .. + 3.
 template <int RB, int N>
-__device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb) {
+__device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb,
+                                           int lane = lane_id()) {
   typedef short short4v __attribute__((ext_vector_type(4)));
   constexpr int RS = row_chunks(RB);
-  const int r16 = lane_id() & 15, row = 4 * (lane_id() >> 4) + (r16 >> 2);
+  const int r16 = lane & 15, row = 4 * (lane >> 4) + (r16 >> 2);
   const int k = (2 * mt + ((r16 & 3) >> 1)) ^ swz<RS>(row);
   const bf16* p = tile + ((32 * kb + row) * RS + k) * 8 + 4 * (r16 & 1);
   Frag<N> f;
@@ -189,6 +190,20 @@ __device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb) {
     f.t[n] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
   return f;
+}
+
+// Four consecutive features of token t: the terms' sum, exactly the input's values.
+template <int RB, int N> __device__ __forceinline__ f32x4 tile_values(const bf16* tile, int t, int f0) {
+  constexpr int RS = row_chunks(RB);
+  const bf16* p = tile + (t * RS + ((f0 >> 3) ^ swz<RS>(t))) * 8 + (f0 & 4);
+  f32x4 x = zero4();
+#pragma unroll
+  for (int n = N - 1; n >= 0; --n) {
+    const bf16x4 v = *reinterpret_cast<const bf16x4*>(p + n * tile_elems(RB));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] += to_f32(v[i]);
+  }
+  return x;
 }
 
 // Where a key sequence's tiles come from.
@@ -232,10 +247,12 @@ __device__ __forceinline__ void stage(void* dst, const void* src, int w) {
       dma16((const char*)src + (u * W + w) * 1024, lane_id() * 16, (char*)dst + (u * W + w) * 1024);
 }
 
-// Between the products of a wide state, where more operands in flight than the next
-// product needs would cost spills.
-template <int RB> __device__ __forceinline__ void narrow_schedule() {
-  if constexpr (RB >= 3) __builtin_amdgcn_sched_barrier(0);
+// The lane, new to the compiler wherever this is called: addresses built from it in a
+// loop are formed there instead of being kept in registers across it.
+__device__ __forceinline__ int fresh_lane() {
+  int l = lane_id();
+  asm volatile("" : "+v"(l));
+  return l;
 }
 
 // A key sequence's tile of chunk c.  Wave w's copies are rows 16 W / .. apart, whole
@@ -366,15 +383,20 @@ __device__ __forceinline__ void chunk_of(const Geo& g, int c, int& t0, int& len)
     len = min(C, g.T - t0);
   }
 }
-__device__ __forceinline__ void run_of(const Geo& g, int i, int& c0, int& c1, int& seg) {
+__device__ __forceinline__ void run_of(const Geo& g, int i, int& c0, int& c1, int& seg,
+                                       bool& first, bool& last) {
   if (g.runs) {
     c0 = g.runs[3 * i];
     c1 = g.runs[3 * i + 1];
     seg = g.runs[3 * i + 2];
+    first = g.segrun[seg] == i;
+    last = g.segrun[seg + 1] == i + 1;
   } else {
     c0 = i * g.K;
     c1 = min(c0 + g.K, g.nch);
     seg = 0;
+    first = i == 0;
+    last = i + 1 == g.nruns;
   }
 }
 
@@ -474,8 +496,7 @@ inline int dispatch(int dtype, int r, F fn) {
 // The checks that the forward and the backward share.
 int check_geo(const char* who, int dtype, const Geo& g);
 // Launches the runs' carry (both directions).
-int launch_carry(const Geo& g, const float* init, const Carry& c, float* fin, bool rev,
-                 hipStream_t st);
+int launch_carry(const Geo& g, const float* init, const Carry& c, bool rev, hipStream_t st);
 
 }  // namespace dl
 }  // namespace smat
