@@ -554,7 +554,8 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  *   o_t = scale S_t^T q_t,  a_t = exp(logA_t)
  * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides, nbk dividing nb
  * (value sequence s reads key sequence s / (nb / nbk)); logA, beta: (nb, T)
- * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256.
+ * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256,
+ * v_st (and the gradient's d_st) < 2^23.
  * Segments: chunks (nch, 2) = first token, tokens (<= 64); runs (nruns, 3) =
  * first chunk, end chunk, segment, every segment's runs together and in order,
  * an empty segment with one empty run; segrun (nseg + 1) the first run of each

@@ -30,7 +30,7 @@ struct ChainIO {
   float* fin;             // state leaving segment j: fin + (j nb + s) r p; or null
   float *save_s, *save_u; // training: states entering chunks, and U, rows padded to p32; or null
   int ptiles;             // value tiles of 16 columns (tiles behind them are M's)
-  bool narrow, ovec;      // v's rows lie within 32-bit offsets; out in groups of four
+  bool ovec;              // out's rows in groups of four
 };
 
 // Bytes of LDS: KD buffers of K and the factors, T; and Q and P with the outputs.
@@ -90,10 +90,9 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
   const In* vs = (const In*)io.v + s * g.v_sb;
   const uint32_t soff = (4 * gq * ld + col) * 4;    // in fp32 rows of ld
   const bool vlive = values && col < g.p;
-  const bool any = on && values && 16 * ct < g.p;
-  In v[16];
+  uint32_t v[16];
   auto load_v = [&](int t0, int len) {
-    load_column(v, vs, g.v_st, io.narrow, t0, len, col, vlive, any);
+    load_column(v, vs, g.v_st, t0, len, values ? col : 0, g.p);
   };
   const TileStage<RB, NT, W> kstage(o.k, g.r, w), qstage(o.q, g.r, w);
   auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
@@ -123,12 +122,12 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     const bf16* kt = kl + buf * TL;
     const float* vec = vl + buf * kVec;
     const int lane = fresh_lane(), fm = lane & 15, f4 = 4 * (lane >> 4);
-    if (more) chunk_of(g, c + 1, t1, len1);
+    chunk_of(g, more ? c + 1 : c, t1, len1);
     wait_vmcnt<0>();
     lds_barrier();
     // ---- K, Q, T and the factors of chunk c are in LDS
     f32x4 x[4];
-    column_values(x, v, vlive);
+    column_values<In>(x, v, vlive, len);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(x[mt]));   // their wait is here
     if (OUT) stage<NO * kTri, W>(pl, o.pm + sc * NO * TB, w);
@@ -146,13 +145,36 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
       f32x4 ks4[4];
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) ks4[mt] = ot[mt] = zero4();
+      constexpr int U = row_step(NT, RB);
+      pipelined<4 / U * RB, Rows<NT, U>>(
+          [&](int st, Rows<NT, U>& b) {
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
+            for (int u = 0; u < U; ++u) {
+              const int mt = st * U % 4 + u, kb = st * U / 4;
+              b.k[u] = rows_of<RB, NT>(kt, mt, kb, lane);
+              if (OUT) b.q[u] = rows_of<RB, NT>(ql, mt, kb, lane);
+            }
+          },
+          [&](int st, Rows<NT, U>& b) {
+            const int m0 = st * U % 4, kb = st * U / 4;
+            f32x4 ca[U], co[U];
+            Frag<NI> sa[U];
+            Frag<NO> so[U];
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          ks4[mt] = mul(ks4[mt], rows_of<RB, NT>(kt, mt, kb, lane), sb[kb]);
-          if (OUT) ot[mt] = mul(ot[mt], lead<NO>(sb[kb]), rows_of<RB, NT>(ql, mt, kb, lane));
-        }
+            for (int u = 0; u < U; ++u) {
+              ca[u] = ks4[m0 + u];
+              co[u] = ot[m0 + u];
+              sa[u] = sb[kb];
+              so[u] = lead<NO>(sb[kb]);
+            }
+            mul_each(ca, b.k, sa);
+            if (OUT) mul_each(co, so, b.q);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              ks4[m0 + u] = ca[u];
+              ot[m0 + u] = co[u];
+            }
+          });
       // b (V - e K S)
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
@@ -165,20 +187,14 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {             // U, in place of x
-        x[mt] = zero4();
-#pragma unroll
-        for (int kb = 0; kb <= mt / 2; ++kb)
-          x[mt] = mul(x[mt], load_frag<NI>(tl + tri(mt, kb) * kFrag, TB, lane), f[kb]);
-      }
+      for (int mt = 0; mt < 4; ++mt) x[mt] = zero4();
+      triangle<false, NI>(x, tl, f, lane);         // U, in place of x
     }
     wait_vmcnt<0>();
     lds_barrier();
     // ---- P of chunk c and the next K are in LDS; Q and T are free
-    if (more) {
-      load_v(t1, len1);
-      stage_qt(c + 1, t1, len1);
-    }
+    load_v(t1, len1);                              // (the last chunk's once more: no branch)
+    if (more) stage_qt(c + 1, t1, len1);
     if (on) {
       if (OUT && io.save_u) {
 #pragma unroll
@@ -198,11 +214,9 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
       if (OUT) {
         const uint32_t ooff = (fm * g.p + f4) * sizeof(In);
         const int left = g.p - 16 * ct - f4;
+        triangle_out<NO>(ot, pl, fo, lane);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
-#pragma unroll
-          for (int kb = 0; kb <= mt / 2; ++kb)
-            ot[mt] = mul(ot[mt], fo[kb], load_frag<NO>(pl + tri(mt, kb) * kFrag, TB, lane));
           In* row = (In*)io.o + ((int64_t)s * g.T + t0 + 16 * mt) * g.p + 16 * ct;
           if (16 * mt + fm < len && left > 0)
             store4(reinterpret_cast<In*>(reinterpret_cast<char*>(row) + ooff), ot[mt],
@@ -210,16 +224,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
         }
       }
       const float aC = vec[3 * C];
-#pragma unroll
-      for (int sk = 0; sk < RB; ++sk) {
-#pragma unroll
-        for (int mt = 2 * sk; mt < 2 * sk + 2; ++mt) {
-          S[mt] *= aC;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb, lane), f[kb]);
-        }
-        sb[sk] = split<NI>(S[2 * sk], S[2 * sk + 1]);
-      }
+      update_state<RB, NT, false>(S, sb, aC, kt, f, kt, f, lane);
     }
     if (KD == 1 && more) {
       lds_barrier();                               // K is read
@@ -399,7 +404,6 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
   io.start = state;
   io.fin = state_out;
   io.ovec = vec4_ok(out, 0, g.p, eb);
-  io.narrow = narrow_stride(g.v_st);
   io.ptiles = (g.p + 15) / 16;
   if (g.nruns > g.nseg) {
     const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);
@@ -464,6 +468,8 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && out), SMAT_EINVAL, "%s: null pointer",
                who);
+  SMAT_REQUIRE(near_rows(v_st), SMAT_EUNSUPPORTED, "%s: rows of v %lld elements apart, beyond 2^23",
+               who, (long long)v_st);
   SMAT_REQUIRE(!save_s == !save_u, SMAT_EINVAL, "%s: save_s and save_u go together", who);
   SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
   const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 0);

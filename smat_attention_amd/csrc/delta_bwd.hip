@@ -34,7 +34,6 @@ struct RChainIO {
   float *save_d, *z;      // dS' of every chunk (R x p32) and Z (64 x p32)
   void* dv;               // (nb, T, p) contiguous
   int ptiles;
-  bool narrow;            // dout's rows lie within 32-bit offsets
 };
 
 // Bytes of LDS: KD buffers of K and the factors, Q, T^T and P^T.
@@ -91,10 +90,9 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
   const In* ds = (const In*)io.dout + s * io.d_sb;
   const uint32_t soff = (4 * gq * ld + col) * 4;    // in fp32 rows of ld
   const bool dlive = values && col < g.p;
-  const bool any = on && values && 16 * ct < g.p;
-  In dv[16];
+  uint32_t dv[16];
   auto load_d = [&](int t0, int len) {
-    load_column(dv, ds, io.d_st, io.narrow, t0, len, col, dlive, any);
+    load_column(dv, ds, io.d_st, t0, len, values ? col : 0, g.p);
   };
   const TileStage<RB, NT, W> kstage(o.k, g.r, w), qstage(o.q, g.r, w);
   auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
@@ -125,12 +123,12 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
     const bf16* kt = kl + buf * TL;
     const float* vec = vl + buf * kVec;
     const int lane = fresh_lane(), f4 = 4 * (lane >> 4);
-    if (more) chunk_of(g, c - 1, t1, len1);
+    chunk_of(g, more ? c - 1 : c, t1, len1);
     wait_vmcnt<0>();
     lds_barrier();
     // ---- K, T^T, P^T and the factors of chunk c are in LDS
     f32x4 d[4], x[4];
-    column_values(d, dv, dlive);
+    column_values<In>(d, dv, dlive, len);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(d[mt]));   // their wait is here
     qstage(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
@@ -144,11 +142,26 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
       }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) x[mt] = zero4();                // dU
+      constexpr int U = row_step(NT, RB);
+      pipelined<4 / U * RB, Rows<NT, U>>(
+          [&](int st, Rows<NT, U>& b) {
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
+            for (int u = 0; u < U; ++u)
+              b.k[u] = rows_of<RB, NT>(kt, st * U % 4 + u, st * U / 4, lane);
+          },
+          [&](int st, Rows<NT, U>& b) {
+            const int m0 = st * U % 4, kb = st * U / 4;
+            f32x4 ca[U];
+            Frag<NI> sa[U];
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-          x[mt] = mul(x[mt], rows_of<RB, NT>(kt, mt, kb, lane), sb[kb]);
+            for (int u = 0; u < U; ++u) {
+              ca[u] = x[m0 + u];
+              sa[u] = sb[kb];
+            }
+            mul_each(ca, b.k, sa);
+#pragma unroll
+            for (int u = 0; u < U; ++u) x[m0 + u] = ca[u];
+          });
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
         x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + f4);
@@ -156,29 +169,19 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
         Frag<NT> df[2];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-          for (int kb = mt / 2; kb < 2; ++kb)
-            x[mt] = mul(x[mt], load_frag<NI>(pl + tri_t(mt, kb) * kFrag, TB, lane), df[kb]);
+        triangle<true, NI>(x, pl, df, lane);
       }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {             // Z
-        x[mt] = zero4();
-#pragma unroll
-        for (int kb = mt / 2; kb < 2; ++kb)
-          x[mt] = mul(x[mt], load_frag<NI>(tl + tri_t(mt, kb) * kFrag, TB, lane), f[kb]);
-      }
+      for (int mt = 0; mt < 4; ++mt) x[mt] = zero4();
+      triangle<true, NI>(x, tl, f, lane);          // Z
     }
     wait_vmcnt<0>();
     lds_barrier();
     // ---- Q of chunk c and the next K are in LDS; T^T and P^T are free
-    if (more) {
-      load_d(t1, len1);
-      stage_tp(c - 1);
-    }
+    load_d(t1, len1);                              // (the last chunk's once more: no branch)
+    if (more) stage_tp(c - 1);
     if (on) {
       if (OUT) {
 #pragma unroll
@@ -208,21 +211,10 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) fd[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
       }
-#pragma unroll
-      for (int sk = 0; sk < RB; ++sk) {
-#pragma unroll
-        for (int mt = 2 * sk; mt < 2 * sk + 2; ++mt) {
-          S[mt] *= aC;
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) S[mt] = mul(S[mt], cols_of<RB, NT>(kt, mt, kb, lane), f[kb]);
-          if (values) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-              S[mt] = mul(S[mt], cols_of<RB, NT>(ql, mt, kb, lane), fd[kb]);
-          }
-        }
-        sb[sk] = split<NI>(S[2 * sk], S[2 * sk + 1]);
-      }
+      if (values)
+        update_state<RB, NT, true>(S, sb, aC, kt, f, ql, fd, lane);
+      else
+        update_state<RB, NT, false>(S, sb, aC, kt, f, ql, fd, lane);
     }
     if (KD == 1 && more) {
       lds_barrier();                               // K is read
@@ -296,8 +288,10 @@ template <typename In, int RB> constexpr int grad_lds() {
 // sums take most registers.
 __device__ __forceinline__ void hold() { __builtin_amdgcn_sched_barrier(0); }
 
-// SHARED: key heads shared by value heads, whose sums take registers of their own.
-template <typename In, int RB, bool SHARED>
+// SHARED: key heads shared by value heads, whose sums take registers of their own.  FULL:
+// rows of V and dO in whole aligned groups, loaded without a branch (at a join the
+// compiler waits for the loads of either side, a step ahead of their use).
+template <typename In, int RB, bool SHARED, bool FULL>
 __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo g, Ops o,
                                                                               GradIO io) {
   constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB, TL = NT * tile_elems(RB);
@@ -346,33 +340,44 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
     const float* vec = o.vec + sc * kVec;
     const In* drow = (const In*)io.dout + s * io.d_sb + row * io.d_st;
     const In* vrow = (const In*)io.v + s * g.v_sb + row * g.v_st;
-    // this wave's loads of a step: tile w of S and dS' (while there is one), and rows of
-    // U (waves of half 0) and Z (waves of the last half)
+    // this wave's loads of a step: tile w of S and dS' (the last one again where there is
+    // no tile w), and rows of U (waves of half 0) and Z (waves of the last half)
+    constexpr bool both = H == 1;
     const bool pairs = w < 2 * RB, has_u = hf == 0, has_z = hf == H - 1;
     const int64_t lane_row = (int64_t)m * ld + 8 * gq;
-    const float* Sp = io.save_s + (sc * R + 16 * w) * ld + lane_row;
-    const float* Dp = io.save_d + (sc * R + 16 * w) * ld + lane_row;
-    const float* Up = io.save_u + (sc * C + 16 * tt) * ld + lane_row;
+    const int tile = min(w, 2 * RB - 1);
+    const float* Sp = io.save_s + (sc * R + 16 * tile) * ld + lane_row;
+    const float* Dp = io.save_d + (sc * R + 16 * tile) * ld + lane_row;
+    const float* Up = (has_u ? io.save_u : io.z) + (sc * C + 16 * tt) * ld + lane_row;
     const float* Zp = io.z + (sc * C + 16 * tt) * ld + lane_row;
-    f32x4 sx[2], ex[2], ux[2], zx[2], dx[2], vx[2];
+    f32x4 sx[2], ex[2], ux[2], zx[2], dx[2], vx[2];   // both = false: ux is U's or Z's rows
+    typedef In In4 __attribute__((ext_vector_type(4)));
+    In4 dr[2], vr[2];
     auto get = [&](f32x4* x, const float* p) {
       x[0] = *reinterpret_cast<const f32x4*>(p);
       x[1] = *reinterpret_cast<const f32x4*>(p + 4);
     };
     auto load_step = [&](int pb) {
-      if (pairs) {
-        get(sx, Sp + pb);
-        get(ex, Dp + pb);
-      }
-      if (has_u) get(ux, Up + pb);
-      if (has_z) get(zx, Zp + pb);
+      get(sx, Sp + pb);
+      get(ex, Dp + pb);
+      get(ux, Up + pb);
+      if (both) get(zx, Zp + pb);
       const int pc = pb + 8 * gq;
-      load8f(dx, drow + pc, live ? g.p - pc : 0, io.dvec);
-      if (has_z) load8f(vx, vrow + pc, live ? g.p - pc : 0, io.vvec);
+      if constexpr (FULL) {
+#pragma unroll
+        for (int h4 = 0; h4 < 2; ++h4) {
+          dr[h4] = *reinterpret_cast<const In4*>(drow + pc + 4 * h4);
+          vr[h4] = *reinterpret_cast<const In4*>(vrow + pc + 4 * h4);
+        }
+      } else {
+        load8f(dx, drow + pc, live ? g.p - pc : 0, io.dvec);
+        load8f(vx, vrow + pc, live ? g.p - pc : 0, io.vvec);
+      }
     };
+    const Gates gates = load_gates(g, io.logA, io.beta, s, t0, len);
     load_step(0);
     __syncthreads();                               // the last head's LDS is read
-    chunk_decays(g, io.logA, io.beta, s, t0, len, Ls, bs);
+    chunk_decays(gates, len, Ls, bs);
 
     f32x4 a[RT], y[RT], kw[RT], gp[4], np[4];
 #pragma unroll
@@ -381,19 +386,30 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
     for (int jt = 0; jt < 4; ++jt) gp[jt] = np[jt] = zero4();
     float zv = 0.f, dots = 0.f;
     for (int pb = 0; pb < ld; pb += 32) {
+      if constexpr (FULL) {
+#pragma unroll
+        for (int h4 = 0; h4 < 2; ++h4)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            dx[h4][i] = live ? to_f32(dr[h4][i]) : 0.f;
+            vx[h4][i] = live ? to_f32(vr[h4][i]) : 0.f;
+          }
+      }
       if (pairs) {
         dots += dot4(sx[0], ex[0]) + dot4(sx[1], ex[1]);
         store_frag<NI>(fr + (FS + w) * kFrag, FP, split<NI>(sx[0], sx[1]));
         store_frag<NI>(fr + (FD + w) * kFrag, FP, split<NI>(ex[0], ex[1]));
       }
-      if (has_u) store_frag<NI>(fr + (FU + tt) * kFrag, FP, split<NI>(ux[0], ux[1]));
-      if (has_z) {
+      store_frag<NI>(fr + ((has_u ? FU : FZ) + tt) * kFrag, FP, split<NI>(ux[0], ux[1]));
+      if (both) {
         zv += dot4(zx[0], vx[0]) + dot4(zx[1], vx[1]);
         store_frag<NI>(fr + (FZ + tt) * kFrag, FP, split<NI>(zx[0], zx[1]));
+      } else if (has_z) {
+        zv += dot4(ux[0], vx[0]) + dot4(ux[1], vx[1]);
       }
       const Frag<NT> df = split<NT>(dx[0], dx[1]);
       __syncthreads();
-      if (pb + 32 < ld) load_step(pb + 32);
+      load_step(min(pb + 32, ld - 32));            // (the last step's once more: no branch)
       {
         const Frag<NI> zf = load_frag<NI>(fr + (FZ + tt) * kFrag, FP);
         const Frag<NI> uf = load_frag<NI>(fr + (FU + tt) * kFrag, FP);
@@ -564,7 +580,6 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   io.d_sb = gr.d_sb;
   io.d_st = gr.d_st;
   io.dv = dv;
-  io.narrow = narrow_stride(gr.d_st);
   io.start = dstate_out;
   io.fin = dstate;
   io.ptiles = (g.p + 15) / 16;
@@ -590,7 +605,11 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   if (g.nch > 0) {
     constexpr int lds = grad_lds<In, RB>();
     static_assert(lds + 4096 <= kMaxLds, "");
-    auto kern = g.nb > g.nbk ? delta_grad_kernel<In, RB, true> : delta_grad_kernel<In, RB, false>;
+    const bool full = g.p % 32 == 0 && gr.vvec && gr.dvec, shared = g.nb > g.nbk;
+    auto kern = shared ? (full ? delta_grad_kernel<In, RB, true, true>
+                               : delta_grad_kernel<In, RB, true, false>)
+                       : (full ? delta_grad_kernel<In, RB, false, true>
+                               : delta_grad_kernel<In, RB, false, false>);
     (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL(kern, dim3(g.nch, g.nbk), dim3(256 * grad_split(RB)), lds, st, g, o, gr);
   }
@@ -621,6 +640,9 @@ extern "C" int smat_delta_scan_backward(
   SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && dout && save_s && save_u && dq && dk &&
                             dv && dlogA && dbeta),
                SMAT_EINVAL, "%s: null pointer", who);
+  SMAT_REQUIRE(near_rows(v_st) && near_rows(d_st), SMAT_EUNSUPPORTED,
+               "%s: rows of v or dout %lld and %lld elements apart, beyond 2^23", who,
+               (long long)v_st, (long long)d_st);
   const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 1);
   SMAT_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
                    ((uintptr_t)workspace & 255) == 0,

@@ -112,6 +112,36 @@ __device__ __forceinline__ f32x4 mul(f32x4 c, const Frag<NA>& a, const Frag<NB>&
   return c;
 }
 
+// The same for U products at once, term by term across them, so that consecutive
+// instructions do not wait for each other's sums.
+template <int U, int NA, int NB>
+__device__ __forceinline__ void mul_each(f32x4 (&c)[U], const Frag<NA> (&a)[U],
+                                         const Frag<NB> (&b)[U]) {
+  constexpr int M = NA > NB ? NA : NB;
+#pragma unroll
+  for (int o = M - 1; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (o - i >= 0 && o - i < NB)
+#pragma unroll
+        for (int u = 0; u < U; ++u) c[u] = mma(c[u], a[u].t[i], b[u].t[o - i]);
+}
+
+// Steps whose operands come from LDS: the next step's reads are issued before a step's
+// products, and stay there.
+template <int STEPS, typename Buf, typename Load, typename Use>
+__device__ __forceinline__ void pipelined(Load load, Use use) {
+  Buf buf[2];
+  load(0, buf[0]);
+#pragma unroll
+  for (int st = 0; st < STEPS; ++st) {
+    if (st + 1 < STEPS) load(st + 1, buf[(st + 1) & 1]);
+    __builtin_amdgcn_sched_barrier(0);
+    use(st, buf[st & 1]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // Terms of a stored fragment: term n lies `ts` elements behind term n - 1.
 template <int N>
 __device__ __forceinline__ Frag<N> load_frag(const bf16* p, int64_t ts, int lane = lane_id()) {
@@ -190,6 +220,111 @@ __device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb,
     f.t[n] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
   }
   return f;
+}
+
+// x += T f for a stored lower triangle (UPPER: its transpose), two row tiles at a time.
+template <int NA> struct Two {
+  Frag<NA> a[2];
+};
+template <bool UPPER, int NA, int NB>
+__device__ __forceinline__ void triangle(f32x4 (&x)[4], const bf16* tl, const Frag<NB> (&f)[2],
+                                         int lane) {
+  // row tiles 0, 1 (of the lower triangle; 2, 3 of the upper) meet one block, the
+  // others two
+  constexpr int TS = kTri * kFrag;
+  auto mt_of = [](int st) { return UPPER ? (st == 0 ? 2 : 0) : (st == 0 ? 0 : 2); };
+  auto kb_of = [](int st) { return UPPER ? (st == 1 ? 0 : 1) : (st == 2 ? 1 : 0); };
+  pipelined<3, Two<NA>>(
+      [&](int st, Two<NA>& b) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int mt = mt_of(st) + u, kb = kb_of(st);
+          b.a[u] = load_frag<NA>(tl + (UPPER ? tri_t(mt, kb) : tri(mt, kb)) * kFrag, TS, lane);
+        }
+      },
+      [&](int st, Two<NA>& b) {
+        const int mt = mt_of(st), kb = kb_of(st);
+        f32x4 c[2] = {x[mt], x[mt + 1]};
+        const Frag<NB> g[2] = {f[kb], f[kb]};
+        mul_each(c, b.a, g);
+        x[mt] = c[0];
+        x[mt + 1] = c[1];
+      });
+}
+// The same with the result transposed: x's columns in registers.
+template <int NA, int NB>
+__device__ __forceinline__ void triangle_out(f32x4 (&x)[4], const bf16* pl, const Frag<NB> (&f)[2],
+                                             int lane) {
+  constexpr int TS = kTri * kFrag;
+  auto mt_of = [](int st) { return st == 0 ? 0 : 2; };
+  auto kb_of = [](int st) { return st == 2 ? 1 : 0; };
+  pipelined<3, Two<NA>>(
+      [&](int st, Two<NA>& b) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          b.a[u] = load_frag<NA>(pl + tri(mt_of(st) + u, kb_of(st)) * kFrag, TS, lane);
+      },
+      [&](int st, Two<NA>& b) {
+        const int mt = mt_of(st), kb = kb_of(st);
+        f32x4 c[2] = {x[mt], x[mt + 1]};
+        const Frag<NB> g[2] = {f[kb], f[kb]};
+        mul_each(c, g, b.a);
+        x[mt] = c[0];
+        x[mt + 1] = c[1];
+      });
+}
+
+// Row tiles a step takes of K S and of K^T U: as many as leave room for the next step's
+// operands.
+constexpr int row_step(int terms, int RB) { return terms == 1 ? (RB == 4 ? 2 : 4) : terms == 2 ? 2 : 1; }
+constexpr int col_step(int terms) { return terms == 1 ? 2 : 1; }
+template <int NT, int U> struct Rows {
+  Frag<NT> k[U], q[U];
+};
+template <int NT, int U, bool Q> struct Cols {
+  Frag<NT> k[2][U], q[Q ? 2 : 1][U];
+};
+
+// S <- aC S + K^T f (+ Q^T h) by feature tiles, and sb its terms.
+template <int RB, int NT, bool Q, int NI>
+__device__ __forceinline__ void update_state(f32x4 (&S)[2 * RB], Frag<NI> (&sb)[RB], float aC,
+                                             const bf16* kt, const Frag<NI> (&f)[2],
+                                             const bf16* qt, const Frag<NI> (&h)[2], int lane) {
+  constexpr int U = col_step(NT);
+  typedef Cols<NT, U, Q> Buf;
+  pipelined<2 * RB / U, Buf>(
+      [&](int st, Buf& b) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            b.k[kb][u] = cols_of<RB, NT>(kt, st * U + u, kb, lane);
+            if constexpr (Q) b.q[kb][u] = cols_of<RB, NT>(qt, st * U + u, kb, lane);
+          }
+      },
+      [&](int st, Buf& b) {
+        f32x4 c[U];
+        Frag<NI> g[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) c[u] = S[st * U + u] * aC;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) g[u] = f[kb];
+          mul_each(c, b.k[kb], g);
+          if constexpr (Q) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) g[u] = h[kb];
+            mul_each(c, b.q[kb], g);
+          }
+        }
+        // the pair of tiles finished a step ago, while this one's products run
+        const int done = st * U - 2;
+        if (done >= 0 && done % 2 == 0) sb[done / 2] = split<NI>(S[done], S[done + 1]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) S[st * U + u] = c[u];
+      });
+  sb[RB - 1] = split<NI>(S[2 * RB - 2], S[2 * RB - 1]);
 }
 
 // Four consecutive features of token t: the terms' sum, exactly the input's values.
@@ -293,39 +428,50 @@ template <int RB, int N, int W> struct TileStage {
 };
 
 // A chunk's 64 values of a column in result-tile order: element j is token
-// 16 (j >> 2) + 4 gq + (j & 3).  Absent tokens, and all if !live, are zero.
+// 16 (j >> 2) + 4 gq + (j & 3), loaded a chunk ahead of their use.  The bits are kept a
+// register each: packed in pairs, they would be waited for where they are loaded.
+template <typename In> __device__ __forceinline__ uint32_t bits_of(const In* p) {
+  if constexpr (sizeof(In) == 4)
+    return *reinterpret_cast<const uint32_t*>(p);
+  else
+    return *reinterpret_cast<const uint16_t*>(p);
+}
+template <typename In> __device__ __forceinline__ float value_of(uint32_t b) {
+  if constexpr (__is_same(In, float))
+    return __uint_as_float(b);
+  else if constexpr (__is_same(In, bf16))
+    return __uint_as_float(b << 16);
+  else
+    return to_f32(__builtin_bit_cast(f16, (uint16_t)b));
+}
+// Without a branch: at a join the compiler waits for the loads of either side.  Absent
+// tokens and columns (col past the last) read the last one there is; column_values drops
+// them.  Rows lie less than 2^23 elements apart, so a chunk's offsets have 32 bits.
 template <typename In>
-__device__ __forceinline__ void load_column(In* v, const In* rows, int64_t st, bool narrow,
-                                            int64_t t0, int len, int col, bool live, bool any) {
-  const int gq = lane_id() >> 4;
-  if (!any) {                                      // uniform: nothing here for the whole wave
+__device__ __forceinline__ void load_column(uint32_t* v, const In* rows, int64_t st, int64_t t0,
+                                            int len, int col, int cols) {
+  const char* p = reinterpret_cast<const char*>(rows + t0 * st);
+  const uint32_t step = (uint32_t)st * sizeof(In), c0 = min(col, cols - 1) * sizeof(In);
+  const uint32_t first = 4 * (lane_id() >> 4) * step + c0, last = (len - 1) * step + c0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = from_f32<In>(0.f);
-    return;
-  }
-  const In* p = rows + t0 * st;
-  if (narrow && len == C) {
-    const uint32_t off = (uint32_t)((4 * gq * (uint32_t)st + (live ? col : 0)) * sizeof(In));
+  for (int j = 0; j < 16; ++j)
+    v[j] = bits_of(reinterpret_cast<const In*>(
+        p + min(first + (16 * (j >> 2) + (j & 3)) * step, last)));
+}
+template <typename In>
+__device__ __forceinline__ void column_values(f32x4* x, const uint32_t* v, bool live, int len) {
+  if (len == C) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      v[j] = *reinterpret_cast<const In*>(reinterpret_cast<const char*>(p) + off);
-      p += (j & 3) == 3 ? 13 * st : st;
-    }
+    for (int j = 0; j < 16; ++j) x[j >> 2][j & 3] = live ? value_of<In>(v[j]) : 0.f;
   } else {
+    const int g4 = 4 * (lane_id() >> 4);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const int t = 16 * (j >> 2) + 4 * gq + (j & 3);
-      v[j] = live && t < len ? p[(int64_t)t * st + col] : from_f32<In>(0.f);
-    }
+    for (int j = 0; j < 16; ++j)
+      x[j >> 2][j & 3] =
+          live && 16 * (j >> 2) + (j & 3) + g4 < len ? value_of<In>(v[j]) : 0.f;
   }
 }
-// (a dead lane of a live wave read column 0)
-template <typename In>
-__device__ __forceinline__ void column_values(f32x4* x, const In* v, bool live) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j) x[j >> 2][j & 3] = live ? to_f32(v[j]) : 0.f;
-}
-inline bool narrow_stride(int64_t st) { return st >= 0 && st < (1 << 24); }
+inline bool near_rows(int64_t st) { return st >= 0 && st < (1 << 23); }
 
 // Four consecutive elements; those at and past nv are zero.
 template <typename In>

@@ -91,18 +91,23 @@ __device__ __forceinline__ void unit_lower_inverse(const float* Am, float* Tm) {
 }
 
 // Running sum of the chunk's logA in fp64, in units of log 2, into Ls (wave 0), beta
-// into bs.  Tokens past the chunk's end count as logA = 0, beta = 0.
-__device__ __forceinline__ void chunk_decays(const Geo& g, const float* logA, const float* beta,
-                                             int s, int t0, int len, double* Ls, float* bs) {
+// into bs.  Tokens past the chunk's end count as logA = 0, beta = 0.  The loads are a
+// call of their own, to be issued ahead.
+struct Gates {
+  float a, b;
+};
+__device__ __forceinline__ Gates load_gates(const Geo& g, const float* logA, const float* beta,
+                                            int s, int t0, int len) {
+  const int64_t t = t0 + min(lane_id(), len - 1);
+  return {logA[s * g.a_sb + t * g.a_st], beta[s * g.b_sb + t * g.b_st]};
+}
+__device__ __forceinline__ void chunk_decays(const Gates& gt, int len, double* Ls, float* bs) {
   const int t = threadIdx.x;
   if (t < C) {
     const bool ok = t < len;
-    double x = 0.0;
-    if (ok) {
-      const float a = logA[s * g.a_sb + (int64_t)(t0 + t) * g.a_st];
-      x = (a < -1e5f ? -1e5 : (double)a) * 1.4426950408889634;   // NaN stays NaN
-    }
-    bs[t] = ok ? beta[s * g.b_sb + (int64_t)(t0 + t) * g.b_st] : 0.f;
+    // NaN stays NaN
+    double x = ok ? (gt.a < -1e5f ? -1e5 : (double)gt.a) * 1.4426950408889634 : 0.0;
+    bs[t] = ok ? gt.b : 0.f;
 #pragma unroll
     for (int d = 1; d < C; d <<= 1) {
       const double y = __shfl_up(x, d);
@@ -191,10 +196,11 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
   const In* krow = k + ks * g.k_sb + (int64_t)(t0 + (live ? tok : 0)) * g.k_st;
   const In* qrow = q + ks * g.q_sb + (int64_t)(t0 + (live ? tok : 0)) * g.q_st;
   const int64_t kc = (ks * g.nch + c) * (int64_t)NT * tile_elems(RB), sc = (int64_t)s * g.nch + c;
+  const Gates gates = load_gates(g, logA, beta, s, t0, len);
   Frag<NT> kf[RB], qf[RB];
   row_frags<In, RB, NT>(kf, krow, live, g.r, kvec, len);
   row_frags<In, RB, NT>(qf, qrow, live, g.r, qvec, len);
-  chunk_decays(g, logA, beta, s, t0, len, Ls, bs);
+  chunk_decays(gates, len, Ls, bs);
 #pragma unroll
   for (int kb = 0; kb < RB; ++kb) store_frag<NT>(rows + (w * RB + kb) * kFrag, KB, kf[kb]);
   if (tiles) {

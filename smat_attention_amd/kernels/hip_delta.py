@@ -89,6 +89,12 @@ class Segments:
         return self._runs[K]
 
 
+def _near_rows(t):
+    """``_rows3``, with rows that lie 2^23 elements and more apart copied together: the kernels
+    reach the rows of a chunk by 32-bit offsets."""
+    return _rows3(t if t.stride(1) < 2 ** 23 else t.contiguous())
+
+
 class _Plan:
     """One call's geometry: its sizes and table addresses in the C entry points' order."""
 
@@ -170,7 +176,7 @@ def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bo
     who = "gated_delta_scan"
     plan = _Plan(who, Q, V, segments)
     code, dev = _code(Q, who), Q.device
-    (Q, q_sb, q_st), (K, k_sb, k_st), (V, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
+    (Q, q_sb, q_st), (K, k_sb, k_st), (V, v_sb, v_st) = _rows3(Q), _rows3(K), _near_rows(V)
     logA, beta = logA.float(), beta.float()
     o = torch.empty(plan.nb, plan.T, plan.p, device=dev, dtype=V.dtype)
     lead = () if segments is None else (plan.nseg,)
@@ -198,7 +204,7 @@ def scan_backward(inputs, save_s, save_u, dO, dS, scale, segments, want_dstate: 
     plan = _Plan(who, Q, V, segments)
     code, dev = _code(Q, who), Q.device
     (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
-    dO, d_sb, d_st = _rows3(dO)
+    dO, d_sb, d_st = _near_rows(dO)
     dQ = torch.empty(plan.nbk, plan.T, plan.r, device=dev, dtype=Q.dtype)
     dK = torch.empty_like(dQ)
     dV = torch.empty(plan.nb, plan.T, plan.p, device=dev, dtype=V.dtype)
