@@ -251,84 +251,98 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
 }
 
 // The states entering the runs of a segment (start): S <- M_i S + E_i past each but
-// the last.  A wave 16 columns, four waves a workgroup; `rev` walks the runs
-// backwards (the gradient's direction).  A step waits on the last one, so
-// what does not depend on it is done ahead: the next M and E are loaded while a step
-// computes, and the waves split M into terms once, in LDS, for each other.
+// the last; `rev` walks the runs backwards (the gradient's direction).  Every step
+// waits on the last one, so a step is made short: a workgroup takes 16 columns only,
+// wave w the rows [32 w, 32 w + 32) of them, M's rows and E's of the next run are
+// loaded while a step computes, and the waves meet once, over their parts of S.
 template <int RB>
-__global__ __launch_bounds__(256) void delta_carry_kernel(Geo g, const float* __restrict__ init,
-                                                          const float* __restrict__ E,
-                                                          const float* __restrict__ M,
-                                                          float* __restrict__ start, bool rev) {
-  constexpr int R = 32 * RB, NI = kMid, NF = 2 * RB * RB, PER = (NF + 3) / 4;
-  extern __shared__ __align__(1024) bf16 lds[];    // NF fragments, a plane a term
-  const int w = wave_id(), m = lane_id() & 15, gq = lane_id() >> 4;
-  const int col = 16 * (4 * blockIdx.x + w) + m, seg = blockIdx.y, s = blockIdx.z;
+__global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float* __restrict__ init,
+                                                              const float* __restrict__ E,
+                                                              const float* __restrict__ M,
+                                                              float* __restrict__ start,
+                                                              bool rev) {
+  constexpr int R = 32 * RB, NI = kMid;
+  __shared__ __align__(16) bf16 parts[2][NI * RB * kFrag];
+  const int w = uniform_wave(), m = lane_id() & 15, gq = lane_id() >> 4;
+  const int col = 16 * blockIdx.x + m, seg = blockIdx.y, s = blockIdx.z;
   const int64_t rp = (int64_t)g.r * g.p;
   const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
-  const bool live = col < g.p;
+  if (r0 >= r1) return;
   auto at = [&](int n) { return (int64_t)(rev ? r0 + r1 - 1 - n : n) * g.nb + s; };
-  auto load_cols = [&](f32x4* x, const float* p) {
+  // element (mt, i) is row 32 w + 16 mt + 4 gq + i; rows and columns past the end read
+  // the last one there is
+  uint32_t off[2][4];
+  bool live[2][4];
 #pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt)
+  for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int a = 16 * mt + 4 * gq + i;
-        x[mt][i] = live && a < g.r ? p[(int64_t)a * g.p + col] : 0.f;
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int a = 32 * w + 16 * mt + 4 * gq + i;
+      live[mt][i] = a < g.r && col < g.p;
+      off[mt][i] = (uint32_t)(min(a, g.r - 1) * g.p + min(col, g.p - 1));
+    }
+  f32x4 S[2], e[2], x[2][RB][2];
+  auto load = [&](f32x4* y, const float* p) {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[mt][i] = p[off[mt][i]];
   };
-  auto store_cols = [&](float* p, const f32x4* x) {
+  auto keep = [&](f32x4* y) {
 #pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt)
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int a = 16 * mt + 4 * gq + i;
-        if (live && a < g.r) p[(int64_t)a * g.p + col] = x[mt][i];
-      }
+      for (int i = 0; i < 4; ++i) y[mt][i] = live[mt][i] ? y[mt][i] : 0.f;
   };
-  f32x4 S[2 * RB], e[2 * RB], x[PER][2];
+  auto store = [&](float* p) {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (live[mt][i]) p[off[mt][i]] = S[mt][i];
+  };
   auto load_m = [&](int n) {
-    const float* p = M + at(n) * R * R + (int64_t)m * R + 4 * gq;
+    const float* p = M + at(n) * R * R + (int64_t)(32 * w + m) * R + 4 * gq;
 #pragma unroll
-    for (int u = 0; u < PER; ++u) {
-      const int f = min(u * 4 + w, NF - 1), mt = f / RB, kb = f % RB;
-      const float* q = p + (int64_t)16 * mt * R + 32 * kb;
-      x[u][0] = *reinterpret_cast<const f32x4*>(q);
-      x[u][1] = *reinterpret_cast<const f32x4*>(q + 16);
-    }
-  };
-#pragma unroll
-  for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = zero4();
-  const int64_t ss = ((int64_t)seg * g.nb + s) * rp;
-  if (init) load_cols(S, init + ss);
-  if (r0 + 1 < r1) {
-    load_m(r0);
-    load_cols(e, E + at(r0) * rp);
-  }
-  for (int n = r0; n + 1 < r1; ++n) {
-    __syncthreads();                               // the last step's fragments are read
-#pragma unroll
-    for (int u = 0; u < PER; ++u)
-      if (u * 4 + w < NF)
-        store_frag<NI>(lds + (u * 4 + w) * kFrag, NF * kFrag, split<NI>(x[u][0], x[u][1]));
-    store_cols(start + at(n) * rp, S);
-    Frag<NI> sb[RB];
-#pragma unroll
-    for (int kb = 0; kb < RB; ++kb) sb[kb] = split<NI>(S[2 * kb], S[2 * kb + 1]);
-#pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt) S[mt] = e[mt];
-    if (n + 2 < r1) {
-      load_m(n + 1);
-      load_cols(e, E + at(n + 1) * rp);
-    }
-    lds_barrier();
-#pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt)
+    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int kb = 0; kb < RB; ++kb)
-        S[mt] = mul(S[mt], load_frag<NI>(lds + (mt * RB + kb) * kFrag, NF * kFrag), sb[kb]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          x[mt][kb][h] = *reinterpret_cast<const f32x4*>(p + 16 * mt * R + 32 * kb + 16 * h);
+  };
+  S[0] = S[1] = zero4();
+  if (init) {
+    load(S, init + ((int64_t)seg * g.nb + s) * rp);
+    keep(S);
   }
-  if (r0 < r1) store_cols(start + at(r1 - 1) * rp, S);
+  load_m(r0 + 1 < r1 ? r0 : r1 - 1);
+  load(e, E + at(r0 + 1 < r1 ? r0 : r1 - 1) * rp);
+  for (int n = r0; n + 1 < r1; ++n) {
+    bf16* part = parts[(n - r0) & 1];
+    store_frag<NI>(part + w * kFrag, RB * kFrag, split<NI>(S[0], S[1]));
+    store(start + at(n) * rp);
+    Frag<NI> mf[2][RB];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) mf[mt][kb] = split<NI>(x[mt][kb][0], x[mt][kb][1]);
+    f32x4 c[2] = {e[0], e[1]};
+    keep(c);
+    const int next = n + 2 < r1 ? n + 1 : n;       // (the last one's once more: no branch)
+    load_m(next);
+    load(e, E + at(next) * rp);
+    lds_barrier();                                 // one a step: the parts alternate
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) {
+      const Frag<NI> sb = load_frag<NI>(part + kb * kFrag, RB * kFrag);
+      const Frag<NI> a[2] = {mf[0][kb], mf[1][kb]}, b[2] = {sb, sb};
+      mul_each(c, a, b);
+    }
+    S[0] = c[0];
+    S[1] = c[1];
+  }
+  store(start + at(r1 - 1) * rp);
 }
 
 int check_geo(const char* who, int dtype, const Geo& g) {
@@ -359,11 +373,8 @@ int check_geo(const char* who, int dtype, const Geo& g) {
 template <int RB>
 static void carry_kernel(const Geo& g, const float* init, const Carry& c, bool rev,
                          hipStream_t st) {
-  constexpr int lds = 2 * RB * RB * kMid * kFrag * 2;
-  auto kern = delta_carry_kernel<RB>;
-  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-  hipLaunchKernelGGL(kern, dim3((g.p + 63) / 64, g.nseg, g.nb), dim3(256), lds, st, g, init, c.E,
-                     c.M, c.start, rev);
+  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3((g.p + 15) / 16, g.nseg, g.nb), dim3(64 * RB), 0,
+                     st, g, init, c.E, c.M, c.start, rev);
 }
 
 int launch_carry(const Geo& g, const float* init, const Carry& c, bool rev, hipStream_t st) {
