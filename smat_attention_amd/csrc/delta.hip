@@ -438,12 +438,31 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 }  // namespace dl
 }  // namespace smat
 
+// Run length: the number of runs a segment, G, that takes least by what a step of a
+// full GPU (512 workgroups of four column tiles) measures, in microseconds: 2.5 + 0.6 RB
+// a chunk of the pass with outputs, 1.5 + 0.4 RB of the first pass, 0.65 RB a run of the
+// carry, 10 for the two launches more.  (8 sequences of 2048 chunks, r = p = 128: 9349
+// whole, 1352 in 32 runs, 2082 in 256; 96 of 64 chunks, r = p = 64, forward and
+// backward: 1074 whole, 930 in 8, 1048 in 2.)
 extern "C" int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p) {
-  // waves that whole segments give, were they all as long as the longest
-  const int64_t work = (int64_t)nb * ((p + 15) / 16) * nch;       // chunk steps
-  if (longest < 32 || work >= (int64_t)1024 * longest) return longest > 0 ? longest : 1;
-  const int64_t K = (work + 2047) / 2048;
-  return (int)(K < 8 ? 8 : K < longest ? K : longest);
+  if (longest < 1 || nb < 1 || r < 1 || p < 1) return 1;
+  const int RB = (r + 31) / 32;
+  // segments as many as the longest would leave of the chunks
+  const double seqs = (double)nb * nch / longest;
+  const int out = (p + 63) / 64, first = ((p + 15) / 16 + 2 * RB + 3) / 4;
+  auto rounds = [](double wgs) { return wgs <= 512 ? 1.0 : wgs / 512; };
+  int best = longest;
+  double least = 0;
+  for (int G = 1; G <= 256 && (G == 1 || longest / G >= 2); ++G) {
+    const int K = (longest + G - 1) / G;
+    double t = rounds(seqs * G * out) * K * (2.5 + 0.6 * RB);
+    if (G > 1) t += rounds(seqs * (G - 1) * first) * K * (1.5 + 0.4 * RB) + G * 0.65 * RB + 10;
+    if (G == 1 || t < least) {
+      least = t;
+      best = K;
+    }
+  }
+  return best;
 }
 
 extern "C" int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg,

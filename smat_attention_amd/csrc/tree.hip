@@ -9,11 +9,12 @@
 //
 // Bound by reading the tables (r p fp32 a level and sequence).  A wave owns 15 value
 // columns and the normaliser's, so its division needs no other wave; it adds S and
-// U_h in registers and multiplies the level's nodes by the sum on bf16 MFMA in three
-// terms (fp32's 24 bits; two for the features in fp16, three in fp32).  The scores
-// phi_j . psi_a are formed once a workgroup; their product with vb runs over the
-// ancestors alone on the vector units, so a value of another branch, infinite or NaN,
-// never meets a zero.
+// U_h in registers, the next level's U_h in flight meanwhile, and multiplies the
+// level's nodes by the sum on bf16 MFMA in three terms (fp32's 24 bits; two for the
+// features in fp16, three in fp32).  What every level needs of the nodes, their Phi
+// rows and all scores phi_j . psi_a, is formed once a workgroup, in LDS.  The masked
+// scores meet vb on MFMA too; a vb that is not finite is left out there, where it would
+// meet other branches' zeros, and added to its descendants alone.
 #include "delta_common.hpp"
 
 namespace smat {
@@ -37,104 +38,151 @@ struct Args {
   int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st;
 };
 
+constexpr int kScLd = kMaxNodes + 4;
+// LDS: Phi's fragments by place in the order, the scores, and each wave's vb columns.
+template <typename In, int RB> constexpr int tree_lds(int W) {
+  return dl::Terms<In>::in * 4 * RB * dl::kFrag * 2 + kMaxNodes * kScLd * 4 +
+         W * kMaxNodes * 16 * 4;
+}
+
 template <typename In, int RB>
 __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
     const In* __restrict__ phi, const In* __restrict__ psi, const In* __restrict__ vb,
     const float* __restrict__ S, const float* __restrict__ U, float* __restrict__ out, Args g,
-    int tiles, bool qvec, bool kvec) {
-  constexpr int NT = dl::Terms<In>::in;
-  __shared__ __align__(16) float sc[16][kMaxNodes + 4];
-  const int s = blockIdx.x, W = blockDim.x >> 6;
-  const int m = lane_id() & 15, gq = lane_id() >> 4;
-  const int tile = blockIdx.y * W + wave_id();     // may lie past the last: computes, never stores
+    bool qvec, bool kvec) {
+  constexpr int NT = dl::Terms<In>::in, FP = 4 * RB * dl::kFrag;
+  extern __shared__ __align__(16) bf16 lds[];
+  bf16* ph = lds;
+  float* sc = reinterpret_cast<float*>(ph + NT * FP);          // [place j][node a]
+  const int s = blockIdx.x, w = dl::uniform_wave(), W = blockDim.x >> 6;
+  float* vl = sc + kMaxNodes * kScLd + w * kMaxNodes * 16;     // [node a][lane's column]
+  const int lane = lane_id(), m = lane & 15, gq = lane >> 4;
   const int tree = g.trees == 1 ? 0 : s / (g.nb / g.trees);
   const int64_t* anc = g.anc + (int64_t)tree * g.M;
   const int32_t* order = g.order + (int64_t)tree * g.M;
   const int32_t* lstart = g.lstart + (int64_t)tree * (g.M + 1);
-  const int nval = g.p - 1;
-  const int v0 = tile * 15;                        // value columns v0 .. v0 + 14, then p - 1
+  const int nval = g.p - 1, used = lstart[g.levels];
+  // value columns v0 .. v0 + 14, then p - 1 (a wave past the last tile: p - 1 alone)
+  const int v0 = (blockIdx.y * W + w) * 15;
   const bool mine = m < 15 && v0 + m < nval;
   const int col = mine ? v0 + m : nval;
   const int64_t at = g.step + (g.ahead ? max(0, g.ahead[s / (g.nb / g.requests)]) : 0);
+  const uint32_t M1 = g.M - 1;
 
-  const float* Sb = S + (int64_t)s * g.r * g.p + col;
-  f32x4 St[2 * RB];
+  // rows past r read the last one; their features are zero
+  uint32_t off[2 * RB];
 #pragma unroll
-  for (int mt = 0; mt < 2 * RB; ++mt)
+  for (int mt = 0; mt < 2 * RB; ++mt) off[mt] = (uint32_t)(16 * mt + 4 * gq) * g.p + col;
+  const uint32_t last = (uint32_t)(g.r - 1) * g.p + col;
+  auto load_table = [&](f32x4* x, const float* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int a = 16 * mt + 4 * gq + i;
-      St[mt][i] = a < g.r ? Sb[(int64_t)a * g.p] : 0.f;
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[mt][i] = p[min(off[mt] + i * (uint32_t)g.p, last)];
+  };
+  auto table = [&](int l) {
+    return U + ((int64_t)s * g.B + (at + l) % g.B) * g.r * g.p;
+  };
+  f32x4 St[2 * RB], Ut[2 * RB];
+  load_table(St, S + (int64_t)s * g.r * g.p);
+  load_table(Ut, table(min((int)blockIdx.z, max(g.levels - 1, 0))));
+
+  // this wave's columns of vb; an unused node's are zero
+  bool odd = false;
+  for (int a0 = 0; a0 < g.M; a0 += 4) {
+    const uint32_t a = min((uint32_t)(a0 + gq), M1);
+    const float x = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)a * g.v_st + col]);
+    const float y = anc[a] ? x : 0.f;
+    vl[(a0 + gq) * 16 + m] = y;
+    odd |= !(fabsf(y) < INFINITY);
+  }
+  odd = __any(odd);
+  // Phi by place, and the scores, tile by tile
+  const int tiles = (g.M + 15) / 16;
+  for (int t = w; t < tiles * tiles; t += W) {
+    const int jt = t / tiles, ta = t % tiles;
+    const uint32_t node = order[min((uint32_t)(16 * jt + m), M1)], a = min((uint32_t)(16 * ta + m), M1);
+    const In* qr = phi + (int64_t)s * g.q_sb + (int64_t)node * g.q_st;
+    const In* kr = psi + (int64_t)s * g.k_sb + (int64_t)a * g.k_st;
+    f32x4 x = zero4();
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) {
+      const int c = 32 * kb + 4 * gq;
+      const Frag<NT> pf =
+          split<NT>(load4(qr + c, g.r - c, qvec), load4(qr + c + 16, g.r - c - 16, qvec));
+      if (ta == 0) dl::store_frag<NT>(ph + (jt * RB + kb) * dl::kFrag, FP, pf);
+      x = mul(x, split<NT>(load4(kr + c, g.r - c, kvec), load4(kr + c + 16, g.r - c - 16, kvec)),
+              pf);                                 // place in the lane, a in registers
     }
+    *reinterpret_cast<f32x4*>(sc + (16 * jt + m) * kScLd + 16 * ta + 4 * gq) = x;
+  }
+  __syncthreads();
+  Frag<NT> vf[2];
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    f32x4 x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = 32 * kb + 16 * h + 4 * gq + i;
+        const float y = a < g.M ? vl[a * 16 + m] : 0.f;
+        x[h][i] = fabsf(y) < INFINITY ? y : 0.f;
+      }
+    vf[kb] = split<NT>(x[0], x[1]);
+  }
+
   for (int l = blockIdx.z; l < g.levels; l += gridDim.z) {
     const int n0 = lstart[l], n1 = lstart[l + 1];
-    if (n0 >= n1) break;                           // this tree has fewer levels (uniform)
-    const int64_t h = (at + l) % g.B;
-    const float* Ub = U + ((int64_t)s * g.B + h) * g.r * g.p + col;
+    if (n0 >= n1) break;                           // this tree has fewer levels
     Frag<3> tb[RB];
-    {
-      f32x4 t[2 * RB];
 #pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int a = 16 * mt + 4 * gq + i;
-          t[mt][i] = a < g.r ? Ub[(int64_t)a * g.p] : 0.f;
-        }
-#pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
-        tb[kb] = split<3>(St[2 * kb] + t[2 * kb], St[2 * kb + 1] + t[2 * kb + 1]);
-    }
+    for (int kb = 0; kb < RB; ++kb)
+      tb[kb] = split<3>(St[2 * kb] + Ut[2 * kb], St[2 * kb + 1] + Ut[2 * kb + 1]);
+    load_table(Ut, table(min(l + (int)gridDim.z, g.levels - 1)));   // (no branch: the last again)
     for (int n = n0; n < n1; n += 16) {
-      const int node = order[min(n + m, n1 - 1)];
-      uint64_t mask = (uint64_t)anc[node];
-      uint64_t all = mask;                         // ancestors of any node of this tile
-#pragma unroll
-      for (int d = 1; d < 16; d <<= 1) all |= __shfl_xor((unsigned long long)all, d);
-      const In* row = phi + (int64_t)s * g.q_sb + (int64_t)node * g.q_st;
-      Frag<NT> pf[RB];
+      const int j = min(n + m, n1 - 1);
+      const uint64_t mask = (uint64_t)anc[order[j]];
       f32x4 acc = zero4();
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) {
-        const int c = 32 * kb + 4 * gq;
-        pf[kb] = split<NT>(load4(row + c, g.r - c, qvec), load4(row + c + 16, g.r - c - 16, qvec));
-        acc = mul(acc, pf[kb], tb[kb]);            // column in the lane, nodes 4 gq + i
-      }
-      __syncthreads();                             // the last tile's scores are read
-      for (int a0 = 16 * wave_id(); a0 < g.M; a0 += 16 * W) {
-        if (((all >> a0) & 0xffff) == 0) continue; // uniform over the wave
-        const int a = min(a0 + m, g.M - 1);
-        const In* kr = psi + (int64_t)s * g.k_sb + (int64_t)a * g.k_st;
-        f32x4 x = zero4();
+      for (int kb = 0; kb < RB; ++kb)              // column in the lane, places 4 gq + i
+        acc = mul(acc,
+                  dl::load_frag<NT>(ph + ((j >> 4) * RB + kb) * dl::kFrag, FP, gq * 16 + (j & 15)),
+                  tb[kb]);
 #pragma unroll
-        for (int kb = 0; kb < RB; ++kb) {
-          const int c = 32 * kb + 4 * gq;
-          x = mul(x, split<NT>(load4(kr + c, g.r - c, kvec), load4(kr + c + 16, g.r - c - 16, kvec)),
-                  pf[kb]);                         // node in the lane, a in registers
+      for (int kb = 0; kb < 2; ++kb)
+        if (32 * kb < g.M) {
+          f32x4 x[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int a = 32 * kb + 16 * h + 4 * gq;
+            const f32x4 y = *reinterpret_cast<const f32x4*>(sc + j * kScLd + a);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[h][i] = (mask >> (a + i)) & 1 ? y[i] : 0.f;
+          }
+          acc = mul(acc, split<3>(x[0], x[1]), vf[kb]);
         }
-        *reinterpret_cast<f32x4*>(&sc[m][a0 + 4 * gq]) = x;
-      }
-      __syncthreads();
-      uint64_t mine4[4];
+      if (odd) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mine4[i] = __shfl((unsigned long long)mask, 4 * gq + i);
-      for (uint64_t left = all; left; left &= left - 1) {
-        const int a = __ffsll((unsigned long long)left) - 1;
-        const float x = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)a * g.v_st + col]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          acc[i] = (mine4[i] >> a) & 1 ? acc[i] + sc[4 * gq + i][a] * x : acc[i];
+        for (int i = 0; i < 4; ++i) {
+          const int ji = min(n + 4 * gq + i, n1 - 1);
+          for (uint64_t left = (uint64_t)anc[order[ji]]; left; left &= left - 1) {
+            const int a = __ffsll((unsigned long long)left) - 1;
+            const float y = vl[a * 16 + m];
+            if (!(fabsf(y) < INFINITY)) acc[i] += sc[ji * kScLd + a] * y;
+          }
+        }
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float den = __shfl(acc[i], gq * 16 + 15);
-        const int j = n + 4 * gq + i;
-        if (mine && j < n1) out[((int64_t)s * g.M + order[j]) * nval + col] = acc[i] / den;
+        const int ji = n + 4 * gq + i;
+        if (mine && ji < n1) out[((int64_t)s * g.M + order[ji]) * nval + col] = acc[i] / den;
       }
     }
   }
   if (blockIdx.z == 0 && mine)                     // unused nodes read nothing and give zeros
-    for (int j = lstart[g.levels] + gq; j < g.M; j += 4)
+    for (int j = used + gq; j < g.M; j += 4)
       out[((int64_t)s * g.M + order[j]) * nval + col] = 0.f;
 }
 
@@ -223,20 +271,22 @@ extern "C" int smat_tree_step(int dtype, const void* phi, const void* psi, const
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(phi && psi && vb && S && U && out && anc && order && lstart, SMAT_EINVAL,
                "%s: null pointer", who);
+  // a workgroup takes half of the column tiles (a third while sequences are few); its waves
+  // walk every z-th level, z as large as leaves the GPU full
   const int tiles = (p - 1 + 14) / 15;
-  // a wave walks every level with S in registers while the sequences fill the GPU;
-  // else levels and columns are spread over workgroups
-  const bool few = nb < 256;
-  const int W = few ? (tiles + 2) / 3 : (tiles + 1) / 2;
-  int z = few ? (256 * 4 + nb * tiles - 1) / (nb * tiles) : 1;
+  const int W = nb < 64 ? (tiles + 2) / 3 : (tiles + 1) / 2;
+  int z = (int)(2048 / ((int64_t)nb * tiles));
   z = z < 1 ? 1 : z > levels ? (levels > 0 ? levels : 1) : z;
   return dl::dispatch(dtype, r, [&](auto in, auto rb) {
     typedef decltype(in) In;
-    constexpr int eb = sizeof(In);
-    hipLaunchKernelGGL((tree_step_kernel<In, decltype(rb)::value>),
-                       dim3(nb, (tiles + W - 1) / W, z), dim3(64 * W), 0, (hipStream_t)stream,
-                       (const In*)phi, (const In*)psi, (const In*)vb, S, U, out, g, tiles,
-                       dl::vec4_ok(phi, q_sb, q_st, eb), dl::vec4_ok(psi, k_sb, k_st, eb));
+    constexpr int eb = sizeof(In), RB = decltype(rb)::value;
+    const int lds = tree_lds<In, RB>(W);
+    auto kern = tree_step_kernel<In, RB>;
+    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
+                              tree_lds<In, RB>(kMaxWaves));
+    hipLaunchKernelGGL(kern, dim3(nb, (tiles + W - 1) / W, z), dim3(64 * W), lds,
+                       (hipStream_t)stream, (const In*)phi, (const In*)psi, (const In*)vb, S, U,
+                       out, g, dl::vec4_ok(phi, q_sb, q_st, eb), dl::vec4_ok(psi, k_sb, k_st, eb));
     return launch_status(who);
   });
 }

@@ -203,10 +203,10 @@ def test_c_entry_points_refuse():
 def test_run_lengths():
     q = lambda *a: _lib.query("smat_delta_run_chunks", *a)
     assert q(512, 1000, 1000, 64, 64) == 1000        # enough sequences: whole segments
-    assert q(1, 10, 10, 64, 64) == 10                # too short to split
+    assert q(1, 3, 3, 64, 64) == 3                   # too short to split
     assert q(1, 0, 0, 64, 64) == 1
-    assert 8 <= q(8, 2048, 2048, 128, 128) < 2048
-    assert 8 <= q(1, 100, 90, 64, 64) < 90           # one long segment among short ones
+    assert 2 <= q(8, 2048, 2048, 128, 128) < 2048
+    assert 2 <= q(1, 100, 90, 64, 64) < 90           # one long segment among short ones
 
 
 def test_oracle_is_the_plain_rule():
