@@ -121,7 +121,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     const int64_t sc = (int64_t)s * g.nch + c;
     const bf16* kt = kl + buf * TL;
     const float* vec = vl + buf * kVec;
-    const int lane = fresh_lane(), fm = lane & 15, f4 = 4 * (lane >> 4);
+    const int lane = RB >= 3 ? fresh_lane() : lane_id(), fm = lane & 15, f4 = 4 * (lane >> 4);
     chunk_of(g, more ? c + 1 : c, t1, len1);
     wait_vmcnt<0>();
     lds_barrier();
