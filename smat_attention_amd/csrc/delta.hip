@@ -393,7 +393,8 @@ static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipS
   constexpr int W = chain_waves<In, RB, OUT>();
   static_assert(lds <= kMaxLds, "");
   auto kern = delta_chain_kernel<In, RB, OUT>;
-  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  static uint64_t done;
+  allow_lds(kern, lds, done);
   hipLaunchKernelGGL(kern, dim3((tiles + W - 1) / W, g.nruns, g.nb), dim3(64 * W), lds, st, g, o,
                      io, tiles);
 }
@@ -508,6 +509,8 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
                SMAT_EINVAL, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who,
                (long long)workspace_bytes, (long long)need);
   hipStream_t st = (hipStream_t)stream;
+  if (!chunks && !save_s && T >= 1 && T <= kFewTokens)
+    return launch_tokens(dtype, g, q, k, v, logA, beta, state, state_out, out, st);
   auto go = [&](auto in, auto rb) {
     typedef decltype(in) In;
     return scan<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, v, logA, beta,

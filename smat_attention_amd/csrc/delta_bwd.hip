@@ -557,7 +557,8 @@ static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hi
   constexpr int lds = rchain_lds<In, RB>(rchain_bufs<In, RB>()), W = rchain_waves<In, RB>();
   static_assert(lds <= kMaxLds, "");
   auto kern = delta_rchain_kernel<In, RB, OUT>;
-  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  static uint64_t done;
+  allow_lds(kern, lds, done);
   hipLaunchKernelGGL(kern, dim3((tiles + W - 1) / W, g.nruns, g.nb), dim3(64 * W), lds, st, g, o,
                      io, tiles);
 }
@@ -610,7 +611,8 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
                                : delta_grad_kernel<In, RB, true, false>)
                        : (full ? delta_grad_kernel<In, RB, false, true>
                                : delta_grad_kernel<In, RB, false, false>);
-    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    static uint64_t done[4];
+    allow_lds(kern, lds, done[2 * shared + full]);
     hipLaunchKernelGGL(kern, dim3(g.nch, g.nbk), dim3(256 * grad_split(RB)), lds, st, g, o, gr);
   }
   return launch_status("smat_delta_scan_backward");

@@ -641,6 +641,21 @@ inline int dispatch(int dtype, int r, F fn) {
 
 // The checks that the forward and the backward share.
 int check_geo(const char* who, int dtype, const Geo& g);
+// Up to this many tokens a sequence are taken one after another (delta_step.hip).
+constexpr int kFewTokens = 16;
+int launch_tokens(int dtype, const Geo& g, const void* q, const void* k, const void* v,
+                  const float* logA, const float* beta, const float* S_in, float* S_out, void* o,
+                  hipStream_t st);
+// hipFuncSetAttribute for a kernel's LDS, once a device.
+template <typename K> inline void allow_lds(K kern, int bytes, uint64_t& done) {
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit) return;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+}
+
 // Launches the runs' carry (both directions).
 int launch_carry(const Geo& g, const float* init, const Carry& c, bool rev, hipStream_t st);
 

@@ -282,8 +282,8 @@ extern "C" int smat_tree_step(int dtype, const void* phi, const void* psi, const
     constexpr int eb = sizeof(In), RB = decltype(rb)::value;
     const int lds = tree_lds<In, RB>(W);
     auto kern = tree_step_kernel<In, RB>;
-    (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              tree_lds<In, RB>(kMaxWaves));
+    static uint64_t done;
+    dl::allow_lds(kern, tree_lds<In, RB>(kMaxWaves), done);
     hipLaunchKernelGGL(kern, dim3(nb, (tiles + W - 1) / W, z), dim3(64 * W), lds,
                        (hipStream_t)stream, (const In*)phi, (const In*)psi, (const In*)vb, S, U,
                        out, g, dl::vec4_ok(phi, q_sb, q_st, eb), dl::vec4_ok(psi, k_sb, k_st, eb));

@@ -8,25 +8,16 @@ raises.  :mod:`smat_attention_amd.attention` has the public entry points.
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import numpy as np
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import call, ptr, stream_of
-from .hip_fwd import _code, _on_gpu, _rows3, _shape
+from ._lib import ptr
+from .hip_fwd import _call_on, _code, _on_gpu, _rows3, _shape
 
 CHUNK = 64
 MAX_R, MAX_P = 128, 256
-
-
-def on_device(t: torch.Tensor):
-    """Launches go to ``t``'s device, whichever is the current one."""
-    if t.get_device() == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(t.device)
 
 
 def same_device(who: str, ref: torch.Tensor, *ts) -> None:
@@ -135,13 +126,17 @@ def check_scan(who, Q, K, V, logA, beta, state, segments):
     """The argument checks of the whole-sequence form."""
     if Q.dim() != 3 or V.dim() != 3:
         raise ValueError(f"{who}: Q, K and V must be (sequences, T, columns)")
-    same_device(who, Q, K, V, logA, beta, state)
+    dev = Q.device
+    if not (Q.is_cuda and dev == K.device == V.device == logA.device == beta.device
+            and (state is None or state.device == dev)):
+        same_device(who, Q, K, V, logA, beta, state)
     nbk, T, r = Q.shape
     nb, _, p = V.shape
-    _shape(who, "K", K, (nbk, T, r))
-    _shape(who, "V", V, (nb, T, p))
-    _shape(who, "logA", logA, (nb, T))
-    _shape(who, "beta", beta, (nb, T))
+    if not (K.shape == Q.shape and V.shape[1] == T and logA.shape == beta.shape == (nb, T)):
+        _shape(who, "K", K, (nbk, T, r))
+        _shape(who, "V", V, (nb, T, p))
+        _shape(who, "logA", logA, (nb, T))
+        _shape(who, "beta", beta, (nb, T))
     if (nbk == 0) != (nb == 0) or (nbk and nb % nbk):
         raise ValueError(f"{who}: {nbk} key sequences do not divide {nb} value sequences")
     _check_types(who, Q, K, V, logA, beta, state)
@@ -189,11 +184,10 @@ def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bo
     ws, n = plan.workspace(code, 0, dev)
     if state is not None:
         state = state.contiguous()
-    with on_device(Q):
-        call("smat_delta_scan", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(), logA.data_ptr(),
-             beta.data_ptr(), ptr(state), o.data_ptr(), ptr(s_out), ptr(save_s) or None,
-             ptr(save_u) or None, *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st,
-             *logA.stride(), *beta.stride(), ws.data_ptr(), n, stream_of(Q))
+    _call_on(Q, "smat_delta_scan", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
+             logA.data_ptr(), beta.data_ptr(), ptr(state) or None, o.data_ptr(),
+             ptr(s_out) or None, ptr(save_s) or None, ptr(save_u) or None, *plan.sizes(scale),
+             q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(), *beta.stride(), ws.data_ptr(), n)
     return o, s_out, save_s, save_u, (Q, K, V, logA, beta)
 
 
@@ -216,12 +210,11 @@ def scan_backward(inputs, save_s, save_u, dO, dS, scale, segments, want_dstate: 
     ws, n = plan.workspace(code, 1, dev)
     if dS is not None:
         dS = dS.contiguous()
-    with on_device(Q):
-        call("smat_delta_scan_backward", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
+    _call_on(Q, "smat_delta_scan_backward", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
              logA.data_ptr(), beta.data_ptr(), dO.data_ptr(), ptr(dS), save_s.data_ptr(),
              save_u.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlogA.data_ptr(),
              dbeta.data_ptr(), ptr(dstate), *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb,
-             v_st, *logA.stride(), *beta.stride(), d_sb, d_st, ws.data_ptr(), n, stream_of(Q))
+             v_st, *logA.stride(), *beta.stride(), d_sb, d_st, ws.data_ptr(), n)
     return dQ, dK, dV, dlogA, dbeta, dstate
 
 
@@ -306,9 +299,5 @@ def step(q, k, v, logA, beta, state, scale, out, out_state):
     args = (_code(q, who), q.data_ptr(), k.data_ptr(), v.data_ptr(), logA.data_ptr(),
             beta.data_ptr(), state.data_ptr(), out_state.data_ptr(), out.data_ptr(), nb,
             max(nbk, 1), r, p, scale, q_sb, k_sb, v_sb, logA.stride(0), beta.stride(0))
-    if dev.index == torch.cuda.current_device():
-        call("smat_delta_step", *args, stream_of(q))
-    else:
-        with torch.cuda.device(dev):
-            call("smat_delta_step", *args, stream_of(q))
+    _call_on(q, "smat_delta_step", *args)
     return out

@@ -724,16 +724,32 @@ def _tree_inputs(who, tree, nb, R, P, device, **rows):
         raise ValueError(f"{who}: the tree is on {tree.device}, the cache on {device}")
     if nb % tree.trees:
         raise ValueError(f"{who}: {tree.trees} trees do not divide {nb} sequences")
-    ref = next(iter(rows.values()))
-    got = []
+    got, M, ref = [], tree.nodes, None
     for name, t in rows.items():
-        _shape(who, name, t, (nb, tree.nodes, P if name == "Vb" else R))
+        if t.shape != (nb, M, P if name == "Vb" else R):
+            _shape(who, name, t, (nb, M, P if name == "Vb" else R))
         if t.device != device:
             raise ValueError(f"{who}: {name} is on {t.device}, the cache on {device}")
-        _same_dtype(who, ref, **{name: t})
-        got += _rows3(t)
+        if ref is None:
+            ref = t
+        elif t.dtype != ref.dtype:
+            _same_dtype(who, ref, **{name: t})
+        sb, st, s1 = t.stride()
+        if s1 != 1:
+            t = t.contiguous()
+            sb, st, _ = t.stride()
+        got += (t, sb, st)
     _code(ref, who)
     return got
+
+
+def _call_on(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` on ``t``'s device, whichever is the current one, and its current stream."""
+    if t.get_device() == torch.cuda.current_device():
+        call(name, *args, stream_of(t))
+    else:
+        with torch.cuda.device(t.device):
+            call(name, *args, stream_of(t))
 
 
 def tree_step(Phi, Psi, Vb, tree: DraftTree, S, U, step: int, *, ahead=None, out=None):
@@ -754,12 +770,11 @@ def tree_step(Phi, Psi, Vb, tree: DraftTree, S, U, step: int, *, ahead=None, out
         raise ValueError(f"{who}: out must be contiguous fp32 {want} on {S.device}")
     if not (S.is_contiguous() and U.is_contiguous() and S.dtype == U.dtype == torch.float32):
         raise ValueError(f"{who}: S and U must be contiguous fp32")
-    with torch.cuda.device(S.device):
-        call("smat_tree_step", _code(Phi, who), Phi.data_ptr(), Psi.data_ptr(), Vb.data_ptr(),
+    _call_on(S, "smat_tree_step", _code(Phi, who), Phi.data_ptr(), Psi.data_ptr(), Vb.data_ptr(),
              S.data_ptr(), U.data_ptr(), out.data_ptr(), tree.anc.data_ptr(),
              tree.order.data_ptr(), tree.lstart.data_ptr(), ptr(ahead) or None, nb, tree.trees,
              ahead.numel() if ahead is not None else 1, tree.nodes, tree.levels, U.shape[1], R, P,
-             int(step), q_sb, q_st, k_sb, k_st, v_sb, v_st, stream_of(S))
+             int(step), q_sb, q_st, k_sb, k_st, v_sb, v_st)
     return out
 
 
@@ -782,8 +797,7 @@ def tree_state(Psi, Vb, tree: DraftTree, nodes, S, S_out, *, ahead=None):
         raise ValueError(f"{who}: S and S_out must be contiguous fp32 on one device")
     if abs(S.data_ptr() - S_out.data_ptr()) < S.numel() * 4:
         raise ValueError(f"{who}: S and S_out must be distinct buffers")
-    with torch.cuda.device(S.device):
-        call("smat_tree_state", _code(Psi, who), Psi.data_ptr(), Vb.data_ptr(), S.data_ptr(),
+    _call_on(S, "smat_tree_state", _code(Psi, who), Psi.data_ptr(), Vb.data_ptr(), S.data_ptr(),
              S_out.data_ptr(), tree.anc.data_ptr(), nodes.data_ptr(), ptr(ahead) or None, nb,
-             tree.trees, nodes.numel(), tree.nodes, R, P, k_sb, k_st, v_sb, v_st, stream_of(S))
+             tree.trees, nodes.numel(), tree.nodes, R, P, k_sb, k_st, v_sb, v_st)
     return S_out
