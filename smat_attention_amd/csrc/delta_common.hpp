@@ -100,16 +100,26 @@ template <int N, int M> __device__ __forceinline__ Frag<N> lead(const Frag<M>& f
   return g;
 }
 
-// c += a b over the terms of order below max(NA, NB), small ones first.
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mul(f32x4 c, const Frag<NA>& a, const Frag<NB>& b) {
-  constexpr int M = NA > NB ? NA : NB;
+// c += a b over the terms of order below M, by default max(NA, NB), small ones first.
+// Two fp16 inputs want order 2 as well: their second terms are 2^-9 of the first, and
+// where fp32 accuracy is due their product counts.
+template <int M, int NA, int NB>
+__device__ __forceinline__ f32x4 mul_below(f32x4 c, const Frag<NA>& a, const Frag<NB>& b) {
 #pragma unroll
   for (int o = M - 1; o >= 0; --o)
 #pragma unroll
     for (int i = 0; i < NA; ++i)
       if (o - i >= 0 && o - i < NB) c = mma(c, a.t[i], b.t[o - i]);
   return c;
+}
+
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mul(f32x4 c, const Frag<NA>& a, const Frag<NB>& b) {
+  return mul_below<(NA > NB ? NA : NB)>(c, a, b);
+}
+template <int N>
+__device__ __forceinline__ f32x4 mul_inputs(f32x4 c, const Frag<N>& a, const Frag<N>& b) {
+  return mul_below<(N == 1 ? 1 : 3)>(c, a, b);
 }
 
 // The same for U products at once, term by term across them, so that consecutive

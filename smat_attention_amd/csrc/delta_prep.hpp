@@ -226,8 +226,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
 #pragma unroll
         for (int kb = 0; kb < RB; ++kb) {
           const Frag<NT> kj = load_frag<NT>(rows + (jt * RB + kb) * kFrag, KB);
-          a = mul(a, kj, kf[kb]);
-          P = mul(P, kj, qf[kb]);
+          a = mul_inputs(a, kj, kf[kb]);
+          P = mul_inputs(P, kj, qf[kb]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -254,7 +254,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
         f32x4 a = zero4();
 #pragma unroll
         for (int kb = 0; kb < RB; ++kb)
-          a = mul(a, load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
+          a = mul_inputs(a, load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int ti = 16 * it + 4 * gq + i;
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
       if (it >= w) {
 #pragma unroll
         for (int kb = 0; kb < RB; ++kb)
-          pacc[it] = mul(pacc[it], load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
+          pacc[it] = mul_inputs(pacc[it], load_frag<NT>(rows + (it * RB + kb) * kFrag, KB), kf[kb]);
         // selected, not multiplied: a query that is not finite stays in its own row
 #pragma unroll
         for (int i = 0; i < 4; ++i)

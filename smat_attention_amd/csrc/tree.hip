@@ -111,7 +111,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
       const Frag<NT> pf =
           split<NT>(load4(qr + c, g.r - c, qvec), load4(qr + c + 16, g.r - c - 16, qvec));
       if (ta == 0) dl::store_frag<NT>(ph + (jt * RB + kb) * dl::kFrag, FP, pf);
-      x = mul(x, split<NT>(load4(kr + c, g.r - c, kvec), load4(kr + c + 16, g.r - c - 16, kvec)),
+      x = dl::mul_inputs(x, split<NT>(load4(kr + c, g.r - c, kvec), load4(kr + c + 16, g.r - c - 16, kvec)),
               pf);                                 // place in the lane, a in registers
     }
     *reinterpret_cast<f32x4*>(sc + (16 * jt + m) * kScLd + 16 * ta + 4 * gq) = x;

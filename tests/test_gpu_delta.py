@@ -119,6 +119,25 @@ def test_scan_and_gradients(dtype, nb, nbk, T, r, p, off, st):
             _check(name, a, b, 2 * chunks, r, p)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_fp32_results_have_fp32_accuracy(dtype):
+    """The state and the gates' gradients are fp32 whatever the inputs' type.  One chunk: each
+    value is off by about sqrt(r + p + 128) independent roundings of 2^-24; twice that in the
+    mean over the values."""
+    nb, T, r, p = 4, 64, 64, 64
+    q, k, v, logA, beta, S = _inputs(nb, nb, T, r, p, dtype, seed=21, state=())
+    x = [t.requires_grad_(True) for t in (q, k, v, logA, beta, S)]
+    o, So = A.gated_delta_scan(*x[:5], state=S, return_state=True)
+    y = [t.detach().double().requires_grad_(True) for t in x]
+    ro, rS = O.delta_scan(*y[:5], state=y[5])
+    dO = torch.randn(o.shape, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    got = (So, *torch.autograd.grad(o, x[3:], dO))
+    ref = (rS, *torch.autograd.grad(ro, y[3:], dO.double()))
+    for name, a, b in zip(("S", "dlogA", "dbeta", "dS0"), got, ref):
+        off = ((a.detach().double() - b.detach()).norm() / b.detach().norm()).item()
+        assert off <= 2 * math.sqrt(r + p + 128) * 2.0 ** -24, (name, off)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("nb,nbk,T,r,p,off,st", [
     (2, 2, 64 * 40 + 5, 64, 64, None, True),
