@@ -39,9 +39,10 @@ struct Args {
 };
 
 constexpr int kScLd = kMaxNodes + 4;
-// LDS: Phi's fragments by place in the order, the scores, and each wave's vb columns.
+// LDS: Phi's fragments by place in the order, Psi's, the scores, and each wave's vb
+// columns.
 template <typename In, int RB> constexpr int tree_lds(int W) {
-  return dl::Terms<In>::in * 4 * RB * dl::kFrag * 2 + kMaxNodes * kScLd * 4 +
+  return 2 * dl::Terms<In>::in * 4 * RB * dl::kFrag * 2 + kMaxNodes * kScLd * 4 +
          W * kMaxNodes * 16 * 4;
 }
 
@@ -52,8 +53,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
     bool qvec, bool kvec) {
   constexpr int NT = dl::Terms<In>::in, FP = 4 * RB * dl::kFrag;
   extern __shared__ __align__(16) bf16 lds[];
-  bf16* ph = lds;
-  float* sc = reinterpret_cast<float*>(ph + NT * FP);          // [place j][node a]
+  bf16 *ph = lds, *ps = ph + NT * FP;
+  float* sc = reinterpret_cast<float*>(ps + NT * FP);          // [place j][node a]
   const int s = blockIdx.x, w = dl::uniform_wave(), W = blockDim.x >> 6;
   float* vl = sc + kMaxNodes * kScLd + w * kMaxNodes * 16;     // [node a][lane's column]
   const int lane = lane_id(), m = lane & 15, gq = lane >> 4;
@@ -69,6 +70,37 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
   const int64_t at = g.step + (g.ahead ? max(0, g.ahead[s / (g.nb / g.requests)]) : 0);
   const uint32_t M1 = g.M - 1;
 
+  // In issue order: vb's columns, Phi and Psi rows, then the tables, which arrive while
+  // the scores are formed.
+  // lane = node: its word; lane = place: the node there and its word; lane = level: its start
+  const uint64_t word = (uint64_t)anc[min((uint32_t)lane, M1)];
+  const int ord = order[min((uint32_t)lane, M1)], begin = lstart[min(lane, g.levels)];
+  const uint64_t path = (uint64_t)anc[ord];
+  float vr[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    vr[i] = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)min((uint32_t)(4 * i + gq), M1) * g.v_st + col]);
+  // tile u < 4: Phi's places 16 u .., else Psi's nodes 16 (u - 4) ..
+  const int tiles = (g.M + 15) / 16;
+  for (int u = w; u < 8; u += W) {
+    const int t = u & 3;
+    if (t >= tiles) continue;
+    const uint32_t place = min((uint32_t)(16 * t + m), M1);
+    const bool q = u < 4;
+    const In* row = q ? phi + (int64_t)s * g.q_sb + (int64_t)__shfl(ord, (int)place) * g.q_st
+                      : psi + (int64_t)s * g.k_sb + (int64_t)place * g.k_st;
+    f32x4 x[RB][2];
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = 32 * kb + 16 * h + 4 * gq;
+        x[kb][h] = load4(row + c, g.r - c, q ? qvec : kvec);
+      }
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb)
+      dl::store_frag<NT>((q ? ph : ps) + (t * RB + kb) * dl::kFrag, FP, split<NT>(x[kb][0], x[kb][1]));
+  }
   // rows past r read the last one; their features are zero
   uint32_t off[2 * RB];
 #pragma unroll
@@ -88,35 +120,27 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
   load_table(Ut, table(min((int)blockIdx.z, max(g.levels - 1, 0))));
 
   // this wave's columns of vb; an unused node's are zero
+  const uint64_t in_use = __ballot(word != 0 && lane < g.M);
   bool odd = false;
-  for (int a0 = 0; a0 < g.M; a0 += 4) {
-    const uint32_t a = min((uint32_t)(a0 + gq), M1);
-    const float x = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)a * g.v_st + col]);
-    const float y = anc[a] ? x : 0.f;
-    vl[(a0 + gq) * 16 + m] = y;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int a = 4 * i + gq;
+    const float y = (in_use >> a) & 1 ? vr[i] : 0.f;
+    vl[a * 16 + m] = y;
     odd |= !(fabsf(y) < INFINITY);
   }
   odd = __any(odd);
-  // Phi by place, and the scores, tile by tile
-  const int tiles = (g.M + 15) / 16;
+  lds_barrier();                                   // Phi and Psi; the tables stay in flight
   for (int t = w; t < tiles * tiles; t += W) {
     const int jt = t / tiles, ta = t % tiles;
-    const uint32_t node = order[min((uint32_t)(16 * jt + m), M1)], a = min((uint32_t)(16 * ta + m), M1);
-    const In* qr = phi + (int64_t)s * g.q_sb + (int64_t)node * g.q_st;
-    const In* kr = psi + (int64_t)s * g.k_sb + (int64_t)a * g.k_st;
     f32x4 x = zero4();
 #pragma unroll
-    for (int kb = 0; kb < RB; ++kb) {
-      const int c = 32 * kb + 4 * gq;
-      const Frag<NT> pf =
-          split<NT>(load4(qr + c, g.r - c, qvec), load4(qr + c + 16, g.r - c - 16, qvec));
-      if (ta == 0) dl::store_frag<NT>(ph + (jt * RB + kb) * dl::kFrag, FP, pf);
-      x = dl::mul_inputs(x, split<NT>(load4(kr + c, g.r - c, kvec), load4(kr + c + 16, g.r - c - 16, kvec)),
-              pf);                                 // place in the lane, a in registers
-    }
+    for (int kb = 0; kb < RB; ++kb)                // place in the lane, a in registers
+      x = dl::mul_inputs(x, dl::load_frag<NT>(ps + (ta * RB + kb) * dl::kFrag, FP),
+                         dl::load_frag<NT>(ph + (jt * RB + kb) * dl::kFrag, FP));
     *reinterpret_cast<f32x4*>(sc + (16 * jt + m) * kScLd + 16 * ta + 4 * gq) = x;
   }
-  __syncthreads();
+  lds_barrier();
   Frag<NT> vf[2];
 #pragma unroll
   for (int kb = 0; kb < 2; ++kb) {
@@ -133,7 +157,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
   }
 
   for (int l = blockIdx.z; l < g.levels; l += gridDim.z) {
-    const int n0 = lstart[l], n1 = lstart[l + 1];
+    const int n0 = __builtin_amdgcn_readlane(begin, l);
+    const int n1 = l + 1 < g.levels ? __builtin_amdgcn_readlane(begin, l + 1) : used;
     if (n0 >= n1) break;                           // this tree has fewer levels
     Frag<3> tb[RB];
 #pragma unroll
@@ -142,7 +167,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
     load_table(Ut, table(min(l + (int)gridDim.z, g.levels - 1)));   // (no branch: the last again)
     for (int n = n0; n < n1; n += 16) {
       const int j = min(n + m, n1 - 1);
-      const uint64_t mask = (uint64_t)anc[order[j]];
+      const uint64_t mask = __shfl((unsigned long long)path, j);
       f32x4 acc = zero4();
 #pragma unroll
       for (int kb = 0; kb < RB; ++kb)              // column in the lane, places 4 gq + i
@@ -166,7 +191,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int ji = min(n + 4 * gq + i, n1 - 1);
-          for (uint64_t left = (uint64_t)anc[order[ji]]; left; left &= left - 1) {
+          for (uint64_t left = __shfl((unsigned long long)path, ji); left; left &= left - 1) {
             const int a = __ffsll((unsigned long long)left) - 1;
             const float y = vl[a * 16 + m];
             if (!(fabsf(y) < INFINITY)) acc[i] += sc[ji * kScLd + a] * y;
@@ -176,14 +201,16 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float den = __shfl(acc[i], gq * 16 + 15);
-        const int ji = n + 4 * gq + i;
-        if (mine && ji < n1) out[((int64_t)s * g.M + order[ji]) * nval + col] = acc[i] / den;
+        const int ji = n + 4 * gq + i, node = __shfl(ord, min(ji, n1 - 1));
+        if (mine && ji < n1) out[((int64_t)s * g.M + node) * nval + col] = acc[i] / den;
       }
     }
   }
-  if (blockIdx.z == 0 && mine)                     // unused nodes read nothing and give zeros
-    for (int j = used + gq; j < g.M; j += 4)
-      out[((int64_t)s * g.M + order[j]) * nval + col] = 0.f;
+  if (blockIdx.z == 0)                             // unused nodes read nothing and give zeros
+    for (int j0 = used; j0 < g.M; j0 += 4) {
+      const int node = __shfl(ord, min(j0 + gq, (int)M1));
+      if (mine && j0 + gq < g.M) out[((int64_t)s * g.M + node) * nval + col] = 0.f;
+    }
 }
 
 // S' = S + sum of psi_a vb_a^T over the accepted path of each request, ancestors in
