@@ -214,14 +214,16 @@ __global__ __launch_bounds__(64 * kMaxWaves) void tree_step_kernel(
 }
 
 // S' = S + sum of psi_a vb_a^T over the accepted path of each request, ancestors in
-// order, sixteen at a time through LDS; `ahead` moves by the path's length.
+// order, eight at a time through LDS (their rows loaded together); `ahead` moves by the
+// path's length.
 constexpr int kElems = 8;          // elements of S a thread
+constexpr int kBatch = 8;          // ancestors a round
 
 template <typename In>
 __global__ __launch_bounds__(256) void tree_state_kernel(
     const In* __restrict__ psi, const In* __restrict__ vb, const float* __restrict__ S,
     float* __restrict__ So, const int32_t* __restrict__ nodes, int32_t* ahead, Args g) {
-  __shared__ float sp[16][128], sv[16][144];
+  __shared__ float sp[kBatch][128], sv[kBatch][144];
   const int s = blockIdx.x, tid = threadIdx.x;
   const int per = g.nb / g.requests, req = s / per;
   const int tree = g.trees == 1 ? 0 : s / (g.nb / g.trees);
@@ -239,19 +241,32 @@ __global__ __launch_bounds__(256) void tree_state_kernel(
     col[j] = min(e, rp - 1) - row[j] * g.p;
     x[j] = S[base + min(e, rp - 1)];
   }
+  const In* pr = psi + (int64_t)s * g.k_sb + min(tid, g.r - 1);
+  const In* vr = vb + (int64_t)s * g.v_sb + min(tid, g.p - 1);
   uint64_t left = path;
   while (left) {
-    int n = 0;
-    for (; left && n < 16; left &= left - 1, ++n) {
-      const int a = __ffsll((unsigned long long)left) - 1;
-      if (tid < g.r) sp[n][tid] = to_f32(psi[(int64_t)s * g.k_sb + (int64_t)a * g.k_st + tid]);
-      if (tid < g.p) sv[n][tid] = to_f32(vb[(int64_t)s * g.v_sb + (int64_t)a * g.v_st + tid]);
+    int n = 0, at = 0;
+    float a[kBatch], b[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {             // past the path's end: the last one again
+      if (left) {
+        at = __ffsll((unsigned long long)left) - 1;
+        left &= left - 1;
+        ++n;
+      }
+      a[i] = to_f32(pr[(int64_t)at * g.k_st]);
+      b[i] = to_f32(vr[(int64_t)at * g.v_st]);
+    }
+    __syncthreads();                               // the last round's are read
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (tid < g.r) sp[i][tid] = a[i];
+      if (tid < g.p) sv[i][tid] = b[i];
     }
     __syncthreads();
     for (int i = 0; i < n; ++i)
 #pragma unroll
       for (int j = 0; j < kElems; ++j) x[j] += sp[i][row[j]] * sv[i][col[j]];
-    __syncthreads();
   }
 #pragma unroll
   for (int j = 0; j < kElems; ++j) {
