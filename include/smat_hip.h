@@ -567,7 +567,9 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  * state: (nseg, nb, r, p) fp32 entering each segment (NULL: zero); state_out
  * the same leaving it (may be NULL; not state itself).
  * Training: save_s (nb, nch, R, P) and save_u (nb, nch, 64, P) fp32, R and P
- * being r and p rounded up to 32, receive the states entering chunks and U.
+ * being r and p rounded up to 32, receive the states entering chunks and U,
+ * and, if nruns > nseg, save_m (nruns, nb, R, R) fp32 the runs' transitions (of
+ * a segment's last run only if state_out is given); else all three are NULL.
  * workspace: smat_delta_workspace_bytes(..., backward) bytes, 256-byte aligned.
  */
 int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p);
@@ -575,27 +577,28 @@ int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg
                                    int r, int p, int backward);
 int smat_delta_scan(int dtype, const void* q, const void* k, const void* v, const float* logA,
                     const float* beta, const float* state, void* out, float* state_out,
-                    float* save_s, float* save_u, const int32_t* chunks, const int32_t* runs,
-                    const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch, int nruns,
-                    int K, int r, int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
-                    int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st,
-                    int64_t b_sb, int64_t b_st, void* workspace, int64_t workspace_bytes,
-                    void* stream);
+                    float* save_s, float* save_u, float* save_m, const int32_t* chunks,
+                    const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T, int nseg,
+                    int nch, int nruns, int K, int r, int p, float scale, int64_t q_sb,
+                    int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st,
+                    int64_t a_sb, int64_t a_st, int64_t b_sb, int64_t b_st, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
 /*
  * Its gradient: dout (nb, T, p) of dtype with strides and dstate_out (the
  * gradient of state_out, or NULL) -> dq, dk (nbk, T, r), dv (nb, T, p) of
  * dtype, dlogA, dbeta (nb, T) fp32, all contiguous, and dstate (nseg, nb, r,
- * p) fp32 or NULL.  Tokens no segment holds are left as they were.
+ * p) fp32 or NULL.  Sizes, runs and tables are the forward's; dstate_out needs
+ * a forward with state_out.  Tokens no segment holds are left as they were.
  */
 int smat_delta_scan_backward(int dtype, const void* q, const void* k, const void* v,
                              const float* logA, const float* beta, const void* dout,
                              const float* dstate_out, const float* save_s, const float* save_u,
-                             void* dq, void* dk, void* dv, float* dlogA, float* dbeta,
-                             float* dstate, const int32_t* chunks, const int32_t* runs,
-                             const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch,
-                             int nruns, int K, int r, int p, float scale, int64_t q_sb,
-                             int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb,
+                             const float* save_m, void* dq, void* dk, void* dv, float* dlogA,
+                             float* dbeta, float* dstate, const int32_t* chunks,
+                             const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T,
+                             int nseg, int nch, int nruns, int K, int r, int p, float scale,
+                             int64_t q_sb, int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb,
                              int64_t v_st, int64_t a_sb, int64_t a_st, int64_t b_sb,
                              int64_t b_st, int64_t d_sb, int64_t d_st, void* workspace,
                              int64_t workspace_bytes, void* stream);

@@ -27,6 +27,8 @@ struct ChainIO {
   const float* start;     // state entering run i of sequence s: start + (i nb + s) r p; or null
   float* end;             // first pass: the state leaving it, same layout
   float* trans;           // first pass: M of run i, (i nb + s) R R row-major (R = 32 RB)
+  float* save_m;          // training, first pass: M transposed, same layout; or null
+  bool first_m, last_m;   // first pass: whether M of a segment's first, last run is wanted
   float* fin;             // state leaving segment j: fin + (j nb + s) r p; or null
   float *save_s, *save_u; // training: states entering chunks, and U, rows padded to p32; or null
   int ptiles;             // value tiles of 16 columns (tiles behind them are M's)
@@ -62,14 +64,19 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
   constexpr int W = chain_waves<In, RB, OUT>();
   const int w = uniform_wave();
   const int ct = blockIdx.x * W + w;
-  const bool on = ct < tiles;                      // else: copies and barriers only
   const int run = blockIdx.y, s = blockIdx.z;
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
   bool head, tail;
   run_of(g, run, c0, c1, seg, head, tail);
-  if (!OUT && tail) return;                        // nothing is carried past a segment's last run
   const bool values = ct < io.ptiles;              // else columns of the transition
+  bool on = ct < tiles;                            // else: copies and barriers only
+  if (!OUT) {                                      // E of all runs but a segment's last, and M
+    const bool e = !tail, t = !(head && tail) && (!head || io.first_m) && (!tail || io.last_m);
+    const int w0 = blockIdx.x * W;
+    if (!(e && w0 < io.ptiles) && !(t && w0 + W > io.ptiles)) return;
+    on = on && (values ? e : t);
+  }
   const int col = 16 * (values ? ct : ct - io.ptiles) + m;
   const int64_t ks = key_of(g, s);
   const int64_t rp = (int64_t)g.r * g.p, sn = (int64_t)run * g.nb + s;
@@ -248,10 +255,16 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
           out[(int64_t)a * g.p + col] = S[mt][i];
       }
   }
+  if (!OUT && !values && io.save_m) {
+#pragma unroll
+    for (int mt = 0; mt < 2 * RB; ++mt)
+      *reinterpret_cast<f32x4*>(io.save_m + (sn * R + col) * R + 16 * mt + 4 * gq) = S[mt];
+  }
 }
 
 // The states entering the runs of a segment (start): S <- M_i S + E_i past each but
-// the last; `rev` walks the runs backwards (the gradient's direction).  Every step
+// the last, from init or from zero (then the first M is not used and need not exist);
+// `rev` walks the runs backwards (the gradient's direction).  Every step
 // waits on the last one, so a step is made short: a workgroup takes 16 columns only,
 // wave w the rows [32 w, 32 w + 32) of them, M's rows and E's of the next run are
 // loaded while a step computes, and the waves meet once, over their parts of S.
@@ -333,11 +346,13 @@ __global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float
     load_m(next);
     load(e, E + at(next) * rp);
     lds_barrier();                                 // one a step: the parts alternate
+    if (n > r0 || init) {
 #pragma unroll
-    for (int kb = 0; kb < RB; ++kb) {
-      const Frag<NI> sb = load_frag<NI>(part + kb * kFrag, RB * kFrag);
-      const Frag<NI> a[2] = {mf[0][kb], mf[1][kb]}, b[2] = {sb, sb};
-      mul_each(c, a, b);
+      for (int kb = 0; kb < RB; ++kb) {
+        const Frag<NI> sb = load_frag<NI>(part + kb * kFrag, RB * kFrag);
+        const Frag<NI> a[2] = {mf[0][kb], mf[1][kb]}, b[2] = {sb, sb};
+        mul_each(c, a, b);
+      }
     }
     S[0] = c[0];
     S[1] = c[1];
@@ -402,7 +417,8 @@ static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipS
 template <typename In, int RB>
 static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v,
                 const float* logA, const float* beta, const float* state, void* out,
-                float* state_out, float* save_s, float* save_u, void* ws, hipStream_t st) {
+                float* state_out, float* save_s, float* save_u, float* save_m, void* ws,
+                hipStream_t st) {
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
   const Ops o = place_ops(ar, dtype, g, q, k, false);
@@ -418,12 +434,15 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
   io.ovec = vec4_ok(out, 0, g.p, eb);
   io.ptiles = (g.p + 15) / 16;
   if (g.nruns > g.nseg) {
-    const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);
+    const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p, true);
     ChainIO first = io;
     first.o = nullptr;
     first.start = nullptr;
     first.end = c.E;
-    first.trans = c.M;
+    first.trans = c.trans;
+    first.save_m = save_m;
+    first.first_m = state != nullptr;
+    first.last_m = save_m && state_out;            // else nothing comes from behind it
     chain<In, RB, false>(g, o, first, io.ptiles + 2 * RB, st);
     const int rc = launch_carry(g, state, c, false, st);
     if (rc) return rc;
@@ -471,7 +490,7 @@ extern "C" int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nc
   using namespace smat::dl;
   Arena ar{nullptr};
   take_ops(ar, dtype, nb, nbk, nch, r, backward != 0, false);
-  if (nruns > nseg) take_carry(ar, nb, nruns, r, p);
+  if (nruns > nseg) take_carry(ar, nb, nruns, r, p, backward == 0);
   if (backward) {
     ar.take<float>((int64_t)nb * nch * 32 * rblocks(r) * p32(p));   // dS' of every chunk
     ar.take<float>((int64_t)nb * nch * C * p32(p));                 // Z
@@ -481,7 +500,7 @@ extern "C" int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nc
 
 extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const void* v,
                                const float* logA, const float* beta, const float* state, void* out,
-                               float* state_out, float* save_s, float* save_u,
+                               float* state_out, float* save_s, float* save_u, float* save_m,
                                const int32_t* chunks, const int32_t* runs, const int32_t* segrun,
                                int nb, int nbk, int T, int nseg, int nch, int nruns, int K, int r,
                                int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
@@ -501,7 +520,9 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
                who);
   SMAT_REQUIRE(near_rows(v_st), SMAT_EUNSUPPORTED, "%s: rows of v %lld elements apart, beyond 2^23",
                who, (long long)v_st);
-  SMAT_REQUIRE(!save_s == !save_u, SMAT_EINVAL, "%s: save_s and save_u go together", who);
+  SMAT_REQUIRE(!save_s == !save_u && (save_s && nruns > nseg ? save_m != nullptr : !save_m),
+               SMAT_EINVAL, "%s: save_s, save_u and (with more runs than segments) save_m go "
+               "together", who);
   SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
   const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 0);
   SMAT_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
@@ -514,7 +535,8 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
   auto go = [&](auto in, auto rb) {
     typedef decltype(in) In;
     return scan<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, v, logA, beta,
-                                         state, out, state_out, save_s, save_u, workspace, st);
+                                         state, out, state_out, save_s, save_u, save_m,
+                                         workspace, st);
   };
   return dispatch(dtype, r, go);
 }

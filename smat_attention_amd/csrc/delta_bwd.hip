@@ -15,7 +15,8 @@
 //
 // Two kernels after the chunks' operands: delta_rchain_kernel walks the chunks
 // backwards through dS as the forward's chain walks them through S (16 columns a
-// wave, operands shared in LDS), storing dS' and Z of every chunk; delta_grad_kernel,
+// wave, operands shared in LDS), storing dS' and Z of every chunk (runs: their
+// transitions are the forward's transposed, which it keeps); delta_grad_kernel,
 // one workgroup a (key sequence, chunk), forms the rest for the group's value heads
 // one after another, so the gradients of a shared key head are sums in registers, in
 // the heads' order.
@@ -29,7 +30,6 @@ struct RChainIO {
   int64_t d_sb, d_st;
   const float* start;     // dS behind run i of sequence s: start + (i nb + s) r p; or null
   float* end;             // first pass: dS before it, same layout
-  float* trans;           // first pass: the run's transition
   float* fin;             // dS before segment j: fin + (j nb + s) r p; or null
   float *save_d, *z;      // dS' of every chunk (R x p32) and Z (64 x p32)
   void* dv;               // (nb, T, p) contiguous
@@ -69,8 +69,7 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
   bool head, tail;
   run_of(g, run, c0, c1, seg, head, tail);
   if (!OUT && head) return;                        // nothing is carried past a segment's first run
-  const bool values = ct < io.ptiles;
-  const int col = 16 * (values ? ct : ct - io.ptiles) + m;
+  const int col = 16 * ct + m;
   const int64_t ks = key_of(g, s);
   const int64_t rp = (int64_t)g.r * g.p, sn = (int64_t)run * g.nb + s;
   const int ld = (g.p + 31) / 32 * 32;
@@ -81,18 +80,15 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int a = 16 * mt + 4 * gq + i;
-      if (!values)
-        S[mt][i] = a == col ? 1.f : 0.f;
-      else
-        S[mt][i] = (io.start && a < g.r && col < g.p) ? io.start[sn * rp + (int64_t)a * g.p + col]
-                                                      : 0.f;
+      S[mt][i] = (io.start && a < g.r && col < g.p) ? io.start[sn * rp + (int64_t)a * g.p + col]
+                                                    : 0.f;
     }
   const In* ds = (const In*)io.dout + s * io.d_sb;
   const uint32_t soff = (4 * gq * ld + col) * 4;    // in fp32 rows of ld
-  const bool dlive = values && col < g.p;
+  const bool dlive = col < g.p;
   uint32_t dv[16];
   auto load_d = [&](int t0, int len) {
-    load_column(dv, ds, io.d_st, t0, len, values ? col : 0, g.p);
+    load_column(dv, ds, io.d_st, t0, len, col, g.p);
   };
   const TileStage<RB, NT, W> kstage(o.k, g.r, w), qstage(o.q, g.r, w);
   auto vec_of = [&](int c) { return o.vec + ((int64_t)s * g.nch + c) * kVec; };
@@ -165,12 +161,10 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
         x[mt] *= *reinterpret_cast<const f32x4*>(vec + C + 16 * mt + f4);
-      if (values) {
-        Frag<NT> df[2];
+      Frag<NT> df[2];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
-        triangle<true, NI>(x, pl, df, lane);
-      }
+      for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
+      triangle<true, NI>(x, pl, df, lane);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
@@ -206,15 +200,11 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
       }
       const float aC = vec[3 * C];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
-      if (values) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) fd[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
+      for (int kb = 0; kb < 2; ++kb) {
+        f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
+        fd[kb] = split<NI>(d[2 * kb], d[2 * kb + 1]);
       }
-      if (values)
-        update_state<RB, NT, true>(S, sb, aC, kt, f, ql, fd, lane);
-      else
-        update_state<RB, NT, false>(S, sb, aC, kt, f, ql, fd, lane);
+      update_state<RB, NT, true>(S, sb, aC, kt, f, ql, fd, lane);
     }
     if (KD == 1 && more) {
       lds_barrier();                               // K is read
@@ -226,16 +216,13 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
   if (!on) return;
   float* out = OUT ? (io.fin && head ? io.fin + ((int64_t)seg * g.nb + s) * rp : nullptr)
                    : io.end + sn * rp;
-  if (values ? out != nullptr : true) {
+  if (out) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int a = 16 * mt + 4 * gq + i;
-        if (!values)
-          io.trans[(sn * R + a) * R + col] = S[mt][i];
-        else if (a < g.r && col < g.p)
-          out[(int64_t)a * g.p + col] = S[mt][i];
+        if (a < g.r && col < g.p) out[(int64_t)a * g.p + col] = S[mt][i];
       }
   }
 }
@@ -565,7 +552,8 @@ static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hi
 
 template <typename In, int RB>
 static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr, void* dv,
-                    const float* dstate_out, float* dstate, void* ws, hipStream_t st) {
+                    const float* dstate_out, float* dstate, const float* save_m, void* ws,
+                    hipStream_t st) {
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
   const Ops o = place_ops(ar, dtype, g, q, k, true);
@@ -585,12 +573,12 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
   io.fin = dstate;
   io.ptiles = (g.p + 15) / 16;
   if (g.nruns > g.nseg) {
-    const Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p);
+    Carry c = take_carry(ar, g.nb, g.nruns, g.r, g.p, false);
+    c.M = save_m;
     RChainIO first = io;
     first.start = nullptr;
     first.end = c.E;
-    first.trans = c.M;
-    rchain<In, RB, false>(g, o, first, io.ptiles + 2 * RB, st);
+    rchain<In, RB, false>(g, o, first, io.ptiles, st);
     const int rc = launch_carry(g, dstate_out, c, true, st);
     if (rc) return rc;
     io.start = c.start;
@@ -623,8 +611,8 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
 
 extern "C" int smat_delta_scan_backward(
     int dtype, const void* q, const void* k, const void* v, const float* logA, const float* beta,
-    const void* dout, const float* dstate_out, const float* save_s, const float* save_u, void* dq,
-    void* dk, void* dv, float* dlogA, float* dbeta, float* dstate, const int32_t* chunks,
+    const void* dout, const float* dstate_out, const float* save_s, const float* save_u,
+    const float* save_m, void* dq, void* dk, void* dv, float* dlogA, float* dbeta, float* dstate, const int32_t* chunks,
     const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch,
     int nruns, int K, int r, int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
     int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st, int64_t b_sb,
@@ -640,7 +628,7 @@ extern "C" int smat_delta_scan_backward(
   if (rc) return rc;
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && dout && save_s && save_u && dq && dk &&
-                            dv && dlogA && dbeta),
+                            dv && dlogA && dbeta && (save_m || nruns == nseg)),
                SMAT_EINVAL, "%s: null pointer", who);
   SMAT_REQUIRE(near_rows(v_st) && near_rows(d_st), SMAT_EUNSUPPORTED,
                "%s: rows of v or dout %lld and %lld elements apart, beyond 2^23", who,
@@ -666,6 +654,7 @@ extern "C" int smat_delta_scan_backward(
   return dispatch(dtype, r, [&](auto in, auto rb) {
     typedef decltype(in) In;
     return backward<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, gr, dv,
-                                             dstate_out, dstate, workspace, (hipStream_t)stream);
+                                             dstate_out, dstate, save_m, workspace,
+                                             (hipStream_t)stream);
   });
 }

@@ -620,16 +620,19 @@ inline Ops place_ops(Arena& ar, int dtype, const Geo& g, const void* q, const vo
   return o;
 }
 
-// What the runs' states take: E, the states entering runs, and M.
+// What the runs' states take: E, the states entering runs, and M (the gradient's is the
+// forward's, kept transposed: `own` = false).
 struct Carry {
-  float *E, *start, *M;
+  float *E, *start;
+  const float* M;
+  float* trans;
 };
-inline Carry take_carry(Arena& ar, int64_t nb, int64_t nruns, int r, int p) {
+inline Carry take_carry(Arena& ar, int64_t nb, int64_t nruns, int r, int p, bool own) {
   const int64_t R = 32 * rblocks(r);
-  Carry c;
+  Carry c = {};
   c.E = ar.take<float>(nruns * nb * r * p);
   c.start = ar.take<float>(nruns * nb * r * p);
-  c.M = ar.take<float>(nruns * nb * R * R);
+  if (own) c.M = c.trans = ar.take<float>(nruns * nb * R * R);
   return c;
 }
 

@@ -131,13 +131,13 @@ SIGNATURES = {
                              _i64, _i64, _p]),
     "smat_delta_run_chunks": (_i, [_i, _i, _i, _i, _i]),
     "smat_delta_workspace_bytes": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
-    "smat_delta_scan": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i,
-                             _i, _i, _i, _i, _i, _i, _f, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-                             _i64, _i64, _i64, _p, _i64, _p]),
+    "smat_delta_scan": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i,
+                             _i, _i, _i, _i, _i, _i, _i, _f, _i64, _i64, _i64, _i64, _i64, _i64,
+                             _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "smat_delta_scan_backward": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
-                                      _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i64,
+                                      _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f,
                                       _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-                                      _i64, _p, _i64, _p]),
+                                      _i64, _i64, _p, _i64, _p]),
     "smat_delta_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _i64, _i64,
                              _i64, _i64, _i64, _p]),
 }

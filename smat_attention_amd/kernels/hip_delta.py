@@ -165,9 +165,9 @@ def _check_widths(who, r, p):
 
 
 def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bool):
-    """``(o, state_out or None, save_s, save_u, inputs)``: the forward over checked arguments;
-    ``inputs`` are the tensors that the kernels read (rows with unit column stride, fp32
-    gates)."""
+    """``(o, state_out or None, saved, inputs)``: the forward over checked arguments; ``saved``
+    is what the backward takes from it, ``inputs`` are the tensors that the kernels read (rows
+    with unit column stride, fp32 gates)."""
     who = "gated_delta_scan"
     plan = _Plan(who, Q, V, segments)
     code, dev = _code(Q, who), Q.device
@@ -177,24 +177,27 @@ def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bo
     lead = () if segments is None else (plan.nseg,)
     s_out = (torch.empty(*lead, plan.nb, plan.r, plan.p, device=dev, dtype=torch.float32)
              if want_state else None)
-    save_s = save_u = None
+    save_s = save_u = save_m = None
     if save:
         save_s = torch.empty(plan.nb, plan.nch, plan.R, plan.P, device=dev)
         save_u = torch.empty(plan.nb, plan.nch, CHUNK, plan.P, device=dev)
+        if plan.nruns > plan.nseg:
+            save_m = torch.empty(plan.nruns, plan.nb, plan.R, plan.R, device=dev)
     ws, n = plan.workspace(code, 0, dev)
     if state is not None:
         state = state.contiguous()
     _call_on(Q, "smat_delta_scan", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
              logA.data_ptr(), beta.data_ptr(), ptr(state) or None, o.data_ptr(),
-             ptr(s_out) or None, ptr(save_s) or None, ptr(save_u) or None, *plan.sizes(scale),
-             q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(), *beta.stride(), ws.data_ptr(), n)
-    return o, s_out, save_s, save_u, (Q, K, V, logA, beta)
+             ptr(s_out) or None, ptr(save_s) or None, ptr(save_u) or None, ptr(save_m) or None,
+             *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(), *beta.stride(), ws.data_ptr(), n)
+    return o, s_out, (save_s, save_u, save_m), (Q, K, V, logA, beta)
 
 
-def scan_backward(inputs, save_s, save_u, dO, dS, scale, segments, want_dstate: bool):
+def scan_backward(inputs, saved, dO, dS, scale, segments, want_dstate: bool):
     """``(dQ, dK, dV, dlogA, dbeta, dstate or None)`` of one forward."""
     who = "gated_delta_scan"
     Q, K, V, logA, beta = inputs
+    save_s, save_u, save_m = saved
     plan = _Plan(who, Q, V, segments)
     code, dev = _code(Q, who), Q.device
     (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
@@ -212,7 +215,7 @@ def scan_backward(inputs, save_s, save_u, dO, dS, scale, segments, want_dstate: 
         dS = dS.contiguous()
     _call_on(Q, "smat_delta_scan_backward", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
              logA.data_ptr(), beta.data_ptr(), dO.data_ptr(), ptr(dS), save_s.data_ptr(),
-             save_u.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlogA.data_ptr(),
+             save_u.data_ptr(), ptr(save_m) or None, dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlogA.data_ptr(),
              dbeta.data_ptr(), ptr(dstate), *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb,
              v_st, *logA.stride(), *beta.stride(), d_sb, d_st, ws.data_ptr(), n)
     return dQ, dK, dV, dlogA, dbeta, dstate
@@ -222,14 +225,15 @@ class GatedDeltaFunction(torch.autograd.Function):
     """The whole-sequence form with gradients of Q, K, V, logA, beta and the state.
 
     The forward keeps, besides its inputs, the state entering every chunk of 64 tokens and
-    the chunk's ``U`` in fp32; the backward forms the chunks' other operands again."""
+    the chunk's ``U`` in fp32, and the transitions of the runs where T is split; the backward
+    forms the chunks' other operands again."""
 
     @staticmethod
     def forward(ctx, Q, K, V, logA, beta, state, scale, segments, want_state):
-        o, s_out, save_s, save_u, inputs = scan(
+        o, s_out, saved, inputs = scan(
             Q.detach(), K.detach(), V.detach(), logA.detach(), beta.detach(),
             None if state is None else state.detach(), scale, segments, want_state, True)
-        ctx.save_for_backward(*inputs, save_s, save_u)
+        ctx.save_for_backward(*inputs, *saved)
         ctx.meta = (scale, segments, logA.dtype, beta.dtype)
         ctx.set_materialize_grads(False)
         return o, s_out
@@ -237,7 +241,7 @@ class GatedDeltaFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dO, dS):
-        *inputs, save_s, save_u = ctx.saved_tensors
+        inputs, saved = ctx.saved_tensors[:5], ctx.saved_tensors[5:]
         scale, segments, a_type, b_type = ctx.meta
         if dO is None and dS is None:
             return (None,) * 9
@@ -245,8 +249,7 @@ class GatedDeltaFunction(torch.autograd.Function):
             V = inputs[2]
             dO = torch.zeros(V.shape, device=V.device, dtype=V.dtype)
         dQ, dK, dV, dlogA, dbeta, dstate = scan_backward(
-            inputs, save_s, save_u, dO.to(inputs[2].dtype), dS, scale, segments,
-            ctx.needs_input_grad[5])
+            inputs, saved, dO.to(inputs[2].dtype), dS, scale, segments, ctx.needs_input_grad[5])
         return (dQ, dK, dV, dlogA.to(a_type), dbeta.to(b_type), dstate, None, None, None)
 
 

@@ -175,15 +175,16 @@ def test_c_entry_points_refuse():
     fake = 1 << 20                     # never dereferenced: validation fails first
 
     def scan(dtype=0, nb=2, nbk=2, T=64, nseg=1, nch=1, nruns=1, K=1, r=64, p=64, q=fake, n=1 << 40,
-             tables=(None, None, None)):
-        _lib.call("smat_delta_scan", dtype, q, fake, fake, fake, fake, None, fake, None, None,
-                  None, *tables, nb, nbk, T, nseg, nch, nruns, K, r, p, 1.0, *[64] * 10, fake, n,
+             tables=(None, None, None), save=None):
+        _lib.call("smat_delta_scan", dtype, q, fake, fake, fake, fake, None, fake, None, save,
+                  save, None, *tables, nb, nbk, T, nseg, nch, nruns, K, r, p, 1.0, *[64] * 10, fake, n,
                   None)
     for kw, what in ((dict(dtype=9), "unknown dtype"), (dict(q=None), "null pointer"),
                      (dict(nbk=3), "does not divide"), (dict(r=129), "beyond"),
                      (dict(p=257), "beyond"), (dict(nch=2), "chunks for T"),
                      (dict(nruns=2), "runs"), (dict(n=16), "workspace"),
-                     (dict(tables=(fake, None, None)), "tables"), (dict(K=0), "runs")):
+                     (dict(tables=(fake, None, None)), "tables"), (dict(K=0), "runs"),
+                     (dict(T=128, nch=2, nruns=2, save=fake), "save_m")):
         with pytest.raises(HipKernelError, match=what):
             scan(**kw)
     with pytest.raises(HipKernelError, match="at most 64"):

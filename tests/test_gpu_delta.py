@@ -168,6 +168,32 @@ def test_split_along_the_sequence(dtype, nb, nbk, T, r, p, off, st):
         _check(name, a, b, 2 * chunks, r, p)
 
 
+@pytest.mark.parametrize("st,want", [(True, True), (False, True), (True, False), (False, False)])
+@pytest.mark.parametrize("off", [None, [0, 64 * 20 + 3, 64 * 20 + 3, 64 * 20 + 40, 64 * 41 + 9]])
+def test_split_gradients_of_the_states(off, st, want):
+    """Runs' transitions are formed where a state enters, or where one leaves and a gradient may
+    come back through it: each of the four, over one sequence and over packed ones."""
+    nb, T, r, p = 2, 64 * 41 + 9, 48, 32
+    lead = () if off is None else (len(off) - 1,)
+    q, k, v, logA, beta, S = _inputs(nb, nb, T, r, p, FP32, seed=13, state=lead if st else None,
+                                     decay=0.02)
+    x = [t.requires_grad_(True) for t in (q, k, v, logA, beta)] + ([S.requires_grad_(True)] if st
+                                                                   else [])
+    seg = None if off is None else A.Segments(off, DEV)
+    got = A.gated_delta_scan(*x[:5], state=S, segments=seg, return_state=want)
+    y = [t.detach().double().requires_grad_(True) for t in x]
+    ref = O.delta_scan(*y[:5], state=y[5] if st else None, offsets=off)
+    got, ref = (got, ref) if want else ((got,), ref[:1])
+    g = torch.Generator().manual_seed(14)
+    d = [torch.randn(t.shape, generator=g).to(DEV) for t in got]
+    got = torch.autograd.grad(got, x, d)
+    ref = torch.autograd.grad(ref, y, [t.double() for t in d])
+    for name, a, b in zip(("dq", "dk", "dv", "dlogA", "dbeta", "dS0"), got, ref):
+        if name == "dlogA" and want:                 # sums terms as large as <dS, S>
+            continue
+        _check(name, a, b, 2 * -(-T // 64), r, p)
+
+
 @pytest.mark.parametrize("kind", ["resets", "strong", "same_keys", "beta2", "beta0", "no_decay"])
 def test_hard_gates(kind):
     """Decays to zero, writes that replace everything, keys that repeat, padding tokens."""
