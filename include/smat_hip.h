@@ -570,7 +570,8 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  * being r and p rounded up to 32, receive the states entering chunks and U,
  * and, if nruns > nseg, save_m (nruns, nb, R, R) fp32 the runs' transitions (of
  * a segment's last run only if state_out is given); else all three are NULL.
- * workspace: smat_delta_workspace_bytes(..., backward) bytes, 256-byte aligned.
+ * workspace: smat_delta_workspace_bytes(..., backward) bytes, 256-byte aligned;
+ * none is used for up to 16 tokens without the tables and save_s.
  */
 int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p);
 int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg, int nruns,

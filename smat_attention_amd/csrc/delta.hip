@@ -524,14 +524,14 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
                SMAT_EINVAL, "%s: save_s, save_u and (with more runs than segments) save_m go "
                "together", who);
   SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
+  hipStream_t st = (hipStream_t)stream;
+  if (!chunks && !save_s && T >= 1 && T <= kFewTokens)
+    return launch_tokens(dtype, g, q, k, v, logA, beta, state, state_out, out, st);
   const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 0);
   SMAT_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
                    ((uintptr_t)workspace & 255) == 0,
                SMAT_EINVAL, "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who,
                (long long)workspace_bytes, (long long)need);
-  hipStream_t st = (hipStream_t)stream;
-  if (!chunks && !save_s && T >= 1 && T <= kFewTokens)
-    return launch_tokens(dtype, g, q, k, v, logA, beta, state, state_out, out, st);
   auto go = [&](auto in, auto rb) {
     typedef decltype(in) In;
     return scan<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, v, logA, beta,

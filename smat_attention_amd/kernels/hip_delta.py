@@ -18,6 +18,7 @@ from .hip_fwd import _call_on, _code, _on_gpu, _rows3, _shape
 
 CHUNK = 64
 MAX_R, MAX_P = 128, 256
+FEW_TOKENS = 16          # calls of up to so many tokens, unpacked, need no workspace
 
 
 def same_device(who: str, ref: torch.Tensor, *ts) -> None:
@@ -102,7 +103,8 @@ class _Plan:
                                  f"{Q.device}")
             self.nseg, self.nch = len(segments), segments.nch
         longest = self.nch if segments is None else segments.longest
-        self.K = _lib.query("smat_delta_run_chunks", self.nb, self.nch, longest, self.r, self.p)
+        self.K = 1 if longest <= 1 else _lib.query("smat_delta_run_chunks", self.nb, self.nch,
+                                                   longest, self.r, self.p)
         if segments is None:
             self.tables = (None, None, None)
             self.nruns = max(1, -(-self.nch // self.K))
@@ -183,13 +185,16 @@ def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bo
         save_u = torch.empty(plan.nb, plan.nch, CHUNK, plan.P, device=dev)
         if plan.nruns > plan.nseg:
             save_m = torch.empty(plan.nruns, plan.nb, plan.R, plan.R, device=dev)
-    ws, n = plan.workspace(code, 0, dev)
+    ws = n = 0
+    if save or segments is not None or plan.T > FEW_TOKENS:
+        buf, n = plan.workspace(code, 0, dev)
+        ws = buf.data_ptr()
     if state is not None:
         state = state.contiguous()
     _call_on(Q, "smat_delta_scan", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
              logA.data_ptr(), beta.data_ptr(), ptr(state) or None, o.data_ptr(),
              ptr(s_out) or None, ptr(save_s) or None, ptr(save_u) or None, ptr(save_m) or None,
-             *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(), *beta.stride(), ws.data_ptr(), n)
+             *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(), *beta.stride(), ws, n)
     return o, s_out, (save_s, save_u, save_m), (Q, K, V, logA, beta)
 
 
