@@ -568,8 +568,9 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  * the same leaving it (may be NULL; not state itself).
  * Training: save_s (nb, nch, R, P) and save_u (nb, nch, 64, P) fp32, R and P
  * being r and p rounded up to 32, receive the states entering chunks and U,
- * and, if nruns > nseg, save_m (nruns, nb, R, R) fp32 the runs' transitions (of
- * a segment's last run only if state_out is given); else all three are NULL.
+ * and, if nruns > nseg, save_m (nruns, nb, R, R, 3) bf16 the runs' transitions in
+ * the kernels' layout (of a segment's last run only if state_out is given);
+ * else all three are NULL.
  * workspace: smat_delta_workspace_bytes(..., backward) bytes, 256-byte aligned;
  * none is used for up to 16 tokens without the tables and save_s.
  */
@@ -578,7 +579,7 @@ int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg
                                    int r, int p, int backward);
 int smat_delta_scan(int dtype, const void* q, const void* k, const void* v, const float* logA,
                     const float* beta, const float* state, void* out, float* state_out,
-                    float* save_s, float* save_u, float* save_m, const int32_t* chunks,
+                    float* save_s, float* save_u, void* save_m, const int32_t* chunks,
                     const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T, int nseg,
                     int nch, int nruns, int K, int r, int p, float scale, int64_t q_sb,
                     int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st,
@@ -595,7 +596,7 @@ int smat_delta_scan(int dtype, const void* q, const void* k, const void* v, cons
 int smat_delta_scan_backward(int dtype, const void* q, const void* k, const void* v,
                              const float* logA, const float* beta, const void* dout,
                              const float* dstate_out, const float* save_s, const float* save_u,
-                             const float* save_m, void* dq, void* dk, void* dv, float* dlogA,
+                             const void* save_m, void* dq, void* dk, void* dv, float* dlogA,
                              float* dbeta, float* dstate, const int32_t* chunks,
                              const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T,
                              int nseg, int nch, int nruns, int K, int r, int p, float scale,

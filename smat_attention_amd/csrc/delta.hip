@@ -26,8 +26,8 @@ struct ChainIO {
   void* o;
   const float* start;     // state entering run i of sequence s: start + (i nb + s) r p; or null
   float* end;             // first pass: the state leaving it, same layout
-  float* trans;           // first pass: M of run i, (i nb + s) R R row-major (R = 32 RB)
-  float* save_m;          // training, first pass: M transposed, same layout; or null
+  bf16* trans;            // first pass: M of run i as fragments (trans_at, index i nb + s)
+  bf16* save_m;           // training, first pass: M transposed, same layout; or null
   bool first_m, last_m;   // first pass: whether M of a segment's first, last run is wanted
   float* fin;             // state leaving segment j: fin + (j nb + s) r p; or null
   float *save_s, *save_u; // training: states entering chunks, and U, rows padded to p32; or null
@@ -240,25 +240,52 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     t0 = t1;
     len = len1;
   }
+  if (!OUT) lds_barrier();                         // the tiles are read: their place is free
   if (!on) return;
+  if (!OUT && !values) {                           // sb: columns of M, the rows in the slots
+    const int tile = ct - io.ptiles;
+    if (io.save_m) {                               // which makes them rows of M transposed
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb)
+        store_frag<NI>(io.save_m + trans_at<RB>(sn, tile, kb), kFrag, sb[kb]);
+    }
+    // rows of M, their 16 columns half a contraction block: transposed a term at a time in
+    // the wave's part of LDS
+    constexpr int LD = R + 4;
+    static_assert(W * 16 * LD * 2 <= chain_lds<In, RB, OUT>(KD), "");
+    bf16* part = lds + w * 16 * LD;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+#pragma unroll
+      for (int kb = 0; kb < RB; ++kb) {
+        const bf16x8 x = sb[kb].t[n];
+        bf16* p = part + m * LD + 32 * kb + 4 * gq;
+        *reinterpret_cast<bf16x4*>(p) = bf16x4{x[0], x[1], x[2], x[3]};
+        *reinterpret_cast<bf16x4*>(p + 16) = bf16x4{x[4], x[5], x[6], x[7]};
+      }
+      asm volatile("" ::: "memory");               // between lanes: a wave's LDS is in order
+#pragma unroll
+      for (int rt = 0; rt < 2 * RB; ++rt) {
+        bf16x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = part[(4 * gq + i) * LD + 16 * rt + m];
+        *reinterpret_cast<bf16x4*>(io.trans + trans_at<RB>(sn, rt, tile >> 1) + n * kFrag +
+                                   lane_id() * 8 + 4 * (tile & 1)) = x;
+      }
+      asm volatile("" ::: "memory");
+    }
+    return;
+  }
   float* out = OUT ? (io.fin && tail ? io.fin + ((int64_t)seg * g.nb + s) * rp : nullptr)
                    : io.end + sn * rp;
-  if (values ? out != nullptr : true) {
+  if (out) {
 #pragma unroll
     for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int a = 16 * mt + 4 * gq + i;
-        if (!values)
-          io.trans[(sn * R + a) * R + col] = S[mt][i];
-        else if (a < g.r && col < g.p)
-          out[(int64_t)a * g.p + col] = S[mt][i];
+        if (a < g.r && col < g.p) out[(int64_t)a * g.p + col] = S[mt][i];
       }
-  }
-  if (!OUT && !values && io.save_m) {
-#pragma unroll
-    for (int mt = 0; mt < 2 * RB; ++mt)
-      *reinterpret_cast<f32x4*>(io.save_m + (sn * R + col) * R + 16 * mt + 4 * gq) = S[mt];
   }
 }
 
@@ -267,17 +294,19 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
 // `rev` walks the runs backwards (the gradient's direction).  Every step
 // waits on the last one, so a step is made short: a workgroup takes 16 columns only,
 // wave w the rows [32 w, 32 w + 32) of them, M's rows and E's of the next run are
-// loaded while a step computes, and the waves meet once, over their parts of S.
+// loaded while a step computes, and the waves meet once, over their parts of S.  The
+// sequences come first in the grid: the workgroups that read one M then mostly share
+// an XCD's L2.
 template <int RB>
 __global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float* __restrict__ init,
                                                               const float* __restrict__ E,
-                                                              const float* __restrict__ M,
+                                                              const bf16* __restrict__ M,
                                                               float* __restrict__ start,
                                                               bool rev) {
-  constexpr int R = 32 * RB, NI = kMid;
+  constexpr int NI = kMid;
   __shared__ __align__(16) bf16 parts[2][NI * RB * kFrag];
   const int w = uniform_wave(), m = lane_id() & 15, gq = lane_id() >> 4;
-  const int col = 16 * blockIdx.x + m, seg = blockIdx.y, s = blockIdx.z;
+  const int col = 16 * blockIdx.y + m, seg = blockIdx.z, s = blockIdx.x;
   const int64_t rp = (int64_t)g.r * g.p;
   const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
   if (r0 >= r1) return;
@@ -294,7 +323,8 @@ __global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float
       live[mt][i] = a < g.r && col < g.p;
       off[mt][i] = (uint32_t)(min(a, g.r - 1) * g.p + min(col, g.p - 1));
     }
-  f32x4 S[2], e[2], x[2][RB][2];
+  f32x4 S[2], e[2];
+  Frag<NI> ma[2][RB], mb[2][RB];                   // M of this step and of the next, in turn
   auto load = [&](f32x4* y, const float* p) {
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
@@ -314,48 +344,44 @@ __global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float
       for (int i = 0; i < 4; ++i)
         if (live[mt][i]) p[off[mt][i]] = S[mt][i];
   };
-  auto load_m = [&](int n) {
-    const float* p = M + at(n) * R * R + (int64_t)(32 * w + m) * R + 4 * gq;
+  auto load_m = [&](Frag<NI> (&x)[2][RB], int n) {
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int kb = 0; kb < RB; ++kb)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          x[mt][kb][h] = *reinterpret_cast<const f32x4*>(p + 16 * mt * R + 32 * kb + 16 * h);
+        x[mt][kb] = load_frag<NI>(M + trans_at<RB>(at(n), 2 * w + mt, kb), kFrag);
   };
   S[0] = S[1] = zero4();
   if (init) {
     load(S, init + ((int64_t)seg * g.nb + s) * rp);
     keep(S);
   }
-  load_m(r0 + 1 < r1 ? r0 : r1 - 1);
+  load_m(ma, r0 + 1 < r1 ? r0 : r1 - 1);
   load(e, E + at(r0 + 1 < r1 ? r0 : r1 - 1) * rp);
-  for (int n = r0; n + 1 < r1; ++n) {
-    bf16* part = parts[(n - r0) & 1];
+  auto step = [&](int n, bf16* part, Frag<NI> (&x)[2][RB], Frag<NI> (&y)[2][RB]) {
     store_frag<NI>(part + w * kFrag, RB * kFrag, split<NI>(S[0], S[1]));
     store(start + at(n) * rp);
-    Frag<NI> mf[2][RB];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int kb = 0; kb < RB; ++kb) mf[mt][kb] = split<NI>(x[mt][kb][0], x[mt][kb][1]);
     f32x4 c[2] = {e[0], e[1]};
     keep(c);
     const int next = n + 2 < r1 ? n + 1 : n;       // (the last one's once more: no branch)
-    load_m(next);
+    load_m(y, next);
     load(e, E + at(next) * rp);
     lds_barrier();                                 // one a step: the parts alternate
     if (n > r0 || init) {
 #pragma unroll
       for (int kb = 0; kb < RB; ++kb) {
         const Frag<NI> sb = load_frag<NI>(part + kb * kFrag, RB * kFrag);
-        const Frag<NI> a[2] = {mf[0][kb], mf[1][kb]}, b[2] = {sb, sb};
+        const Frag<NI> a[2] = {x[0][kb], x[1][kb]}, b[2] = {sb, sb};
         mul_each(c, a, b);
       }
     }
     S[0] = c[0];
     S[1] = c[1];
+  };
+  for (int n = r0; n + 1 < r1; n += 2) {
+    step(n, parts[0], ma, mb);
+    if (n + 2 >= r1) break;
+    step(n + 1, parts[1], mb, ma);
   }
   store(start + at(r1 - 1) * rp);
 }
@@ -388,7 +414,7 @@ int check_geo(const char* who, int dtype, const Geo& g) {
 template <int RB>
 static void carry_kernel(const Geo& g, const float* init, const Carry& c, bool rev,
                          hipStream_t st) {
-  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3((g.p + 15) / 16, g.nseg, g.nb), dim3(64 * RB), 0,
+  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3(g.nb, (g.p + 15) / 16, g.nseg), dim3(64 * RB), 0,
                      st, g, init, c.E, c.M, c.start, rev);
 }
 
@@ -417,7 +443,7 @@ static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipS
 template <typename In, int RB>
 static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v,
                 const float* logA, const float* beta, const float* state, void* out,
-                float* state_out, float* save_s, float* save_u, float* save_m, void* ws,
+                float* state_out, float* save_s, float* save_u, bf16* save_m, void* ws,
                 hipStream_t st) {
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
@@ -500,7 +526,7 @@ extern "C" int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nc
 
 extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const void* v,
                                const float* logA, const float* beta, const float* state, void* out,
-                               float* state_out, float* save_s, float* save_u, float* save_m,
+                               float* state_out, float* save_s, float* save_u, void* save_m,
                                const int32_t* chunks, const int32_t* runs, const int32_t* segrun,
                                int nb, int nbk, int T, int nseg, int nch, int nruns, int K, int r,
                                int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
@@ -535,8 +561,8 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
   auto go = [&](auto in, auto rb) {
     typedef decltype(in) In;
     return scan<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, v, logA, beta,
-                                         state, out, state_out, save_s, save_u, save_m,
-                                         workspace, st);
+                                         state, out, state_out, save_s, save_u,
+                                         (bf16*)save_m, workspace, st);
   };
   return dispatch(dtype, r, go);
 }

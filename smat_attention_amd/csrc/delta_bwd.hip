@@ -552,7 +552,7 @@ static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hi
 
 template <typename In, int RB>
 static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr, void* dv,
-                    const float* dstate_out, float* dstate, const float* save_m, void* ws,
+                    const float* dstate_out, float* dstate, const bf16* save_m, void* ws,
                     hipStream_t st) {
   constexpr int eb = sizeof(In);
   Arena ar{(char*)ws};
@@ -612,7 +612,7 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
 extern "C" int smat_delta_scan_backward(
     int dtype, const void* q, const void* k, const void* v, const float* logA, const float* beta,
     const void* dout, const float* dstate_out, const float* save_s, const float* save_u,
-    const float* save_m, void* dq, void* dk, void* dv, float* dlogA, float* dbeta, float* dstate, const int32_t* chunks,
+    const void* save_m, void* dq, void* dk, void* dv, float* dlogA, float* dbeta, float* dstate, const int32_t* chunks,
     const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch,
     int nruns, int K, int r, int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
     int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st, int64_t b_sb,
@@ -654,7 +654,7 @@ extern "C" int smat_delta_scan_backward(
   return dispatch(dtype, r, [&](auto in, auto rb) {
     typedef decltype(in) In;
     return backward<In, decltype(rb)::value>(dtype, g, (const In*)q, (const In*)k, gr, dv,
-                                             dstate_out, dstate, save_m, workspace,
+                                             dstate_out, dstate, (const bf16*)save_m, workspace,
                                              (hipStream_t)stream);
   });
 }

@@ -620,19 +620,24 @@ inline Ops place_ops(Arena& ar, int dtype, const Geo& g, const void* q, const vo
   return o;
 }
 
-// What the runs' states take: E, the states entering runs, and M (the gradient's is the
-// forward's, kept transposed: `own` = false).
+// What the runs' states take: E, the states entering runs, and M as the carry's operand,
+// split into terms where it is formed (in the carry every step would wait for that).  The
+// gradient's M is the forward's, kept transposed: `own` = false.
 struct Carry {
   float *E, *start;
-  const float* M;
-  float* trans;
+  const bf16* M;
+  bf16* trans;
 };
+// Fragment (row tile rt, contraction block kb) of the M at index sn.
+template <int RB> __device__ __forceinline__ int64_t trans_at(int64_t sn, int rt, int kb) {
+  return ((sn * 2 * RB + rt) * RB + kb) * kMid * kFrag;
+}
 inline Carry take_carry(Arena& ar, int64_t nb, int64_t nruns, int r, int p, bool own) {
   const int64_t R = 32 * rblocks(r);
   Carry c = {};
   c.E = ar.take<float>(nruns * nb * r * p);
   c.start = ar.take<float>(nruns * nb * r * p);
-  if (own) c.M = c.trans = ar.take<float>(nruns * nb * R * R);
+  if (own) c.M = c.trans = ar.take<bf16>(nruns * nb * R * R * kMid);
   return c;
 }
 

@@ -184,7 +184,8 @@ def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bo
         save_s = torch.empty(plan.nb, plan.nch, plan.R, plan.P, device=dev)
         save_u = torch.empty(plan.nb, plan.nch, CHUNK, plan.P, device=dev)
         if plan.nruns > plan.nseg:
-            save_m = torch.empty(plan.nruns, plan.nb, plan.R, plan.R, device=dev)
+            save_m = torch.empty(plan.nruns, plan.nb, plan.R, plan.R, 3, device=dev,
+                                 dtype=torch.bfloat16)
     ws = n = 0
     if save or segments is not None or plan.T > FEW_TOKENS:
         buf, n = plan.workspace(code, 0, dev)
