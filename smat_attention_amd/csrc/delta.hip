@@ -291,18 +291,18 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
 
 // The states entering the runs of a segment (start): S <- M_i S + E_i past each but
 // the last, from init or from zero (then the first M is not used and need not exist);
-// `rev` walks the runs backwards (the gradient's direction).  Every step
-// waits on the last one, so a step is made short: a workgroup takes 16 columns only,
-// wave w the rows [32 w, 32 w + 32) of them, M's rows and E's of the next run are
-// loaded while a step computes, and the waves meet once, over their parts of S.  The
-// sequences come first in the grid: the workgroups that read one M then mostly share
-// an XCD's L2.
+// `rev` walks the runs backwards (the gradient's direction).  Every step waits on the
+// last one, so a step is made short: a workgroup takes 16 columns only, wave w the rows
+// [16 w, 16 w + 16) of them, M's rows and E's are loaded two steps ahead of their use,
+// and the waves meet once, over their parts of S.  The sequences come first in the
+// grid: the workgroups that read one M then mostly share an XCD's L2.
 template <int RB>
-__global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float* __restrict__ init,
-                                                              const float* __restrict__ E,
-                                                              const bf16* __restrict__ M,
-                                                              float* __restrict__ start,
-                                                              bool rev) {
+__global__ __launch_bounds__(128 * RB) void delta_carry_kernel(Geo g,
+                                                               const float* __restrict__ init,
+                                                               const float* __restrict__ E,
+                                                               const bf16* __restrict__ M,
+                                                               float* __restrict__ start,
+                                                               bool rev) {
   constexpr int NI = kMid;
   __shared__ __align__(16) bf16 parts[2][NI * RB * kFrag];
   const int w = uniform_wave(), m = lane_id() & 15, gq = lane_id() >> 4;
@@ -311,79 +311,74 @@ __global__ __launch_bounds__(64 * RB) void delta_carry_kernel(Geo g, const float
   const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
   if (r0 >= r1) return;
   auto at = [&](int n) { return (int64_t)(rev ? r0 + r1 - 1 - n : n) * g.nb + s; };
-  // element (mt, i) is row 32 w + 16 mt + 4 gq + i; rows and columns past the end read
-  // the last one there is
-  uint32_t off[2][4];
-  bool live[2][4];
+  // element i is row 16 w + 4 gq + i; rows and columns past the end read the last one
+  // there is
+  uint32_t off[4];
+  bool live[4];
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int a = 32 * w + 16 * mt + 4 * gq + i;
-      live[mt][i] = a < g.r && col < g.p;
-      off[mt][i] = (uint32_t)(min(a, g.r - 1) * g.p + min(col, g.p - 1));
-    }
-  f32x4 S[2], e[2];
-  Frag<NI> ma[2][RB], mb[2][RB];                   // M of this step and of the next, in turn
-  auto load = [&](f32x4* y, const float* p) {
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[mt][i] = p[off[mt][i]];
-  };
-  auto keep = [&](f32x4* y) {
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[mt][i] = live[mt][i] ? y[mt][i] : 0.f;
-  };
-  auto store = [&](float* p) {
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (live[mt][i]) p[off[mt][i]] = S[mt][i];
-  };
-  auto load_m = [&](Frag<NI> (&x)[2][RB], int n) {
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int kb = 0; kb < RB; ++kb)
-        x[mt][kb] = load_frag<NI>(M + trans_at<RB>(at(n), 2 * w + mt, kb), kFrag);
-  };
-  S[0] = S[1] = zero4();
-  if (init) {
-    load(S, init + ((int64_t)seg * g.nb + s) * rp);
-    keep(S);
+  for (int i = 0; i < 4; ++i) {
+    const int a = 16 * w + 4 * gq + i;
+    live[i] = a < g.r && col < g.p;
+    off[i] = (uint32_t)(min(a, g.r - 1) * g.p + min(col, g.p - 1));
   }
-  load_m(ma, r0 + 1 < r1 ? r0 : r1 - 1);
-  load(e, E + at(r0 + 1 < r1 ? r0 : r1 - 1) * rp);
-  auto step = [&](int n, bf16* part, Frag<NI> (&x)[2][RB], Frag<NI> (&y)[2][RB]) {
-    store_frag<NI>(part + w * kFrag, RB * kFrag, split<NI>(S[0], S[1]));
-    store(start + at(n) * rp);
-    f32x4 c[2] = {e[0], e[1]};
-    keep(c);
-    const int next = n + 2 < r1 ? n + 1 : n;       // (the last one's once more: no branch)
-    load_m(y, next);
-    load(e, E + at(next) * rp);
+  struct Run {
+    Frag<NI> m[RB];
+    f32x4 e;
+  };
+  Run a, b, c;                                     // this step's, the next one's, and past it
+  auto load = [&](const float* p) {
+    f32x4 y;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = p[off[i]];
+    return y;
+  };
+  auto keep = [&](f32x4 y) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = live[i] ? y[i] : 0.f;
+    return y;
+  };
+  auto store = [&](float* p, const f32x4& y) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (live[i]) p[off[i]] = y[i];
+  };
+  const int last = max(r1 - 2, r0);                // (read once more at the end: no branch)
+  auto load_run = [&](Run& x, int n) {
+    const int64_t sn = at(min(n, last));
+#pragma unroll
+    for (int kb = 0; kb < RB; ++kb) x.m[kb] = load_frag<NI>(M + trans_at<RB>(sn, w, kb), kFrag);
+    x.e = load(E + sn * rp);
+  };
+  f32x4 S = zero4();
+  if (init) S = keep(load(init + ((int64_t)seg * g.nb + s) * rp));
+  load_run(a, r0);
+  load_run(b, r0 + 1);
+  auto step = [&](int n, const Run& x, Run& behind) {
+    bf16* part = parts[(n - r0) & 1];
+    const Frag<NI> f = split<NI>(S, zero4());
+#pragma unroll
+    for (int t = 0; t < NI; ++t)                   // half a fragment: the wave's 16 rows
+      *reinterpret_cast<bf16x4*>(part + (t * RB + (w >> 1)) * kFrag + lane_id() * 8 +
+                                 4 * (w & 1)) =
+          bf16x4{f.t[t][0], f.t[t][1], f.t[t][2], f.t[t][3]};
+    store(start + at(n) * rp, S);
+    load_run(behind, n + 2);
     lds_barrier();                                 // one a step: the parts alternate
+    S = keep(x.e);
     if (n > r0 || init) {
 #pragma unroll
-      for (int kb = 0; kb < RB; ++kb) {
-        const Frag<NI> sb = load_frag<NI>(part + kb * kFrag, RB * kFrag);
-        const Frag<NI> a[2] = {x[0][kb], x[1][kb]}, b[2] = {sb, sb};
-        mul_each(c, a, b);
-      }
+      for (int kb = 0; kb < RB; ++kb)
+        S = mul(S, x.m[kb], load_frag<NI>(part + kb * kFrag, RB * kFrag));
     }
-    S[0] = c[0];
-    S[1] = c[1];
   };
-  for (int n = r0; n + 1 < r1; n += 2) {
-    step(n, parts[0], ma, mb);
+  for (int n = r0; n + 1 < r1; n += 3) {
+    step(n, a, c);
     if (n + 2 >= r1) break;
-    step(n + 1, parts[1], mb, ma);
+    step(n + 1, b, a);
+    if (n + 3 >= r1) break;
+    step(n + 2, c, b);
   }
-  store(start + at(r1 - 1) * rp);
+  store(start + at(r1 - 1) * rp, S);
 }
 
 int check_geo(const char* who, int dtype, const Geo& g) {
@@ -414,7 +409,7 @@ int check_geo(const char* who, int dtype, const Geo& g) {
 template <int RB>
 static void carry_kernel(const Geo& g, const float* init, const Carry& c, bool rev,
                          hipStream_t st) {
-  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3(g.nb, (g.p + 15) / 16, g.nseg), dim3(64 * RB), 0,
+  hipLaunchKernelGGL(delta_carry_kernel<RB>, dim3(g.nb, (g.p + 15) / 16, g.nseg), dim3(128 * RB), 0,
                      st, g, init, c.E, c.M, c.start, rev);
 }
 
