@@ -446,7 +446,8 @@ def gated_delta_scan(Q, K, V, logA, beta, *, scale: float = 1.0, state=None,
     with contiguous columns are read in place, so packed ``(tokens, heads, columns)`` tensors
     come as their transposed views.  r <= 128, p <= 256; the values of a chunk of 64 tokens
     meet in products, so inputs are expected to be finite (``logA = -inf`` counts as a decay to
-    zero).  A token with ``beta = 0, logA = 0`` leaves the state as it is: padding.
+    zero; positive ones are taken while the exp of their sum over a chunk stays within fp32).
+    A token with ``beta = 0, logA = 0`` leaves the state as it is: padding.
 
     ``segments`` (:class:`Segments`) packs sequences of any lengths along T; each starts from
     its own state.  ``state`` fp32 ``(nb, r, p)``, with segments ``(segments, nb, r, p)``
@@ -470,8 +471,9 @@ def gated_delta_step(q, k, v, logA, beta, state, *, scale: float = 1.0, out=None
                      out_state=None):
     """One token of :func:`gated_delta_scan` for a batch of sequences: ``q, k (nbk, r)``,
     ``v (nb, p)``, ``logA, beta (nb,)``, ``state (nb, r, p)`` fp32.  The new state goes to
-    ``out_state``, or replaces ``state`` if that is None; returns ``o (nb, p)`` in v's type.
-    One launch, for serving: no gradients."""
+    ``out_state``, or replaces ``state`` if that is None; returns ``o (nb, p)`` in v's type
+    (``out``, if given, must not share memory with the inputs).  One launch, for serving: no
+    gradients."""
     return _delta.step(q, k, v, logA, beta, state, float(scale), out, out_state)
 
 
@@ -953,9 +955,15 @@ class SmatDecoder:
         """Take each request's accepted path into its state and move its position by the
         path's length.  Requests may accept different numbers of tokens: from the first commit
         on, ``ahead`` (int32, on the device) holds how far each is past the step counter
-        ``i``, and :meth:`step` and :meth:`tree_step` read it there."""
+        ``i``, and :meth:`step` and :meth:`tree_step` read it there.  The first commit makes
+        ``ahead``, so it cannot be captured into a graph; as with :meth:`step`, a graph holds an
+        even number of commits and steps (the state buffers take turns)."""
         if self.ahead is None:
             _hip._check_requests("SmatDecoder.commit", "nodes", nodes, self.nb, self.S.device)
+            if torch.cuda.is_current_stream_capturing():     # every replay would clear them
+                raise RuntimeError("SmatDecoder.commit: the first one makes the requests' "
+                                   "positions and cannot be captured; commit once before, or "
+                                   "give from_cache ahead")
             ahead = torch.zeros_like(nodes)
         else:
             ahead = self.ahead

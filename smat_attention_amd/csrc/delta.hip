@@ -481,7 +481,7 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 
 // Run length: the number of runs a segment, G, that takes least by what a step of a
 // full GPU (512 workgroups of four column tiles) measures, in microseconds: 2.5 + 0.6 RB
-// a chunk of the pass with outputs, 1.5 + 0.4 RB of the first pass, 0.65 RB a run of the
+// a chunk of the pass with outputs, 1.5 + 0.4 RB of the first pass, 0.55 RB a run of the
 // carry, 10 for the two launches more.  (8 sequences of 2048 chunks, r = p = 128: 9349
 // whole, 1352 in 32 runs, 2082 in 256; 96 of 64 chunks, r = p = 64, forward and
 // backward: 1074 whole, 930 in 8, 1048 in 2.)
@@ -497,7 +497,7 @@ extern "C" int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p)
   for (int G = 1; G <= 256 && (G == 1 || longest / G >= 2); ++G) {
     const int K = (longest + G - 1) / G;
     double t = rounds(seqs * G * out) * K * (2.5 + 0.6 * RB);
-    if (G > 1) t += rounds(seqs * (G - 1) * first) * K * (1.5 + 0.4 * RB) + G * 0.65 * RB + 10;
+    if (G > 1) t += rounds(seqs * (G - 1) * first) * K * (1.5 + 0.4 * RB) + G * 0.55 * RB + 10;
     if (G == 1 || t < least) {
       least = t;
       best = K;

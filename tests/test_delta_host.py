@@ -109,6 +109,9 @@ def test_scan_refusals(anywhere):
         _scan_check(a)
     with pytest.raises(ValueError, match="sequences, T, columns"):
         _scan_check([t[0] for t in _args()])
+    long = [t[:, :1].expand(2, 2 ** 31, *t.shape[2:]) for t in _args()]
+    with pytest.raises(ValueError, match="at most 2\\^31"):
+        _scan_check(long)
     with pytest.raises(ValueError, match="segments end at 3"):
         hip_delta._Plan("gated_delta_scan", *[_args(T=4)[i] for i in (0, 2)], seg)
 
@@ -145,6 +148,19 @@ def test_tree_refusals(anywhere):
                      ((torch.zeros(4, **i32),), dict(tree=hip_fwd.DraftTree([[-1, 0]] * 2, "cpu")))):
         with pytest.raises(ValueError):
             state(*args, **kw)
+    same = torch.zeros(2, **i32)
+    with pytest.raises(ValueError, match="must not be nodes"):
+        state(same, ahead=same)
+
+
+def test_first_commit_is_not_captured(anywhere, monkeypatch):
+    """A captured first commit would clear the positions in every replay."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    dec = A.SmatDecoder.from_cache(torch.zeros(2, 3, 8, 9), torch.zeros(2, 8, 9))
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        dec.commit(torch.zeros(2, 2, 8), torch.zeros(2, 2, 9), hip_fwd.DraftTree([-1, 0], "cpu"),
+                   torch.zeros(2, dtype=torch.int32))
+    assert dec.ahead is None
 
 
 def test_step_refusals(anywhere):

@@ -301,6 +301,84 @@ def test_offsets_past_32_bits():
                        A.gated_delta_scan(q, k, v, logA, beta))
 
 
+def test_far_key_rows():
+    """Queries and keys whose rows lie 2^24 elements and more apart."""
+    T, r, p, st = 66, 32, 32, 2 ** 24 + 8
+    q, k, v, logA, beta, _ = _inputs(1, 1, T, r, p, BF16, seed=7)
+    buf = torch.empty(2 * T * st, device=DEV, dtype=BF16).view(2, 1, T, st)[..., :r]
+    buf[0].copy_(q)
+    buf[1].copy_(k)
+    assert torch.equal(A.gated_delta_scan(buf[0], buf[1], v, logA, beta),
+                       A.gated_delta_scan(q, k, v, logA, beta))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_segments_and_sequences_keep_apart(dtype, bad):
+    """What is not finite in one segment or sequence reaches no other one: outputs, states and
+    gradients of the others stay the same bits."""
+    nb, T, r, p, off = 3, 64 * 40, 64, 40, [0, 64 * 20 + 5, 64 * 20 + 35, 64 * 40]
+    x = _inputs(nb, nb, T, r, p, dtype, seed=15, state=(3,), decay=0.1)
+    dO = torch.randn(nb, T, p, generator=torch.Generator().manual_seed(3)).to(dtype).to(DEV)
+    seg = A.Segments(off, DEV)
+
+    def run(x, dO):
+        x = [t.clone().requires_grad_(True) for t in x]
+        o, S = A.gated_delta_scan(*x[:5], state=x[5], segments=seg, return_state=True)
+        return [o.detach(), S.detach(), *torch.autograd.grad(o, x, dO)]
+    want = run(x, dO)
+    for lo, hi in ((off[0], off[1]), (off[1], off[2]), (off[2], off[3])):
+        y, dO2 = [t.clone() for t in x], dO.clone()
+        for t in (*y[:5], dO2):
+            t[1, lo:hi] = bad
+        got = run(y, dO2)
+        keep = torch.ones(nb, T, dtype=torch.bool, device=DEV)
+        keep[1, lo:hi] = False
+        skeep = torch.ones(3, nb, dtype=torch.bool, device=DEV)
+        skeep[off.index(lo), 1] = False
+        for n, (a, b) in enumerate(zip(got, want)):
+            m = skeep if n in (1, 7) else keep
+            assert torch.equal(a[m], b[m]), (n, lo)
+
+
+def test_gradient_with_resets():
+    """Decays to zero inside chunks, at their borders and at both ends."""
+    nb, T, r, p = 2, 150, 32, 40
+    q, k, v, logA, beta, S = _inputs(nb, nb, T, r, p, FP32, seed=16, state=())
+    logA[:, [0, 3, 4, 63, 64, 100, 149]] = -math.inf
+    x = [t.requires_grad_(True) for t in (q, k, v, logA, beta, S)]
+    o, So = A.gated_delta_scan(*x[:5], state=S, return_state=True)
+    y = [t.detach().double().requires_grad_(True) for t in x]
+    ro, rS = O.delta_scan(*y[:5], state=y[5])
+    g = torch.Generator().manual_seed(17)
+    d = [torch.randn(t.shape, generator=g).to(DEV) for t in (o, So)]
+    got = torch.autograd.grad((o, So), x, d)
+    ref = torch.autograd.grad((ro, rS), y, [t.double() for t in d])
+    for name, a, b in zip(("dq", "dk", "dv", "dlogA", "dbeta", "dS0"), got, ref):
+        assert torch.isfinite(a).all() and torch.isfinite(b).all(), name
+        if name == "dlogA":                          # sums terms as large as <dS, S> (see above)
+            lim = 3 * (r + p + 128) * 2.0 ** -24 * r * p * (rS.abs().max() * d[1].abs().max())
+            assert (a.double() - b).abs().max() <= lim
+        else:
+            _check(name, a, b, 6, r, p)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, each with its own workspaces."""
+    cases = [_inputs(2, 2, 64 * 36, 64, 64, BF16, seed=s) for s in (18, 19)]
+    want = [A.gated_delta_scan(*c[:5]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(A.gated_delta_scan(*cases[i][:5]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
 def test_empty():
     q, k, v, logA, beta, S = _inputs(2, 2, 0, 8, 8, BF16, state=())
     o, So = A.gated_delta_scan(q, k, v, logA, beta, state=S, return_state=True)
