@@ -16,6 +16,12 @@
 // (its columns are more columns of the same recurrence, with V = 0), a kernel
 // carries the states across the runs, S <- M S + E, and the second pass takes every
 // run from its own state.
+//
+// What bounds it: the vector ALUs, which split every product's result into terms (eight
+// operations a value), and MFMA issue beside them.  8 sequences of 131072 tokens, r = p =
+// 128 in bf16: 672 us for the first pass, 71 for the carry over 32 runs, 515 for the
+// second, 0.81 PFLOP/s of issued products.  In training the second pass also writes S and
+// U and runs at 5 TB/s (96 x 4096, r = p = 64: 119 us).
 #include "delta_prep.hpp"
 
 namespace smat {
@@ -482,9 +488,9 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 // Run length: the number of runs a segment, G, that takes least by what a step of a
 // full GPU (512 workgroups of four column tiles) measures, in microseconds: 2.5 + 0.6 RB
 // a chunk of the pass with outputs, 1.5 + 0.4 RB of the first pass, 0.55 RB a run of the
-// carry, 10 for the two launches more.  (8 sequences of 2048 chunks, r = p = 128: 9349
-// whole, 1352 in 32 runs, 2082 in 256; 96 of 64 chunks, r = p = 64, forward and
-// backward: 1074 whole, 930 in 8, 1048 in 2.)
+// carry, 10 for the two launches more.  (8 sequences of 2048 chunks, r = p = 128: 9367
+// whole, 1377 in 32 runs, 1457 in 64, 1670 in 128; 96 of 64 chunks, r = p = 64, forward
+// and backward: 1053 whole, 902 in 8 runs, 982 in 2.)
 extern "C" int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p) {
   if (longest < 1 || nb < 1 || r < 1 || p < 1) return 1;
   const int RB = (r + 31) / 32;

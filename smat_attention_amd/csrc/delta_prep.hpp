@@ -10,6 +10,9 @@
 // L is summed and subtracted in fp64, so that a decay that has cost the chunk
 // hundreds of nats leaves the differences of later tokens exact; logA below -1e5
 // (a = 0 many times over) counts as -1e5, which keeps -inf - -inf out.
+//
+// Bound by HBM, what it writes above all (T in three terms, 18 KB): 194 us for 8
+// sequences of 131072 tokens, r = 128 in bf16, 5.4 TB/s.
 #pragma once
 
 #include "delta_common.hpp"

@@ -7,8 +7,9 @@
 // registers, so that one exchange through LDS settles u, o and the update.  A workgroup
 // takes 4 CL columns; thread (row group, column lane) holds every RG-th row of four
 // columns, all loaded before the first exchange.  Columns do not mix, so S' may be S.
-// 2048 sequences of 128 x 128: 52 us a token, 5.2 TB/s.  Seven tokens of 8 sequences of
-// 64 x 64 take one launch here; as a chunk they are 18 us of two dependent kernels.
+// 2048 sequences of 128 x 128: 45 us a token, 6 TB/s (the state partly stays in the
+// last-level cache).  Seven tokens of 8 sequences of 64 x 64 take one launch of 12.5 us
+// here; as a chunk they are 18 us of two dependent kernels.
 #include "delta_common.hpp"
 
 namespace smat {
