@@ -32,7 +32,8 @@ template <typename In, int CL, bool VEC, bool ONE>
 __global__ __launch_bounds__(kStepThreads, ONE ? 4 : 2) void delta_tokens_kernel(Tokens g) {
   constexpr int RG = kStepThreads / CL, ROWS = kMaxR / RG, WAVES = kStepThreads / 64;
   constexpr int MOST = ONE ? 1 : kFewTokens, BUFS = ONE ? 1 : 2;
-  __shared__ float sq[MOST][kMaxR], sk[MOST][kMaxR];
+  __shared__ float sq[MOST][kMaxR], sk[MOST][kMaxR], sa[MOST], sb[MOST];
+  __shared__ __align__(16) f32x4 sv[ONE ? 1 : MOST][ONE ? 1 : CL];
   __shared__ __align__(16) f32x4 rk[BUFS][WAVES][CL], rq[BUFS][WAVES][CL];
   __shared__ float rqk[BUFS][WAVES];
   const int T = ONE ? 1 : g.T;
@@ -60,22 +61,55 @@ __global__ __launch_bounds__(kStepThreads, ONE ? 4 : 2) void delta_tokens_kernel
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) S[j] = zero4();
   }
-  for (int e = tid; e < T * kMaxR; e += kStepThreads) {
-    const int t = e / kMaxR, a = e % kMaxR;
-    sq[t][a] = a < g.r ? to_f32(((const In*)g.q)[ks * g.q_sb + t * g.q_st + a]) : 0.f;
-    sk[t][a] = a < g.r ? to_f32(((const In*)g.k)[ks * g.k_sb + t * g.k_st + a]) : 0.f;
+  // four rows of q and k a thread in flight; those past the last token's are not kept
+  constexpr int ROUND = ONE ? 1 : 4, STEP = kStepThreads / kMaxR;
+  const int a0 = tid % kMaxR, ac = min(a0, g.r - 1);
+  const In *qs = (const In*)g.q + ks * g.q_sb + ac, *kk = (const In*)g.k + ks * g.k_sb + ac;
+  for (int t0 = tid / kMaxR; t0 < T; t0 += ROUND * STEP) {
+    In xq[ROUND], xk[ROUND];
+#pragma unroll
+    for (int i = 0; i < ROUND; ++i) {
+      const int t = min(t0 + i * STEP, T - 1);
+      xq[i] = qs[t * g.q_st];
+      xk[i] = kk[t * g.k_st];
+    }
+#pragma unroll
+    for (int i = 0; i < ROUND; ++i)
+      if (t0 + i * STEP < T) {
+        sq[t0 + i * STEP][a0] = a0 < g.r ? to_f32(xq[i]) : 0.f;
+        sk[t0 + i * STEP][a0] = a0 < g.r ? to_f32(xk[i]) : 0.f;
+      }
   }
-  float la = g.logA[s * g.a_sb], b = g.beta[s * g.b_sb];
-  const In* vs = (const In*)g.v + s * g.v_sb + c0;
-  f32x4 vv = load4(vs, nv, false);
+  // the tokens' gates and values too: a load inside the loop would be waited for in it
+  const In* vs = (const In*)g.v + s * g.v_sb;
+  auto values = [&](const In* row, int c) {        // columns past the last: the last one's
+    f32x4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = to_f32(row[min(c + i, g.p - 1)]);
+    return x;
+  };
+  float a = 0.f, b = 0.f;
+  f32x4 v = zero4();
+  if constexpr (ONE) {
+    a = expf(g.logA[s * g.a_sb]);
+    b = g.beta[s * g.b_sb];
+    v = values(vs, c0);
+  } else {
+    if (tid < T) {
+      sa[tid] = expf(g.logA[s * g.a_sb + tid * g.a_st]);
+      sb[tid] = g.beta[s * g.b_sb + tid * g.b_st];
+    }
+    for (int e = tid; e < T * CL; e += kStepThreads) {
+      const int t = e / CL;
+      sv[t][e % CL] = values(vs + t * g.v_st, (blockIdx.y * CL + e % CL) * 4);
+    }
+  }
   __syncthreads();
   for (int t = 0; t < T; ++t) {
-    const float a = expf(la), bt = b;
-    const f32x4 vt = vv;
-    if (t + 1 < T) {                             // the next token's, ahead of the exchange
-      la = g.logA[s * g.a_sb + (t + 1) * g.a_st];
-      b = g.beta[s * g.b_sb + (t + 1) * g.b_st];
-      vv = load4(vs + (t + 1) * g.v_st, nv, false);
+    if constexpr (!ONE) {
+      a = sa[t];
+      b = sb[t];
+      v = sv[t][cl];
     }
     f32x4 ks4 = zero4(), qs4 = zero4();
     float qk = 0.f;
@@ -111,7 +145,7 @@ __global__ __launch_bounds__(kStepThreads, ONE ? 4 : 2) void delta_tokens_kernel
       qs4 += rq[buf][i][cl];
       qk += rqk[buf][i];
     }
-    const f32x4 u = bt * (vt - a * ks4);
+    const f32x4 u = b * (v - a * ks4);
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) S[j] = a * S[j] + sk[t][rg + j * RG] * u;
     if (rg == 0)
