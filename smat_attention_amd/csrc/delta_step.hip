@@ -7,8 +7,8 @@
 // registers, so that one exchange through LDS settles u, o and the update.  A workgroup
 // takes 4 CL columns; thread (row group, column lane) holds every RG-th row of four
 // columns, all loaded before the first exchange.  Columns do not mix, so S' may be S.
-// 2048 sequences of 128 x 128: 45 us a token, 6 TB/s (the state partly stays in the
-// last-level cache).  Seven tokens of 8 sequences of 64 x 64 take one launch of 12.5 us
+// 2048 sequences of 128 x 128: 43 us a token, 6.3 TB/s (the state partly stays in the
+// last-level cache).  Seven tokens of 8 sequences of 64 x 64 take one launch of 9 us
 // here; as a chunk they are 18 us of two dependent kernels.
 #include "delta_common.hpp"
 
@@ -26,6 +26,26 @@ struct Tokens {
   float scale;
   int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st, a_sb, a_st, b_sb, b_st, o_sb, o_st;
 };
+
+// x of this lane and of lane ^ D, summed in registers (a shuffle through LDS takes ten
+// times as long, and a token is a chain of them).
+template <int D> __device__ __forceinline__ float sum_across(float x) {
+  static_assert(D == 8 || D == 16 || D == 32, "");
+  if constexpr (D == 8) {                          // a rotation within 16 lanes
+    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf,
+                                                           false));
+  } else {
+    const uint32_t b = __float_as_uint(x);
+    const auto r = D == 16 ? __builtin_amdgcn_permlane16_swap(b, b, false, false)
+                           : __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+}
+template <int CL> __device__ __forceinline__ float sum_rows(float x) {
+  if constexpr (CL <= 8) x = sum_across<8>(x);
+  if constexpr (CL <= 16) x = sum_across<16>(x);
+  return sum_across<32>(x);
+}
 
 // ONE: a single token (less LDS and fewer registers, so more of the state in flight).
 template <typename In, int CL, bool VEC, bool ONE>
@@ -121,14 +141,11 @@ __global__ __launch_bounds__(kStepThreads, ONE ? 4 : 2) void delta_tokens_kernel
       qk += kr * qr;
     }
 #pragma unroll
-    for (int d = CL; d < 64; d <<= 1) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        ks4[i] += __shfl_xor(ks4[i], d);
-        qs4[i] += __shfl_xor(qs4[i], d);
-      }
-      qk += __shfl_xor(qk, d);
+    for (int i = 0; i < 4; ++i) {
+      ks4[i] = sum_rows<CL>(ks4[i]);
+      qs4[i] = sum_rows<CL>(qs4[i]);
     }
+    qk = sum_rows<CL>(qk);
     const int buf = ONE ? 0 : t & 1;                         // alternating: one barrier a token
     if (lane_id() < CL) {
       rk[buf][w][cl] = ks4;
