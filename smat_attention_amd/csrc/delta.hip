@@ -69,8 +69,8 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
   float* vl = reinterpret_cast<float*>(pl + (OUT ? NO * TB : 0));
   constexpr int W = chain_waves<In, RB, OUT>();
   const int w = uniform_wave();
-  const int ct = blockIdx.x * W + w;
-  const int run = blockIdx.y, s = blockIdx.z;
+  const int ct = blockIdx.y * W + w;
+  const int run = blockIdx.z, s = blockIdx.x;      // sequences first: see below
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
   bool head, tail;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
   bool on = ct < tiles;                            // else: copies and barriers only
   if (!OUT) {                                      // E of all runs but a segment's last, and M
     const bool e = !tail, t = !(head && tail) && (!head || io.first_m) && (!tail || io.last_m);
-    const int w0 = blockIdx.x * W;
+    const int w0 = blockIdx.y * W;
     if (!(e && w0 < io.ptiles) && !(t && w0 + W > io.ptiles)) return;
     on = on && (values ? e : t);
   }
@@ -437,7 +437,9 @@ static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipS
   auto kern = delta_chain_kernel<In, RB, OUT>;
   static uint64_t done;
   allow_lds(kern, lds, done);
-  hipLaunchKernelGGL(kern, dim3((tiles + W - 1) / W, g.nruns, g.nb), dim3(64 * W), lds, st, g, o,
+  // workgroups go to the XCDs in turn: with the sequences first, runs that are shorter or
+  // not wanted leave every XCD as much
+  hipLaunchKernelGGL(kern, dim3(g.nb, (tiles + W - 1) / W, g.nruns), dim3(64 * W), lds, st, g, o,
                      io, tiles);
 }
 

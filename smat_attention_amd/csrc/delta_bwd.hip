@@ -65,9 +65,9 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
   float* vl = reinterpret_cast<float*>(pl + NI * TB);
   constexpr int W = rchain_waves<In, RB>();
   const int w = uniform_wave();
-  const int ct = blockIdx.x * W + w;
+  const int ct = blockIdx.y * W + w;
   const bool on = ct < tiles;                      // else: copies and barriers only
-  const int run = blockIdx.y, s = blockIdx.z;
+  const int run = blockIdx.z, s = blockIdx.x;      // sequences first, as in the forward
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int c0, c1, seg;
   bool head, tail;
@@ -550,7 +550,7 @@ static void rchain(const Geo& g, const Ops& o, const RChainIO& io, int tiles, hi
   auto kern = delta_rchain_kernel<In, RB, OUT>;
   static uint64_t done;
   allow_lds(kern, lds, done);
-  hipLaunchKernelGGL(kern, dim3((tiles + W - 1) / W, g.nruns, g.nb), dim3(64 * W), lds, st, g, o,
+  hipLaunchKernelGGL(kern, dim3(g.nb, (tiles + W - 1) / W, g.nruns), dim3(64 * W), lds, st, g, o,
                      io, tiles);
 }
 
