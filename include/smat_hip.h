@@ -556,14 +556,16 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  * (value sequence s reads key sequence s / (nb / nbk)); logA, beta: (nb, T)
  * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256,
  * v_st (and the gradient's d_st) < 2^23.
- * Segments: chunks (nch, 2) = first token, tokens (<= 64); runs (nruns, 3) =
+ * Segments: chunks (nch, 2) = first token, tokens (<= 64); runs (nruns, 4) =
  * first chunk, end chunk, segment, every segment's runs together and in order,
- * an empty segment with one empty run; segrun (nseg + 1) the first run of each
+ * an empty segment with one empty run, and in the last column the runs' order
+ * of work (a permutation: the longest first); segrun (nseg + 1) the first run of each
  * segment.  Entries are trusted.  All three NULL: one segment, chunks of 64,
  * runs of K chunks, nch = ceil(T / 64), nruns = max(1, ceil(nch / K)).
  * With more runs than segments the sequences are also split along T.
- * smat_delta_run_chunks: the run length that fills the GPU (longest: the
- * chunks of the longest segment).
+ * smat_delta_run_chunks: the run length that takes least time, for times[i]
+ * (host arrays) segments of lengths[i] chunks each, or, with NULL arrays, for
+ * one of nch.
  * state: (nseg, nb, r, p) fp32 entering each segment (NULL: zero); state_out
  * the same leaving it (may be NULL; not state itself).
  * Training: save_s (nb, nch, R, P) and save_u (nb, nch, 64, P) fp32, R and P
@@ -574,7 +576,8 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  * workspace: smat_delta_workspace_bytes(..., backward) bytes, 256-byte aligned;
  * none is used for up to 16 tokens without the tables and save_s.
  */
-int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p);
+int smat_delta_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
+                          const int32_t* times, int n, int r, int p);
 int64_t smat_delta_workspace_bytes(int dtype, int nb, int nbk, int nch, int nseg, int nruns,
                                    int r, int p, int backward);
 int smat_delta_scan(int dtype, const void* q, const void* k, const void* v, const float* logA,

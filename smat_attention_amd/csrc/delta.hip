@@ -70,11 +70,11 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
   constexpr int W = chain_waves<In, RB, OUT>();
   const int w = uniform_wave();
   const int ct = blockIdx.y * W + w;
-  const int run = blockIdx.z, s = blockIdx.x;      // sequences first: see below
+  const int s = blockIdx.x;                        // sequences first: see below
   const int m = lane_id() & 15, gq = lane_id() >> 4;
-  int c0, c1, seg;
+  int run, c0, c1, seg;
   bool head, tail;
-  run_of(g, run, c0, c1, seg, head, tail);
+  run_of(g, blockIdx.z, run, c0, c1, seg, head, tail);
   const bool values = ct < io.ptiles;              // else columns of the transition
   bool on = ct < tiles;                            // else: copies and barriers only
   if (!OUT) {                                      // E of all runs but a segment's last, and M
@@ -438,7 +438,7 @@ static void chain(const Geo& g, const Ops& o, const ChainIO& io, int tiles, hipS
   static uint64_t done;
   allow_lds(kern, lds, done);
   // workgroups go to the XCDs in turn: with the sequences first, runs that are shorter or
-  // not wanted leave every XCD as much
+  // not wanted leave every XCD as much; the runs table has the longest go first
   hipLaunchKernelGGL(kern, dim3(g.nb, (tiles + W - 1) / W, g.nruns), dim3(64 * W), lds, st, g, o,
                      io, tiles);
 }
@@ -487,27 +487,59 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 }  // namespace dl
 }  // namespace smat
 
-// Run length: the number of runs a segment, G, that takes least by what a step of a
-// full GPU (512 workgroups of four column tiles) measures, in microseconds: 2.5 + 0.6 RB
-// a chunk of the pass with outputs, 1.5 + 0.4 RB of the first pass, 0.55 RB a run of the
-// carry, 10 for the two launches more.  (8 sequences of 2048 chunks, r = p = 128: 9367
-// whole, 1377 in 32 runs, 1457 in 64, 1670 in 128; 96 of 64 chunks, r = p = 64, forward
-// and backward: 1053 whole, 902 in 8 runs, 982 in 2.)
-extern "C" int smat_delta_run_chunks(int nb, int nch, int longest, int r, int p) {
-  if (longest < 1 || nb < 1 || r < 1 || p < 1) return 1;
-  const int RB = (r + 31) / 32;
-  // segments as many as the longest would leave of the chunks
-  const double seqs = (double)nb * nch / longest;
-  const int out = (p + 63) / 64, first = ((p + 15) / 16 + 2 * RB + 3) / 4;
-  auto rounds = [](double wgs) { return wgs <= 512 ? 1.0 : wgs / 512; };
+// Run length: of the lengths that cut the longest segment into 1 to 256 runs, the one
+// whose passes take least by what their steps measure, in microseconds a chunk with a
+// workgroup on every CU: 3.4 + 0.375 RB with outputs, 1.9 + 0.24 RB in the first pass,
+// 1.9 times that where inputs have several terms; 0.55 RB a run of the carry and 10 for
+// the two launches more.  Workgroups of four waves share a CU in pairs, which then take
+// 1.64 times as long; more than are resident follow one another, the last ones alone.
+// (8 sequences of 2048 chunks, r = p = 128: 9367 whole, 1377 in 32 runs, 1457 in 64,
+// 1670 in 128; 12 of 5 segments and 158 chunks, r = p = 96 in fp16: 640 whole, 251 in
+// runs of 10, 303 of 8, 285 of 16.)
+extern "C" int smat_delta_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
+                                     const int32_t* times, int n, int r, int p) {
+  using namespace smat::dl;
+  const bool packed = lengths && times && n > 0;
+  int longest = packed ? 0 : nch;
+  for (int i = 0; packed && i < n; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
+  if (longest < 1 || nb < 1 || r < 1 || p < 1 || r > kMaxR || dtype < SMAT_BF16 ||
+      dtype > SMAT_F32)
+    return 1;
+  const int RB = rblocks(r), tiles = (p + 15) / 16;
+  int wout = 4, wfirst = 4;
+  dispatch(dtype, r, [&](auto in, auto rb) {
+    wout = chain_waves<decltype(in), decltype(rb)::value, true>();
+    wfirst = chain_waves<decltype(in), decltype(rb)::value, false>();
+    return 0;
+  });
+  const double terms = dtype == SMAT_BF16 ? 1.0 : 1.9;
+  // a pass of wgs workgroups of up to K chunks, `steps` chunks in all
+  auto pass = [&](double wgs, double steps, int K, int waves, double cost) {
+    const double share = waves == 4 ? 0.82 : 1.0;
+    if (wgs <= 256) return K * cost;
+    if (waves == 4 && wgs <= 512) return 2 * share * K * cost;
+    return (share * steps / 256 + 0.4 * K) * cost;
+  };
   int best = longest;
   double least = 0;
   for (int G = 1; G <= 256 && (G == 1 || longest / G >= 2); ++G) {
     const int K = (longest + G - 1) / G;
-    double t = rounds(seqs * G * out) * K * (2.5 + 0.6 * RB);
-    if (G > 1) t += rounds(seqs * (G - 1) * first) * K * (1.5 + 0.4 * RB) + G * 0.55 * RB + 10;
-    if (G == 1 || t < least) {
-      least = t;
+    double runs = 0, chunks = 0, ends = 0;         // `ends`: runs with one behind them
+    for (int i = 0; i < (packed ? n : 1); ++i) {
+      const double len = packed ? lengths[i] : nch, t = packed ? times[i] : 1;
+      const double cut = len > K ? (int)((len + K - 1) / K) : 1;
+      runs += t * cut;
+      ends += t * (cut - 1);
+      chunks += t * len;
+    }
+    const double out = (double)nb * ((tiles + wout - 1) / wout);
+    const double first = (double)nb * ((tiles + 2 * RB + wfirst - 1) / wfirst);
+    double us = pass(runs * out, chunks * out, K, wout, terms * (3.4 + 0.375 * RB));
+    if (ends > 0)
+      us += pass(ends * first, ends * K * first, K, wfirst, terms * (1.9 + 0.24 * RB)) +
+            G * 0.55 * RB + 10;
+    if (G == 1 || us < least) {
+      least = us;
       best = K;
     }
   }

@@ -67,11 +67,11 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
   const int w = uniform_wave();
   const int ct = blockIdx.y * W + w;
   const bool on = ct < tiles;                      // else: copies and barriers only
-  const int run = blockIdx.z, s = blockIdx.x;      // sequences first, as in the forward
+  const int s = blockIdx.x;                        // sequences first, as in the forward
   const int m = lane_id() & 15, gq = lane_id() >> 4;
-  int c0, c1, seg;
+  int run, c0, c1, seg;
   bool head, tail;
-  run_of(g, run, c0, c1, seg, head, tail);
+  run_of(g, blockIdx.z, run, c0, c1, seg, head, tail);
   if (!OUT && head) return;                        // nothing is carried past a segment's first run
   const int col = 16 * ct + m;
   const int64_t ks = key_of(g, s);

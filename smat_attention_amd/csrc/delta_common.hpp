@@ -539,12 +539,14 @@ __device__ __forceinline__ void chunk_of(const Geo& g, int c, int& t0, int& len)
     len = min(C, g.T - t0);
   }
 }
-__device__ __forceinline__ void run_of(const Geo& g, int i, int& c0, int& c1, int& seg,
+__device__ __forceinline__ void run_of(const Geo& g, int turn, int& i, int& c0, int& c1, int& seg,
                                        bool& first, bool& last) {
+  i = turn;
   if (g.runs) {
-    c0 = g.runs[3 * i];
-    c1 = g.runs[3 * i + 1];
-    seg = g.runs[3 * i + 2];
+    i = g.runs[4 * turn + 3];
+    c0 = g.runs[4 * i];
+    c1 = g.runs[4 * i + 1];
+    seg = g.runs[4 * i + 2];
     first = g.segrun[seg] == i;
     last = g.segrun[seg + 1] == i + 1;
   } else {

@@ -129,7 +129,7 @@ SIGNATURES = {
                             _i, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "smat_tree_state": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i64, _i64,
                              _i64, _i64, _p]),
-    "smat_delta_run_chunks": (_i, [_i, _i, _i, _i, _i]),
+    "smat_delta_run_chunks": (_i, [_i, _i, _i, _p, _p, _i, _i, _i]),
     "smat_delta_workspace_bytes": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "smat_delta_scan": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i,
                              _i, _i, _i, _i, _i, _i, _i, _f, _i64, _i64, _i64, _i64, _i64, _i64,

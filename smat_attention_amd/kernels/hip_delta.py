@@ -56,8 +56,10 @@ class Segments:
         # one row at least, so that the table's address says that there is one
         self.chunks = torch.from_numpy(rows if len(rows) else
                                        np.zeros((1, 2), np.int32)).to(self.device)
-        self.nch, self.longest = int(first[-1]), int(counts.max())
-        self._runs = {}
+        self.nch = int(first[-1])
+        self._lengths, self._times = (np.ascontiguousarray(x, dtype=np.int32) for x in
+                                      np.unique(counts, return_counts=True))
+        self._runs, self._best = {}, {}
 
     def __len__(self):
         return len(self.offsets) - 1
@@ -65,6 +67,15 @@ class Segments:
     @property
     def T(self):
         return self.offsets[-1]
+
+    def run_chunks(self, code: int, nb: int, r: int, p: int) -> int:
+        """The run length for inputs of these sizes, searched at the first call with them."""
+        key = (code, nb, r, p)
+        if key not in self._best:
+            self._best[key] = _lib.query("smat_delta_run_chunks", code, nb, self.nch,
+                                         self._lengths.ctypes.data, self._times.ctypes.data,
+                                         len(self._lengths), r, p)
+        return self._best[key]
 
     def runs(self, K: int):
         """``(runs, segrun)`` on the device for runs of ``K`` chunks; staged at the first call
@@ -76,7 +87,10 @@ class Segments:
                 for a in range(0, max(int(n), 1), K):
                     rows.append((c0 + a, c0 + min(a + K, int(n)), s))
                 segrun.append(len(rows))
-            self._runs[K] = tuple(torch.tensor(x, dtype=torch.int32).to(self.device)
+            rows = np.array(rows)
+            turns = np.argsort(rows[:, 0] - rows[:, 1], kind="stable")    # the longest first
+            rows = np.concatenate([rows, turns[:, None]], 1)
+            self._runs[K] = tuple(torch.from_numpy(np.asarray(x, np.int32)).to(self.device)
                                   for x in (rows, segrun))
         return self._runs[K]
 
@@ -102,9 +116,14 @@ class _Plan:
                 raise ValueError(f"{who}: segments are on {segments.device}, the inputs on "
                                  f"{Q.device}")
             self.nseg, self.nch = len(segments), segments.nch
-        longest = self.nch if segments is None else segments.longest
-        self.K = 1 if longest <= 1 else _lib.query("smat_delta_run_chunks", self.nb, self.nch,
-                                                   longest, self.r, self.p)
+        code = _code(Q, who)
+        if segments is not None:
+            self.K = segments.run_chunks(code, self.nb, self.r, self.p)
+        elif self.nch <= 1:
+            self.K = 1
+        else:
+            self.K = _lib.query("smat_delta_run_chunks", code, self.nb, self.nch, None, None, 0,
+                                self.r, self.p)
         if segments is None:
             self.tables = (None, None, None)
             self.nruns = max(1, -(-self.nch // self.K))

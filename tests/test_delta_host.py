@@ -14,7 +14,7 @@ def test_segments_tables():
     assert len(s) == 4 and s.T == 194 and s.nch == 5
     assert s.chunks.tolist() == [[0, 1], [1, 64], [65, 64], [129, 1], [130, 64]]
     runs, segrun = s.runs(2)
-    assert runs.tolist() == [[0, 1, 0], [1, 1, 1], [1, 3, 2], [3, 4, 2], [4, 5, 3]]
+    assert runs.tolist() == [[0, 1, 0, 2], [1, 1, 1, 0], [1, 3, 2, 3], [3, 4, 2, 4], [4, 5, 3, 1]]
     assert segrun.tolist() == [0, 1, 2, 4, 5]
     assert s.runs(2)[0] is runs
     assert hip_delta.Segments(torch.tensor([0, 0]), "cpu").nch == 0
@@ -218,12 +218,18 @@ def test_c_entry_points_refuse():
 
 
 def test_run_lengths():
-    q = lambda *a: _lib.query("smat_delta_run_chunks", *a)
-    assert q(512, 1000, 1000, 64, 64) == 1000        # enough sequences: whole segments
-    assert q(1, 3, 3, 64, 64) == 3                   # too short to split
-    assert q(1, 0, 0, 64, 64) == 1
-    assert 2 <= q(8, 2048, 2048, 128, 128) < 2048
-    assert 2 <= q(1, 100, 90, 64, 64) < 90           # one long segment among short ones
+    for code in range(3):
+        def q(nb, nch, r, p):
+            return _lib.query("smat_delta_run_chunks", code, nb, nch, None, None, 0, r, p)
+        assert q(512, 1000, 64, 64) == 1000          # enough sequences: whole segments
+        assert q(1, 3, 64, 64) == 3                  # too short to split
+        assert q(1, 0, 64, 64) == 1
+        assert 2 <= q(8, 2048, 128, 128) < 2048
+        # one long segment among short ones and an empty one
+        off = [0, 64, 64, 64 * 91, 64 * 93, 64 * 100]
+        assert 2 <= hip_delta.Segments(off, "cpu").run_chunks(code, 1, 64, 64) < 90
+        assert hip_delta.Segments([0, 5], "cpu").run_chunks(code, 1, 64, 64) == 1
+        assert hip_delta.Segments([0, 0], "cpu").run_chunks(code, 1, 64, 64) == 1
 
 
 def test_oracle_is_the_plain_rule():

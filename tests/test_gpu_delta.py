@@ -150,10 +150,8 @@ def test_split_along_the_sequence(dtype, nb, nbk, T, r, p, off, st):
     q, k, v, logA, beta, S = _inputs(nb, nbk, T, r, p, dtype, seed=3, state=lead if st else None,
                                      decay=0.1)
     seg = None if off is None else A.Segments(off, DEV)
-    from smat_attention_amd.kernels import _lib
-    nch = seg.nch if seg else -(-T // 64)
-    longest = seg.longest if seg else nch
-    assert _lib.query("smat_delta_run_chunks", nb, nch, longest, r, p) < longest
+    from smat_attention_amd.kernels.hip_delta import _Plan
+    assert _Plan("test", q, v, seg).nruns > (len(seg) if seg else 1)
     leaves = [t.requires_grad_(True) for t in (q, k, v, logA, beta)]
     o, So = A.gated_delta_scan(*leaves, state=S, segments=seg, return_state=True)
     ref_in = [t.detach().double().requires_grad_(True) for t in leaves]
