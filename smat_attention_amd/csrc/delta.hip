@@ -19,9 +19,9 @@
 //
 // What bounds it: the vector ALUs, which split every product's result into terms (eight
 // operations a value), and MFMA issue beside them.  8 sequences of 131072 tokens, r = p =
-// 128 in bf16: 672 us for the first pass, 71 for the carry over 32 runs, 515 for the
-// second, 0.81 PFLOP/s of issued products.  In training the second pass also writes S and
-// U and runs at 5 TB/s (96 x 4096, r = p = 64: 119 us).
+// 128 in bf16: 675 us for the first pass, 61 for the carry over 32 runs, 498 for the
+// second, 0.82 PFLOP/s of issued products.  In training the second pass also writes S and
+// U and runs at 5 TB/s (96 x 4096, r = p = 64: 120 us).
 #include "delta_prep.hpp"
 
 namespace smat {
