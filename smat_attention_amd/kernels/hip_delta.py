@@ -81,6 +81,9 @@ class Segments:
         """``(runs, segrun)`` on the device for runs of ``K`` chunks; staged at the first call
         with that K (outside a graph capture)."""
         if K not in self._runs:
+            if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Segments: the first call with inputs of these sizes stages a "
+                                   "table and cannot be captured; make one before")
             rows, segrun = [], [0]
             for s, n in enumerate(self._counts):
                 c0 = int(self._first[s])

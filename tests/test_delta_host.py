@@ -153,6 +153,16 @@ def test_tree_refusals(anywhere):
         state(same, ahead=same)
 
 
+def test_run_tables_are_not_staged_in_a_capture(monkeypatch):
+    seg = hip_delta.Segments([0, 100, 300], "cpu")
+    kept = seg.runs(2)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    seg.device = torch.device("cuda", 0)
+    assert seg.runs(2) is kept
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        seg.runs(3)
+
+
 def test_first_commit_is_not_captured(anywhere, monkeypatch):
     """A captured first commit would clear the positions in every replay."""
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
