@@ -616,12 +616,12 @@ static int backward(int dtype, const Geo& g, const In* q, const In* k, GradIO gr
 extern "C" int smat_delta_scan_backward(
     int dtype, const void* q, const void* k, const void* v, const float* logA, const float* beta,
     const void* dout, const float* dstate_out, const float* save_s, const float* save_u,
-    const void* save_m, void* dq, void* dk, void* dv, float* dlogA, float* dbeta, float* dstate, const int32_t* chunks,
-    const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T, int nseg, int nch,
-    int nruns, int K, int r, int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
-    int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st, int64_t b_sb,
-    int64_t b_st, int64_t d_sb, int64_t d_st, void* workspace, int64_t workspace_bytes,
-    void* stream) {
+    const void* save_m, void* dq, void* dk, void* dv, float* dlogA, float* dbeta, float* dstate,
+    const int32_t* chunks, const int32_t* runs, const int32_t* segrun, int nb, int nbk, int T,
+    int nseg, int nch, int nruns, int K, int r, int p, float scale, int64_t q_sb, int64_t q_st,
+    int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st, int64_t a_sb, int64_t a_st,
+    int64_t b_sb, int64_t b_st, int64_t d_sb, int64_t d_st, void* workspace,
+    int64_t workspace_bytes, void* stream) {
   using namespace smat;
   using namespace smat::dl;
   clear_error();

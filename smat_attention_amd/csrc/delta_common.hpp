@@ -87,10 +87,6 @@ __device__ __forceinline__ Frag<N> split(const f32x4& a, const f32x4& b) {
   return f;
 }
 
-template <int N> __device__ __forceinline__ Frag<N> zero_frag() {
-  return split<N>(zero4(), zero4());
-}
-
 // The leading N terms.
 template <int N, int M> __device__ __forceinline__ Frag<N> lead(const Frag<M>& f) {
   static_assert(N <= M, "");

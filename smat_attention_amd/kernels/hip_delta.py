@@ -137,8 +137,8 @@ class _Plan:
         self.R, self.P = -(-self.r // 32) * 32, -(-self.p // 32) * 32
 
     def sizes(self, scale):
-        return (*self.tables, self.nb, max(self.nbk, 1), self.T, self.nseg, self.nch, self.nruns, self.K,
-                self.r, self.p, float(scale))
+        return (*self.tables, self.nb, max(self.nbk, 1), self.T, self.nseg, self.nch, self.nruns,
+                self.K, self.r, self.p, float(scale))
 
     def workspace(self, code, backward, device):
         n = _lib.query("smat_delta_workspace_bytes", code, self.nb, self.nbk, self.nch, self.nseg,
@@ -219,7 +219,8 @@ def scan(Q, K, V, logA, beta, state, scale, segments, want_state: bool, save: bo
     _call_on(Q, "smat_delta_scan", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
              logA.data_ptr(), beta.data_ptr(), ptr(state) or None, o.data_ptr(),
              ptr(s_out) or None, ptr(save_s) or None, ptr(save_u) or None, ptr(save_m) or None,
-             *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(), *beta.stride(), ws, n)
+             *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb, v_st, *logA.stride(),
+             *beta.stride(), ws, n)
     return o, s_out, (save_s, save_u, save_m), (Q, K, V, logA, beta)
 
 
