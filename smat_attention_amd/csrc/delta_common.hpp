@@ -366,13 +366,15 @@ __device__ __forceinline__ int uniform_wave() {
 }
 
 // One copy of 16 bytes a lane into LDS, as lds_dma16<true>, from a uniform address
-// and a lane's byte offset: no vector address arithmetic.
+// and a lane's byte offset: no vector address arithmetic.  Five wait states lie before
+// the copy, for a base that a vector instruction has just written (a reload from a
+// spill); the last three also serve the write of m0.
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, const void* dst) {
   const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
   uint32_t keep;
   asm volatile(
-      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
+      "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 2\n\t"
+      "global_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
       : "=&s"(keep)
       : "v"(off), "s"(base), "s"(m0)
       : "memory");

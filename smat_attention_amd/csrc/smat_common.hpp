@@ -297,7 +297,8 @@ __device__ __forceinline__ void wait_vmcnt() {
 // the compiler does track must then not be pending across such a copy, or
 // their compiler waits (counting only tracked loads) drain it as well.  m0
 // (the LDS address) is saved and restored around the copy: the compiler
-// reserves it and may keep a value of its own there.
+// reserves it and may keep a value of its own there.  The copy needs a wait
+// state after the write of m0, which the compiler does not insert in assembly.
 template <bool UNTRACKED>
 __device__ __forceinline__ void lds_dma16(const void* src, void* dst) {
   typedef __attribute__((address_space(3))) char lds_char;
@@ -306,8 +307,8 @@ __device__ __forceinline__ void lds_dma16(const void* src, void* dst) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)dst);
     uint32_t keep;
     asm volatile(
-        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-        "s_mov_b32 m0, %0"
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t"
+        "global_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
         : "=&s"(keep)
         : "v"(src), "s"(m0)
         : "memory");
