@@ -43,9 +43,9 @@ struct ChainIO {
 
 // Bytes of LDS: KD buffers of K and the factors, T; and Q and P with the outputs.
 template <typename In, int RB, bool OUT> constexpr int chain_lds(int KD) {
-  constexpr int NT = Terms<In>::in, NO = Terms<In>::out;
+  constexpr int NT = Terms<In>::in, TB = kLow * kFrag * kMid;
   return KD * (2 * NT * tile_elems(RB) + kVec * 4) +
-         2 * (kTri * kFrag * kMid + (OUT ? NT * tile_elems(RB) + kTri * kFrag * NO : 0));
+         2 * (TB + (OUT ? NT * tile_elems(RB) + TB : 0));
 }
 // fp32 tiles of more than 64 features fit once only: their next K is copied between
 // the chunks.
@@ -61,12 +61,12 @@ template <typename In, int RB, bool OUT> constexpr int chain_waves() {
 template <typename In, int RB, bool OUT>
 __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_chain_kernel(
     Geo g, Ops o, ChainIO io, int tiles) {
-  constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid, R = 32 * RB;
-  constexpr int TL = NT * tile_elems(RB), TB = kTri * kFrag;
+  constexpr int NT = Terms<In>::in, NI = kMid, R = 32 * RB;
+  constexpr int TL = NT * tile_elems(RB), TB = NI * kLow * kFrag;
   constexpr int KD = chain_bufs<In, RB, OUT>();
   extern __shared__ __align__(1024) bf16 lds[];
-  bf16 *kl = lds, *tl = lds + KD * TL, *ql = tl + NI * TB, *pl = ql + (OUT ? TL : 0);
-  float* vl = reinterpret_cast<float*>(pl + (OUT ? NO * TB : 0));
+  bf16 *kl = lds, *tl = lds + KD * TL, *ql = tl + TB, *pl = ql + (OUT ? TL : 0);
+  float* vl = reinterpret_cast<float*>(pl + (OUT ? TB : 0));
   constexpr int W = chain_waves<In, RB, OUT>();
   const int w = uniform_wave();
   const int ct = blockIdx.y * W + w;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     stage<1, W>(vl + buf * kVec, vec_of(c), W - 1 - w);
   };
   auto stage_qt = [&](int c, int t0, int len) {
-    stage<NI * kTri, W>(tl, o.tm + ((int64_t)s * g.nch + c) * NI * TB, w);
+    stage<NI * kLow, W>(tl, o.tm + ((int64_t)s * g.nch + c) * TB, w);
     if (OUT) qstage(ql, o.q, ks, g.nch, c, t0, len, g.r, vec_of(c), w);
   };
 
@@ -143,7 +143,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
     column_values<In>(x, v, vlive, len);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) asm volatile("" : "+v"(x[mt]));   // their wait is here
-    if (OUT) stage<NO * kTri, W>(pl, o.pm + sc * NO * TB, w);
+    if (OUT) stage<NI * kLow, W>(pl, o.pm + sc * TB, w);
     if (KD == 2 && more) stage_k(c + 1, t1, len1, 1 - buf);
 
     f32x4 ot[4];
@@ -172,16 +172,14 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
             const int m0 = st * U % 4, kb = st * U / 4;
             f32x4 ca[U], co[U];
             Frag<NI> sa[U];
-            Frag<NO> so[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               ca[u] = ks4[m0 + u];
               co[u] = ot[m0 + u];
               sa[u] = sb[kb];
-              so[u] = lead<NO>(sb[kb]);
             }
             mul_each(ca, b.k, sa);
-            if (OUT) mul_each(co, so, b.q);
+            if (OUT) mul_each(co, sa, b.q);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
               ks4[m0 + u] = ca[u];
@@ -214,10 +212,10 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
         for (int mt = 0; mt < 4; ++mt)
           put_rows(io.save_u + (sc * C + 16 * mt) * ld, soff, ld, x[mt]);
       }
-      Frag<NO> fo[2];
+      Frag<NI> fo[2];
       if (OUT) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NO>(x[2 * kb], x[2 * kb + 1]);
+        for (int kb = 0; kb < 2; ++kb) fo[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
       }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
@@ -227,7 +225,7 @@ __global__ __launch_bounds__((64 * chain_waves<In, RB, OUT>()), 2) void delta_ch
       if (OUT) {
         const uint32_t ooff = (fm * g.p + f4) * sizeof(In);
         const int left = g.p - 16 * ct - f4;
-        triangle_out<NO>(ot, pl, fo, lane);
+        triangle<true, NI>(ot, pl, fo, lane);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           In* row = (In*)io.o + ((int64_t)s * g.T + t0 + 16 * mt) * g.p + 16 * ct;

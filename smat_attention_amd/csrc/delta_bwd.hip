@@ -168,12 +168,12 @@ __global__ __launch_bounds__((64 * rchain_waves<In, RB>()), 2) void delta_rchain
       Frag<NT> df[2];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) df[kb] = split<NT>(d[2 * kb], d[2 * kb + 1]);
-      triangle<true, NI>(x, pl, df, lane);
+      triangle_t<NI>(x, pl, df, lane);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) f[kb] = split<NI>(x[2 * kb], x[2 * kb + 1]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) x[mt] = zero4();
-      triangle<true, NI>(x, tl, f, lane);          // Z
+      triangle_t<NI>(x, tl, f, lane);              // Z
     }
     wait_vmcnt<0>();
     lds_barrier();

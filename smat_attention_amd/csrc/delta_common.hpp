@@ -18,18 +18,20 @@
 // Operands.  Every product runs on v_mfma_f32_16x16x32_bf16.  A value held in
 // fewer than its own bits is a sum of bf16 terms: bf16 inputs are one term, fp16
 // inputs two (exact: 11 bits), fp32 inputs and everything that is computed in fp32
-// on the way to a state or a gradient three (24 bits), so that states and the fp32
-// gradients have fp32's accuracy.  What ends in a 16-bit output alone (Q S, P U)
-// takes two terms, 2^-17 of the value and 2^8 finer than the output's rounding.  A
-// product keeps the terms whose orders sum below the larger count.  (fp32 MFMA
-// needs 16 times the cycles of one bf16 product, these forms three to six.)
+// on the way three (24 bits), so that states, gradients and outputs have fp32's
+// accuracy and 16-bit ones are rounded once, at the end.  A product keeps the terms
+// whose orders sum below the larger count.  (fp32 MFMA needs 16 times the cycles of
+// one bf16 product, these forms three to six.)
 //
 // Contraction slots.  A 16x16 result has its column in lane & 15 and rows 4g + i
 // (g = lane >> 4) in registers.  Slot (g, j) of a 32-long contraction stands for
 // index 4g + j (j < 4) or 16 + 4g + j - 4: then two stacked result tiles are an
 // operand of the next product as they lie in registers, and the chain needs no
 // exchange between lanes.  T and P are stored as fragments in that order, 16 x 32
-// in 1 KB, lane by lane.
+// in 1 KB, lane by lane.  Of a lower triangle's six the first and the fifth have
+// values in the first half of their slots only; they share a place, 15 KB in three
+// terms, so that two workgroups of four waves still fit a CU where the tiles take 8 KB
+// a term and two of them are copied ahead.
 //
 // K and Q are read both by rows (contraction over features) and transposed (over
 // tokens).  Both reads come from one LDS tile of 64 rows: 8-byte reads of a row's
@@ -52,13 +54,14 @@ constexpr int C = 64;              // tokens a chunk
 constexpr int kFrag = 512;         // elements a 16 x 32 fragment
 constexpr int kVec = 256;          // floats a chunk: e[64], w[64], b[64], exp(L_C), zeros
 constexpr int kZero = 3 * C + 4;   // where 16 bytes of zeros lie in it
-constexpr int kTri = 6;            // fragments of a 64 x 64 triangle
+constexpr int kLow = 5;            // places of a 64 x 64 lower triangle's fragments
+constexpr int kTri = 6;            // and of an upper one's
 constexpr int kMaxR = 128, kMaxP = 256;
 
 template <typename In> struct Terms;
-template <> struct Terms<bf16> { static constexpr int in = 1, out = 2; };
-template <> struct Terms<f16> { static constexpr int in = 2, out = 2; };
-template <> struct Terms<float> { static constexpr int in = 3, out = 3; };
+template <> struct Terms<bf16> { static constexpr int in = 1; };
+template <> struct Terms<f16> { static constexpr int in = 2; };
+template <> struct Terms<float> { static constexpr int in = 3; };
 constexpr int kMid = 3;            // terms of what is computed in fp32
 
 template <int N> struct Frag { bf16x8 t[N]; };
@@ -85,15 +88,6 @@ __device__ __forceinline__ Frag<N> split(const f32x4& a, const f32x4& b) {
     }
   }
   return f;
-}
-
-// The leading N terms.
-template <int N, int M> __device__ __forceinline__ Frag<N> lead(const Frag<M>& f) {
-  static_assert(N <= M, "");
-  Frag<N> g;
-#pragma unroll
-  for (int n = 0; n < N; ++n) g.t[n] = f.t[n];
-  return g;
 }
 
 // c += a b over the terms of order below M, by default max(NA, NB), small ones first.
@@ -162,11 +156,13 @@ __device__ __forceinline__ void store_frag(bf16* p, int64_t ts, const Frag<N>& f
   for (int n = 0; n < N; ++n) *reinterpret_cast<bf16x8*>(p + n * ts + lane_id() * 8) = f.t[n];
 }
 
-// Fragment of a lower triangle's row tile mt, contraction block kb (kb <= mt / 2),
-// and of its transpose (kb >= mt / 2).
+// Place of a lower triangle's fragment: row tile mt, contraction block kb (kb <= mt / 2).
+// (0, 0) has the first half of each lane's eight elements of place 0, (2, 1) the second.
 __device__ __forceinline__ constexpr int tri(int mt, int kb) {
-  return mt < 2 ? mt : 2 * mt - 2 + kb;
+  return mt < 2 ? mt : mt == 2 ? (kb == 0 ? 2 : 0) : 3 + kb;
 }
+__device__ __forceinline__ constexpr bool half_tri(int mt, int kb) { return mt == 2 * kb; }
+// and of its transpose's (kb >= mt / 2), each a place of its own.
 __device__ __forceinline__ constexpr int tri_t(int mt, int kb) {
   return mt < 2 ? 2 * mt + kb : mt + 2;
 }
@@ -228,53 +224,82 @@ __device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb,
   return f;
 }
 
-// x += T f for a stored lower triangle (UPPER: its transpose), two row tiles at a time.
+// The first sixteen slots of a fragment.
+template <int N> struct Half { bf16x4 t[N]; };
+__device__ __forceinline__ bf16x4 low_half(const bf16x8& x) {
+  return __builtin_shufflevector(x, x, 0, 1, 2, 3);
+}
+__device__ __forceinline__ f32x4 mma_half(f32x4 c, const bf16x4& a, const bf16x4& b) {
+  typedef short short4v __attribute__((ext_vector_type(4)));
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4v, a),
+                                                   __builtin_bit_cast(short4v, b), c, 0, 0, 0);
+}
+
+// x += T f for a stored lower triangle, two row tiles at a time; OUT: the result
+// transposed, x's columns in registers.
 template <int NA> struct Two {
   Frag<NA> a[2];
+  Half<NA> h;
 };
-template <bool UPPER, int NA, int NB>
+template <bool OUT, int NA, int NB>
 __device__ __forceinline__ void triangle(f32x4 (&x)[4], const bf16* tl, const Frag<NB> (&f)[2],
                                          int lane) {
-  // row tiles 0, 1 (of the lower triangle; 2, 3 of the upper) meet one block, the
-  // others two
-  constexpr int TS = kTri * kFrag;
-  auto mt_of = [](int st) { return UPPER ? (st == 0 ? 2 : 0) : (st == 0 ? 0 : 2); };
-  auto kb_of = [](int st) { return UPPER ? (st == 1 ? 0 : 1) : (st == 2 ? 1 : 0); };
-  pipelined<3, Two<NA>>(
-      [&](int st, Two<NA>& b) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int mt = mt_of(st) + u, kb = kb_of(st);
-          b.a[u] = load_frag<NA>(tl + (UPPER ? tri_t(mt, kb) : tri(mt, kb)) * kFrag, TS, lane);
-        }
-      },
-      [&](int st, Two<NA>& b) {
-        const int mt = mt_of(st), kb = kb_of(st);
-        f32x4 c[2] = {x[mt], x[mt + 1]};
-        const Frag<NB> g[2] = {f[kb], f[kb]};
-        mul_each(c, b.a, g);
-        x[mt] = c[0];
-        x[mt + 1] = c[1];
-      });
-}
-// The same with the result transposed: x's columns in registers.
-template <int NA, int NB>
-__device__ __forceinline__ void triangle_out(f32x4 (&x)[4], const bf16* pl, const Frag<NB> (&f)[2],
-                                             int lane) {
-  constexpr int TS = kTri * kFrag;
+  // row tiles 0, 1 meet one block, 2, 3 two; the first of a pair's last block is half
+  constexpr int TS = kLow * kFrag, M = NA > NB ? NA : NB;
   auto mt_of = [](int st) { return st == 0 ? 0 : 2; };
   auto kb_of = [](int st) { return st == 2 ? 1 : 0; };
   pipelined<3, Two<NA>>(
       [&](int st, Two<NA>& b) {
+        const int mt = mt_of(st), kb = kb_of(st);
+        b.a[1] = load_frag<NA>(tl + tri(mt + 1, kb) * kFrag, TS, lane);
+        if (half_tri(mt, kb)) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          b.a[u] = load_frag<NA>(pl + tri(mt_of(st) + u, kb_of(st)) * kFrag, TS, lane);
+          for (int n = 0; n < NA; ++n)
+            b.h.t[n] = *reinterpret_cast<const bf16x4*>(tl + n * TS + lane * 8 + 4 * kb);
+        } else {
+          b.a[0] = load_frag<NA>(tl + tri(mt, kb) * kFrag, TS, lane);
+        }
       },
       [&](int st, Two<NA>& b) {
         const int mt = mt_of(st), kb = kb_of(st);
+        const Frag<NB>& g = f[kb];
+#pragma unroll
+        for (int o = M - 1; o >= 0; --o)
+#pragma unroll
+          for (int i = 0; i < NA; ++i)
+            if (o - i >= 0 && o - i < NB) {
+              const bf16x8 y = g.t[o - i];
+              if (half_tri(mt, kb))
+                x[mt] = OUT ? mma_half(x[mt], low_half(y), b.h.t[i])
+                            : mma_half(x[mt], b.h.t[i], low_half(y));
+              else
+                x[mt] = OUT ? mma(x[mt], y, b.a[0].t[i]) : mma(x[mt], b.a[0].t[i], y);
+              x[mt + 1] = OUT ? mma(x[mt + 1], y, b.a[1].t[i]) : mma(x[mt + 1], b.a[1].t[i], y);
+            }
+      });
+}
+// x += T^T f for a stored upper triangle.
+template <int NA, int NB>
+__device__ __forceinline__ void triangle_t(f32x4 (&x)[4], const bf16* tl, const Frag<NB> (&f)[2],
+                                           int lane) {
+  // row tiles 2, 3 meet one block, 0, 1 two
+  constexpr int TS = kTri * kFrag;
+  auto mt_of = [](int st) { return st == 0 ? 2 : 0; };
+  auto kb_of = [](int st) { return st == 1 ? 0 : 1; };
+  struct Pair {
+    Frag<NA> a[2];
+  };
+  pipelined<3, Pair>(
+      [&](int st, Pair& b) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          b.a[u] = load_frag<NA>(tl + tri_t(mt_of(st) + u, kb_of(st)) * kFrag, TS, lane);
+      },
+      [&](int st, Pair& b) {
+        const int mt = mt_of(st), kb = kb_of(st);
         f32x4 c[2] = {x[mt], x[mt + 1]};
         const Frag<NB> g[2] = {f[kb], f[kb]};
-        mul_each(c, g, b.a);
+        mul_each(c, b.a, g);
         x[mt] = c[0];
         x[mt + 1] = c[1];
       });
@@ -583,7 +608,6 @@ constexpr int kMaxLds = 160 * 1024;
 inline int rblocks(int r) { return (r + 31) / 32; }
 inline int p32(int p) { return (p + 31) / 32 * 32; }
 inline int in_terms(int dtype) { return dtype == SMAT_BF16 ? 1 : dtype == SMAT_F16 ? 2 : 3; }
-inline int out_terms(int dtype) { return dtype == SMAT_F32 ? 3 : 2; }
 
 // Whether rows can be copied as they are: bf16 in aligned groups of eight.
 inline bool raw_ok(int dtype, const void* p, int64_t sb, int64_t st, int r) {
@@ -594,7 +618,7 @@ inline bool raw_ok(int dtype, const void* p, int64_t sb, int64_t st, int r) {
 inline Ops take_ops(Arena& ar, int dtype, int64_t nb, int64_t nbk, int64_t nch, int r, bool bwd,
                     bool raw) {
   const int64_t tiles = nbk * nch * in_terms(dtype) * tile_elems(rblocks(r));
-  const int64_t tris = nb * nch * kTri * kFrag;
+  const int64_t tris = nb * nch * (bwd ? kTri : kLow) * kFrag * kMid;
   Ops o = {};
   if (!raw) {
     o.kw = ar.take<bf16>(tiles);
@@ -602,8 +626,8 @@ inline Ops take_ops(Arena& ar, int dtype, int64_t nb, int64_t nbk, int64_t nch, 
     o.k.ws = o.kw;
     o.q.ws = o.qw;
   }
-  (bwd ? o.tt : o.tm) = ar.take<bf16>(tris * kMid);
-  (bwd ? o.pt : o.pm) = ar.take<bf16>(tris * (bwd ? kMid : out_terms(dtype)));
+  (bwd ? o.tt : o.tm) = ar.take<bf16>(tris);
+  (bwd ? o.pt : o.pm) = ar.take<bf16>(tris);
   o.vec = ar.take<float>(nb * nch * kVec);
   return o;
 }

@@ -11,7 +11,7 @@
 // hundreds of nats leaves the differences of later tokens exact; logA below -1e5
 // (a = 0 many times over) counts as -1e5, which keeps -inf - -inf out.
 //
-// Bound by HBM, what it writes above all (T in three terms, 18 KB): 194 us for 8
+// Bound by HBM, what it writes above all (T and P in three terms, 30 KB): 194 us for 8
 // sequences of 131072 tokens, r = 128 in bf16, 5.4 TB/s.
 #pragma once
 
@@ -152,6 +152,18 @@ __device__ __forceinline__ void row_frags(Frag<N>* f, const In* row, bool ok, in
   for (int kb = 0; kb < RB; ++kb) f[kb] = row_frag<In, N>(row, ok, 32 * kb + 4 * gq, r, vec);
 }
 
+// A lower triangle's fragment of row tile mt and block kb into its place, or its half.
+__device__ __forceinline__ void store_tri(bf16* p, int mt, int kb, const Frag<kMid>& f) {
+  if (half_tri(mt, kb)) {
+#pragma unroll
+    for (int n = 0; n < kMid; ++n)
+      *reinterpret_cast<bf16x4*>(p + n * kLow * kFrag + lane_id() * 8 + 4 * kb) =
+          __builtin_shufflevector(f.t[n], f.t[n], 0, 1, 2, 3);
+  } else {
+    store_frag<kMid>(p + tri(mt, kb) * kFrag, kLow * kFrag, f);
+  }
+}
+
 // A token's slots of contraction block kb into its row of a tile (a tile a term).
 template <int RB, int N>
 __device__ __forceinline__ void store_row(bf16* tile, int t, int kb, const Frag<N>& f) {
@@ -180,7 +192,7 @@ template <typename In, int RB, bool BWD>
 __global__ __launch_bounds__(256) void delta_prep_kernel(
     const In* __restrict__ q, const In* __restrict__ k, const float* __restrict__ logA,
     const float* __restrict__ beta, Geo g, Ops o, bool qvec, bool kvec) {
-  constexpr int NT = Terms<In>::in, NO = Terms<In>::out, NI = kMid;
+  constexpr int NT = Terms<In>::in, NI = kMid;
   constexpr int KB = 4 * RB * kFrag;               // elements of one term of a chunk's rows
   __shared__ __align__(16) char mem[prep_rows<In, RB, BWD>()];
   __shared__ __align__(16) float Am[C * kLd];
@@ -244,8 +256,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
       if (kb <= w / 2)
-        store_frag<NO>(o.pm + (sc * NO * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
-                       split<NO>(pacc[2 * kb], pacc[2 * kb + 1]));
+        store_tri(o.pm + sc * NI * kLow * kFrag, w, kb, split<NI>(pacc[2 * kb], pacc[2 * kb + 1]));
     __syncthreads();                               // Am whole; the rows are read
   } else {
     // token j = 16 w + m in the lane, rows i = 16 it + 4 gq + .. in registers: the same
@@ -305,8 +316,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(
       const float* row = Tm + tok * kLd + 32 * kb + 4 * gq;
       const f32x4 x0 = *reinterpret_cast<const f32x4*>(row);
       const f32x4 x1 = 2 * kb + 1 <= w ? *reinterpret_cast<const f32x4*>(row + 16) : zero4();
-      store_frag<NI>(o.tm + (sc * NI * kTri + tri(w, kb)) * kFrag, kTri * kFrag,
-                     split<NI>(x0, x1));
+      store_tri(o.tm + sc * NI * kLow * kFrag, w, kb, split<NI>(x0, x1));
     }
   }
   if (threadIdx.x < C) {
