@@ -66,7 +66,9 @@ constexpr int kMid = 3;            // terms of what is computed in fp32
 
 template <int N> struct Frag { bf16x8 t[N]; };
 
-// Eight fp32 values as N bf16 terms each.
+// Eight fp32 values as N bf16 terms each.  Values that would round to infinity (beyond
+// (2 - 2^-8) 2^127) take bf16's largest as their first term, and the others make up the
+// rest.  (Two terms are fp16 values', which end at 65504.)
 template <int N>
 __device__ __forceinline__ Frag<N> split(const f32x4& a, const f32x4& b) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -77,7 +79,15 @@ __device__ __forceinline__ Frag<N> split(const f32x4& a, const f32x4& b) {
     f32x2 v = q < 2 ? f32x2{a[2 * q], a[2 * q + 1]} : f32x2{b[2 * q - 4], b[2 * q - 3]};
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const bf16x2 h = __builtin_convertvector(v, bf16x2);
+      bf16x2 h;
+      if (N == 3 && n == 0) {
+        constexpr float most = 0x1.fefffep127f;    // rounds to bf16's largest
+        h = __builtin_convertvector((f32x2{__builtin_amdgcn_fmed3f(v[0], -most, most),
+                                           __builtin_amdgcn_fmed3f(v[1], -most, most)}),
+                                    bf16x2);
+      } else {
+        h = __builtin_convertvector(v, bf16x2);
+      }
       f.t[n][2 * q] = h[0];
       f.t[n][2 * q + 1] = h[1];
       if (n + 1 < N) {
