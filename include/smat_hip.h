@@ -555,7 +555,8 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides, nbk dividing nb
  * (value sequence s reads key sequence s / (nb / nbk)); logA, beta: (nb, T)
  * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256,
- * v_st (and the gradient's d_st) < 2^23.
+ * v_st (and the gradient's d_st) < 2^23, but for calls of up to 16 tokens that use no
+ * workspace (below).
  * Segments: chunks (nch, 2) = first token, tokens (<= 64); runs (nruns, 4) =
  * first chunk, end chunk, segment, every segment's runs together and in order,
  * an empty segment with one empty run, and in the last column the runs' order

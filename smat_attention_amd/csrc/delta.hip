@@ -577,8 +577,6 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && out), SMAT_EINVAL, "%s: null pointer",
                who);
-  SMAT_REQUIRE(near_rows(v_st), SMAT_EUNSUPPORTED, "%s: rows of v %lld elements apart, beyond 2^23",
-               who, (long long)v_st);
   SMAT_REQUIRE(!save_s == !save_u && (save_s && nruns > nseg ? save_m != nullptr : !save_m),
                SMAT_EINVAL, "%s: save_s, save_u and (with more runs than segments) save_m go "
                "together", who);
@@ -586,6 +584,8 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
   hipStream_t st = (hipStream_t)stream;
   if (!chunks && !save_s && T >= 1 && T <= kFewTokens)
     return launch_tokens(dtype, g, q, k, v, logA, beta, state, state_out, out, st);
+  SMAT_REQUIRE(near_rows(v_st), SMAT_EUNSUPPORTED, "%s: rows of v %lld elements apart, beyond 2^23",
+               who, (long long)v_st);
   const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 0);
   SMAT_REQUIRE(workspace_bytes >= need && (workspace || need == 0) &&
                    ((uintptr_t)workspace & 255) == 0,

@@ -100,7 +100,11 @@ class Segments:
 
 def _near_rows(t):
     """``_rows3``, with rows that lie 2^23 elements and more apart copied together: the kernels
-    reach the rows of a chunk by 32-bit offsets."""
+    reach the rows of a chunk by 32-bit offsets.  A single row's stride is anything (torch
+    ignores it, in ``contiguous`` too) and means nothing: it becomes the row's length."""
+    if t.shape[1] <= 1:
+        t, sb, _ = _rows3(t)
+        return t, sb, t.shape[2]
     return _rows3(t if t.stride(1) < 2 ** 23 else t.contiguous())
 
 
@@ -231,7 +235,7 @@ def scan_backward(inputs, saved, dO, dS, scale, segments, want_dstate: bool):
     save_s, save_u, save_m = saved
     plan = _Plan(who, Q, V, segments)
     code, dev = _code(Q, who), Q.device
-    (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
+    (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = _rows3(Q), _rows3(K), _near_rows(V)
     dO, d_sb, d_st = _near_rows(dO)
     dQ = torch.empty(plan.nbk, plan.T, plan.r, device=dev, dtype=Q.dtype)
     dK = torch.empty_like(dQ)
