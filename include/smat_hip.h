@@ -528,8 +528,8 @@ int smat_decode_step_at(int dtype, const void* phi_t, const void* psi_t, const v
  * over the path that ends in nodes[request] (a value outside [0, M): none)
  * and, with ahead not NULL, adds the path's length to ahead[request].
  * Phi, Psi: (nb, M, r), Vb: (nb, M, p) of dtype; S: (nb, r, p), U: (nb, B, r,
- * p), out: (nb, M, p-1) fp32 contiguous; nb is a multiple of trees and of
- * requests (heads innermost).  Tables of each tree: anc (trees, M), bit a of
+ * p), out: (nb, M, p-1) fp32 contiguous; nb < 2^23 is a multiple of trees and
+ * of requests (heads innermost).  Tables of each tree: anc (trees, M), bit a of
  * word j set when a is j or an ancestor of j (0: an unused node, whose out row
  * is zero); order (trees, M) the used nodes by level, then the unused ones;
  * lstart (trees, M + 1) the first of each level in order, at and past the
@@ -554,9 +554,9 @@ int smat_tree_state(int dtype, const void* psi, const void* vb, const float* S, 
  *   o_t = scale S_t^T q_t,  a_t = exp(logA_t)
  * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides, nbk dividing nb
  * (value sequence s reads key sequence s / (nb / nbk)); logA, beta: (nb, T)
- * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256,
- * v_st (and the gradient's d_st) < 2^23, but for calls of up to 16 tokens that use no
- * workspace (below).
+ * fp32 with strides; out: (nb, T, p) of dtype, contiguous.  r <= 128, p <= 256.
+ * nb, nseg and nruns <= 65535, v_st (and the gradient's d_st) < 2^23; calls of
+ * up to 16 tokens that use no workspace (below) take any v_st and nb < 2^24.
  * Segments: chunks (nch, 2) = first token, tokens (<= 64); runs (nruns, 4) =
  * first chunk, end chunk, segment, every segment's runs together and in order,
  * an empty segment with one empty run, and in the last column the runs' order
@@ -612,7 +612,7 @@ int smat_delta_scan_backward(int dtype, const void* q, const void* k, const void
 /*
  * One token of it: S_out from S_in (both (nb, r, p) fp32 contiguous; they may
  * be the same buffer) and out (nb, p) of dtype, contiguous.  q, k: (nbk, r),
- * v: (nb, p), logA, beta: (nb) fp32, with batch strides.
+ * v: (nb, p), logA, beta: (nb) fp32, with batch strides; nb < 2^24.
  */
 int smat_delta_step(int dtype, const void* q, const void* k, const void* v, const float* logA,
                     const float* beta, const float* S_in, float* S_out, void* out, int nb,

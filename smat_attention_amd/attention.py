@@ -447,6 +447,8 @@ def gated_delta_scan(Q, K, V, logA, beta, *, scale: float = 1.0, state=None,
     come as their transposed views.  r <= 128, p <= 256; the values of a chunk of 64 tokens
     meet in products, so inputs are expected to be finite (``logA = -inf`` counts as a decay to
     zero; positive ones are taken while the exp of their sum over a chunk stays within fp32).
+    At most 65535 value sequences and segments (2^24 - 1 sequences where at most 16 tokens each,
+    unpacked and without gradients, are taken one after another).
     A token with ``beta = 0, logA = 0`` leaves the state as it is: padding.
 
     ``segments`` (:class:`Segments`) packs sequences of any lengths along T; each starts from

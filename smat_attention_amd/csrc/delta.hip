@@ -395,9 +395,6 @@ int check_geo(const char* who, int dtype, const Geo& g) {
                g.nb);
   SMAT_REQUIRE(g.r >= 1 && g.r <= kMaxR && g.p >= 1 && g.p <= kMaxP, SMAT_EUNSUPPORTED,
                "%s: r=%d p=%d beyond r<=%d, p<=%d", who, g.r, g.p, kMaxR, kMaxP);
-  SMAT_REQUIRE(g.nb <= 65535 && g.nruns <= 65535 && g.nseg <= 65535, SMAT_EUNSUPPORTED,
-               "%s: nb=%d, %d segments and %d runs must stay within 65535", who, g.nb, g.nseg,
-               g.nruns);
   if (g.chunks || g.runs || g.segrun) {
     SMAT_REQUIRE(g.chunks && g.runs && g.segrun && g.nruns >= g.nseg, SMAT_EINVAL,
                  "%s: segments need the chunk, run and segment tables", who);
@@ -407,6 +404,14 @@ int check_geo(const char* who, int dtype, const Geo& g) {
     SMAT_REQUIRE(g.K >= 1 && g.nruns == (g.nch > 0 ? (g.nch + g.K - 1) / g.K : 1), SMAT_EINVAL,
                  "%s: %d runs of %d chunks for %d chunks", who, g.nruns, g.K, g.nch);
   }
+  return SMAT_OK;
+}
+
+// The chunks' kernels have sequences, segments and runs along a grid's second and third axes.
+int check_grid(const char* who, const Geo& g) {
+  SMAT_REQUIRE(g.nb <= kMaxGrid && g.nruns <= kMaxGrid && g.nseg <= kMaxGrid, SMAT_EUNSUPPORTED,
+               "%s: nb=%d, %d segments and %d runs must stay within %d", who, g.nb, g.nseg,
+               g.nruns, kMaxGrid);
   return SMAT_OK;
 }
 
@@ -583,7 +588,9 @@ extern "C" int smat_delta_scan(int dtype, const void* q, const void* k, const vo
   SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
   hipStream_t st = (hipStream_t)stream;
   if (!chunks && !save_s && T >= 1 && T <= kFewTokens)
-    return launch_tokens(dtype, g, q, k, v, logA, beta, state, state_out, out, st);
+    return launch_tokens(who, dtype, g, q, k, v, logA, beta, state, state_out, out, st);
+  const int fits = check_grid(who, g);
+  if (fits) return fits;
   SMAT_REQUIRE(near_rows(v_st), SMAT_EUNSUPPORTED, "%s: rows of v %lld elements apart, beyond 2^23",
                who, (long long)v_st);
   const int64_t need = smat_delta_workspace_bytes(dtype, nb, nbk, nch, nseg, nruns, r, p, 0);

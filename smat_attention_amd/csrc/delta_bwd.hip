@@ -628,7 +628,8 @@ extern "C" int smat_delta_scan_backward(
   const char* who = "smat_delta_scan_backward";
   const Geo g = {chunks, runs, segrun, nb, nbk, T, nseg, nch, nruns, K, r, p, scale,
                  q_sb, q_st, k_sb, k_st, v_sb, v_st, a_sb, a_st, b_sb, b_st};
-  const int rc = check_geo(who, dtype, g);
+  int rc = check_geo(who, dtype, g);
+  if (rc == SMAT_OK) rc = check_grid(who, g);
   if (rc) return rc;
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(nch == 0 || (q && k && v && logA && beta && dout && save_s && save_u && dq && dk &&

@@ -691,11 +691,13 @@ inline int dispatch(int dtype, int r, F fn) {
   return rows(float());
 }
 
-// The checks that the forward and the backward share.
+// The checks that the forward and the backward share, and those of the chunks' kernels.
 int check_geo(const char* who, int dtype, const Geo& g);
+constexpr int kMaxGrid = 65535;
+int check_grid(const char* who, const Geo& g);
 // Up to this many tokens a sequence are taken one after another (delta_step.hip).
 constexpr int kFewTokens = 16;
-int launch_tokens(int dtype, const Geo& g, const void* q, const void* k, const void* v,
+int launch_tokens(const char* who, int dtype, const Geo& g, const void* q, const void* k, const void* v,
                   const float* logA, const float* beta, const float* S_in, float* S_out, void* o,
                   hipStream_t st);
 // hipFuncSetAttribute for a kernel's LDS, once a device.

@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kStepThreads, ONE ? 4 : 2) void delta_tokens_kernel
 }
 
 template <typename In>
-static int tokens(const Tokens& g, int nb, hipStream_t st) {
+static int tokens(const char* who, const Tokens& g, int nb, hipStream_t st) {
   auto go = [&](auto kern, int CL) {
     hipLaunchKernelGGL(kern, dim3(nb, (g.p + 4 * CL - 1) / (4 * CL)), dim3(kStepThreads), 0, st, g);
   };
@@ -198,18 +198,20 @@ static int tokens(const Tokens& g, int nb, hipStream_t st) {
     cols(std::true_type());
   else
     cols(std::false_type());
-  return launch_status("smat_delta_step");
+  return launch_status(who);
 }
 
-int launch_tokens(int dtype, const Geo& g, const void* q, const void* k, const void* v,
-                  const float* logA, const float* beta, const float* S_in, float* S_out, void* o,
-                  hipStream_t st) {
+int launch_tokens(const char* who, int dtype, const Geo& g, const void* q, const void* k,
+                  const void* v, const float* logA, const float* beta, const float* S_in,
+                  float* S_out, void* o, hipStream_t st) {
+  // a grid has less than 2^32 threads along an axis
+  SMAT_REQUIRE(g.nb < (1 << 24), SMAT_EUNSUPPORTED, "%s: nb=%d must stay below 2^24", who, g.nb);
   const Tokens t = {q, k, v, logA, beta, S_in, S_out, o, g.T, g.nb / g.nbk, g.r, g.p, g.scale,
                     g.q_sb, g.q_st, g.k_sb, g.k_st, g.v_sb, g.v_st, g.a_sb, g.a_st, g.b_sb,
                     g.b_st, (int64_t)g.T * g.p, g.p};
-  if (dtype == SMAT_BF16) return tokens<bf16>(t, g.nb, st);
-  if (dtype == SMAT_F16) return tokens<f16>(t, g.nb, st);
-  return tokens<float>(t, g.nb, st);
+  if (dtype == SMAT_BF16) return tokens<bf16>(who, t, g.nb, st);
+  if (dtype == SMAT_F16) return tokens<f16>(who, t, g.nb, st);
+  return tokens<float>(who, t, g.nb, st);
 }
 
 }  // namespace dl
@@ -245,5 +247,5 @@ extern "C" int smat_delta_step(int dtype, const void* q, const void* k, const vo
   g.v_sb = v_sb;
   g.a_sb = a_sb;
   g.b_sb = b_sb;
-  return launch_tokens(dtype, g, q, k, v, logA, beta, S_in, S_out, out, (hipStream_t)stream);
+  return launch_tokens(who, dtype, g, q, k, v, logA, beta, S_in, S_out, out, (hipStream_t)stream);
 }

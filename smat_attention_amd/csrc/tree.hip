@@ -290,6 +290,8 @@ static int check(const char* who, int dtype, const Args& g) {
                g.M, kMaxNodes);
   SMAT_REQUIRE(g.r >= 1 && g.r <= kMaxR && g.p >= 2 && g.p <= kMaxP, SMAT_EUNSUPPORTED,
                "%s: r=%d p=%d beyond r<=%d, 2<=p<=%d", who, g.r, g.p, kMaxR, kMaxP);
+  // a grid has less than 2^32 threads along an axis
+  SMAT_REQUIRE(g.nb < (1 << 23), SMAT_EUNSUPPORTED, "%s: nb=%d must stay below 2^23", who, g.nb);
   return SMAT_OK;
 }
 

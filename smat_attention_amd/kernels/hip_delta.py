@@ -325,9 +325,9 @@ def step(q, k, v, logA, beta, state, scale, out, out_state):
                         f"{out_state.dtype}")
     if not (state.is_contiguous() and out_state.is_contiguous() and out.is_contiguous()):
         raise ValueError(f"{who}: state, out_state and out must be contiguous")
-    if r > MAX_R or p > MAX_P or r < 1 or p < 1 or nb >= 2 ** 31:
+    if r > MAX_R or p > MAX_P or r < 1 or p < 1 or nb >= 2 ** 24:
         _check_widths(who, r, p)
-        raise ValueError(f"{who}: {nb} sequences, at most 2^31 - 1")
+        raise ValueError(f"{who}: {nb} sequences, at most 2^24 - 1")
     if out_state is not state and out_state.data_ptr() != state.data_ptr():
         lo, hi = sorted((state.data_ptr(), out_state.data_ptr()))
         if hi < lo + state.numel() * 4:

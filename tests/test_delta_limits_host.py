@@ -1,7 +1,11 @@
 """The limits of the gated delta rule's sizes and strides, on the CPU."""
+import pytest
 import torch
 
-from smat_attention_amd.kernels import hip_delta
+from smat_attention_amd.kernels import _lib, hip_delta
+from smat_attention_amd.kernels._lib import HipKernelError
+
+FAKE = 1 << 20                         # never dereferenced: the refusal comes first
 
 
 def test_a_single_row_is_near():
@@ -11,3 +15,23 @@ def test_a_single_row_is_near():
     t, sb, st = hip_delta._near_rows(far)
     assert t.data_ptr() == far.data_ptr() and (sb, st) == (4, 4)
     assert hip_delta._near_rows(torch.empty(2, 0, 4))[2] == 4
+
+
+def test_sequences_beyond_a_grid_are_refused():
+    """In chunks 65535 sequences; token by token, and trees, what a grid's first axis holds."""
+    def scan(nb, T):
+        _lib.call("smat_delta_scan", 0, FAKE, FAKE, FAKE, FAKE, FAKE, None, FAKE, None, None, None,
+                  None, None, None, None, nb, nb, T, 1, 1, 1, 1, 8, 8, 1.0, *[64] * 10, FAKE,
+                  1 << 50, None)
+    with pytest.raises(HipKernelError, match="within 65535"):
+        scan(65536, 17)
+    with pytest.raises(HipKernelError, match="below 2\\^24"):
+        scan(1 << 24, 16)
+    with pytest.raises(HipKernelError, match="below 2\\^24"):
+        _lib.call("smat_delta_step", 0, *[FAKE] * 8, 1 << 24, 1, 8, 8, 1.0, 8, 8, 8, 1, 1, None)
+    with pytest.raises(HipKernelError, match="below 2\\^23"):
+        _lib.call("smat_tree_step", 0, *[FAKE] * 9, None, 1 << 23, 1, 1, 2, 1, 1, 8, 9, 0,
+                  *[0] * 6, None)
+    with pytest.raises(HipKernelError, match="below 2\\^23"):
+        _lib.call("smat_tree_state", 0, *[FAKE] * 3, FAKE + 64, FAKE, FAKE, None, 1 << 23, 1, 1, 2,
+                  8, 9, *[0] * 4, None)

@@ -54,3 +54,18 @@ def test_few_tokens_take_any_row_stride():
 def _lib_code(t):
     from smat_attention_amd.kernels.hip_fwd import _code
     return _code(t, "test")
+
+
+def test_few_tokens_of_many_sequences():
+    """More sequences than a grid's second axis holds, for one and for a few tokens."""
+    nb, r, p = 70000, 4, 5
+    q, k, v, logA, beta, S = _inputs(nb, nb // 2, 3, r, p, FP32, seed=3, state=())
+    ro, rS = O.delta_scan(q, k, v, logA, beta, state=S)
+    o, So = A.gated_delta_scan(q, k, v, logA, beta, state=S, return_state=True)
+    _check("o", o, ro, 1, r, p)
+    _check("S", So, rS, 1, r, p)
+    x = [t[:, :1] for t in (q, k, v, logA, beta)]
+    o, So = A.gated_delta_scan(*x, state=S, return_state=True)
+    new = torch.empty_like(S)
+    o1 = A.gated_delta_step(*(t[:, 0] for t in x), S, out_state=new)
+    assert torch.equal(o[:, 0], o1) and torch.equal(So, new)
