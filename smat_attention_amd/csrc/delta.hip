@@ -535,6 +535,7 @@ extern "C" int smat_delta_run_chunks(int dtype, int nb, int nch, const int32_t* 
       ends += t * (cut - 1);
       chunks += t * len;
     }
+    if (G > 1 && runs > kMaxGrid) continue;        // more than a grid holds
     const double out = (double)nb * ((tiles + wout - 1) / wout);
     const double first = (double)nb * ((tiles + 2 * RB + wfirst - 1) / wfirst);
     double us = pass(runs * out, chunks * out, K, wout, terms * (3.4 + 0.375 * RB));

@@ -35,3 +35,15 @@ def test_sequences_beyond_a_grid_are_refused():
     with pytest.raises(HipKernelError, match="below 2\\^23"):
         _lib.call("smat_tree_state", 0, *[FAKE] * 3, FAKE + 64, FAKE, FAKE, None, 1 << 23, 1, 1, 2,
                   8, 9, *[0] * 4, None)
+
+
+def test_run_lengths_keep_within_the_grid():
+    """Many short segments and a long one: cut so that the runs stay within 65535, where a call
+    without cuts does."""
+    short = list(range(65501))
+    for off in (short + [short[-1] + 64 * 4096], short + [short[-1] + 64 * 4096 + 1]):
+        seg = hip_delta.Segments(off, "cpu")
+        assert len(seg) == 65501
+        for code in range(3):
+            K = seg.run_chunks(code, 1, 64, 64)
+            assert seg.runs(K)[0].shape[0] <= 65535, (code, K)
