@@ -526,7 +526,8 @@ int smat_decode_step_at(int dtype, const void* phi_t, const void* psi_t, const v
  * decode steps along j's path give.  smat_tree_state forms
  *   S_out = S + sum_a Psi_a Vb_a^T
  * over the path that ends in nodes[request] (a value outside [0, M): none)
- * and, with ahead not NULL, adds the path's length to ahead[request].
+ * and, with ahead not NULL, adds the path's length to ahead[request] (ahead
+ * shares no memory with nodes).
  * Phi, Psi: (nb, M, r), Vb: (nb, M, p) of dtype; S: (nb, r, p), U: (nb, B, r,
  * p), out: (nb, M, p-1) fp32 contiguous; nb < 2^23 is a multiple of trees and
  * of requests (heads innermost).  Tables of each tree: anc (trees, M), bit a of

@@ -790,8 +790,8 @@ def tree_state(Psi, Vb, tree: DraftTree, nodes, S, S_out, *, ahead=None):
         _check_requests(who, "ahead", ahead, nb, S.device)
         if ahead.numel() != nodes.numel():
             raise ValueError(f"{who}: {nodes.numel()} accepted nodes for {ahead.numel()} requests")
-        if ahead.data_ptr() == nodes.data_ptr():
-            raise ValueError(f"{who}: ahead must not be nodes")
+        if abs(ahead.data_ptr() - nodes.data_ptr()) < 4 * nodes.numel():
+            raise ValueError(f"{who}: ahead must not be nodes, nor share memory with them")
     if tree.trees not in (1, nodes.numel()):
         raise ValueError(f"{who}: {nodes.numel()} accepted nodes for {tree.trees} trees")
     if not (S.is_contiguous() and S_out.is_contiguous() and S.dtype == S_out.dtype
