@@ -493,8 +493,9 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 // Run length: of the lengths that cut the longest segment into 1 to 256 runs, the one
 // whose passes take least by what their steps measure, in microseconds a chunk with a
 // workgroup on every CU: 3.4 + 0.375 RB with outputs, 1.9 + 0.24 RB in the first pass,
-// 1.9 times that where inputs have several terms; 0.55 RB a run of the carry and 10 for
-// the two launches more.  Workgroups of four waves share a CU in pairs, which then take
+// 1.9 times that where inputs have several terms (measured in fp16; fp32, with three and
+// one buffer of K from 96 features on, is taken for the same); 0.55 RB a run of the carry
+// and 10 for the two launches more.  Workgroups of four waves share a CU in pairs, which then take
 // 1.64 times as long; more than are resident follow one another, the last ones alone.
 // (8 sequences of 2048 chunks, r = p = 128: 9367 whole, 1377 in 32 runs, 1457 in 64,
 // 1670 in 128; 12 of 5 segments and 158 chunks, r = p = 96 in fp16: 640 whole, 251 in

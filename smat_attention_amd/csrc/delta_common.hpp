@@ -195,7 +195,8 @@ __device__ __forceinline__ Frag<N> rows_of(const bf16* tile, int mt, int kb,
   const int k0 = (4 * kb + (g >> 1)) ^ swz<RS>(m), k1 = (4 * kb + 2 + (g >> 1)) ^ swz<RS>(m);
   int at = (16 * mt + m) * RS * 8 + 4 * (g & 1);
   // odd row tiles take an address the compiler cannot relate to the even ones': fused
-  // into ds_read2st64_b64 the pair would be read at half the rate
+  // into ds_read2st64_b64 the pair would be read at half the rate (with two and three
+  // terms it still fuses the terms of one tile)
   if (mt & 1) asm("" : "+v"(at));
   const bf16* p = tile + at;
   Frag<N> f;
@@ -557,7 +558,7 @@ inline bool vec4_ok(const void* p, int64_t sb, int64_t st, int eb) {
 // arithmetic: chunk c is tokens [64 c, 64 c + 64), run g chunks [g K, g K + K).
 struct Geo {
   const int32_t* chunks;   // (nch, 2): first token, tokens; or null
-  const int32_t* runs;     // (nruns, 3): first chunk, end chunk, segment; or null
+  const int32_t* runs;     // (nruns, 4): first chunk, end chunk, segment, turn; or null
   const int32_t* segrun;   // (nseg + 1): first run of each segment; or null
   int nb, nbk, T, nseg, nch, nruns, K, r, p;
   float scale;
@@ -695,7 +696,8 @@ inline int dispatch(int dtype, int r, F fn) {
 int check_geo(const char* who, int dtype, const Geo& g);
 constexpr int kMaxGrid = 65535;
 int check_grid(const char* who, const Geo& g);
-// Up to this many tokens a sequence are taken one after another (delta_step.hip).
+// Up to this many tokens a sequence are taken one after another (delta_step.hip; callers,
+// who give such calls no workspace, hold the same number).
 constexpr int kFewTokens = 16;
 int launch_tokens(const char* who, int dtype, const Geo& g, const void* q, const void* k, const void* v,
                   const float* logA, const float* beta, const float* S_in, float* S_out, void* o,

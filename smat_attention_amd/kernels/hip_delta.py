@@ -18,7 +18,7 @@ from .hip_fwd import _call_on, _code, _on_gpu, _rows3, _shape
 
 CHUNK = 64
 MAX_R, MAX_P = 128, 256
-FEW_TOKENS = 16          # calls of up to so many tokens, unpacked, need no workspace
+FEW_TOKENS = 16          # calls of up to so many tokens, unpacked, need no workspace (kFewTokens)
 
 
 def same_device(who: str, ref: torch.Tensor, *ts) -> None:
@@ -250,8 +250,8 @@ def scan_backward(inputs, saved, dO, dS, scale, segments, want_dstate: bool):
         dS = dS.contiguous()
     _call_on(Q, "smat_delta_scan_backward", code, Q.data_ptr(), K.data_ptr(), V.data_ptr(),
              logA.data_ptr(), beta.data_ptr(), dO.data_ptr(), ptr(dS), save_s.data_ptr(),
-             save_u.data_ptr(), ptr(save_m) or None, dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlogA.data_ptr(),
-             dbeta.data_ptr(), ptr(dstate), *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb,
+             save_u.data_ptr(), ptr(save_m) or None, dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(),
+             dlogA.data_ptr(), dbeta.data_ptr(), ptr(dstate), *plan.sizes(scale), q_sb, q_st, k_sb, k_st, v_sb,
              v_st, *logA.stride(), *beta.stride(), d_sb, d_st, ws.data_ptr(), n)
     return dQ, dK, dV, dlogA, dbeta, dstate
 

@@ -1,4 +1,7 @@
 """The limits of the gated delta rule's sizes and strides, on the CPU."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -47,3 +50,11 @@ def test_run_lengths_keep_within_the_grid():
         for code in range(3):
             K = seg.run_chunks(code, 1, 64, 64)
             assert seg.runs(K)[0].shape[0] <= 65535, (code, K)
+
+
+def test_few_tokens_are_the_same_number_on_both_sides():
+    """Calls of up to FEW_TOKENS tokens bring no workspace, which kFewTokens says is needed."""
+    src = os.path.join(os.path.dirname(hip_delta.__file__), "..", "csrc", "delta_common.hpp")
+    with open(src) as f:
+        (n,) = re.findall(r"constexpr int kFewTokens = (\d+);", f.read())
+    assert int(n) == hip_delta.FEW_TOKENS
