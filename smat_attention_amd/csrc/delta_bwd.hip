@@ -10,6 +10,9 @@
 //   db_i = Z_i.V_i + k_i.y_i
 //   dlogA_t = sum_{i >= t} (q_i.dQ_i + b_i k_i.y_i - k_i.(dK_i - b_i y_i)) + <dS', S'>
 //
+// Where the state entering a chunk is zero, dlogA of its first token is zero, and is
+// stored as that: its terms cancel only up to their roundings.
+//
 // (L_i enters as q_i e^{L_i}, as the e^{L_i} of the reading k_i and as the e^{-L_i}
 // of the writing one, and everything behind the chunk as e^{L_C} in S'.)
 //
@@ -294,6 +297,7 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
   float *G = reinterpret_cast<float*>(fr), *N = G + C * kLd;
   __shared__ double Ls[C];
   __shared__ float bs[C], zvs[C], pair[W], sums[H][4][C];
+  __shared__ bool holds[W];
   const int c = blockIdx.x, ks = blockIdx.y, group = SHARED ? g.nb / g.nbk : 1;
   const int w = uniform_wave(), tt = w & 3, hf = w >> 2;
   const int ld = (g.p + 31) / 32 * 32, rt0 = hf * RT;
@@ -376,6 +380,7 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) gp[jt] = np[jt] = zero4();
     float zv = 0.f, dots = 0.f;
+    uint32_t held = 0;                             // whether the state entering holds anything
     for (int pb = 0; pb < ld; pb += 32) {
       if constexpr (FULL) {
 #pragma unroll
@@ -388,6 +393,8 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
       }
       if (pairs) {
         dots += dot4(sx[0], ex[0]) + dot4(sx[1], ex[1]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) held |= __float_as_uint(sx[0][i]) | __float_as_uint(sx[1][i]);
         store_frag<NI>(fr + (FS + w) * kFrag, FP, split<NI>(sx[0], sx[1]));
         store_frag<NI>(fr + (FD + w) * kFrag, FP, split<NI>(ex[0], ex[1]));
       }
@@ -427,7 +434,11 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) dots += __shfl_xor(dots, d);
     }
-    if (lane_id() == 0) pair[w] = dots;
+    const bool any = __any((held << 1) != 0);      // (a zero may have a sign)
+    if (lane_id() == 0) {
+      pair[w] = dots;
+      holds[w] = any;
+    }
     if (has_z) {
       zv = sum_groups(zv);
       if (gq == 0) zvs[tok] = zv;
@@ -530,8 +541,11 @@ __global__ __launch_bounds__(256 * grad_split(RB), 2) void delta_grad_kernel(Geo
 #pragma unroll
       for (int n = 0; n < W; ++n) ds += pair[n];
       sum += vec[3 * C] * ds;                      // <dS', S'>
+      bool enters = false;
+#pragma unroll
+      for (int n = 0; n < W; ++n) enters |= holds[n];
       if (t < len) {
-        io.dlogA[(int64_t)s * g.T + t0 + t] = x + sum;
+        io.dlogA[(int64_t)s * g.T + t0 + t] = t > 0 || enters ? x + sum : 0.f;
         io.dbeta[(int64_t)s * g.T + t0 + t] = zvs[t] + v4[1];
       }
     }
