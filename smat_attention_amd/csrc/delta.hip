@@ -18,10 +18,11 @@
 // run from its own state.
 //
 // What bounds it: the vector ALUs, which split every product's result into terms (eight
-// operations a value), and MFMA issue beside them.  8 sequences of 131072 tokens, r = p =
-// 128 in bf16: 675 us for the first pass, 61 for the carry over 32 runs, 498 for the
-// second, 0.82 PFLOP/s of issued products.  In training the second pass also writes S and
-// U and runs at 5 TB/s (96 x 4096, r = p = 64: 120 us).
+// operations a value), with the reloads of addresses spilled to vector lanes, and MFMA
+// issue beside them.  8 sequences of 131072 tokens, r = p = 128 in bf16: 699 us for the
+// first pass, 65 for the carry over 32 runs, 588 for the second, 0.76 PFLOP/s of issued
+// products.  In training the second pass also writes S and U and runs at 4.7 TB/s (96 x
+// 4096, r = p = 64: 127 us).
 #include "delta_prep.hpp"
 
 namespace smat {
@@ -497,9 +498,12 @@ static int scan(int dtype, const Geo& g, const In* q, const In* k, const void* v
 // one buffer of K from 96 features on, is taken for the same); 0.55 RB a run of the carry
 // and 10 for the two launches more.  Workgroups of four waves share a CU in pairs, which then take
 // 1.64 times as long; more than are resident follow one another, the last ones alone.
-// (8 sequences of 2048 chunks, r = p = 128: 9367 whole, 1377 in 32 runs, 1457 in 64,
-// 1670 in 128; 12 of 5 segments and 158 chunks, r = p = 96 in fp16: 640 whole, 251 in
-// runs of 10, 303 of 8, 285 of 16.)
+// (8 sequences of 2048 chunks, r = p = 128: 10915 whole, 1446 in 32 runs, 1496 in 64,
+// 1648 in 128; 12 of 5 segments and 158 chunks, r = p = 96 in fp16: 734 whole, 242 in
+// runs of 9, 247 of 8, 294 of 16.)  A step with outputs takes 4.0 + 0.43 RB by now; priced
+// so, the rule cuts finer, which suits forwards alone (32 x 128 chunks, r = p = 64: 188,
+// not 198) and costs training, whose backward walks the same runs (79 x 18 chunks, r = 64,
+// p = 128: 365, not 337): over the ten of 123 sizes that it moves, 2 % lost.
 extern "C" int smat_delta_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
                                      const int32_t* times, int n, int r, int p) {
   using namespace smat::dl;

@@ -25,8 +25,8 @@
 // the heads' order.
 //
 // Both move fp32 states and rows of every chunk through HBM and are bound by that: 96 x
-// 4096 tokens, r = p = 64 in bf16: the walk 138 us at 4.6 TB/s (its first pass 81), the
-// rest 220 us for 113 KB a chunk, 3.2 TB/s, its loads one step of 32 columns ahead.
+// 4096 tokens, r = p = 64 in bf16: the walk 140 us at 4.5 TB/s (its first pass 84), the
+// rest 225 us for 113 KB a chunk, 3.1 TB/s, its loads one step of 32 columns ahead.
 #include "delta_prep.hpp"
 
 namespace smat {

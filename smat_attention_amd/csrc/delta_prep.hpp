@@ -11,8 +11,8 @@
 // hundreds of nats leaves the differences of later tokens exact; logA below -1e5
 // (a = 0 many times over) counts as -1e5, which keeps -inf - -inf out.
 //
-// Bound by HBM, what it writes above all (T and P in three terms, 30 KB): 194 us for 8
-// sequences of 131072 tokens, r = 128 in bf16, 5.4 TB/s.
+// Bound by HBM, what it writes above all (T and P in three terms, 30 KB): 196 us for 8
+// sequences of 131072 tokens, r = 128 in bf16, 5.3 TB/s.
 #pragma once
 
 #include "delta_common.hpp"

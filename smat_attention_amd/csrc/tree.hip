@@ -15,7 +15,7 @@
 // rows and all scores phi_j . psi_a, is formed once a workgroup, in LDS.  The masked
 // scores meet vb on MFMA too; a vb that is not finite is left out there, where it would
 // meet other branches' zeros, and added to its descendants alone.  16 trees of 64 nodes
-// and 8 heads of 128: 34 us, 2.3 TB/s (a chain of levels: sum, split, products, store),
+// and 8 heads of 128: 35 us, 2.2 TB/s (a chain of levels: sum, split, products, store),
 // the accepted paths' states 9.
 #include "delta_common.hpp"
 
