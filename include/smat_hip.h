@@ -621,6 +621,62 @@ int smat_delta_step(int dtype, const void* q, const void* k, const void* v, cons
                     int64_t a_sb, int64_t b_sb, void* stream);
 
 /*
+ * Linear attention with a decay for each head over whole sequences:
+ *   S_t = a S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,  a = exp(logA[head]),
+ * fp32 state S (r, p).  No counterpart in the reference's path (its decayed scan, model.py:41-82,
+ * has a decay a token).
+ * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides (any; unit column stride); value
+ * sequence s reads key sequence s / (nb / nbk) and has head s % heads (nbk and heads divide nb).
+ * logA: (heads) fp32.  out: (nb, T, p) of dtype, contiguous.  8 <= r, p <= 128; nb < 2^23; at
+ * most 65535 segments and runs.  Segments and runs: the tables of smat_delta_scan;
+ * smat_head_decay_run_chunks is its rule for the run length here.
+ * state: (nseg, nb, r, p) fp32 entering each segment (NULL: zero); state_out the same leaving
+ * it (may be NULL; not state itself).
+ * Training: save_start (nruns, nb, r, p) fp32 receives the states entering runs (only where
+ * nruns > nseg; may be NULL), save_s (nb, nch, P, R) fp32 those entering chunks, R being r
+ * rounded up to 32 and P 64 or 128 (may be NULL: needed for dlogA).
+ * workspace: smat_head_decay_workspace_bytes(..., backward, learn) bytes, 256-byte aligned.
+ */
+int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
+                               const int32_t* times, int n, int r, int p);
+int64_t smat_head_decay_workspace_bytes(int nb, int nbk, int T, int nseg, int nruns, int r, int p,
+                                        int backward, int learn);
+int smat_head_decay_scan(int dtype, const void* q, const void* k, const void* v, const float* logA,
+                         const float* state, void* out, float* state_out, float* save_start,
+                         float* save_s, const int32_t* chunks, const int32_t* runs,
+                         const int32_t* segrun, int nb, int nbk, int heads, int T, int nseg,
+                         int nch, int nruns, int K, int r, int p, float scale, int64_t q_sb,
+                         int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its gradient: dout (nb, T, p) of dtype with strides and dstate_out (the gradient of
+ * state_out, or NULL) -> dq, dk (nbk, T, r), dv (nb, T, p) of dtype, contiguous, dstate (nseg,
+ * nb, r, p) fp32 or NULL, and dlogA (heads) fp32 or NULL (learn = 0).  start: the forward's
+ * save_start, or its state where nruns == nseg.  Sizes, runs and tables are the forward's.
+ */
+int smat_head_decay_scan_backward(int dtype, const void* q, const void* k, const void* v,
+                                  const float* logA, const void* dout, const float* dstate_out,
+                                  const float* start, const float* save_s, void* dq, void* dk,
+                                  void* dv, float* dstate, float* dlogA, const int32_t* chunks,
+                                  const int32_t* runs, const int32_t* segrun, int nb, int nbk,
+                                  int heads, int T, int nseg, int nch, int nruns, int K, int r,
+                                  int p, float scale, int64_t q_sb, int64_t q_st, int64_t k_sb,
+                                  int64_t k_st, int64_t v_sb, int64_t v_st, int64_t d_sb,
+                                  int64_t d_st, void* workspace, int64_t workspace_bytes,
+                                  void* stream);
+
+/*
+ * One token of it: S_out from S_in (both (nb, r, p) fp32 contiguous; they may be the same
+ * buffer) and out (nb, p) of dtype, contiguous.  q, k: (nbk, r), v: (nb, p) with batch strides;
+ * 1 <= r, p <= 128; nb < 2^24.
+ */
+int smat_head_decay_step(int dtype, const void* q, const void* k, const void* v, const float* logA,
+                         const float* S_in, float* S_out, void* out, int nb, int nbk, int heads,
+                         int r, int p, float scale, int64_t q_sb, int64_t k_sb, int64_t v_sb,
+                         void* stream);
+
+/*
  * Unpooled long-range sums  U_h = sum_{j in cols_h} Psi_{n_P+j}^T Vb_{n_P+j}
  * (fp32, U: (nb, B, r, p) contiguous), one row type per list: cols (B, kappa)
  * int32 landmark columns, row h holding its counts[h] columns first.

@@ -34,6 +34,7 @@ from typing import Callable, Dict, Optional
 import numpy as np
 import torch
 
+from .kernels import hip_decay as _decay
 from .kernels import hip_delta as _delta
 from .kernels import hip_fwd as _hip
 from .kernels.hip_delta import Segments
@@ -47,6 +48,7 @@ __all__ = [
     "query_by_type", "zeta_transform", "walsh_incidence", "direct_long_range",
     "smat_attention", "smat_attention_fused", "dense_masked_kernel_attention", "SmatDecoder",
     "DraftTree", "Segments", "gated_delta_scan", "gated_delta_step", "GatedDeltaDecoder",
+    "head_decay_scan", "head_decay_step", "HeadDecayDecoder",
     "have_triton", "have_hip",
 ]
 
@@ -477,6 +479,61 @@ def gated_delta_step(q, k, v, logA, beta, state, *, scale: float = 1.0, out=None
     (``out``, if given, must not share memory with the inputs).  One launch, for serving: no
     gradients."""
     return _delta.step(q, k, v, logA, beta, state, float(scale), out, out_state)
+
+
+def head_decay_scan(Q, K, V, logA, *, scale: float = 1.0, state=None,
+                    segments: Optional[Segments] = None, return_state: bool = False):
+    """Linear attention with a decay for each head, over whole sequences::
+
+        S_t = a S_{t-1} + k_t v_t^T,   o_t = scale S_t^T q_t,   a = exp(logA) of the head
+
+    the decayed scan's state where the decay is the head's and not the token's.  It has no
+    counterpart in the reference's path.
+
+    ``Q, K (nbk, T, r)`` and ``V (nb, T, p)`` in one of bf16, fp16 and fp32; ``nbk`` divides
+    ``nb`` and value sequence s reads key sequence ``s // (nb // nbk)`` (value heads innermost).
+    ``logA (heads,)`` in fp32 (16-bit ones are taken to fp32 first), heads dividing ``nb``: value
+    sequence s has head ``s % heads``, so sequences are batch-major.  ``logA <= 0``, ``-inf``
+    among them: the state is then the last token's.  (Positive ones are taken while the exp of 64
+    of them, and of a sequence's, stay within fp32.)  Any strides with contiguous columns are read
+    in place, so packed ``(tokens, heads, columns)`` tensors come as their transposed views.
+    r, p <= 128; at most 2^23 - 1 sequences.  The values of a chunk of 64 tokens meet in
+    products, so one that is not finite spoils its sequence from its chunk on.
+
+    ``segments`` (:class:`Segments`) packs sequences of any lengths along T; each starts from
+    its own state.  ``state`` fp32 ``(nb, r, p)``, with segments ``(segments, nb, r, p)``
+    (zero if None), is the state entering; ``return_state`` returns ``(o, state_out)``, else
+    ``o (nb, T, p)`` in the inputs' type.  Few long sequences are also split along T.
+    Differentiable in Q, K, V, logA and state.
+    """
+    who = "head_decay_scan"
+    _decay.check_scan(who, Q, K, V, logA, state, segments)
+    r, p = Q.shape[2], V.shape[2]
+    if min(r, p) < _decay.MIN_D:                     # rows are read eight values at a time
+        more = [max(0, _decay.MIN_D - n) for n in (r, p)]
+        pad = torch.nn.functional.pad
+        o, S = head_decay_scan(
+            pad(Q, (0, more[0])), pad(K, (0, more[0])), pad(V, (0, more[1])), logA, scale=scale,
+            state=None if state is None else pad(state, (0, more[1], 0, more[0])),
+            segments=segments, return_state=True)
+        o = o[..., :p].contiguous()
+        return (o, S[..., :r, :p].contiguous()) if return_state else o
+    if _wants_grad(Q, K, V, logA, state):
+        o, s_out = _decay.HeadDecayFunction.apply(Q, K, V, logA, state, float(scale), segments,
+                                                  return_state)
+    else:
+        o, s_out = _decay.scan(Q, K, V, logA, state, scale, segments, return_state, False,
+                               False)[:2]
+    return (o, s_out) if return_state else o
+
+
+def head_decay_step(q, k, v, logA, state, *, scale: float = 1.0, out=None, out_state=None):
+    """One token of :func:`head_decay_scan` for a batch of sequences: ``q, k (nbk, r)``,
+    ``v (nb, p)``, ``logA (heads,)``, ``state (nb, r, p)`` fp32.  The new state goes to
+    ``out_state``, or replaces ``state`` if that is None; returns ``o (nb, p)`` in v's type
+    (``out``, if given, must not share memory with the inputs).  One launch, for serving: no
+    gradients."""
+    return _decay.step(q, k, v, logA, state, float(scale), out, out_state)
 
 
 def pool_profiles(Psi, Vb, spec: MaskSpec, acc_dtype=None, backend: str = "auto"):
@@ -1006,6 +1063,38 @@ class GatedDeltaDecoder:
     def step(self, q, k, v, logA, beta, *, out=None) -> torch.Tensor:
         """One token; returns ``o (nb, p)``."""
         return gated_delta_step(q, k, v, logA, beta, self.S, scale=self.scale, out=out)
+
+    def cache_words(self) -> int:
+        return int(self.S.numel())
+
+
+class HeadDecayDecoder:
+    """A decayed linear attention layer's state in serving: a prompt in chunks, then token by
+    token.
+
+    ``state`` fp32 ``(nb, r, p)`` is taken over and updated in place (zero it for a new
+    sequence, copy it to branch); ``logA (heads,)`` is the layer's.  The arguments of the calls
+    are :func:`head_decay_scan`'s and :func:`head_decay_step`'s."""
+
+    def __init__(self, state: torch.Tensor, logA: torch.Tensor, *, scale: float = 1.0):
+        who = "HeadDecayDecoder"
+        _delta.same_device(who, state, logA)
+        if state.dim() != 3 or state.dtype != torch.float32 or not state.is_contiguous():
+            raise ValueError(f"{who}: the state must be contiguous fp32 (nb, r, p)")
+        _decay.check_sizes(who, state.shape[0], state.shape[0], logA, *state.shape[1:])
+        self.S, self.logA, self.scale = state, logA.detach().float().contiguous(), float(scale)
+
+    @torch.no_grad()
+    def prefill(self, Q, K, V) -> torch.Tensor:
+        """Any number of tokens at once; returns ``o (nb, T, p)``."""
+        o, S = head_decay_scan(Q, K, V, self.logA, scale=self.scale, state=self.S,
+                               return_state=True)
+        self.S.copy_(S)
+        return o
+
+    def step(self, q, k, v, *, out=None) -> torch.Tensor:
+        """One token; returns ``o (nb, p)``."""
+        return head_decay_step(q, k, v, self.logA, self.S, scale=self.scale, out=out)
 
     def cache_words(self) -> int:
         return int(self.S.numel())

@@ -1,0 +1,372 @@
+// Linear attention with a decay for each head: the entry points over whole sequences
+// (head_decay_scan and its gradient).  The mathematics and the walk are in decay_walk.hpp.
+//
+// A workgroup walks a whole segment where sequences give enough workgroups.  Where they do
+// not, segments are cut into runs: a first pass takes every run but the last from the zero
+// state for its end E, the carry adds them up, S <- a^(tokens of the run) S + E, and the
+// second pass takes every run from its own state.
+#include "decay_walk.hpp"
+
+namespace smat {
+namespace hd {
+
+// The states entering the runs of a segment, from init or from zero; `rev`: the runs in
+// turned order.  Every element on its own, eight runs' E in flight.
+__global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* __restrict__ init,
+                                                          const float* __restrict__ E,
+                                                          float* __restrict__ start) {
+  const int s = blockIdx.x, seg = blockIdx.z;
+  const int64_t rp = (int64_t)g.r * g.p, e = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
+  if (r0 >= r1 || e >= rp) return;
+  const double la = g.logA[s % g.heads];
+  auto at = [&](int n) { return ((int64_t)(g.rev ? r0 + r1 - 1 - n : n) * g.nb + s) * rp + e; };
+  auto decay = [&](int n) {                        // of the run's tokens
+    const int i = g.rev ? r0 + r1 - 1 - n : n;
+    int tokens;
+    if (g.runs) {
+      const int a = g.runs[4 * i], b = g.runs[4 * i + 1];
+      tokens = b > a ? g.chunks[2 * b - 2] + g.chunks[2 * b - 1] - g.chunks[2 * a] : 0;
+    } else {
+      tokens = min((i + 1) * g.K * C, g.T) - i * g.K * C;
+    }
+    return tokens ? (float)exp(la * tokens) : 1.f;
+  };
+  float S = init ? init[((int64_t)seg * g.nb + s) * rp + e] : 0.f;
+  constexpr int U = 8;
+  for (int n = r0; n < r1; n += U) {
+    float x[U], a[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {                  // past the last but one: its own once more
+      const int i = min(n + u, max(r1 - 2, r0));
+      x[u] = r1 - r0 > 1 ? E[at(i)] : 0.f;
+      a[u] = decay(i);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (n + u >= r1) break;
+      start[at(n + u)] = S;
+      S = a[u] * S + x[u];
+    }
+  }
+}
+
+// out = the sum over a key head's value heads of fp32 rows, rounded once.
+template <typename In>
+__global__ __launch_bounds__(256) void decay_heads_kernel(const float* __restrict__ part,
+                                                          In* __restrict__ out, int group,
+                                                          int64_t n) {
+  const int64_t ks = blockIdx.y;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n;
+       i += (int64_t)gridDim.x * 1024) {
+    const int nv = (int)(n - i < 4 ? n - i : 4);
+    f32x4 x = zero4();
+    for (int j = 0; j < group; ++j) x += dl::load4(part + (ks * group + j) * n + i, nv, n % 4 == 0);
+    dl::store4(out + ks * n + i, x, nv, n % 4 == 0);
+  }
+}
+
+// dlogA of a head: its parts of the three walks, in the same order every time.
+__global__ __launch_bounds__(256) void decay_grad_kernel(const float* p0, const float* p1,
+                                                         const float* p2, int W0, int W1, int W2,
+                                                         int nruns, int nb, int heads,
+                                                         float* __restrict__ dlogA) {
+  const int h = blockIdx.x;
+  const float* ps[3] = {p0, p1, p2};
+  const int Ws[3] = {W0, W1, W2};
+  double x = 0;
+  for (int k = 0; k < 3; ++k) {
+    const int64_t n = (int64_t)nruns * (nb / heads) * Ws[k];
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+      const int64_t sn = i / Ws[k];                // run, batch
+      const int64_t run = sn / (nb / heads), b = sn % (nb / heads);
+      x += ps[k][(run * nb + b * heads + h) * Ws[k] + i % Ws[k]];
+    }
+  }
+  __shared__ double sum[256];
+  sum[threadIdx.x] = x;
+  __syncthreads();
+  for (int d = 128; d > 0; d >>= 1) {
+    if (threadIdx.x < d) sum[threadIdx.x] += sum[threadIdx.x + d];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) dlogA[h] = (float)sum[0];
+}
+
+static int walk_any(int dtype, const Walk& g, bool out, hipStream_t st) {
+  if (dtype == SMAT_BF16) return launch_walk<bf16>(g, out, st);
+  if (dtype == SMAT_F16) return launch_walk<f16>(g, out, st);
+  return launch_walk<float>(g, out, st);
+}
+
+// First pass and carry of a walk (k, v, rev and upd set): start from init.
+static int carry(int dtype, const Walk& base, const float* init, float* E, float* start,
+                 hipStream_t st) {
+  Walk g = base;
+  g.start = nullptr;
+  g.fin = E;
+  int rc = walk_any(dtype, g, false, st);
+  if (rc) return rc;
+  const int64_t rp = (int64_t)g.r * g.p;
+  hipLaunchKernelGGL(decay_carry_kernel, dim3(g.nb, (rp + 255) / 256, g.nseg), dim3(256), 0, st, g,
+                     init, E, start);
+  return launch_status("smat_head_decay_scan: carry");
+}
+
+static int check(const char* who, int dtype, const Walk& g, int nbk, int r, int p) {
+  SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
+               "%s: unknown dtype %d", who, dtype);
+  SMAT_REQUIRE(g.nb >= 0 && nbk >= 1 && g.heads >= 1 && g.T >= 0 && g.nseg >= 1 && g.nch >= 0,
+               SMAT_EINVAL, "%s: bad sizes (nb=%d nbk=%d heads=%d T=%d nseg=%d nch=%d)", who, g.nb,
+               nbk, g.heads, g.T, g.nseg, g.nch);
+  SMAT_REQUIRE(g.nb % nbk == 0 && g.nb % g.heads == 0, SMAT_EINVAL,
+               "%s: nbk=%d and heads=%d must divide nb=%d", who, nbk, g.heads, g.nb);
+  SMAT_REQUIRE(r >= kMinD && r <= kMaxD && p >= kMinD && p <= kMaxD, SMAT_EUNSUPPORTED,
+               "%s: r=%d p=%d must lie in %d..%d", who, r, p, kMinD, kMaxD);
+  if (g.chunks || g.runs || g.segrun) {
+    SMAT_REQUIRE(g.chunks && g.runs && g.segrun && g.nruns >= g.nseg, SMAT_EINVAL,
+                 "%s: segments need the chunk, run and segment tables", who);
+  } else {
+    SMAT_REQUIRE(g.nseg == 1 && g.nch == (g.T + C - 1) / C, SMAT_EINVAL,
+                 "%s: %d chunks for T=%d", who, g.nch, g.T);
+    SMAT_REQUIRE(g.K >= 1 && g.nruns == (g.nch > 0 ? (g.nch + g.K - 1) / g.K : 1), SMAT_EINVAL,
+                 "%s: %d runs of %d chunks for %d chunks", who, g.nruns, g.K, g.nch);
+  }
+  // a grid has less than 2^32 threads along its first axis and 65535 workgroups along others
+  SMAT_REQUIRE(g.nb < (1 << 23) && g.nruns <= dl::kMaxGrid && g.nseg <= dl::kMaxGrid,
+               SMAT_EUNSUPPORTED, "%s: nb=%d must stay below 2^23, %d segments and %d runs within %d",
+               who, g.nb, g.nseg, g.nruns, dl::kMaxGrid);
+  return SMAT_OK;
+}
+
+static int check_workspace(const char* who, const void* ws, int64_t got, int64_t need) {
+  SMAT_REQUIRE(got >= need && (ws || need == 0) && ((uintptr_t)ws & 255) == 0, SMAT_EINVAL,
+               "%s: workspace of %lld bytes, %lld needed (256-byte aligned)", who, (long long)got,
+               (long long)need);
+  return SMAT_OK;
+}
+
+struct Scratch {
+  float *E, *start;        // the runs' ends and starts
+  float *dq, *dk;          // rows of every value head, where they share key heads
+  float* part[3];          // the parts of dlogA
+};
+static Scratch take(dl::Arena& ar, int64_t nb, int64_t nbk, int64_t T, int nseg, int64_t nruns,
+                    int r, int p, bool backward, bool learn) {
+  Scratch c = {};
+  if (nruns > nseg) {
+    c.E = ar.take<float>(nruns * nb * r * p);
+    c.start = ar.take<float>(nruns * nb * r * p);
+  }
+  if (backward && nb > nbk) {
+    c.dq = ar.take<float>(nb * T * r);
+    c.dk = ar.take<float>(nb * T * r);
+  }
+  if (backward && learn)
+    for (float*& x : c.part) x = ar.take<float>(nruns * nb * 8);
+  return c;
+}
+
+}  // namespace hd
+}  // namespace smat
+
+// Run length: of the lengths that cut the longest segment into 1 to 256 runs, the one whose
+// passes take least.
+extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
+                                          const int32_t* times, int n, int r, int p) {
+  using namespace smat;
+  const bool packed = lengths && times && n > 0;
+  int longest = packed ? 0 : nch;
+  for (int i = 0; packed && i < n; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
+  if (longest < 1 || nb < 1 || r < 1 || p < 1) return 1;
+  const int slots = hd::waves_of(p) == 4 ? 512 : 256;
+  int best = longest;
+  double least = 0;
+  for (int G = 1; G <= 256 && (G == 1 || longest / G >= 2); ++G) {
+    const int K = (longest + G - 1) / G;
+    double runs = 0, chunks = 0, ends = 0;
+    for (int i = 0; i < (packed ? n : 1); ++i) {
+      const double len = packed ? lengths[i] : nch, t = packed ? times[i] : 1;
+      const double cut = len > K ? (int)((len + K - 1) / K) : 1;
+      runs += t * cut;
+      ends += t * (cut - 1);
+      chunks += t * len;
+    }
+    if (G > 1 && runs > dl::kMaxGrid) continue;
+    auto pass = [&](double wgs, double steps, double cost) {
+      return wgs <= slots ? K * cost : (steps / slots + 0.5 * K) * cost;
+    };
+    double us = pass(runs * nb, chunks * nb, 3.0);
+    if (ends > 0) us += pass(ends * nb, ends * K * nb, 1.5) + 10 + 0.1 * G;
+    if (G == 1 || us < least) {
+      least = us;
+      best = K;
+    }
+  }
+  return best;
+}
+
+extern "C" int64_t smat_head_decay_workspace_bytes(int nb, int nbk, int T, int nseg, int nruns,
+                                                   int r, int p, int backward, int learn) {
+  using namespace smat;
+  dl::Arena ar{nullptr};
+  hd::take(ar, nb, nbk, T, nseg, nruns, r, p, backward != 0, learn != 0);
+  return ar.used;
+}
+
+extern "C" int smat_head_decay_scan(int dtype, const void* q, const void* k, const void* v,
+                                    const float* logA, const float* state, void* out,
+                                    float* state_out, float* save_start, float* save_s,
+                                    const int32_t* chunks, const int32_t* runs,
+                                    const int32_t* segrun, int nb, int nbk, int heads, int T,
+                                    int nseg, int nch, int nruns, int K, int r, int p, float scale,
+                                    int64_t q_sb, int64_t q_st, int64_t k_sb, int64_t k_st,
+                                    int64_t v_sb, int64_t v_st, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  using namespace smat;
+  using namespace smat::hd;
+  clear_error();
+  const char* who = "smat_head_decay_scan";
+  Walk g = {chunks, runs, segrun, nb, T, nseg, nch, nruns, K, r, p};
+  g.heads = heads;
+  int rc = check(who, dtype, g, nbk, r, p);
+  if (rc) return rc;
+  if (nb == 0) return SMAT_OK;
+  SMAT_REQUIRE(logA && (nch == 0 || (q && k && v && out)), SMAT_EINVAL, "%s: null pointer", who);
+  SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
+  rc = check_workspace(who, workspace, workspace_bytes,
+                       smat_head_decay_workspace_bytes(nb, nbk, T, nseg, nruns, r, p, 0, 0));
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  dl::Arena ar{(char*)workspace};
+  const Scratch sc = take(ar, nb, nbk, T, nseg, nruns, r, p, false, false);
+  const int group = nb / nbk;
+  g.q = {q, q_sb, q_st, group};
+  g.k = {k, k_sb, k_st, group};
+  g.v = {v, v_sb, v_st, 1};
+  g.logA = logA;
+  g.upd = 1.f;
+  g.inter = g.intra = scale;
+  g.start = state;
+  g.s_row = p;
+  g.s_col = 1;
+  if (nruns > nseg) {
+    float* start = save_start ? save_start : sc.start;
+    rc = carry(dtype, g, state, sc.E, start, st);
+    if (rc) return rc;
+    g.start = start;
+  }
+  g.fin = state_out;
+  g.o = out;
+  g.save_s = save_s;
+  return walk_any(dtype, g, true, st);
+}
+
+extern "C" int smat_head_decay_scan_backward(
+    int dtype, const void* q, const void* k, const void* v, const float* logA, const void* dout,
+    const float* dstate_out, const float* start, const float* save_s, void* dq, void* dk, void* dv,
+    float* dstate, float* dlogA, const int32_t* chunks, const int32_t* runs, const int32_t* segrun,
+    int nb, int nbk, int heads, int T, int nseg, int nch, int nruns, int K, int r, int p,
+    float scale, int64_t q_sb, int64_t q_st, int64_t k_sb, int64_t k_st, int64_t v_sb, int64_t v_st,
+    int64_t d_sb, int64_t d_st, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace smat;
+  using namespace smat::hd;
+  clear_error();
+  const char* who = "smat_head_decay_scan_backward";
+  Walk base = {chunks, runs, segrun, nb, T, nseg, nch, nruns, K, r, p};
+  base.heads = heads;
+  int rc = check(who, dtype, base, nbk, r, p);
+  if (rc) return rc;
+  const bool learn = dlogA != nullptr;
+  if (nb == 0) return SMAT_OK;
+  SMAT_REQUIRE(logA && (nch == 0 || (q && k && v && dout && dq && dk && dv)), SMAT_EINVAL,
+               "%s: null pointer", who);
+  SMAT_REQUIRE((nruns == nseg || start) && (!learn || save_s || nch == 0), SMAT_EINVAL,
+               "%s: the states that the forward kept are missing", who);
+  rc = check_workspace(
+      who, workspace, workspace_bytes,
+      smat_head_decay_workspace_bytes(nb, nbk, T, nseg, nruns, r, p, 1, learn));
+  if (rc) return rc;
+  hipStream_t st = (hipStream_t)stream;
+  dl::Arena ar{(char*)workspace};
+  const Scratch sc = take(ar, nb, nbk, T, nseg, nruns, r, p, true, learn);
+  const int group = nb / nbk;
+  base.logA = logA;
+  base.intra = scale;
+  const Side Q = {q, q_sb, q_st, group}, Kk = {k, k_sb, k_st, group}, V = {v, v_sb, v_st, 1},
+             dO = {dout, d_sb, d_st, 1};
+  // backwards: the gradients of v and k
+  Walk g = base;
+  g.rev = true;
+  g.q = Kk;
+  g.k = Q;
+  g.v = dO;
+  g.upd = scale;
+  g.inter = 1.f;
+  g.start = dstate_out;
+  g.s_row = p;
+  g.s_col = 1;
+  if (nruns > nseg) {
+    rc = carry(dtype, g, dstate_out, sc.E, sc.start, st);
+    if (rc) return rc;
+    g.start = sc.start;
+  }
+  g.fin = dstate;
+  g.o = dv;
+  g.load_s = save_s;
+  g.learn = learn ? kDv : kNone;
+  g.part = sc.part[0];
+  rc = walk_any(dtype, g, true, st);
+  if (rc) return rc;
+  g.q = V;
+  g.k = dO;
+  g.v = Q;
+  g.r = p;
+  g.p = r;
+  g.s_row = 1;
+  g.s_col = p;
+  g.fin = nullptr;
+  g.o = group > 1 ? (void*)sc.dk : dk;
+  g.wide = group > 1;
+  g.x = Kk;
+  g.learn = learn ? kDk : kNone;
+  g.part = sc.part[1];
+  rc = walk_any(dtype, g, true, st);
+  if (rc) return rc;
+  // forward: that of q
+  g.rev = false;
+  g.q = dO;
+  g.k = V;
+  g.v = Kk;
+  g.upd = 1.f;
+  g.inter = scale;
+  g.start = start;
+  g.o = group > 1 ? (void*)sc.dq : dq;
+  g.x = Q;
+  g.learn = learn ? kDq : kNone;
+  g.part = sc.part[2];
+  rc = walk_any(dtype, g, true, st);
+  if (rc) return rc;
+  if (group > 1 && nch > 0) {
+    const int64_t n = (int64_t)T * r;
+    const int blocks = (int)((n + 1023) / 1024 < 4096 ? (n + 1023) / 1024 : 4096);
+    auto sum = [&](auto in) {
+      typedef decltype(in) In;
+      for (int ks = 0; ks < nbk; ks += dl::kMaxGrid) {   // (a grid's second axis)
+        const int many = nbk - ks < dl::kMaxGrid ? nbk - ks : dl::kMaxGrid;
+        const int64_t in0 = (int64_t)ks * group * n, out0 = (int64_t)ks * n;
+        hipLaunchKernelGGL(decay_heads_kernel<In>, dim3(blocks, many), dim3(256), 0, st,
+                           sc.dq + in0, (In*)dq + out0, group, n);
+        hipLaunchKernelGGL(decay_heads_kernel<In>, dim3(blocks, many), dim3(256), 0, st,
+                           sc.dk + in0, (In*)dk + out0, group, n);
+      }
+    };
+    if (dtype == SMAT_BF16) sum(bf16());
+    else if (dtype == SMAT_F16) sum(f16());
+    else sum(float());
+  }
+  if (learn)
+    hipLaunchKernelGGL(decay_grad_kernel, dim3(heads), dim3(256), 0, st, sc.part[0], sc.part[1],
+                       sc.part[2], waves_of(p), waves_of(r), waves_of(r), nruns, nb, heads, dlogA);
+  return launch_status(who);
+}

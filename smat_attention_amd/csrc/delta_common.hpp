@@ -517,6 +517,26 @@ __device__ __forceinline__ void column_values(f32x4* x, const uint32_t* v, bool 
 }
 inline bool near_rows(int64_t st) { return st >= 0 && st < (1 << 23); }
 
+// x of this lane and of lane ^ D, summed in registers (a shuffle through LDS takes ten
+// times as long, and a token is a chain of them).
+template <int D> __device__ __forceinline__ float sum_across(float x) {
+  static_assert(D == 8 || D == 16 || D == 32, "");
+  if constexpr (D == 8) {                          // a rotation within 16 lanes
+    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf,
+                                                           false));
+  } else {
+    const uint32_t b = __float_as_uint(x);
+    const auto r = D == 16 ? __builtin_amdgcn_permlane16_swap(b, b, false, false)
+                           : __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+}
+template <int CL> __device__ __forceinline__ float sum_rows(float x) {
+  if constexpr (CL <= 8) x = sum_across<8>(x);
+  if constexpr (CL <= 16) x = sum_across<16>(x);
+  return sum_across<32>(x);
+}
+
 // Four consecutive elements; those at and past nv are zero.
 template <typename In>
 __device__ __forceinline__ f32x4 load4(const In* p, int nv, bool vec) {

@@ -27,26 +27,6 @@ struct Tokens {
   int64_t q_sb, q_st, k_sb, k_st, v_sb, v_st, a_sb, a_st, b_sb, b_st, o_sb, o_st;
 };
 
-// x of this lane and of lane ^ D, summed in registers (a shuffle through LDS takes ten
-// times as long, and a token is a chain of them).
-template <int D> __device__ __forceinline__ float sum_across(float x) {
-  static_assert(D == 8 || D == 16 || D == 32, "");
-  if constexpr (D == 8) {                          // a rotation within 16 lanes
-    return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x128, 0xf, 0xf,
-                                                           false));
-  } else {
-    const uint32_t b = __float_as_uint(x);
-    const auto r = D == 16 ? __builtin_amdgcn_permlane16_swap(b, b, false, false)
-                           : __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-}
-template <int CL> __device__ __forceinline__ float sum_rows(float x) {
-  if constexpr (CL <= 8) x = sum_across<8>(x);
-  if constexpr (CL <= 16) x = sum_across<16>(x);
-  return sum_across<32>(x);
-}
-
 // ONE: a single token (less LDS and fewer registers, so more of the state in flight).
 template <typename In, int CL, bool VEC, bool ONE>
 __global__ __launch_bounds__(kStepThreads, ONE ? 4 : 2) void delta_tokens_kernel(Tokens g) {

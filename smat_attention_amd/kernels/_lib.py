@@ -140,6 +140,17 @@ SIGNATURES = {
                                       _i64, _i64, _p, _i64, _p]),
     "smat_delta_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _i64, _i64,
                              _i64, _i64, _i64, _p]),
+    "smat_head_decay_run_chunks": (_i, [_i, _i, _i, _p, _p, _i, _i, _i]),
+    "smat_head_decay_workspace_bytes": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "smat_head_decay_scan": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i,
+                                  _i, _i, _i, _i, _i, _i, _i, _f, _i64, _i64, _i64, _i64, _i64,
+                                  _i64, _p, _i64, _p]),
+    "smat_head_decay_scan_backward": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                                           _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f,
+                                           _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p,
+                                           _i64, _p]),
+    "smat_head_decay_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _i64,
+                                  _i64, _i64, _p]),
 }
 
 _lock = threading.Lock()

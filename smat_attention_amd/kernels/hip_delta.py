@@ -68,11 +68,12 @@ class Segments:
     def T(self):
         return self.offsets[-1]
 
-    def run_chunks(self, code: int, nb: int, r: int, p: int) -> int:
+    def run_chunks(self, code: int, nb: int, r: int, p: int,
+                   rule: str = "smat_delta_run_chunks") -> int:
         """The run length for inputs of these sizes, searched at the first call with them."""
-        key = (code, nb, r, p)
+        key = (rule, code, nb, r, p)
         if key not in self._best:
-            self._best[key] = _lib.query("smat_delta_run_chunks", code, nb, self.nch,
+            self._best[key] = _lib.query(rule, code, nb, self.nch,
                                          self._lengths.ctypes.data, self._times.ctypes.data,
                                          len(self._lengths), r, p)
         return self._best[key]
