@@ -677,6 +677,44 @@ int smat_head_decay_step(int dtype, const void* q, const void* k, const void* v,
                          void* stream);
 
 /*
+ * The end of a block, a row of D columns at a time:
+ *   y = post f / rms(f),  u = m gate(z) y,  h2 = h + s u,  x = pre h2 / rms(h2),
+ * rms(t)^2 = mean t^2 + eps.  No counterpart in the reference's path.
+ * f, z, x: (rows, D) of dtype; h, h2: of h_dtype (dtype or fp32); f, h, z with row strides and
+ * unit column stride, outputs contiguous.  gate: 0 none (z NULL), 1 z itself, 2 sigmoid, 3 silu.
+ * post, s, pre: (D) of types post_t, s_t, pre_t, or NULL: no norm after the block, `scale` for
+ * every column, no x.  p: dropout in [0, 1); place (row, column) is kept, times 1 / (1 - p),
+ * where its word of Philox 4x32 (ten rounds; key = *seed's low and high halves, counter =
+ * column / 4, row, salt, 0; word column % 4) is at least p 2^32.  seed: one int64 on the device,
+ * or NULL where p = 0.
+ * factors: (rows + 1, 2) fp32, 8-byte aligned, receive 1 / rms(f) and 1 / rms(h2) of every row
+ * and the seed's eight bytes for the gradient, or NULL.
+ * 8 <= D <= 8192, rows < 2^31.
+ */
+int smat_block_join(int dtype, int h_dtype, const void* f, const void* h, const void* z,
+                    const void* post, const void* s, const void* pre, int post_t, int s_t,
+                    int pre_t, const int64_t* seed, void* h2, void* x, float* factors,
+                    int64_t rows, int D, int gate, float eps, float scale, double p, uint32_t salt,
+                    int64_t f_st, int64_t h_st, int64_t z_st, void* stream);
+
+/*
+ * Its gradient, from dh (of h2) and dx (of x), (rows, D) with row strides, either NULL for
+ * zero: df, dz of dtype, dh_out of h_dtype, contiguous, and the columns' sums dpost, ds, dpre
+ * (D) fp32, each NULL where it is not wanted.  The other arguments are the forward's.
+ * workspace: smat_block_join_workspace_bytes(rows, D) bytes, 16-byte aligned; none without the
+ * sums.
+ */
+int64_t smat_block_join_workspace_bytes(int64_t rows, int D);
+int smat_block_join_backward(int dtype, int h_dtype, const void* f, const void* h, const void* z,
+                             const void* post, const void* s, const void* pre, int post_t, int s_t,
+                             int pre_t, const float* factors, const void* dh, const void* dx,
+                             void* df, void* dh_out, void* dz, float* dpost, float* ds,
+                             float* dpre, int64_t rows, int D, int gate, float eps, float scale,
+                             double p, uint32_t salt, int64_t f_st, int64_t h_st, int64_t z_st,
+                             int64_t dh_st, int64_t dx_st, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/*
  * Unpooled long-range sums  U_h = sum_{j in cols_h} Psi_{n_P+j}^T Vb_{n_P+j}
  * (fp32, U: (nb, B, r, p) contiguous), one row type per list: cols (B, kappa)
  * int32 landmark columns, row h holding its counts[h] columns first.

@@ -37,6 +37,7 @@ import torch
 from .kernels import hip_decay as _decay
 from .kernels import hip_delta as _delta
 from .kernels import hip_fwd as _hip
+from .kernels import hip_join as _join
 from .kernels.hip_delta import Segments
 from .kernels.hip_fwd import DraftTree
 from .mask import MaskSpec
@@ -48,7 +49,7 @@ __all__ = [
     "query_by_type", "zeta_transform", "walsh_incidence", "direct_long_range",
     "smat_attention", "smat_attention_fused", "dense_masked_kernel_attention", "SmatDecoder",
     "DraftTree", "Segments", "gated_delta_scan", "gated_delta_step", "GatedDeltaDecoder",
-    "head_decay_scan", "head_decay_step", "HeadDecayDecoder",
+    "head_decay_scan", "head_decay_step", "HeadDecayDecoder", "block_join",
     "have_triton", "have_hip",
 ]
 
@@ -348,6 +349,42 @@ def combine_normalise(H, Y, n: int, eps: float = 1e-6, out_dtype=torch.float32):
         raise ValueError(f"{who}: out_dtype must be float32, bfloat16 or float16")
     from .kernels.hip_bwd import CombineNormaliseFunction
     return CombineNormaliseFunction.apply(H, Y, n, eps, out_dtype)
+
+
+def block_join(f, h, *, post_weight=None, gate=None, gate_kind: str = "sigmoid", scale=1.0,
+               pre_weight=None, eps: float = 1e-6, dropout: float = 0.0, seed=None, salt: int = 0):
+    """The end of a block in one kernel each way: the norm after it, its gate, dropout, the
+    residual scale and sum, and the next block's norm, a row of columns at a time::
+
+        y  = post_weight * f / rms(f)          rms(t)^2 = mean(t^2) + eps
+        u  = drop(gate(z) * y)
+        h' = h + scale * u
+        x  = pre_weight * h' / rms(h')
+
+    ``f (..., D)`` is the block's output, ``h`` the residual stream, of f's type or fp32, and
+    ``gate`` = z, of f's type; 8 <= D <= 8192.  ``gate_kind`` is ``"sigmoid"``, ``"silu"``
+    (``z sigmoid(z)``) or ``"linear"`` (z itself).  ``post_weight, pre_weight (D,)`` and ``scale``,
+    a number or ``(D,)``, in any of the three types.  Without ``post_weight`` y is f, without
+    ``gate`` u is y, and without ``pre_weight`` there is no x.  Returns ``(h', x)`` in h's and f's
+    types, x None if there is none; computed in fp32 and rounded once.
+
+    ``dropout`` keeps a place with probability ``1 - dropout`` and scales it by its inverse.
+    Which ones is a function of ``seed`` (an int64 tensor of one element on the GPU: a captured
+    graph reads it at every replay), ``salt`` (a number below 2^32, one a layer), the row and the
+    column, from a counter-based generator; no mask is stored, and the gradient forms it again.
+
+    Differentiable in f, h, gate, the weights and a tensor ``scale``.  The rows of a tensor with
+    one stride between them are read in place; others (a gate expanded over tokens) are copied.
+    """
+    _join.check(f, h, gate, post_weight, scale, pre_weight, dropout, seed)
+    opt = _join.Options(gate, gate_kind, scale, eps, dropout, salt)
+    vector = scale if isinstance(scale, torch.Tensor) else None
+    if not opt.dropout:
+        seed = None
+    ts = (f, h, gate, post_weight, vector, pre_weight)
+    if _wants_grad(*ts):
+        return _join.BlockJoinFunction.apply(*ts, seed, opt)
+    return _join.forward(*ts, seed, opt, False)[:2]
 
 
 def _causal_scan(Phi, Psi, Vb, n: int, C: int):

@@ -30,6 +30,7 @@
 #pragma once
 
 #include "delta_common.hpp"
+#include "row_groups.hpp"
 
 namespace smat {
 namespace hd {
@@ -80,69 +81,6 @@ struct Walk {
   float* part;             // LEARN: (nruns, nb, W)
 };
 
-// Eight consecutive values of a row as they come, at the element's own alignment.
-template <typename In> struct Raw {
-  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-  typedef uint32_t u4h __attribute__((ext_vector_type(4), aligned(2)));
-  typedef uint32_t u4f __attribute__((ext_vector_type(4), aligned(4)));
-  typedef typename std::conditional<sizeof(In) == 2, u4h, u4f>::type u4u;
-  static constexpr int N = sizeof(In) / 2;
-  u4 x[N];
-  __device__ __forceinline__ void load(const In* p) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = reinterpret_cast<const u4u*>(p)[i];
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = u4{0, 0, 0, 0};
-  }
-  // Drops the first `by` values (0 <= by < 8): later ones move up, zeros follow.
-  __device__ __forceinline__ void drop(int by) {
-    uint32_t* d = reinterpret_cast<uint32_t*>(x);
-    constexpr int W = 4 * N;
-    if constexpr (sizeof(In) == 4) {
-#pragma unroll
-      for (int b = 4; b > 0; b >>= 1)
-        if (by & b) {
-#pragma unroll
-          for (int i = 0; i < W; ++i) d[i] = i + b < W ? d[i + b] : 0;
-        }
-    } else {
-#pragma unroll
-      for (int b = 2; b > 0; b >>= 1)
-        if (by & (2 * b)) {
-#pragma unroll
-          for (int i = 0; i < W; ++i) d[i] = i + b < W ? d[i + b] : 0;
-        }
-      if (by & 1) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) d[i] = (d[i] >> 16) | (i + 1 < W ? d[i + 1] << 16 : 0);
-      }
-    }
-  }
-  __device__ __forceinline__ void put(bf16* p, int64_t ts) const {
-    if constexpr (__is_same(In, bf16)) {
-      *reinterpret_cast<u4*>(p) = x[0];
-    } else {
-      f32x4 a, b;
-      if constexpr (__is_same(In, f16)) {
-        const f16x8 h = __builtin_bit_cast(f16x8, x[0]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] = (float)h[i];
-          b[i] = (float)h[i + 4];
-        }
-      } else {
-        a = __builtin_bit_cast(f32x4, x[0]);
-        b = __builtin_bit_cast(f32x4, x[1]);
-      }
-      const Frag<Terms<In>::in> f = dl::split<Terms<In>::in>(a, b);
-#pragma unroll
-      for (int n = 0; n < Terms<In>::in; ++n) *reinterpret_cast<bf16x8*>(p + n * ts) = f.t[n];
-    }
-  }
-};
-
 // One operand's rows of a chunk on their way to LDS: loaded a chunk ahead into registers,
 // then written as a tile (delta_common.hpp), a tile a term.  B: 32-column blocks.
 template <typename In, int B, int W> struct Rows {
@@ -175,7 +113,17 @@ template <typename In, int B, int W> struct Rows {
       if (UNITS % (64 * W) && t >= C) break;
       if (over && 8 * k + 8 > cols && 8 * k < cols) x[u].drop(8 - over);
       if (t >= len || 8 * k >= cols) x[u].zero();
-      x[u].put(tile + (t * RS + (k ^ dl::swz<RS>(t))) * 8, dl::tile_elems(B));
+      bf16* at = tile + (t * RS + (k ^ dl::swz<RS>(t))) * 8;
+      if constexpr (__is_same(In, bf16)) {
+        *reinterpret_cast<typename Raw<In>::u4*>(at) = x[u].x[0];
+      } else {
+        f32x4 a, b;
+        x[u].values(a, b);
+        const Frag<Terms<In>::in> f = dl::split<Terms<In>::in>(a, b);
+#pragma unroll
+        for (int n = 0; n < Terms<In>::in; ++n)
+          *reinterpret_cast<bf16x8*>(at + n * dl::tile_elems(B)) = f.t[n];
+      }
     }
   }
 };

@@ -36,6 +36,7 @@ class HipKernelError(RuntimeError):
 
 
 _i, _i64, _p, _f = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+_d, _u = ctypes.c_double, ctypes.c_uint32
 
 # name -> (restype, argtypes); must match include/smat_hip.h
 SIGNATURES = {
@@ -140,6 +141,12 @@ SIGNATURES = {
                                       _i64, _i64, _p, _i64, _p]),
     "smat_delta_step": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _f, _i64, _i64,
                              _i64, _i64, _i64, _p]),
+    "smat_block_join": (_i, [_i, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p, _p, _i64, _i,
+                             _i, _f, _f, _d, _u, _i64, _i64, _i64, _p]),
+    "smat_block_join_workspace_bytes": (_i64, [_i64, _i]),
+    "smat_block_join_backward": (_i, [_i, _i, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _p, _p, _p,
+                                      _p, _p, _p, _p, _p, _i64, _i, _i, _f, _f, _d, _u, _i64,
+                                      _i64, _i64, _i64, _i64, _p, _i64, _p]),
     "smat_head_decay_run_chunks": (_i, [_i, _i, _i, _p, _p, _i, _i, _i]),
     "smat_head_decay_workspace_bytes": (_i64, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "smat_head_decay_scan": (_i, [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i,
