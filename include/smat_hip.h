@@ -625,8 +625,8 @@ int smat_delta_step(int dtype, const void* q, const void* k, const void* v, cons
  *   S_t = a S_{t-1} + k_t v_t^T,  o_t = scale S_t^T q_t,  a = exp(logA[head]),
  * fp32 state S (r, p).  No counterpart in the reference's path (its decayed scan, model.py:41-82,
  * has a decay a token).
- * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides (any; unit column stride); value
- * sequence s reads key sequence s / (nb / nbk) and has head s % heads (nbk and heads divide nb).
+ * q, k: (nbk, T, r), v: (nb, T, p) of dtype with strides (rows 0 to 2^23 - 1 elements apart,
+ * unit column stride; likewise dout below); value sequence s reads key sequence s / (nb / nbk) and has head s % heads (nbk and heads divide nb).
  * logA: (heads) fp32.  out: (nb, T, p) of dtype, contiguous.  8 <= r, p <= 128; nb < 2^23; at
  * most 65535 segments and runs.  Segments and runs: the tables of smat_delta_scan;
  * smat_head_decay_run_chunks is its rule for the run length here.

@@ -5,6 +5,8 @@
 // not, segments are cut into runs: a first pass takes every run but the last from the zero
 // state for its end E, the carry adds them up, S <- a^(tokens of the run) S + E, and the
 // second pass takes every run from its own state.
+#include <initializer_list>
+
 #include "decay_walk.hpp"
 
 namespace smat {
@@ -74,15 +76,13 @@ __global__ __launch_bounds__(256) void decay_grad_kernel(const float* p0, const 
   const int h = blockIdx.x;
   const float* ps[3] = {p0, p1, p2};
   const int Ws[3] = {W0, W1, W2};
+  const int64_t batch = nb / heads;
   double x = 0;
-  for (int k = 0; k < 3; ++k) {
-    const int64_t n = (int64_t)nruns * (nb / heads) * Ws[k];
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-      const int64_t sn = i / Ws[k];                // run, batch
-      const int64_t run = sn / (nb / heads), b = sn % (nb / heads);
-      x += ps[k][(run * nb + b * heads + h) * Ws[k] + i % Ws[k]];
+  for (int k = 0; k < 3; ++k)
+    for (int64_t i = threadIdx.x; i < nruns * batch * Ws[k]; i += 256) {
+      const int64_t rb = i / Ws[k];                // run, batch
+      x += ps[k][(rb / batch * nb + rb % batch * heads + h) * Ws[k] + i % Ws[k]];
     }
-  }
   __shared__ double sum[256];
   sum[threadIdx.x] = x;
   __syncthreads();
@@ -113,7 +113,8 @@ static int carry(int dtype, const Walk& base, const float* init, float* E, float
   return launch_status("smat_head_decay_scan: carry");
 }
 
-static int check(const char* who, int dtype, const Walk& g, int nbk, int r, int p) {
+static int check(const char* who, int dtype, const Walk& g, int nbk, int r, int p,
+                 std::initializer_list<int64_t> rows) {
   SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
                "%s: unknown dtype %d", who, dtype);
   SMAT_REQUIRE(g.nb >= 0 && nbk >= 1 && g.heads >= 1 && g.T >= 0 && g.nseg >= 1 && g.nch >= 0,
@@ -121,6 +122,9 @@ static int check(const char* who, int dtype, const Walk& g, int nbk, int r, int 
                nbk, g.heads, g.T, g.nseg, g.nch);
   SMAT_REQUIRE(g.nb % nbk == 0 && g.nb % g.heads == 0, SMAT_EINVAL,
                "%s: nbk=%d and heads=%d must divide nb=%d", who, nbk, g.heads, g.nb);
+  for (int64_t st : rows)
+    SMAT_REQUIRE(g.T <= 1 || dl::near_rows(st), SMAT_EUNSUPPORTED,
+                 "%s: rows %lld elements apart, not 0 to 2^23", who, (long long)st);
   SMAT_REQUIRE(r >= kMinD && r <= kMaxD && p >= kMinD && p <= kMaxD, SMAT_EUNSUPPORTED,
                "%s: r=%d p=%d must lie in %d..%d", who, r, p, kMinD, kMaxD);
   if (g.chunks || g.runs || g.segrun) {
@@ -163,7 +167,7 @@ static Scratch take(dl::Arena& ar, int64_t nb, int64_t nbk, int64_t T, int nseg,
     c.dk = ar.take<float>(nb * T * r);
   }
   if (backward && learn)
-    for (float*& x : c.part) x = ar.take<float>(nruns * nb * 8);
+    for (float*& x : c.part) x = ar.take<float>(nruns * nb * kMaxWaves);
   return c;
 }
 
@@ -179,7 +183,7 @@ extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int3
   int longest = packed ? 0 : nch;
   for (int i = 0; packed && i < n; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
   if (longest < 1 || nb < 1 || r < 1 || p < 1) return 1;
-  const int slots = hd::waves_of(p) == 4 ? 512 : 256;
+  const int slots = 512;
   int best = longest;
   double least = 0;
   for (int G = 1; G <= 256 && (G == 1 || longest / G >= 2); ++G) {
@@ -229,7 +233,7 @@ extern "C" int smat_head_decay_scan(int dtype, const void* q, const void* k, con
   const char* who = "smat_head_decay_scan";
   Walk g = {chunks, runs, segrun, nb, T, nseg, nch, nruns, K, r, p};
   g.heads = heads;
-  int rc = check(who, dtype, g, nbk, r, p);
+  int rc = check(who, dtype, g, nbk, r, p, {q_st, k_st, v_st});
   if (rc) return rc;
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(logA && (nch == 0 || (q && k && v && out)), SMAT_EINVAL, "%s: null pointer", who);
@@ -275,7 +279,7 @@ extern "C" int smat_head_decay_scan_backward(
   const char* who = "smat_head_decay_scan_backward";
   Walk base = {chunks, runs, segrun, nb, T, nseg, nch, nruns, K, r, p};
   base.heads = heads;
-  int rc = check(who, dtype, base, nbk, r, p);
+  int rc = check(who, dtype, base, nbk, r, p, {q_st, k_st, v_st, d_st});
   if (rc) return rc;
   const bool learn = dlogA != nullptr;
   if (nb == 0) return SMAT_OK;
@@ -367,6 +371,7 @@ extern "C" int smat_head_decay_scan_backward(
   }
   if (learn)
     hipLaunchKernelGGL(decay_grad_kernel, dim3(heads), dim3(256), 0, st, sc.part[0], sc.part[1],
-                       sc.part[2], waves_of(p), waves_of(r), waves_of(r), nruns, nb, heads, dlogA);
+                       sc.part[2], learn_waves(p), learn_waves(r),
+                       learn_waves(r), nruns, nb, heads, dlogA);
   return launch_status(who);
 }

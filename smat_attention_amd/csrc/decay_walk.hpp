@@ -19,8 +19,8 @@
 // A walk backwards takes the tokens in turned order; then its in-chunk part is the forward
 // one's, and its factors are e_i = a^i, w_j = a^(n-j).
 //
-// The columns of the state do not mix, so a wave takes 16 of them with all key rows in
-// registers (fp32).  A workgroup has all columns of a sequence: its waves share the
+// The columns of the state do not mix, so a wave takes 16 or 32 of them with all key rows in
+// registers (fp32).  A workgroup has all columns of a sequence: its four waves share the
 // chunk's rows in LDS and one P = (Q K^T) o D, of which each forms a few tiles.
 //
 // Operands: every product runs on v_mfma_f32_16x16x32_bf16, values held in fewer than
@@ -81,89 +81,230 @@ struct Walk {
   float* part;             // LEARN: (nruns, nb, W)
 };
 
-// One operand's rows of a chunk on their way to LDS: loaded a chunk ahead into registers,
-// then written as a tile (delta_common.hpp), a tile a term.  B: 32-column blocks.
-template <typename In, int B, int W> struct Rows {
-  static constexpr int LC = 4 * B, RS = dl::row_chunks(B), UNITS = C * LC;
-  static constexpr int U = (UNITS + 64 * W - 1) / (64 * W);
-  Raw<In> x[U];
-
-  __device__ __forceinline__ static void place(int u, int& t, int& k) {
-    const int i = u * 64 * W + (int)threadIdx.x;
-    t = i / LC;
-    k = i % LC;
-  }
-  // base: the walk's first row of the chunk, st: to the next one in the walk's order.  Rows
-  // past the last are the last one's, and a group that would pass the row's end is read
-  // earlier in it (cols >= 8): every address lies in the operand.
-  __device__ __forceinline__ void load(const In* base, int64_t st, int len, int cols) {
+// fp32 values as three bf16 terms, exactly: each term takes the next eight bits, so none is
+// rounded up past the type's end.
+__device__ __forceinline__ Frag<kMid> cut(const f32x4& a, const f32x4& b) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  u4 t[kMid];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      int t, k;
-      place(u, t, k);
-      x[u].load(base + min(t, len - 1) * st + min(8 * k, cols - 8));
+  for (int q = 0; q < 4; ++q) {
+    float x = q < 2 ? a[2 * q] : b[2 * q - 4], y = q < 2 ? a[2 * q + 1] : b[2 * q - 3];
+#pragma unroll
+    for (int n = 0; n < kMid; ++n) {
+      const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+      t[n][q] = __builtin_amdgcn_perm(v, u, 0x07060302);     // the upper halves
+      if (n + 1 < kMid) {
+        x -= __uint_as_float(u & 0xffff0000u);
+        y -= __uint_as_float(v & 0xffff0000u);
+      }
     }
   }
-  __device__ __forceinline__ void put(bf16* tile, int len, int cols) {
-    const int over = cols & 7;
+  Frag<kMid> f;
+#pragma unroll
+  for (int n = 0; n < kMid; ++n) f.t[n] = __builtin_bit_cast(bf16x8, t[n]);
+  return f;
+}
+// For products with one-term operands, which keep every term; others drop products of low
+// terms, and rounded terms are half as large and of either sign.
+template <int NT> __device__ __forceinline__ Frag<kMid> terms(const f32x4& a, const f32x4& b) {
+  if constexpr (NT == 1)
+    return cut(a, b);
+  else
+    return dl::split<kMid>(a, b);
+}
+
+// A chunk's rows in LDS, 32 B columns of 16 bits: row t at t (64 B + 32) bytes, and 16 more in
+// every second eight rows.  That keeps both reads free of bank conflicts (64 banks, 32 lanes
+// a phase): rows of 16 bytes from 16 rows, and transposing ones of 32 bytes from 8 rows; and
+// every address is one a lane and constants.
+constexpr int pitch(int B) { return 32 * B + 16; }
+constexpr int tile_elems(int B) { return C * pitch(B); }
+__device__ __forceinline__ int row_at(int B, int t) { return t * pitch(B) + ((t >> 3) & 1) * 8; }
+
+// Rows fragment: token 16 mt + (lane & 15), the column slots of block kb (delta_common.hpp).
+template <int B, int N, typename T = bf16>
+__device__ __forceinline__ Frag<N> rows_of(const T* tile, int mt, int kb) {
+  const int m = lane_id() & 15, g = lane_id() >> 4;
+  const T* p = tile + row_at(B, m) + 4 * g + 16 * mt * pitch(B) + 32 * kb;
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const bf16x4 a = *reinterpret_cast<const bf16x4*>(p + n * tile_elems(B));
+    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p + n * tile_elems(B) + 16);
+    f.t[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// Transposed fragment: column 16 mt + (lane & 15), the token slots of block kb.  Lane 4 e + q
+// of each sixteen addresses token 4 (lane >> 4) + e, columns 4 q .. + 3.
+template <int B, int N>
+__device__ __forceinline__ Frag<N> cols_of(const bf16* tile, int mt, int kb) {
+  typedef short short4v __attribute__((ext_vector_type(4)));
+  const int r16 = lane_id() & 15, t = 4 * (lane_id() >> 4) + (r16 >> 2);
+  const bf16* p = tile + row_at(B, t) + 4 * (r16 & 3) + 16 * mt + 32 * kb * pitch(B);
+  Frag<N> f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    bf16x4 h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      h[i] = __builtin_bit_cast(
+          bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                      (__attribute__((address_space(3))) short4v*)(uintptr_t)(uint32_t)(uintptr_t)(
+                          p + n * tile_elems(B) + i * 16 * pitch(B))));
+    f.t[n] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  return f;
+}
+
+// A value that is new to the compiler here: what only a rare path needs of it is formed there,
+// and not kept in registers across the walk.
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// One operand's rows of a chunk on their way to LDS: loaded a chunk ahead into registers,
+// then written as a tile a term, or (V) as they are.  B: 32-column blocks.  A thread has the
+// same eight columns of every STEP-th row.
+template <typename In, int B, int W, bool RAW> struct Rows {
+  static constexpr int MIN = B == 1 ? 4 : B == 2 ? 8 : 16, LC = MIN < W ? W : MIN;
+  static constexpr int STEP = 64 * W / LC, U = C / STEP;
+  static_assert(STEP % 16 == 0 && U * STEP == C, "");
+  Raw<In> x[U];
+
+  __device__ __forceinline__ static int row(int tid = threadIdx.x) { return tid / LC; }
+  __device__ __forceinline__ static int group(int tid = threadIdx.x) { return tid % LC; }
+  // The lane's offset in bytes from a chunk's first row, sb bytes to the next one; turned order
+  // counts from the last of 64.  Columns past the end are read earlier in the row (cols >= 8).
+  __device__ __forceinline__ static uint32_t offset(uint32_t sb, int cols, bool rev) {
+    const int t = rev ? STEP - 1 - row() : row();
+    return t * sb + min(8 * group(), cols - 8) * (int)sizeof(In);
+  }
+  __device__ __forceinline__ void load(const char* base, uint32_t off, uint32_t sb, bool rev) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      x[u].load(reinterpret_cast<const In*>(base + (int64_t)((rev ? U - 1 - u : u) * STEP) * sb +
+                                            off));
+  }
+  // Of len < 64 rows: those past the last are the last one's, so every address lies in the
+  // operand.
+  __device__ __forceinline__ void load_part(const char* base, uint32_t sb, int len, int cols,
+                                            bool rev) {
+    const int tid = fresh((int)threadIdx.x);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      int t, k;
-      place(u, t, k);
-      if (UNITS % (64 * W) && t >= C) break;
+      const int t = min(u * STEP + row(tid), len - 1);
+      x[u].load(reinterpret_cast<const In*>(base + (int64_t)(rev ? len - 1 - t : t) * sb) +
+                min(8 * group(tid), cols - 8));
+    }
+  }
+  __device__ __forceinline__ void put(bf16* tile) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) put_one(u, tile, threadIdx.x);
+  }
+  __device__ __forceinline__ void put_part(bf16* tile, int len, int cols) {
+    const int tid = fresh((int)threadIdx.x), k = group(tid), over = cols & 7;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
       if (over && 8 * k + 8 > cols && 8 * k < cols) x[u].drop(8 - over);
-      if (t >= len || 8 * k >= cols) x[u].zero();
-      bf16* at = tile + (t * RS + (k ^ dl::swz<RS>(t))) * 8;
-      if constexpr (__is_same(In, bf16)) {
-        *reinterpret_cast<typename Raw<In>::u4*>(at) = x[u].x[0];
+      if (u * STEP + row(tid) >= len || 8 * k >= cols) x[u].zero();
+      put_one(u, tile, tid);
+    }
+  }
+  __device__ __forceinline__ void put_one(int u, bf16* tile, int tid) {
+    const int t = row(tid), k = group(tid);
+    if (LC > 4 * B && k >= 4 * B) return;
+    typedef typename Raw<In>::u4 u4;
+    if constexpr (RAW && sizeof(In) == 4) {
+      float* at = reinterpret_cast<float*>(tile) + (u * STEP + t) * (32 * B + 4) + 8 * k;
+      reinterpret_cast<u4*>(at)[0] = x[u].x[0];
+      reinterpret_cast<u4*>(at)[1] = x[u].x[1];
+    } else {
+      bf16* at = tile + row_at(B, t) + 8 * k + u * STEP * pitch(B);
+      if constexpr (RAW || __is_same(In, bf16)) {
+        *reinterpret_cast<u4*>(at) = x[u].x[0];
       } else {
         f32x4 a, b;
         x[u].values(a, b);
         const Frag<Terms<In>::in> f = dl::split<Terms<In>::in>(a, b);
 #pragma unroll
         for (int n = 0; n < Terms<In>::in; ++n)
-          *reinterpret_cast<bf16x8*>(at + n * dl::tile_elems(B)) = f.t[n];
+          *reinterpret_cast<bf16x8*>(at + n * tile_elems(B)) = f.t[n];
       }
     }
   }
 };
 
-template <int W> __device__ __host__ constexpr int value_blocks() { return W / 2; }
+// V's tile holds values as they come (fp32: rows of 32 B + 4 floats).  A lane's eight values of
+// a column, the token slots of block kb, and of a row (token 16 mt + lane & 15).
+template <typename In, int B>
+__device__ __forceinline__ void value_cols(const bf16* tile, int ct, int kb, f32x4& a, f32x4& b) {
+  if constexpr (sizeof(In) == 4) {
+    const float* p = reinterpret_cast<const float*>(tile) +
+                     (32 * kb + 4 * (lane_id() >> 4)) * (32 * B + 4) + 16 * ct + (lane_id() & 15);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = p[i * (32 * B + 4)];
+      b[i] = p[(16 + i) * (32 * B + 4)];
+    }
+  } else {
+    Raw<In> x;
+    x.x[0] = __builtin_bit_cast(typename Raw<In>::u4, cols_of<B, 1>(tile, ct, kb).t[0]);
+    x.values(a, b);
+  }
+}
+template <typename In, int B>
+__device__ __forceinline__ Frag<Terms<In>::in> value_rows(const bf16* tile, int mt, int kb) {
+  if constexpr (__is_same(In, bf16)) {
+    return rows_of<B, 1>(tile, mt, kb);
+  } else {
+    f32x4 a, b;
+    if constexpr (sizeof(In) == 4) {
+      const float* p = reinterpret_cast<const float*>(tile) +
+                       (16 * mt + (lane_id() & 15)) * (32 * B + 4) + 32 * kb + 4 * (lane_id() >> 4);
+      a = *reinterpret_cast<const f32x4*>(p);
+      b = *reinterpret_cast<const f32x4*>(p + 16);
+    } else {
+      Raw<In> x;
+      x.x[0] = __builtin_bit_cast(typename Raw<In>::u4, rows_of<B, 1>(tile, mt, kb).t[0]);
+      x.values(a, b);
+    }
+    return dl::split<Terms<In>::in>(a, b);
+  }
+}
 
-// Elements of a set of tiles, Q (where there are outputs), K and V, and bytes of LDS.
-template <typename In, int RB, int W, bool OUT> constexpr int set_elems() {
-  return Terms<In>::in *
-         ((OUT ? 2 : 1) * dl::tile_elems(RB) + dl::tile_elems(value_blocks<W>()));
+// The column tiles of a wave and the waves of a workgroup, by the columns of all (64 or 128):
+// two tiles a wave share the reads of K, Q and P; with LEARN they would not fit the registers.
+template <int P, bool LEARN> constexpr int tiles() { return P == 64 || LEARN ? 1 : 2; }
+template <int P, bool LEARN> constexpr int waves() { return P / 16 / tiles<P, LEARN>(); }
+constexpr int kMaxWaves = 8;
+template <typename In, int P> constexpr int value_elems() {
+  return sizeof(In) == 4 ? 2 * C * (P + 4) : tile_elems(P / 32);
+}
+template <typename In, int RB, int P, bool OUT> constexpr int set_elems() {
+  return Terms<In>::in * (OUT ? 2 : 1) * tile_elems(RB) + value_elems<In, P>();
 }
 constexpr int kTab = C + 4 + 2 * C;   // floats: a^0 .. a^64; the update's factors, zeros behind
-template <typename In, int RB, int W, bool OUT> constexpr int walk_lds(int KD) {
-  return KD * set_elems<In, RB, W, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) +
-         kTab * 4;
+template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets) {
+  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) + kTab * 4;
 }
-// Two sets, so that the next chunk's rows are written beside this one's use, where that
-// fits half (W = 4) or all of a CU's LDS.
-template <typename In, int RB, int W, bool OUT> constexpr int walk_sets() {
-  return walk_lds<In, RB, W, OUT>(2) <= (W == 4 ? dl::kMaxLds / 2 : dl::kMaxLds) ? 2 : 1;
+// Waves a SIMD: as many as registers and LDS have room for.
+template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_occ() {
+  const int fit = dl::kMaxLds / walk_lds<In, RB, P, OUT>(1) * waves<P, LEARN>() / 4;
+  const int most = LEARN ? 2 : !OUT ? (P == 64 ? 4 : RB > 2 ? 2 : 3) : P == 64 && RB < 3 ? 3 : 2;
+  return fit < most ? fit : most;
 }
-
-// Rows fragment of a tile at a row tile known at run time only.
-template <int B, int N>
-__device__ __forceinline__ Frag<N> row_frag(const bf16* tile, int mt, int kb) {
-  constexpr int RS = dl::row_chunks(B);
-  const int m = lane_id() & 15, g = lane_id() >> 4;
-  const int k0 = (4 * kb + (g >> 1)) ^ dl::swz<RS>(m), k1 = (4 * kb + 2 + (g >> 1)) ^ dl::swz<RS>(m);
-  const bf16* p = tile + (16 * mt + m) * RS * 8 + 4 * (g & 1);
-  Frag<N> f;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const bf16x4 a = *reinterpret_cast<const bf16x4*>(p + n * dl::tile_elems(B) + k0 * 8);
-    const bf16x4 b = *reinterpret_cast<const bf16x4*>(p + n * dl::tile_elems(B) + k1 * 8);
-    f.t[n] = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-  }
-  return f;
+// Two sets, so that the next chunk's rows are written beside this one's use, where that many
+// still fit.
+template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_sets() {
+  return walk_lds<In, RB, P, OUT>(2) * walk_occ<In, RB, P, OUT, LEARN>() * 4 /
+                     waves<P, LEARN>() <= dl::kMaxLds ? 2 : 1;
 }
 
-// The same fragment from the caller's rows: row tile mt of the chunk, 32-column block kb.
+// A rows fragment from the caller's rows: row tile mt of the chunk (in the walk's order),
+// 32-column block kb.
 template <typename In>
 __device__ __forceinline__ Frag<Terms<In>::in> global_frag(const In* base, int64_t st, int len,
                                                            int cols, int mt, int kb) {
@@ -181,17 +322,6 @@ __device__ __forceinline__ Frag<Terms<In>::in> global_frag(const In* base, int64
   return dl::split<Terms<In>::in>(h[0], h[1]);
 }
 
-template <int N> __device__ __forceinline__ void values_of(const Frag<N>& f, f32x4& a, f32x4& b) {
-  a = b = zero4();
-#pragma unroll
-  for (int n = N - 1; n >= 0; --n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] += to_f32(f.t[n][i]);
-      b[i] += to_f32(f.t[n][i + 4]);
-    }
-}
-
 // A product rounded here, not fused into what reads it: results keep their bits whichever
 // variant of the kernel forms them.
 __device__ __forceinline__ f32x4 rounded(f32x4 x) {
@@ -204,11 +334,28 @@ __device__ __forceinline__ void tile_of(int i, int& mt, int& jt) {
   jt = i - mt * (mt + 1) / 2;
 }
 
-template <typename In, int RB, int W, bool OUT, bool LEARN>
-__global__ __launch_bounds__(64 * W, 2) void decay_walk_kernel(Walk g) {
-  constexpr int NT = Terms<In>::in, NI = kMid, VB = value_blocks<W>();
-  constexpr int KT = NT * dl::tile_elems(RB), SET = set_elems<In, RB, W, OUT>();
-  constexpr int KD = walk_sets<In, RB, W, OUT>(), TP = (kTiles + W - 1) / W;
+// Steps whose operands come from LDS: AHEAD issues the next step's reads before a step's
+// products, and keeps them there; else they come as the compiler likes (several terms: registers).
+template <int STEPS, bool AHEAD, typename Buf, typename Load, typename Use>
+__device__ __forceinline__ void steps(Load load, Use use) {
+  if constexpr (AHEAD) {
+    dl::pipelined<STEPS, Buf>(load, use);
+  } else {
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+      Buf b;
+      load(st, b);
+      use(st, b);
+    }
+  }
+}
+
+template <typename In, int RB, int P, bool OUT, bool LEARN>
+__global__ __launch_bounds__((64 * waves<P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void decay_walk_kernel(
+    Walk g) {
+  constexpr int W = waves<P, LEARN>(), CT = tiles<P, LEARN>(), NT = Terms<In>::in, NI = kMid, VB = P / 32;
+  constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>(), SET = set_elems<In, RB, P, OUT>();
+  constexpr int KD = walk_sets<In, RB, P, OUT, LEARN>(), TP = (kTiles + W - 1) / W;
   extern __shared__ __align__(1024) bf16 lds[];
   bf16* pl = lds + KD * SET;
   float* tab = reinterpret_cast<float*>(pl + (OUT ? NI * kLow * kFrag : 0));   // a^0 .. a^64
@@ -229,19 +376,54 @@ __global__ __launch_bounds__(64 * W, 2) void decay_walk_kernel(Walk g) {
     dl::run_of(geo, blockIdx.y, run, c0, c1, seg, head, tail);
   }
   if (!OUT && (g.rev ? head : tail)) return;       // no run follows it
-  auto chunk_at = [&](int i, int& t0, int& len) {
-    const int c = g.rev ? c1 - 1 - i : c0 + i;
-    if (g.chunks) {
-      t0 = g.chunks[2 * c];
-      len = g.chunks[2 * c + 1];
+  const int chunks = c1 - c0, tile0 = w * CT;      // the wave's first column tile
+  const int64_t sn = (int64_t)run * g.nb + s, rp = (int64_t)g.r * g.p;
+  // a run's chunks lie one behind the other, all but its last whole
+  int begin = 0, end = 0;
+  if (chunks > 0) {
+    begin = g.chunks ? g.chunks[2 * c0] : c0 * C;
+    end = g.chunks ? g.chunks[2 * c1 - 2] + g.chunks[2 * c1 - 1] : min(c1 * C, g.T);
+  }
+  Rows<In, RB, W, false> rq, rk;
+  Rows<In, VB, W, true> rv;
+  constexpr uint32_t EB = sizeof(In);
+  const uint32_t qb = (uint32_t)g.q.st * EB, kb_ = (uint32_t)g.k.st * EB, vb_ = (uint32_t)g.v.st * EB;
+  auto rows_at = [&](const Side& x, int t) {
+    return (const char*)x.p + (s / x.div * x.sb + (int64_t)t * x.st) * EB;
+  };
+  const char *qp = rows_at(g.q, begin), *kp = rows_at(g.k, begin), *vp = rows_at(g.v, begin);
+  const uint32_t qo = rq.offset(qb, g.r, g.rev), ko = rk.offset(kb_, g.r, g.rev),
+                 vo = rv.offset(vb_, g.p, g.rev);
+  // chunk i of the walk: its first token from the run's, its tokens
+  auto first_of = [&](int i) { return (g.rev ? chunks - 1 - i : i) * C; };
+  auto load = [&](int i) {
+    const int64_t t = first_of(i);
+    const int len = min(C, end - begin - (int)t);
+    if (len == C) {
+      if (OUT) rq.load(qp + t * qb, qo, qb, g.rev);
+      rk.load(kp + t * kb_, ko, kb_, g.rev);
+      rv.load(vp + t * vb_, vo, vb_, g.rev);
     } else {
-      t0 = c * C;
-      len = min(C, g.T - t0);
+      if (OUT) rq.load_part(qp + t * qb, qb, len, g.r, g.rev);
+      rk.load_part(kp + t * kb_, kb_, len, g.r, g.rev);
+      rv.load_part(vp + t * vb_, vb_, len, g.p, g.rev);
     }
   };
-  const int chunks = c1 - c0, col = 16 * w + m;
-  const bool on = 16 * w < g.p;                    // else: copies, tiles of P and barriers only
-  const int64_t sn = (int64_t)run * g.nb + s, rp = (int64_t)g.r * g.p;
+  const bool full = g.r == 32 * RB && g.p == 32 * VB;
+  auto put = [&](int i) {
+    bf16* set = lds + (KD == 2 ? (i & 1) * SET : 0);
+    const int len = min(C, end - begin - first_of(i));
+    if (full && len == C) {
+      rk.put(set);
+      rv.put(set + KT);
+      if (OUT) rq.put(set + KT + VT);
+    } else {
+      rk.put_part(set, len, g.r);
+      rv.put_part(set + KT, len, g.p);
+      if (OUT) rq.put_part(set + KT + VT, len, g.r);
+    }
+  };
+  if (chunks > 0) load(0);
   {
     // powers from 64 bits: a^i is then rounded once, however long the product
     const double la = g.logA[s % g.heads];
@@ -252,45 +434,20 @@ __global__ __launch_bounds__(64 * W, 2) void decay_walk_kernel(Walk g) {
       wt[i] = i < C ? (e == 0 ? 1.f : (float)exp(la * e)) * g.upd : 0.f;
     }
   }
-  f32x4 S[2 * RB];
+  // element i of S[ct][mt]: row 16 mt + 4 gq + i of column 16 (tile0 + ct) + m
+  f32x4 S[CT][2 * RB];
 #pragma unroll
-  for (int mt = 0; mt < 2 * RB; ++mt)
+  for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int a = 16 * mt + 4 * gq + i;
-      S[mt][i] = g.start && a < g.r && col < g.p
-                     ? g.start[sn * rp + (int64_t)a * g.s_row + (int64_t)col * g.s_col]
-                     : 0.f;
-    }
-  const In *qs = (const In*)g.q.p + s / g.q.div * g.q.sb, *ks = (const In*)g.k.p + s / g.k.div * g.k.sb,
-           *vs = (const In*)g.v.p + s / g.v.div * g.v.sb;
-  auto first_row = [&](const In* p, int64_t st, int t0, int len) {
-    return p + (int64_t)(g.rev ? t0 + len - 1 : t0) * st;
-  };
-  auto step_of = [&](int64_t st) { return g.rev ? -st : st; };
-  Rows<In, RB, W> rq, rk;
-  Rows<In, VB, W> rv;
-  auto load = [&](int t0, int len) {
-    if (OUT) rq.load(first_row(qs, g.q.st, t0, len), step_of(g.q.st), len, g.r);
-    rk.load(first_row(ks, g.k.st, t0, len), step_of(g.k.st), len, g.r);
-    rv.load(first_row(vs, g.v.st, t0, len), step_of(g.v.st), len, g.p);
-  };
-  auto put = [&](bf16* set, int len) {
-    rk.put(set, len, g.r);
-    rv.put(set + KT, len, g.p);
-    if (OUT) rq.put(set + KT + NT * dl::tile_elems(VB), len, g.r);
-  };
-  int t0 = 0, len = 0;
-  if (chunks > 0) {
-    chunk_at(0, t0, len);
-    load(t0, len);
-    put(lds, len);
-  }
-  Frag<NI> sb[OUT ? RB : 1];                       // S as the next product's operand
-  if (OUT) {
+    for (int mt = 0; mt < 2 * RB; ++mt)
 #pragma unroll
-    for (int kb = 0; kb < RB; ++kb) sb[kb] = dl::split<NI>(S[2 * kb], S[2 * kb + 1]);
-  }
+      for (int i = 0; i < 4; ++i) {
+        const int a = 16 * mt + 4 * gq + i, col = 16 * (tile0 + ct) + m;
+        S[ct][mt][i] = g.start && a < g.r && col < g.p
+                           ? g.start[sn * rp + (int64_t)a * g.s_row + (int64_t)col * g.s_col]
+                           : 0.f;
+      }
+  if (chunks > 0) put(0);
   lds_barrier();
   float e[4];
   f32x4 D[OUT ? TP : 1];
@@ -309,131 +466,144 @@ __global__ __launch_bounds__(64 * W, 2) void decay_walk_kernel(Walk g) {
     }
   }
   float acc = 0.f;                                 // LEARN: this lane's part of the gradient
+  const In* xs = LEARN ? (const In*)g.x.p + s / g.x.div * g.x.sb : nullptr;
+  const int64_t x_st = g.rev ? -g.x.st : g.x.st;
 
   for (int c = 0; c < chunks; ++c) {
     bf16* set = lds + (KD == 2 ? (c & 1) * SET : 0);
-    const bf16 *kt = set, *vt = set + KT, *qt = vt + NT * dl::tile_elems(VB);
+    const bf16 *kt = set, *vt = set + KT, *qt = vt + VT;
     const bool more = c + 1 < chunks;
-    int t1 = t0, len1 = len;
+    const int t0 = begin + first_of(c), len = min(C, end - t0);
     if (c > 0) lds_barrier();
     // ---- the chunk's rows are in LDS
-    if (more) {
-      chunk_at(c + 1, t1, len1);
-      load(t1, len1);
-    }
+    if (more) load(c + 1);
     const float aC = tab[len];
-    f32x4 ot[OUT ? 4 : 1];
+    const In* xrow = LEARN ? xs + (int64_t)(g.rev ? t0 + len - 1 : t0) * g.x.st : nullptr;
+    f32x4 ot[OUT ? CT : 1][OUT ? 4 : 1];
     if constexpr (OUT) {
+      if (g.save_s) {
+        f32x4* to = reinterpret_cast<f32x4*>(g.save_s) +
+                    (((int64_t)s * g.nch + c0 + c) * W + w) * (CT * 2 * RB * 64) + lane_id();
 #pragma unroll
-      for (int u = 0; u < TP; ++u) {
-        if (w + u * W >= kTiles) break;
-        int mt, jt;
-        tile_of(w + u * W, mt, jt);
-        // transposed: rows are tokens j, columns i
-        f32x4 x = zero4();
-#pragma unroll
-        for (int kb = 0; kb < RB; ++kb)
-          x = dl::mul_inputs(x, row_frag<RB, NT>(kt, jt, kb), row_frag<RB, NT>(qt, mt, kb));
-        x = rounded(x * D[u]);
-        if constexpr (LEARN) {
-          if (g.learn == kDq) {                    // here i: dO, j: V; and V's place has K
-            const In* xs = (const In*)g.x.p + s / g.x.div * g.x.sb;
-            f32x4 z = zero4();
-            for (int kb = 0; kb < VB; ++kb)
-              z = dl::mul_inputs(z, row_frag<VB, NT>(vt, jt, kb),
-                                 global_frag(first_row(xs, g.x.st, t0, len), step_of(g.x.st), len,
-                                             g.p, mt, kb));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              acc += (float)(16 * (mt - jt) + m - 4 * gq - i) * (x[i] * z[i]);
-          }
-        }
-        const Frag<NI> f = dl::split<NI>(x, zero4());
-        const int half = mt == 2 && jt == 2 ? 1 : jt & 1;
-        bf16* at = pl + dl::tri(mt, jt >> 1) * kFrag + lane_id() * 8 + 4 * half;
-#pragma unroll
-        for (int n = 0; n < NI; ++n)
-          *reinterpret_cast<bf16x4*>(at + n * kLow * kFrag) = dl::low_half(f.t[n]);
+        for (int i = 0; i < CT * 2 * RB; ++i) to[i * 64] = S[i / (2 * RB)][i % (2 * RB)];
       }
-      if (on) {
-        if (g.save_s) {
-          f32x4* to = reinterpret_cast<f32x4*>(g.save_s) +
-                      (((int64_t)s * g.nch + c0 + c) * W + w) * (2 * RB * 64) + lane_id();
+      // tiles of P, transposed: rows are tokens j, columns i (the last ones twice: no branch)
+      struct Pair {
+        Frag<NT> k[RB], q[RB];
+      };
+      steps<TP, NT == 1, Pair>(
+          [&](int u, Pair& b) {
+            int mt, jt;
+            tile_of(min(w + u * W, kTiles - 1), mt, jt);
 #pragma unroll
-          for (int mt = 0; mt < 2 * RB; ++mt) to[mt * 64] = S[mt];
-        }
-        // (Q S)^T: columns in registers, the token in the lane
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) ot[mt] = zero4();
-#pragma unroll
-        for (int kb = 0; kb < RB; ++kb)
-#pragma unroll
-          for (int mt = 0; mt < 4; ++mt)
-            ot[mt] = dl::mul(ot[mt], sb[kb], dl::rows_of<RB, NT>(qt, mt, kb));
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) ot[mt] = rounded(ot[mt] * e[mt]);
-        if constexpr (LEARN) {
-          if (g.learn == kDq || g.learn == kDk) {  // (i + 1) q . dq, and i k . dk in turned order
-            const In* xs = (const In*)g.x.p + s / g.x.div * g.x.sb;
-            const In* base = first_row(xs, g.x.st, t0, len);
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-              const int t = 16 * mt + m;
-              const In* row = base + min(t, len - 1) * step_of(g.x.st);
-              float dot = 0.f;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int cc = 16 * w + 4 * gq + i;
-                const float x = to_f32(row[min(cc, g.p - 1)]);
-                dot += cc < g.p ? x * ot[mt][i] : 0.f;
-              }
-              if (t < len) acc += (float)(t + (g.rev ? 0 : 1)) * dot;
+            for (int kb = 0; kb < RB; ++kb) {
+              b.k[kb] = rows_of<RB, NT>(kt, jt, kb);
+              b.q[kb] = rows_of<RB, NT>(qt, mt, kb);
             }
-          } else if (g.learn == kDv) {             // n a^n <S, Y>
-            const f32x4* from = reinterpret_cast<const f32x4*>(g.load_s) +
-                                (((int64_t)s * g.nch + c1 - 1 - c) * W + w) * (2 * RB * 64) +
-                                lane_id();
+          },
+          [&](int u, Pair& b) {
+            int mt, jt;
+            tile_of(min(w + u * W, kTiles - 1), mt, jt);
+            f32x4 x = zero4();
+#pragma unroll
+            for (int kb = 0; kb < RB; ++kb) x = dl::mul_inputs(x, b.k[kb], b.q[kb]);
+            x = rounded(x * D[u]);
+            if constexpr (LEARN) {
+              if (g.learn == kDq && w + u * W < kTiles) {   // here i: dO, j: V; K in V's place
+                f32x4 z = zero4();
+                for (int kb = 0; kb < VB; ++kb)
+                  z = dl::mul_inputs(z, value_rows<In, VB>(vt, jt, kb),
+                                     global_frag(xrow, x_st, len, g.p, mt, kb));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  acc += (float)(16 * (mt - jt) + m - 4 * gq - i) * (x[i] * z[i]);
+              }
+            }
+            const Frag<NI> f = terms<NT>(x, zero4());
+            const int half = mt == 2 && jt == 2 ? 1 : jt & 1;
+            bf16* at = pl + dl::tri(mt, jt >> 1) * kFrag + lane_id() * 8 + 4 * half;
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+              *reinterpret_cast<bf16x4*>(at + n * kLow * kFrag) = dl::low_half(f.t[n]);
+          });
+      // (Q S)^T: columns in registers, the token in the lane
+#pragma unroll
+      for (int i = 0; i < CT * 4; ++i) ot[i / 4][i % 4] = zero4();
+      struct Four {
+        Frag<NT> q[4];
+      };
+      steps<RB, NT == 1, Four>(
+          [&](int kb, Four& b) {
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) b.q[mt] = rows_of<RB, NT>(qt, mt, kb);
+          },
+          [&](int kb, Four& b) {
+            Frag<NI> sb[CT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) sb[ct] = terms<NT>(S[ct][2 * kb], S[ct][2 * kb + 1]);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              Frag<NI> all[4];
+#pragma unroll
+              for (int mt = 0; mt < 4; ++mt) all[mt] = sb[ct];
+              dl::mul_each(ot[ct], all, b.q);
+            }
+          });
+#pragma unroll
+      for (int i = 0; i < CT * 4; ++i) ot[i / 4][i % 4] = rounded(ot[i / 4][i % 4] * e[i % 4]);
+      if constexpr (LEARN) {
+        if (g.learn == kDq || g.learn == kDk) {    // (i + 1) q . dq, and i k . dk in turned order
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            const int t = 16 * mt + m;
+            const In* row = xrow + min(t, len - 1) * x_st;
             float dot = 0.f;
 #pragma unroll
-            for (int mt = 0; mt < 2 * RB; ++mt) {
-              const f32x4 x = from[mt * 64];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) dot += x[i] * S[mt][i];
+            for (int i = 0; i < CT * 4; ++i) {
+              const int cc = 16 * (tile0 + i / 4) + 4 * gq + i % 4;
+              const float x = to_f32(row[min(cc, g.p - 1)]);
+              dot += cc < g.p ? x * ot[i / 4][mt][i % 4] : 0.f;
             }
-            acc += (float)len * aC * dot;
+            if (t < len) acc += (float)(t + (g.rev ? 0 : 1)) * dot;
           }
+        } else if (g.learn == kDv) {               // n a^n <S, Y>
+          const f32x4* from = reinterpret_cast<const f32x4*>(g.load_s) +
+                              (((int64_t)s * g.nch + c1 - 1 - c) * W + w) * (CT * 2 * RB * 64) +
+                              lane_id();
+          float dot = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < CT * 2 * RB; ++mt) {
+            const f32x4 x = from[mt * 64];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot += x[i] * S[mt / (2 * RB)][mt % (2 * RB)][i];
+          }
+          acc += (float)len * aC * dot;
         }
       }
+    }
+    // the wave's columns of V by token slots: what P meets
+    Frag<NT> vf[OUT || NT == 1 ? CT : 1][2];
+    if constexpr (OUT || NT == 1) {
+#pragma unroll
+      for (int i = 0; i < CT * 2; ++i) {
+        if constexpr (NT == 1) {
+          vf[i / 2][i % 2] = cols_of<VB, 1>(vt, tile0 + i / 2, i % 2);
+        } else {
+          f32x4 a, b;
+          value_cols<In, VB>(vt, tile0 + i / 2, i % 2, a, b);
+          vf[i / 2][i % 2] = dl::split<NT>(a, b);
+        }
+      }
+    }
+    if constexpr (OUT) {
       lds_barrier();
       // ---- P is in LDS
-    }
-    if (on) {
-      Frag<NT> vf[2];
-      Frag<NI> f[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        vf[kb] = dl::cols_of<VB, NT>(vt, w, kb);
-        f32x4 a, b, wa, wb;
-        values_of(vf[kb], a, b);
-        const float* wp = wt + C - len + 32 * kb + 4 * gq;
-        if (len == C) {
-          wa = *reinterpret_cast<const f32x4*>(wp);
-          wb = *reinterpret_cast<const f32x4*>(wp + 16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            wa[i] = wp[i];
-            wb[i] = wp[16 + i];
-          }
-        }
-        f[kb] = dl::split<NI>(rounded(wa * a), rounded(wb * b));
-      }
-      if constexpr (OUT) {
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-          for (int kb = 0; kb <= mt / 2; ++kb) {
-            Frag<NI> pf;
+      struct One {
+        Frag<NI> p;
+      };
+      steps<6, NT == 1, One>(
+          [&](int st, One& b) {
+            const int mt = st < 2 ? st : st < 4 ? 2 : 3, kb = st < 2 ? 0 : st & 1;
             const bf16* at = pl + dl::tri(mt, kb) * kFrag + lane_id() * 8;
 #pragma unroll
             for (int n = 0; n < NI; ++n) {
@@ -441,110 +611,175 @@ __global__ __launch_bounds__(64 * W, 2) void decay_walk_kernel(Walk g) {
                 const bf16x4 h =
                     *reinterpret_cast<const bf16x4*>(at + n * kLow * kFrag + (mt == 2 ? 4 : 0));
                 const bf16x4 no = {(bf16)0.f, (bf16)0.f, (bf16)0.f, (bf16)0.f};
-                pf.t[n] = __builtin_shufflevector(h, no, 0, 1, 2, 3, 4, 5, 6, 7);
+                b.p.t[n] = __builtin_shufflevector(h, no, 0, 1, 2, 3, 4, 5, 6, 7);
               } else {
-                pf.t[n] = *reinterpret_cast<const bf16x8*>(at + n * kLow * kFrag);
+                b.p.t[n] = *reinterpret_cast<const bf16x8*>(at + n * kLow * kFrag);
               }
             }
-            ot[mt] = dl::mul(ot[mt], vf[kb], pf);
-          }
-        const int c4 = 16 * w + 4 * gq;
+          },
+          [&](int st, One& b) {
+            const int mt = st < 2 ? st : st < 4 ? 2 : 3, kb = st < 2 ? 0 : st & 1;
+            f32x4 x[CT];
+            Frag<NT> v[CT];
+            Frag<NI> all[CT];
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          const int t = 16 * mt + m;
-          if (t >= len || c4 >= g.p) continue;
-          const int64_t at = ((int64_t)s * g.T + (g.rev ? t0 + len - 1 - t : t0 + t)) * g.p + c4;
-          auto store = [&](auto* o) {
-            typedef typename std::remove_pointer<decltype(o)>::type Out;
-            typedef Out out4u __attribute__((ext_vector_type(4), aligned(sizeof(Out))));
-            if (c4 + 4 <= g.p) {
-              out4u y;
-#pragma unroll
-              for (int i = 0; i < 4; ++i) y[i] = from_f32<Out>(ot[mt][i]);
-              *reinterpret_cast<out4u*>(o + at) = y;
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (c4 + i < g.p) o[at + i] = from_f32<Out>(ot[mt][i]);
+            for (int ct = 0; ct < CT; ++ct) {
+              x[ct] = ot[ct][mt];
+              v[ct] = vf[ct][kb];
+              all[ct] = b.p;
             }
-          };
-          if (!__is_same(In, float) && g.wide)
-            store((float*)g.o);
-          else
-            store((In*)g.o);
+            dl::mul_each(x, v, all);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) ot[ct][mt] = x[ct];
+          });
+      auto store = [&](auto* o) {
+        typedef typename std::remove_pointer<decltype(o)>::type Out;
+        typedef Out out4u __attribute__((ext_vector_type(4), aligned(sizeof(Out))));
+        // the chunk's lowest row, the lane's place in a row tile from its lowest
+        char* base = reinterpret_cast<char*>(o + ((int64_t)s * g.T + t0 + (g.rev ? len - C : 0)) *
+                                                     g.p + 16 * tile0);
+        const int lane = fresh(lane_id()), m = lane & 15, gq = lane >> 4;
+        const uint32_t at = ((g.rev ? 15 - m : m) * g.p + 4 * gq) * (uint32_t)sizeof(Out);
+        const int tile = 16 * g.p * (int)sizeof(Out);
+        auto row = [&](int mt) {
+          return reinterpret_cast<Out*>(base + (g.rev ? 3 - mt : mt) * tile + at);
+        };
+        if (full && len == C) {
+#pragma unroll
+          for (int i = 0; i < CT * 4; ++i) {
+            out4u y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = from_f32<Out>(ot[i % CT][i / CT][j]);
+            *reinterpret_cast<out4u*>(row(i / CT) + 16 * (i % CT)) = y;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < CT * 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (16 * (i / CT) + m < len && 16 * (tile0 + i % CT) + 4 * gq + j < g.p)
+                row(i / CT)[16 * (i % CT) + j] = from_f32<Out>(ot[i % CT][i / CT][j]);
+        }
+      };
+      if (!__is_same(In, float) && g.wide)
+        store((float*)g.o);
+      else
+        store((In*)g.o);
+    }
+    // S <- a^n S + K^T (w V), half the tokens at a time
+#pragma unroll
+    for (int i = 0; i < CT * 2 * RB; ++i) S[i / (2 * RB)][i % (2 * RB)] *= aC;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x4 wa, wb;
+      const float* wp = wt + C - len + 32 * kb + 4 * gq;
+      if (len == C) {
+        wa = *reinterpret_cast<const f32x4*>(wp);
+        wb = *reinterpret_cast<const f32x4*>(wp + 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          wa[i] = wp[i];
+          wb[i] = wp[16 + i];
         }
       }
-      // S <- a^n S + K^T (w V)
+      Frag<NI> f[CT];
 #pragma unroll
-      for (int mt = 0; mt < 2 * RB; ++mt) {
-        f32x4 x = S[mt] * aC;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) x = dl::mul(x, dl::cols_of<RB, NT>(kt, mt, kb), f[kb]);
-        S[mt] = x;
+      for (int ct = 0; ct < CT; ++ct) {
+        f32x4 a, b;
+        if constexpr (NT == 1) {
+          Raw<bf16> x;
+          x.x[0] = __builtin_bit_cast(Raw<bf16>::u4, vf[ct][kb].t[0]);
+          x.values(a, b);
+        } else {
+          value_cols<In, VB>(vt, tile0 + ct, kb, a, b);
+        }
+        f[ct] = terms<NT>(rounded(wa * a), rounded(wb * b));
       }
-      if constexpr (OUT) {
+      constexpr int U = NT == 1 ? 2 : 1;
+      struct Some {
+        Frag<NT> k[U];
+      };
+      steps<2 * RB / U, NT == 1, Some>(
+          [&](int st, Some& b) {
 #pragma unroll
-        for (int kb = 0; kb < RB; ++kb) sb[kb] = dl::split<NI>(S[2 * kb], S[2 * kb + 1]);
-      }
+            for (int u = 0; u < U; ++u) b.k[u] = cols_of<RB, NT>(kt, st * U + u, kb);
+          },
+          [&](int st, Some& b) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+              f32x4 x[U];
+              Frag<NI> all[U];
+#pragma unroll
+              for (int u = 0; u < U; ++u) {
+                x[u] = S[ct][st * U + u];
+                all[u] = f[ct];
+              }
+              dl::mul_each(x, b.k, all);
+#pragma unroll
+              for (int u = 0; u < U; ++u) S[ct][st * U + u] = x[u];
+            }
+          });
     }
     if (more) {
       if (KD == 1) lds_barrier();                  // the tiles are read
-      put(lds + (KD == 2 ? ((c + 1) & 1) * SET : 0), len1);
+      put(c + 1);
     }
-    t0 = t1;
-    len = len1;
   }
   if (LEARN && g.learn) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) acc += __shfl_xor(acc, d);
     if (lane_id() == 0) g.part[sn * W + w] = acc;
   }
-  if (!on || !g.fin || (OUT && !(g.rev ? head : tail))) return;
+  if (!g.fin || (OUT && !(g.rev ? head : tail))) return;
   float* out = g.fin + (OUT ? (int64_t)seg * g.nb + s : sn) * rp;
+  const int lane = fresh(lane_id());
 #pragma unroll
-  for (int mt = 0; mt < 2 * RB; ++mt)
+  for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int a = 16 * mt + 4 * gq + i;
-      if (a < g.r && col < g.p)
-        out[(int64_t)a * g.s_row + (int64_t)col * g.s_col] = S[mt][i];
-    }
+    for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int a = 16 * mt + 4 * (lane >> 4) + i, col = 16 * (tile0 + ct) + (lane & 15);
+        if (a < g.r && col < g.p)
+          out[(int64_t)a * g.s_row + (int64_t)col * g.s_col] = S[ct][mt][i];
+      }
 }
 
-inline int waves_of(int p) { return p <= 64 ? 4 : 8; }
+inline int learn_waves(int p) { return p <= 64 ? waves<64, true>() : waves<128, true>(); }
 
-template <typename In, int RB, int W, bool OUT, bool LEARN>
+template <typename In, int RB, int P, bool OUT, bool LEARN>
 static void walk(const Walk& g, hipStream_t st) {
-  constexpr int lds = walk_lds<In, RB, W, OUT>(walk_sets<In, RB, W, OUT>());
+  constexpr int lds = walk_lds<In, RB, P, OUT>(walk_sets<In, RB, P, OUT, LEARN>());
   static_assert(lds <= dl::kMaxLds, "");
-  auto kern = decay_walk_kernel<In, RB, W, OUT, LEARN>;
+  auto kern = decay_walk_kernel<In, RB, P, OUT, LEARN>;
   static uint64_t done;
   dl::allow_lds(kern, lds, done);
-  hipLaunchKernelGGL(kern, dim3(g.nb, g.nruns), dim3(64 * W), lds, st, g);
+  hipLaunchKernelGGL(kern, dim3(g.nb, g.nruns), dim3(64 * waves<P, LEARN>()), lds, st, g);
 }
 
 // One file a type instantiates it.
 template <typename In> int launch_walk(const Walk& g, bool out, hipStream_t st) {
-  auto go = [&](auto rb, auto wv) {
-    constexpr int RB = decltype(rb)::value, W = decltype(wv)::value;
+  auto go = [&](auto rb, auto cols) {
+    constexpr int RB = decltype(rb)::value, P = decltype(cols)::value;
     if (!out)
-      walk<In, RB, W, false, false>(g, st);
+      walk<In, RB, P, false, false>(g, st);
     else if (g.learn)
-      walk<In, RB, W, true, true>(g, st);
+      walk<In, RB, P, true, true>(g, st);
     else
-      walk<In, RB, W, true, false>(g, st);
+      walk<In, RB, P, true, false>(g, st);
     return launch_status("smat_head_decay_scan");
   };
-  auto rows = [&](auto wv) {
+  auto rows = [&](auto cols) {
     switch (dl::rblocks(g.r)) {
-      case 1: return go(std::integral_constant<int, 1>(), wv);
-      case 2: return go(std::integral_constant<int, 2>(), wv);
-      case 3: return go(std::integral_constant<int, 3>(), wv);
-      default: return go(std::integral_constant<int, 4>(), wv);
+      case 1: return go(std::integral_constant<int, 1>(), cols);
+      case 2: return go(std::integral_constant<int, 2>(), cols);
+      case 3: return go(std::integral_constant<int, 3>(), cols);
+      default: return go(std::integral_constant<int, 4>(), cols);
     }
   };
-  return waves_of(g.p) == 4 ? rows(std::integral_constant<int, 4>())
-                            : rows(std::integral_constant<int, 8>());
+  return g.p <= 64 ? rows(std::integral_constant<int, 64>())
+                   : rows(std::integral_constant<int, 128>());
 }
 extern template int launch_walk<bf16>(const Walk&, bool, hipStream_t);
 extern template int launch_walk<f16>(const Walk&, bool, hipStream_t);

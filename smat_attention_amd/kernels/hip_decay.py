@@ -14,8 +14,8 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import ptr
-from .hip_delta import CHUNK, same_device
-from .hip_fwd import _call_on, _code, _rows3, _shape
+from .hip_delta import CHUNK, _near_rows, same_device
+from .hip_fwd import _call_on, _code, _shape
 
 MAX_D = 128
 MIN_D = 8                # rows are read eight values at a time (kMinD)
@@ -105,7 +105,7 @@ def scan(Q, K, V, logA, state, scale, segments, want_state: bool, save: bool, le
     those entering the chunks), ``inputs`` are the tensors that the kernels read."""
     plan = _Plan("head_decay_scan", Q, V, len(logA), segments)
     code, dev = _code(Q, "head_decay_scan"), Q.device
-    (Q, q_sb, q_st), (K, k_sb, k_st), (V, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
+    (Q, q_sb, q_st), (K, k_sb, k_st), (V, v_sb, v_st) = map(_near_rows, (Q, K, V))
     logA = logA.float().contiguous()
     o = torch.empty(plan.nb, plan.T, plan.p, device=dev, dtype=V.dtype)
     lead = () if segments is None else (plan.nseg,)
@@ -133,8 +133,8 @@ def scan_backward(inputs, kept, dO, dS, scale, segments, want_dstate: bool, lear
     start, chunk_states = kept
     plan = _Plan("head_decay_scan", Q, V, len(logA), segments)
     code, dev = _code(Q, "head_decay_scan"), Q.device
-    (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = _rows3(Q), _rows3(K), _rows3(V)
-    dO, d_sb, d_st = _rows3(dO)
+    (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = map(_near_rows, (Q, K, V))
+    dO, d_sb, d_st = _near_rows(dO)
     dQ = torch.empty(plan.nbk, plan.T, plan.r, device=dev, dtype=Q.dtype)
     dK = torch.empty_like(dQ)
     dV = torch.empty(plan.nb, plan.T, plan.p, device=dev, dtype=V.dtype)
