@@ -13,42 +13,46 @@ namespace smat {
 namespace hd {
 
 // The states entering the runs of a segment, from init or from zero; `rev`: the runs in
-// turned order.  Every element on its own, eight runs' E in flight.
+// turned order.  Every element on its own, sixteen runs' E in flight.
 __global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* __restrict__ init,
                                                           const float* __restrict__ E,
                                                           float* __restrict__ start) {
+  constexpr int U = 16, BLOCK = 256;
+  __shared__ float decay[BLOCK];                   // of the tokens of a block of runs
   const int s = blockIdx.x, seg = blockIdx.z;
   const int64_t rp = (int64_t)g.r * g.p, e = (int64_t)blockIdx.y * 256 + threadIdx.x;
   const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
-  if (r0 >= r1 || e >= rp) return;
-  const double la = g.logA[s % g.heads];
-  auto at = [&](int n) { return ((int64_t)(g.rev ? r0 + r1 - 1 - n : n) * g.nb + s) * rp + e; };
-  auto decay = [&](int n) {                        // of the run's tokens
-    const int i = g.rev ? r0 + r1 - 1 - n : n;
-    int tokens;
-    if (g.runs) {
-      const int a = g.runs[4 * i], b = g.runs[4 * i + 1];
-      tokens = b > a ? g.chunks[2 * b - 2] + g.chunks[2 * b - 1] - g.chunks[2 * a] : 0;
-    } else {
-      tokens = min((i + 1) * g.K * C, g.T) - i * g.K * C;
+  auto run_at = [&](int n) { return g.rev ? r0 + r1 - 1 - n : n; };
+  const int64_t step = g.nb * rp;                  // between a sequence's runs
+  const float* E0 = E + s * rp + min(e, rp - 1);
+  float* start0 = start + s * rp + e;
+  float S = init && e < rp ? init[((int64_t)seg * g.nb + s) * rp + e] : 0.f;
+  for (int b = r0; b < r1; b += BLOCK) {
+    __syncthreads();
+    if (b + (int)threadIdx.x < r1) {
+      const int i = run_at(b + threadIdx.x);
+      int tokens;
+      if (g.runs) {
+        const int first = g.runs[4 * i], last = g.runs[4 * i + 1];
+        tokens = last > first ? g.chunks[2 * last - 2] + g.chunks[2 * last - 1] - g.chunks[2 * first]
+                              : 0;
+      } else {
+        tokens = (int)min((int64_t)(i + 1) * g.K * C, (int64_t)g.T) - i * g.K * C;
+      }
+      decay[threadIdx.x] = tokens ? (float)exp((double)g.logA[s % g.heads] * tokens) : 1.f;
     }
-    return tokens ? (float)exp(la * tokens) : 1.f;
-  };
-  float S = init ? init[((int64_t)seg * g.nb + s) * rp + e] : 0.f;
-  constexpr int U = 8;
-  for (int n = r0; n < r1; n += U) {
-    float x[U], a[U];
+    __syncthreads();
+    for (int n = b; n < min(b + BLOCK, r1); n += U) {
+      float x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {                  // past the last but one: its own once more
-      const int i = min(n + u, max(r1 - 2, r0));
-      x[u] = r1 - r0 > 1 ? E[at(i)] : 0.f;
-      a[u] = decay(i);
-    }
+      for (int u = 0; u < U; ++u)                  // a segment's last run has no E: another's
+        x[u] = r1 - r0 > 1 ? E0[run_at(min(n + u, r1 - 2)) * step] : 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (n + u >= r1) break;
-      start[at(n + u)] = S;
-      S = a[u] * S + x[u];
+      for (int u = 0; u < U; ++u)
+        if (n + u < r1) {
+          if (e < rp) start0[run_at(n + u) * step] = S;
+          S = decay[n + u - b] * S + x[u];
+        }
     }
   }
 }

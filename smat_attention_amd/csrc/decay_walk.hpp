@@ -276,9 +276,14 @@ __device__ __forceinline__ Frag<Terms<In>::in> value_rows(const bf16* tile, int 
 }
 
 // The column tiles of a wave and the waves of a workgroup, by the columns of all (64 or 128):
-// two tiles a wave share the reads of K, Q and P; with LEARN they would not fit the registers.
-template <int P, bool LEARN> constexpr int tiles() { return P == 64 || LEARN ? 1 : 2; }
-template <int P, bool LEARN> constexpr int waves() { return P / 16 / tiles<P, LEARN>(); }
+// two tiles a wave share the reads of K, Q and P.  With LEARN they would not fit the registers,
+// and inputs of several terms leave LDS for one workgroup a CU, which eight waves fill better.
+template <typename In, int P, bool LEARN> constexpr int tiles() {
+  return P == 64 || LEARN || Terms<In>::in > 1 ? 1 : 2;
+}
+template <typename In, int P, bool LEARN> constexpr int waves() {
+  return P / 16 / tiles<In, P, LEARN>();
+}
 constexpr int kMaxWaves = 8;
 template <typename In, int P> constexpr int value_elems() {
   return sizeof(In) == 4 ? 2 * C * (P + 4) : tile_elems(P / 32);
@@ -292,7 +297,7 @@ template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets)
 }
 // Waves a SIMD: as many as registers and LDS have room for.
 template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_occ() {
-  const int fit = dl::kMaxLds / walk_lds<In, RB, P, OUT>(1) * waves<P, LEARN>() / 4;
+  const int fit = dl::kMaxLds / walk_lds<In, RB, P, OUT>(1) * waves<In, P, LEARN>() / 4;
   const int most = LEARN ? 2 : !OUT ? (P == 64 ? 4 : RB > 2 ? 2 : 3) : P == 64 && RB < 3 ? 3 : 2;
   return fit < most ? fit : most;
 }
@@ -300,7 +305,7 @@ template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_o
 // still fit.
 template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_sets() {
   return walk_lds<In, RB, P, OUT>(2) * walk_occ<In, RB, P, OUT, LEARN>() * 4 /
-                     waves<P, LEARN>() <= dl::kMaxLds ? 2 : 1;
+                     waves<In, P, LEARN>() <= dl::kMaxLds ? 2 : 1;
 }
 
 // A rows fragment from the caller's rows: row tile mt of the chunk (in the walk's order),
@@ -351,9 +356,9 @@ __device__ __forceinline__ void steps(Load load, Use use) {
 }
 
 template <typename In, int RB, int P, bool OUT, bool LEARN>
-__global__ __launch_bounds__((64 * waves<P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void decay_walk_kernel(
+__global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void decay_walk_kernel(
     Walk g) {
-  constexpr int W = waves<P, LEARN>(), CT = tiles<P, LEARN>(), NT = Terms<In>::in, NI = kMid, VB = P / 32;
+  constexpr int W = waves<In, P, LEARN>(), CT = tiles<In, P, LEARN>(), NT = Terms<In>::in, NI = kMid, VB = P / 32;
   constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>(), SET = set_elems<In, RB, P, OUT>();
   constexpr int KD = walk_sets<In, RB, P, OUT, LEARN>(), TP = (kTiles + W - 1) / W;
   extern __shared__ __align__(1024) bf16 lds[];
@@ -746,7 +751,7 @@ __global__ __launch_bounds__((64 * waves<P, LEARN>()), (walk_occ<In, RB, P, OUT,
       }
 }
 
-inline int learn_waves(int p) { return p <= 64 ? waves<64, true>() : waves<128, true>(); }
+inline int learn_waves(int p) { return p <= 64 ? 4 : 8; }
 
 template <typename In, int RB, int P, bool OUT, bool LEARN>
 static void walk(const Walk& g, hipStream_t st) {
@@ -755,7 +760,7 @@ static void walk(const Walk& g, hipStream_t st) {
   auto kern = decay_walk_kernel<In, RB, P, OUT, LEARN>;
   static uint64_t done;
   dl::allow_lds(kern, lds, done);
-  hipLaunchKernelGGL(kern, dim3(g.nb, g.nruns), dim3(64 * waves<P, LEARN>()), lds, st, g);
+  hipLaunchKernelGGL(kern, dim3(g.nb, g.nruns), dim3(64 * waves<In, P, LEARN>()), lds, st, g);
 }
 
 // One file a type instantiates it.
