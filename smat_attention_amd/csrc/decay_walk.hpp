@@ -279,7 +279,11 @@ __device__ __forceinline__ Frag<Terms<In>::in> value_rows(const bf16* tile, int 
 // two tiles a wave share the reads of K, Q and P.  With LEARN they would not fit the registers,
 // and inputs of several terms leave LDS for one workgroup a CU, which eight waves fill better.
 template <typename In, int P, bool LEARN> constexpr int tiles() {
+#ifdef V8
+  return 1;
+#else
   return P == 64 || LEARN || Terms<In>::in > 1 ? 1 : 2;
+#endif
 }
 template <typename In, int P, bool LEARN> constexpr int waves() {
   return P / 16 / tiles<In, P, LEARN>();
@@ -291,9 +295,13 @@ template <typename In, int P> constexpr int value_elems() {
 template <typename In, int RB, int P, bool OUT> constexpr int set_elems() {
   return Terms<In>::in * (OUT ? 2 : 1) * tile_elems(RB) + value_elems<In, P>();
 }
-constexpr int kTab = C + 4 + 2 * C;   // floats: a^0 .. a^64; the update's factors, zeros behind
+// Floats: a^0 .. a^64; the update's factors, zeros behind; and, where inputs of one term leave
+// room and four registers a tile are dear, D by the tiles' distances, lane by lane.
+template <typename In> constexpr int tab_floats() {
+  return C + 4 + 2 * C + (Terms<In>::in == 1 ? 4 * 256 : 0);
+}
 template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets) {
-  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) + kTab * 4;
+  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) + tab_floats<In>() * 4;
 }
 // Waves a SIMD: as many as registers and LDS have room for.
 template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_occ() {
@@ -455,18 +463,29 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
   if (chunks > 0) put(0);
   lds_barrier();
   float e[4];
-  f32x4 D[OUT ? TP : 1];
+  f32x4* dt = reinterpret_cast<f32x4*>(wt + 2 * C);
+  f32x4 D[OUT && NT > 1 ? TP : 1];
   if (OUT) {
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) e[mt] = g.inter * tab[16 * mt + m + (g.rev ? 0 : 1)];
-#pragma unroll
-    for (int u = 0; u < TP; ++u) {
-      int mt, jt;
-      tile_of(min(w + u * W, kTiles - 1), mt, jt);
+    auto factors = [&](int q) {                    // of tiles 16 q tokens apart
+      f32x4 x;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int d = 16 * (mt - jt) + m - 4 * gq - i;
-        D[u][i] = d >= 0 ? g.intra * tab[d] : 0.f;
+        const int d = 16 * q + m - 4 * gq - i;
+        x[i] = d >= 0 ? g.intra * tab[d] : 0.f;
+      }
+      return x;
+    };
+    if constexpr (NT == 1) {
+      for (int q = w; q < 4; q += W) dt[q * 64 + lane_id()] = factors(q);
+      lds_barrier();
+    } else {
+#pragma unroll
+      for (int u = 0; u < TP; ++u) {
+        int mt, jt;
+        tile_of(min(w + u * W, kTiles - 1), mt, jt);
+        D[u] = factors(mt - jt);
       }
     }
   }
@@ -478,6 +497,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
     bf16* set = lds + (KD == 2 ? (c & 1) * SET : 0);
     const bf16 *kt = set, *vt = set + KT, *qt = vt + VT;
     const bool more = c + 1 < chunks;
+    __builtin_amdgcn_s_setprio(0);
     const int t0 = begin + first_of(c), len = min(C, end - t0);
     if (c > 0) lds_barrier();
     // ---- the chunk's rows are in LDS
@@ -495,6 +515,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
       // tiles of P, transposed: rows are tokens j, columns i (the last ones twice: no branch)
       struct Pair {
         Frag<NT> k[RB], q[RB];
+        f32x4 d;
       };
       steps<TP, NT == 1, Pair>(
           [&](int u, Pair& b) {
@@ -505,6 +526,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
               b.k[kb] = rows_of<RB, NT>(kt, jt, kb);
               b.q[kb] = rows_of<RB, NT>(qt, mt, kb);
             }
+            b.d = NT == 1 ? dt[(mt - jt) * 64 + lane_id()] : D[NT == 1 ? 0 : u];
           },
           [&](int u, Pair& b) {
             int mt, jt;
@@ -512,7 +534,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
             f32x4 x = zero4();
 #pragma unroll
             for (int kb = 0; kb < RB; ++kb) x = dl::mul_inputs(x, b.k[kb], b.q[kb]);
-            x = rounded(x * D[u]);
+            x = rounded(x * b.d);
             if constexpr (LEARN) {
               if (g.learn == kDq && w + u * W < kTiles) {   // here i: dO, j: V; K in V's place
                 f32x4 z = zero4();
@@ -603,6 +625,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
     if constexpr (OUT) {
       lds_barrier();
       // ---- P is in LDS
+      __builtin_amdgcn_s_setprio(1);
       struct One {
         Frag<NI> p;
       };
