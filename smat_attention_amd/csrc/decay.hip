@@ -179,20 +179,47 @@ static Scratch take(dl::Arena& ar, int64_t nb, int64_t nbk, int64_t T, int nseg,
 }  // namespace smat
 
 // Run length: of the lengths that cut the longest segment into 1 to 256 runs, the one whose
-// passes take least.
+// passes take least by what their steps measure, in microseconds a chunk of a workgroup with
+// its CU to itself: 1.6 + 0.7 RB with outputs, half as much again at 128 columns, 1.35 and 1.7
+// times that where inputs have two and three terms, and 0.42 of it in the first pass.  Two
+// workgroups on a CU take 1.45 times as long each, three (bf16, 64 columns) 1.9; more than fit
+// follow one another.  The carry moves its states at 4 TB/s, and two launches more
+// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 8511 whole, 606 in 32 runs, 474 in
+// 64, 508 in 128; 32 of 128 chunks, 64 x 64: 341 whole, 80 in 8, 64 in 16, 67 in 22; 96 of 64
+// chunks with gradients: 714 whole, 313 in 4, 262 in 8; fp16, 12 of 157 chunks, 96 x 96: 131 in
+// 16, 113 in 20, 123 in 40.)
 extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
                                           const int32_t* times, int n, int r, int p) {
   using namespace smat;
   const bool packed = lengths && times && n > 0;
   int longest = packed ? 0 : nch;
   for (int i = 0; packed && i < n; ++i) longest = lengths[i] > longest ? lengths[i] : longest;
-  if (longest < 1 || nb < 1 || r < 1 || p < 1) return 1;
-  const int slots = 512;
+  if (longest < 1 || nb < 1 || r < 1 || p < 1 || r > hd::kMaxD || p > hd::kMaxD ||
+      dtype < SMAT_BF16 || dtype > SMAT_F32)
+    return 1;
+  int on = 1;                                      // workgroups a CU
+  dl::dispatch(dtype, r, [&](auto in, auto rb) {
+    typedef decltype(in) In;
+    constexpr int RB = decltype(rb)::value;
+    on = p <= 64 ? hd::walk_occ<In, RB, 64, true, false>() * 4 / hd::waves<In, 64, false>()
+                 : hd::walk_occ<In, RB, 128, true, false>() * 4 / hd::waves<In, 128, false>();
+    return 0;
+  });
+  static const double terms[] = {1.0, 1.35, 1.7}, share[] = {0.0, 1.0, 1.45, 1.9};
+  const double step = (1.6 + 0.7 * dl::rblocks(r)) * (p <= 64 ? 1.0 : 1.5) *
+                      terms[dl::in_terms(dtype) - 1];
+  // wgs workgroups of up to K chunks, `steps` chunks in all
+  auto pass = [&](double wgs, double steps, int K) {
+    const double rounds = (double)(int64_t)(wgs / (256 * on)), left = wgs - rounds * 256 * on;
+    const int most = left <= 0 ? 0 : left <= 256 ? 1 : left <= 512 ? 2 : 3;
+    const double even = steps / (wgs * K);         // runs shorter than K end earlier
+    return K * (rounds * share[on] * even + share[most < on ? most : on]);
+  };
   int best = longest;
   double least = 0;
   for (int G = 1; G <= 256 && (G == 1 || longest / G >= 2); ++G) {
     const int K = (longest + G - 1) / G;
-    double runs = 0, chunks = 0, ends = 0;
+    double runs = 0, chunks = 0, ends = 0;         // `ends`: runs with one behind them
     for (int i = 0; i < (packed ? n : 1); ++i) {
       const double len = packed ? lengths[i] : nch, t = packed ? times[i] : 1;
       const double cut = len > K ? (int)((len + K - 1) / K) : 1;
@@ -200,12 +227,10 @@ extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int3
       ends += t * (cut - 1);
       chunks += t * len;
     }
-    if (G > 1 && runs > dl::kMaxGrid) continue;
-    auto pass = [&](double wgs, double steps, double cost) {
-      return wgs <= slots ? K * cost : (steps / slots + 0.5 * K) * cost;
-    };
-    double us = pass(runs * nb, chunks * nb, 3.0);
-    if (ends > 0) us += pass(ends * nb, ends * K * nb, 1.5) + 10 + 0.1 * G;
+    if (G > 1 && runs > dl::kMaxGrid) continue;    // more than a grid holds
+    double us = step * pass(runs * nb, chunks * nb, K);
+    if (ends > 0)
+      us += 0.42 * step * pass(ends * nb, ends * K * nb, K) + 9 + runs * nb * r * p * 16 / 4e6;
     if (G == 1 || us < least) {
       least = us;
       best = K;
