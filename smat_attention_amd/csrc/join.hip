@@ -15,10 +15,9 @@
 //
 // Bandwidth kernels: each tensor is read once and written once.  The backward reads f, h and
 // z and forms y, u and h' again in fp32 as the forward did, the rows' two factors r1 and r2
-// are kept; so no rounded h' enters the gradients.  A row is one wave's up to 512 columns, else
-// a workgroup's of up to eight, each lane with one or two groups of eight columns; rows are
-// walked with the weights, and in the backward the columns' sums, in registers.  The sums leave
-// through the workgroups' parts, added in a fixed order.
+// are kept; so no rounded h' enters the gradients.  A row is a group of waves', a lane has eight
+// of its columns; rows are walked with the weights, and in the backward the columns' sums, in
+// registers.  The sums leave through the workgroups' parts, added in a fixed order.
 //
 // Dropout's mask is never stored: place (row, column) is kept where its word of Philox 4x32,
 // ten rounds (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC 2011),
@@ -30,7 +29,7 @@
 namespace smat {
 namespace join {
 
-constexpr int kMinD = 8, kMaxD = 8192, kMost = 512;   // columns, and threads a workgroup
+constexpr int kMinD = 8, kMaxD = 8192;   // columns
 enum Gate { kAbsent = 0, kLinear = 1, kSigmoid = 2, kSilu = 3 };
 
 struct Args {
@@ -50,9 +49,12 @@ struct Args {
   const void *dh, *dx;                     // or null: zero
   int64_t dh_st, dx_st;
   void *df, *dz, *dh_out;                  // dz: null without a gate
-  float* part;                             // (groups, 3, D); or null
+  float* part;                             // (workgroups, 3, D); or null
 };
 
+// The four words of a place's block of columns.  Rows are a wave's, so the first two rounds
+// cost a lane nothing in the rows' loop: every product in them is of the columns or of the
+// row alone.
 __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
@@ -67,337 +69,319 @@ __device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k
   }
 }
 
-__device__ __forceinline__ float weight(const void* w, int type, int c) {
-  return type == SMAT_F32   ? ((const float*)w)[c]
-         : type == SMAT_BF16 ? to_f32(((const bf16*)w)[c])
-                             : to_f32(((const f16*)w)[c]);
+// What a lane has of a row: eight columns.
+typedef float f8 __attribute__((ext_vector_type(8)));
+template <typename In>
+__device__ __forceinline__ f8 eight(Raw<In> x, int c, int D) {
+  if ((D & 7) && c + 8 > D && c < D) x.drop(8 - (D & 7));
+  if (c >= D) x.zero();
+  f32x4 a, b;
+  x.values(a, b);
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+template <typename Out>
+__device__ __forceinline__ void put(Out* row, const f8& y, int c, int D) {
+  if (c < D)
+    store8(row + c, __builtin_shufflevector(y, y, 0, 1, 2, 3),
+           __builtin_shufflevector(y, y, 4, 5, 6, 7), D - c);
+}
+__device__ __forceinline__ float sum8(const f8& x) {
+  return ((x[0] + x[4]) + (x[1] + x[5])) + ((x[2] + x[6]) + (x[3] + x[7]));
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
+// Eight weights; `absent` where there are none, and past the last column.
+__device__ __forceinline__ f8 weights(const void* w, int type, float absent, int c, int D) {
+  f8 y;
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
-  return x;
-}
-// A row's sum over its threads: a wave's, or a workgroup's through LDS (sums of either
-// parity of calls alternate between two places, so one barrier a sum).
-__device__ __forceinline__ float row_sum(float x, int group, float (*lds)[16], int& turn) {
-  x = wave_sum(x);
-  if (group > 64) {
-    float* at = lds[turn];
-    turn ^= 1;
-    if (lane_id() == 0) at[wave_id()] = x;
-    __syncthreads();
-    x = at[0];
-    for (int i = 1; i < group / 64; ++i) x += at[i];
-  }
-  return x;
-}
-
-// What a lane has of a row: NV groups of eight columns.
-template <typename In, int NV> struct Cols {
-  Raw<In> x[NV];
-  __device__ __forceinline__ void load(const In* row, const int (&c)[NV], int D) {
+  for (int i = 0; i < 8; ++i) y[i] = absent;
+  if (!w) return y;
+  auto read = [&](auto t) {
+    typedef decltype(t) T;
+    Raw<T> x;
+    x.load((const T*)w + min(c, D - 8));
+    return eight(x, c, D);
+  };
+  const f8 x = type == SMAT_F32 ? read(float()) : type == SMAT_BF16 ? read(bf16()) : read(f16());
 #pragma unroll
-    for (int v = 0; v < NV; ++v) x[v].load(row + min(c[v], D - 8));
-  }
-  // Element i of group v as fp32; columns past the last are zero.
-  __device__ __forceinline__ void get(float (&y)[NV][8], const int (&c)[NV], int D) {
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      if ((D & 7) && c[v] + 8 > D && c[v] < D) x[v].drop(8 - (D & 7));
-      if (c[v] >= D) x[v].zero();
-      f32x4 a, b;
-      x[v].values(a, b);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        y[v][i] = a[i];
-        y[v][i + 4] = b[i];
-      }
-    }
-  }
-};
-template <typename Out, int NV>
-__device__ __forceinline__ void put(Out* row, const float (&y)[NV][8], const int (&c)[NV], int D) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-    if (c[v] < D)
-      store8(row + c[v], f32x4{y[v][0], y[v][1], y[v][2], y[v][3]},
-             f32x4{y[v][4], y[v][5], y[v][6], y[v][7]}, D - c[v]);
+  for (int i = 0; i < 8; ++i) y[i] = c + i < D ? x[i] : absent;
+  return y;
 }
 
 // gate(z), and its slope.  The exp is of -|z|, and 1 - sigmoid(z) is sigmoid(-z): neither
-// overflows, and nothing cancels at either end.
-__device__ __forceinline__ float gate_of(int kind, float z, float& slope) {
+// overflows, and nothing cancels at either end.  exp(x) is 2^(x log2 e) with the product's
+// rounding error put back, since the hardware's exponential takes it as it is, and as the square
+// of 2^(x log2 e / 2), since that instruction gives no subnormal results.
+__device__ __forceinline__ void sigmoid(float z, float& s, float& t) {
+  constexpr float high = 0x1.715476p+0f, low = 0x1.4ae0cp-26f;     // log2 e
+  const float x = -fabsf(z), y = x * high;
+  const float off = fmaf(x, low, fmaf(x, high, -y));
+  const float root = __builtin_amdgcn_exp2f(0.5f * y);
+  const float e = root * fmaf(off, 0x1.62e43p-1f, 1.f) * root;
+  const float d = __builtin_amdgcn_rcpf(1.f + e);
+  s = z >= 0.f ? d : e * d;
+  t = z >= 0.f ? e * d : d;
+}
+template <bool SLOPE>
+__device__ __forceinline__ void gate_of(int kind, const f8& z, f8& a, f8& slope) {
   if (kind == kLinear) {
-    slope = 1.f;
-    return z;
+    a = z;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) slope[i] = 1.f;
+  } else if (kind == kSigmoid) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float s, t;
+      sigmoid(z[i], s, t);
+      a[i] = s;
+      if (SLOPE) slope[i] = s * t;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float s, t;
+      sigmoid(z[i], s, t);
+      a[i] = z[i] * s;
+      if (SLOPE) slope[i] = s * (1.f + z[i] * t);
+    }
   }
-  const float e = expf(-fabsf(z)), d = 1.f / (1.f + e);
-  const float s = z >= 0.f ? d : e * d, t = z >= 0.f ? e * d : d;
-  slope = kind == kSigmoid ? s * t : s * (1.f + z * t);
-  return kind == kSigmoid ? s : z * s;
 }
 
-template <int NV> struct Lane {
-  int c[NV];
-  __device__ __forceinline__ Lane(int group) {
+// The rows' walk.  A workgroup has `per` groups of threads, one row each, and takes `per` rows
+// at a time; all its groups make as many turns, since those of several waves share barriers.
+// A turn's rows are loaded while the last one's are worked on.
+struct Walk {
+  int c, in_group, group, of, per, turn = 0;       // `of`: which group this thread is of
+  float (*sums)[16];
+  __device__ __forceinline__ Walk(int group, float (*sums)[16]) : group(group), sums(sums) {
+    in_group = (int)threadIdx.x % group;
+    of = __builtin_amdgcn_readfirstlane((int)threadIdx.x / group);
+    per = blockDim.x / group;
+    c = in_group * 8;
+  }
+  // A row's sum over its threads: a wave's, or several waves' through LDS (sums alternate
+  // between two places, so one barrier a sum).
+  __device__ __forceinline__ float sum(float x) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) c[v] = (v * group + (int)threadIdx.x % group) * 8;
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    if (group > 64) {
+      float* at = sums[turn];
+      turn ^= 1;
+      if (lane_id() == 0) at[wave_id()] = x;
+      __syncthreads();
+      const int waves = group / 64, w0 = of * waves;
+      x = at[w0];
+      for (int i = 1; i < waves; ++i) x += at[w0 + i];
+    }
+    return x;
   }
 };
 
-// u of the gate's factor a and y, and the mask's factors m.
-template <int NV>
-__device__ __forceinline__ void masks(const Args& g, float (&m)[NV][8], const int (&c)[NV],
-                                      int64_t row, uint32_t k0, uint32_t k1) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      uint32_t w[4] = {(uint32_t)(c[v] / 4 + b), (uint32_t)row, g.salt, 0};
-      philox(w, k0, k1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) m[v][4 * b + i] = w[i] >= g.threshold ? g.keep : 0.f;
-    }
-}
-
-template <int NV>
-__device__ __forceinline__ void weights(float (&y)[NV][8], const void* w, int type, float absent,
-                                        const int (&c)[NV], int D) {
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      y[v][i] = w && c[v] + i < D ? weight(w, type, c[v] + i) : absent;
-}
-
-template <typename In, typename H, int NV>
-__global__ __launch_bounds__(kMost) void join_kernel(Args g) {
-  __shared__ float sums[2][16];
-  int turn = 0;
-  const int group = g.group, D = g.D;
-  const Lane<NV> l(group);
-  const int64_t per = blockDim.x / group, step = per * gridDim.x;
-  float post[NV][8], s[NV][8], pre[NV][8];
-  weights<NV>(post, g.post, g.wt[0], 1.f, l.c, D);
-  weights<NV>(s, g.s, g.wt[1], g.scale, l.c, D);
-  weights<NV>(pre, g.pre, g.wt[2], 0.f, l.c, D);
-  uint32_t k0 = 0, k1 = 0;
-  if (g.seed) {
-    const uint32_t* k = reinterpret_cast<const uint32_t*>(g.seed);
-    k0 = k[0];
-    k1 = k[1];
+template <typename In, typename H> struct RowIn {
+  Raw<In> f, z;
+  Raw<H> h;
+  __device__ __forceinline__ void load(const Args& g, int64_t row, int c) {
+    c = min(c, g.D - 8);
+    f.load((const In*)g.f + row * g.f_st + c);
+    h.load((const H*)g.h + row * g.h_st + c);
+    if (g.gate) z.load((const In*)g.z + row * g.z_st + c);
   }
+};
+template <typename In, typename H> struct RowBack : RowIn<In, H> {
+  Raw<In> x;
+  Raw<H> d;
+  float r1, r2;
+  __device__ __forceinline__ void load(const Args& g, int64_t row, int c) {
+    RowIn<In, H>::load(g, row, c);
+    c = min(c, g.D - 8);
+    if (g.dx) x.load((const In*)g.dx + row * g.dx_st + c);
+    if (g.dh) d.load((const H*)g.dh + row * g.dh_st + c);
+    r1 = g.factors[2 * row];
+    r2 = g.factors[2 * row + 1];
+  }
+};
+
+__device__ __forceinline__ f8 mask_of(const Args& g, int c, uint32_t row, uint32_t k0,
+                                      uint32_t k1) {
+  f8 m;
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    uint32_t w[4] = {(uint32_t)(c / 4 + b), row, g.salt, 0};
+    philox(w, k0, k1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[4 * b + i] = w[i] >= g.threshold ? g.keep : 0.f;
+  }
+  return m;
+}
+
+// What a kernel's lane keeps through its rows.
+struct Kept {
+  f8 post, s, pre;
+  uint32_t k0 = 0, k1 = 0;
+  float mean;
+  __device__ __forceinline__ Kept(const Args& g, int c) {
+    post = weights(g.post, g.wt[0], 1.f, c, g.D);
+    s = weights(g.s, g.wt[1], g.scale, c, g.D);
+    pre = weights(g.pre, g.wt[2], 0.f, c, g.D);
+    if (g.seed) {
+      const uint32_t* k = reinterpret_cast<const uint32_t*>(g.seed);
+      k0 = k[0];
+      k1 = k[1];
+    }
+    mean = 1.f / (float)g.D;
+  }
+};
+
+// MOST: threads a workgroup.
+template <typename In, typename H, int MOST>
+__global__ __launch_bounds__(MOST) void join_kernel(Args g) {
+  __shared__ float sums[2][16];
+  Walk l(g.group, sums);
+  const int D = g.D, c = l.c;
+  const Kept k(g, c);
   if (g.factors && g.seed && blockIdx.x == 0 && threadIdx.x == 0) {
     uint32_t* kept = reinterpret_cast<uint32_t*>(g.factors + 2 * g.rows);
-    kept[0] = k0;
-    kept[1] = k1;
+    kept[0] = k.k0;
+    kept[1] = k.k1;
   }
-  const float mean = 1.f / (float)D;
-  for (int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / group; row < g.rows; row += step) {
-    Cols<In, NV> fc, zc;
-    Cols<H, NV> hc;
-    fc.load((const In*)g.f + row * g.f_st, l.c, D);
-    hc.load((const H*)g.h + row * g.h_st, l.c, D);
-    if (g.gate) zc.load((const In*)g.z + row * g.z_st, l.c, D);
-    float y[NV][8], h[NV][8];
-    fc.get(y, l.c, D);
+  const int64_t step = (int64_t)l.per * gridDim.x;
+  int64_t r0 = (int64_t)blockIdx.x * l.per;
+  RowIn<In, H> next;
+  next.load(g, min(r0 + l.of, g.rows - 1), c);
+  for (; r0 < g.rows; r0 += step) {
+    const int64_t row = r0 + l.of;
+    const bool live = row < g.rows;
+    const RowIn<In, H> in = next;
+    if (r0 + step < g.rows) next.load(g, min(row + step, g.rows - 1), c);
+    f8 y = eight(in.f, c, D);
     float r1 = 1.f, r2 = 1.f;
     if (g.post) {
-      float q = 0.f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q += y[v][i] * y[v][i];
-      r1 = rsqrtf(row_sum(q, group, sums, turn) * mean + g.eps);
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[v][i] = y[v][i] * r1 * post[v][i];
+      r1 = rsqrtf(l.sum(sum8(y * y)) * k.mean + g.eps);
+      y = y * r1 * k.post;
     }
     if (g.gate) {
-      float z[NV][8];
-      zc.get(z, l.c, D);
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float slope;
-          y[v][i] *= gate_of(g.gate, z[v][i], slope);
-        }
+      f8 a, slope;
+      gate_of<false>(g.gate, eight(in.z, c, D), a, slope);
+      y *= a;
     }
     if (g.seed) {
-      float m[NV][8];
-      masks<NV>(g, m, l.c, row, k0, k1);
+      const f8 m = mask_of(g, c, (uint32_t)row, k.k0, k.k1);
 #pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[v][i] = m[v][i] != 0.f ? y[v][i] * m[v][i] : 0.f;
+      for (int i = 0; i < 8; ++i) y[i] = m[i] != 0.f ? y[i] * m[i] : 0.f;
     }
-    hc.get(h, l.c, D);
-    float q = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        h[v][i] += s[v][i] * y[v][i];
-        if (l.c[v] + i < D) q += h[v][i] * h[v][i];
-      }
-    put((H*)g.h2 + row * D, h, l.c, D);
+    y = eight(in.h, c, D) + k.s * y;
+    if (live) put((H*)g.h2 + row * D, y, c, D);
     if (g.pre) {
-      r2 = rsqrtf(row_sum(q, group, sums, turn) * mean + g.eps);
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[v][i] = h[v][i] * r2 * pre[v][i];
-      put((In*)g.x + row * D, h, l.c, D);
+      r2 = rsqrtf(l.sum(sum8(y * y)) * k.mean + g.eps);
+      if (live) put((In*)g.x + row * D, y * r2 * k.pre, c, D);
     }
-    if (g.factors && threadIdx.x % group == 0) {
+    if (g.factors && live && l.in_group == 0) {
       g.factors[2 * row] = r1;
       g.factors[2 * row + 1] = r2;
     }
   }
 }
 
-template <typename In, typename H, int NV>
-__global__ __launch_bounds__(kMost) void join_backward_kernel(Args g) {
+template <typename In, typename H, int MOST>
+__global__ __launch_bounds__(MOST) void join_backward_kernel(Args g) {
   __shared__ float sums[2][16];
-  int turn = 0;
-  const int group = g.group, D = g.D;
-  const Lane<NV> l(group);
-  const int64_t per = blockDim.x / group, step = per * gridDim.x;
-  float post[NV][8], s[NV][8], pre[NV][8];
-  weights<NV>(post, g.post, g.wt[0], 1.f, l.c, D);
-  weights<NV>(s, g.s, g.wt[1], g.scale, l.c, D);
-  weights<NV>(pre, g.pre, g.wt[2], 0.f, l.c, D);
-  uint32_t k0 = 0, k1 = 0;
-  if (g.seed) {
-    const uint32_t* k = reinterpret_cast<const uint32_t*>(g.seed);
-    k0 = k[0];
-    k1 = k[1];
-  }
-  const float mean = 1.f / (float)D;
-  float apost[NV][8], as[NV][8], apre[NV][8];
-#pragma unroll
-  for (int v = 0; v < NV; ++v)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) apost[v][i] = as[v][i] = apre[v][i] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / group; row < g.rows; row += step) {
-    Cols<In, NV> fc, zc, xc;
-    Cols<H, NV> hc, dc;
-    fc.load((const In*)g.f + row * g.f_st, l.c, D);
-    hc.load((const H*)g.h + row * g.h_st, l.c, D);
-    if (g.gate) zc.load((const In*)g.z + row * g.z_st, l.c, D);
-    if (g.dx) xc.load((const In*)g.dx + row * g.dx_st, l.c, D);
-    if (g.dh) dc.load((const H*)g.dh + row * g.dh_st, l.c, D);
-    const float r1 = g.factors[2 * row], r2 = g.factors[2 * row + 1];
-    // a = gate m, y, and z's part of dz
-    float f[NV][8], z[NV][8], a[NV][8], d[NV][8];
-    fc.get(f, l.c, D);
-    if (g.gate) zc.get(z, l.c, D);
-    if (g.seed) masks<NV>(g, a, l.c, row, k0, k1);
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
+  extern __shared__ __align__(16) float part[];    // the columns' sums of the groups: 3 D
+  Walk l(g.group, sums);
+  const int D = g.D, c = l.c;
+  const Kept k(g, c);
+  const f8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  f8 apost = zero, as = zero, apre = zero;
+  const int64_t step = (int64_t)l.per * gridDim.x;
+  int64_t r0 = (int64_t)blockIdx.x * l.per;
+  RowBack<In, H> next;
+  next.load(g, min(r0 + l.of, g.rows - 1), c);
+  for (; r0 < g.rows; r0 += step) {
+    const int64_t row = r0 + l.of;
+    const bool live = row < g.rows;
+    const RowBack<In, H> in = next;
+    if (r0 + step < g.rows) next.load(g, min(row + step, g.rows - 1), c);
+    const float r1 = in.r1, r2 = in.r2;            // (r1 is one without a norm after the block)
+    const f8 f = eight(in.f, c, D), y = f * r1 * k.post;
+    f8 a = zero + 1.f, z = zero;                   // gate m, and m gate'
+    if (g.gate) gate_of<true>(g.gate, eight(in.z, c, D), a, z);
+    if (g.seed) {
+      const f8 m = mask_of(g, c, (uint32_t)row, k.k0, k.k1);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float m = g.seed ? a[v][i] : 1.f;
-        float slope = 0.f;
-        const float gate = g.gate ? gate_of(g.gate, z[v][i], slope) : 1.f;
-        a[v][i] = m != 0.f ? m * gate : 0.f;
-        z[v][i] = m != 0.f ? m * slope : 0.f;
+        a[i] = m[i] != 0.f ? m[i] * a[i] : 0.f;
+        z[i] = m[i] != 0.f ? m[i] * z[i] : 0.f;
       }
-    if (g.dh) {
-      dc.get(d, l.c, D);
-    } else {
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[v][i] = 0.f;
     }
+    f8 d = g.dh ? eight(in.d, c, D) : zero;        // dh', then dh
     if (g.dx) {
-      float h[NV][8], t[NV][8];
-      hc.get(h, l.c, D);
-      xc.get(t, l.c, D);
-      float q = 0.f;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = g.post ? f[v][i] * r1 * post[v][i] : f[v][i];
-          h[v][i] += s[v][i] * (a[v][i] * y);
-          apre[v][i] += t[v][i] * h[v][i] * r2;
-          t[v][i] *= pre[v][i];
-          q += t[v][i] * h[v][i];
-        }
-      q = row_sum(q, group, sums, turn) * mean * r2 * r2 * r2;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[v][i] += r2 * t[v][i] - h[v][i] * q;
+      const f8 h = eight(in.h, c, D) + k.s * (a * y);
+      f8 t = eight(in.x, c, D);
+      if (live) apre += t * h * r2;
+      t *= k.pre;
+      const float q = l.sum(sum8(t * h)) * k.mean * r2 * r2 * r2;
+      d += r2 * t - h * q;
     }
-    put((H*)g.dh_out + row * D, d, l.c, D);
-    float q = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = g.post ? f[v][i] * r1 * post[v][i] : f[v][i];
-        as[v][i] += d[v][i] * (a[v][i] * y);
-        const float du = d[v][i] * s[v][i];
-        z[v][i] *= du * y;
-        d[v][i] = du * a[v][i];                    // dy
-        if (g.post) {
-          apost[v][i] += d[v][i] * f[v][i] * r1;
-          d[v][i] *= post[v][i];
-          q += d[v][i] * f[v][i];
-        }
-      }
-    if (g.gate) put((In*)g.dz + row * D, z, l.c, D);
+    if (live) {
+      put((H*)g.dh_out + row * D, d, c, D);
+      as += d * (a * y);
+    }
+    d *= k.s;
+    if (g.gate && live) put((In*)g.dz + row * D, z * (d * y), c, D);
+    d *= a;                                        // dy
     if (g.post) {
-      q = row_sum(q, group, sums, turn) * mean * r1 * r1 * r1;
-#pragma unroll
-      for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[v][i] = r1 * d[v][i] - f[v][i] * q;
+      if (live) apost += d * f * r1;
+      d *= k.post;
+      const float q = l.sum(sum8(d * f)) * k.mean * r1 * r1 * r1;
+      d = r1 * d - f * q;
     }
-    put((In*)g.df + row * D, d, l.c, D);
+    if (live) put((In*)g.df + row * D, d, c, D);
   }
   if (!g.part) return;
-  const int64_t at = (int64_t)blockIdx.x * per + threadIdx.x / group;
-  float* p = g.part + at * 3 * D;
-  put(p, apost, l.c, D);
-  put(p + D, as, l.c, D);
-  put(p + 2 * D, apre, l.c, D);
+  // the groups' sums one after another into LDS, the last into the workgroup's part
+  float* out = g.part + (int64_t)blockIdx.x * 3 * D;
+  for (int n = 0; n < l.per; ++n) {
+    if (n) __syncthreads();
+    if (l.of != n) continue;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (c + i >= D) break;
+      float x[3] = {apost[i], as[i], apre[i]};
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        if (n) x[j] += part[j * D + c + i];
+        (n + 1 < l.per ? part : out)[j * D + c + i] = x[j];
+      }
+    }
+  }
 }
 
-// The columns' sums of the groups' parts, in the same order every time.
-__global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict__ part, int groups,
-                                                        int D, float* post, float* s, float* pre) {
-  __shared__ float sums[16][17];
-  const int c = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16, n = 3 * D;
+// The columns' sums of the workgroups' parts, in the same order every time.
+__global__ __launch_bounds__(1024) void join_sums_kernel(const float* __restrict__ part, int parts,
+                                                         int D, float* post, float* s,
+                                                         float* pre) {
+  __shared__ float sums[64][17];
+  const int i = threadIdx.x % 16, c = blockIdx.x * 16 + i, k = threadIdx.x / 16, n = 3 * D;
   float x = 0.f;
-  if (c < n)
-    for (int i = k; i < groups; i += 16) x += part[(int64_t)i * n + c];
-  sums[k][threadIdx.x % 16] = x;
+  if (c < n) {
+#pragma unroll 8
+    for (int j = k; j < parts; j += 64) x += part[(int64_t)j * n + c];
+  }
+  sums[k][i] = x;
   __syncthreads();
   if (k == 0 && c < n) {
-    for (int i = 1; i < 16; ++i) x += sums[i][threadIdx.x];
+    for (int j = 1; j < 64; ++j) x += sums[j][i];
     float* to = c < D ? post : c < 2 * D ? s : pre;
     if (to) to[c % D] = x;
   }
 }
 
-// Threads a row: whole waves, a lane for eight columns up to 4096, for sixteen beyond.
-inline int group_of(int D) {
-  const int lanes = (D + 7) / 8;
-  return ((lanes <= kMost ? lanes : (lanes + 1) / 2) + 63) / 64 * 64;
-}
-// Rows a workgroup, and workgroups: up to as many as stay on the CUs, each walking its rows.
-inline int rows_of(int D) { return group_of(D) == 64 ? 4 : 1; }
+// Threads a row (whole waves, eight columns a lane), rows a workgroup takes at a time, and
+// workgroups: as many as stay on the CUs, each walking its rows (16 waves a CU, 8 in the
+// backward).
+inline int group_of(int D) { return (D + 511) / 512 * 64; }
+inline int rows_of(int D) { return group_of(D) < 512 ? 512 / group_of(D) : 1; }
 inline int64_t grid_of(int64_t rows, int D, bool backward) {
-  const int waves = group_of(D) * rows_of(D) / 64;
-  const int64_t most = 256 * ((backward ? 12 : 20) / waves > 1 ? (backward ? 12 : 20) / waves : 1);
-  const int64_t need = (rows + rows_of(D) - 1) / rows_of(D);
+  const int waves = group_of(D) * rows_of(D) / 64, on = (backward ? 8 : 16) / waves;
+  const int64_t most = 256 * (on > 1 ? on : 1), need = (rows + rows_of(D) - 1) / rows_of(D);
   return need < most ? need : most;
 }
 
@@ -408,17 +392,18 @@ static int launch_join(int dtype, int h_dtype, Args& g, hipStream_t st) {
   auto go = [&](auto in, auto h) {
     typedef decltype(in) In;
     typedef decltype(h) H;
-    auto kern = [&](auto nv) {
-      constexpr int NV = decltype(nv)::value;
+    auto kern = [&](auto most) {
+      constexpr int MOST = decltype(most)::value;
       if constexpr (BACKWARD)
-        hipLaunchKernelGGL((join_backward_kernel<In, H, NV>), grid, block, 0, st, g);
+        hipLaunchKernelGGL((join_backward_kernel<In, H, MOST>), grid, block,
+                           rows_of(g.D) > 1 ? 12 * g.D : 0, st, g);
       else
-        hipLaunchKernelGGL((join_kernel<In, H, NV>), grid, block, 0, st, g);
+        hipLaunchKernelGGL((join_kernel<In, H, MOST>), grid, block, 0, st, g);
     };
-    if (g.D <= 8 * kMost)
-      kern(std::integral_constant<int, 1>());
+    if (g.group <= 512)
+      kern(std::integral_constant<int, 512>());
     else
-      kern(std::integral_constant<int, 2>());
+      kern(std::integral_constant<int, 1024>());
     return launch_status(BACKWARD ? "smat_block_join_backward" : "smat_block_join");
   };
   if (dtype == SMAT_BF16) return h_dtype == SMAT_F32 ? go(bf16(), float()) : go(bf16(), bf16());
@@ -503,7 +488,7 @@ extern "C" int smat_block_join(int dtype, int h_dtype, const void* f, const void
 extern "C" int64_t smat_block_join_workspace_bytes(int64_t rows, int D) {
   using namespace smat::join;
   if (rows <= 0 || D < kMinD || D > kMaxD) return 0;
-  return grid_of(rows, D, true) * rows_of(D) * 12 * D;
+  return grid_of(rows, D, true) * 12 * D;
 }
 
 extern "C" int smat_block_join_backward(
@@ -542,8 +527,8 @@ extern "C" int smat_block_join_backward(
   hipStream_t st = (hipStream_t)stream;
   const int rl = launch_join<true>(dtype, h_dtype, g, st);
   if (rl || !sums) return rl;
-  const int groups = (int)(need / (12 * D));
-  hipLaunchKernelGGL(join_sums_kernel, dim3((3 * D + 15) / 16), dim3(256), 0, st, g.part, groups, D,
+  const int parts = (int)(need / (12 * D));
+  hipLaunchKernelGGL(join_sums_kernel, dim3((3 * D + 15) / 16), dim3(1024), 0, st, g.part, parts, D,
                      dpost, ds, dpre);
   return launch_status(who);
 }
