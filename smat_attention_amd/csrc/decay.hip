@@ -121,7 +121,8 @@ static int check(const char* who, int dtype, const Walk& g, int nbk, int r, int 
                  std::initializer_list<int64_t> rows) {
   SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
                "%s: unknown dtype %d", who, dtype);
-  SMAT_REQUIRE(g.nb >= 0 && nbk >= 1 && g.heads >= 1 && g.T >= 0 && g.nseg >= 1 && g.nch >= 0,
+  SMAT_REQUIRE(g.nb >= 0 && nbk >= 1 && g.heads >= 1 && g.T >= 0 && g.T <= 0x7fffffff - C + 1 &&
+                   g.nseg >= 1 && g.nch >= 0,
                SMAT_EINVAL, "%s: bad sizes (nb=%d nbk=%d heads=%d T=%d nseg=%d nch=%d)", who, g.nb,
                nbk, g.heads, g.T, g.nseg, g.nch);
   SMAT_REQUIRE(g.nb % nbk == 0 && g.nb % g.heads == 0, SMAT_EINVAL,

@@ -40,6 +40,8 @@ class Options:
 
 def check(f, h, gate, post, scale, pre, dropout, seed):
     vector = scale if isinstance(scale, torch.Tensor) else None
+    if dropout and not isinstance(seed, torch.Tensor):
+        raise ValueError(f"{_WHO}: dropout needs a seed, an int64 tensor of one element on the GPU")
     same_device(_WHO, f, h, gate, post, vector, pre, seed if dropout else None)
     if f.dim() < 1:
         raise ValueError(f"{_WHO}: f must be (..., columns)")
@@ -61,9 +63,6 @@ def check(f, h, gate, post, scale, pre, dropout, seed):
             _shape(_WHO, name, w, (D,))
             _code(w, _WHO)
     if dropout:
-        if not isinstance(seed, torch.Tensor):
-            raise ValueError(f"{_WHO}: dropout needs a seed, an int64 tensor of one element on "
-                             f"the GPU")
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise ValueError(f"{_WHO}: seed must be an int64 tensor of one element, got "
                              f"{seed.dtype} {tuple(seed.shape)}")
