@@ -97,10 +97,10 @@ __global__ __launch_bounds__(256) void decay_grad_kernel(const float* p0, const 
   if (threadIdx.x == 0) dlogA[h] = (float)sum[0];
 }
 
-static int walk_any(int dtype, const Walk& g, bool out, hipStream_t st) {
-  if (dtype == SMAT_BF16) return launch_walk<bf16>(g, out, st);
-  if (dtype == SMAT_F16) return launch_walk<f16>(g, out, st);
-  return launch_walk<float>(g, out, st);
+static int walk_any(int dtype, const Walk& g, bool out, int learn, hipStream_t st) {
+  if (dtype == SMAT_BF16) return launch_walk<bf16>(g, out, learn, st);
+  if (dtype == SMAT_F16) return launch_walk<f16>(g, out, learn, st);
+  return launch_walk<float>(g, out, learn, st);
 }
 
 // First pass and carry of a walk (k, v, rev and upd set): start from init.
@@ -109,7 +109,7 @@ static int carry(int dtype, const Walk& base, const float* init, float* E, float
   Walk g = base;
   g.start = nullptr;
   g.fin = E;
-  int rc = walk_any(dtype, g, false, st);
+  int rc = walk_any(dtype, g, false, kNone, st);
   if (rc) return rc;
   const int64_t rp = (int64_t)g.r * g.p;
   hipLaunchKernelGGL(decay_carry_kernel, dim3(g.nb, (rp + 255) / 256, g.nseg), dim3(256), 0, st, g,
@@ -202,8 +202,8 @@ extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int3
   dl::dispatch(dtype, r, [&](auto in, auto rb) {
     typedef decltype(in) In;
     constexpr int RB = decltype(rb)::value;
-    on = p <= 64 ? hd::walk_occ<In, RB, 64, true, false>() * 4 / hd::waves<In, 64, false>()
-                 : hd::walk_occ<In, RB, 128, true, false>() * 4 / hd::waves<In, 128, false>();
+    on = p <= 64 ? hd::walk_occ<In, RB, 64, true, 0>() * 4 / hd::waves<In, 64, 0>()
+                 : hd::walk_occ<In, RB, 128, true, 0>() * 4 / hd::waves<In, 128, 0>();
     return 0;
   });
   static const double terms[] = {1.0, 1.35, 1.7}, share[] = {0.0, 1.0, 1.45, 1.9};
@@ -293,7 +293,7 @@ extern "C" int smat_head_decay_scan(int dtype, const void* q, const void* k, con
   g.fin = state_out;
   g.o = out;
   g.save_s = save_s;
-  return walk_any(dtype, g, true, st);
+  return walk_any(dtype, g, true, kNone, st);
 }
 
 extern "C" int smat_head_decay_scan_backward(
@@ -348,9 +348,8 @@ extern "C" int smat_head_decay_scan_backward(
   g.fin = dstate;
   g.o = dv;
   g.load_s = save_s;
-  g.learn = learn ? kDv : kNone;
   g.part = sc.part[0];
-  rc = walk_any(dtype, g, true, st);
+  rc = walk_any(dtype, g, true, learn ? kDv : kNone, st);
   if (rc) return rc;
   g.q = V;
   g.k = dO;
@@ -363,9 +362,8 @@ extern "C" int smat_head_decay_scan_backward(
   g.o = group > 1 ? (void*)sc.dk : dk;
   g.wide = group > 1;
   g.x = Kk;
-  g.learn = learn ? kDk : kNone;
   g.part = sc.part[1];
-  rc = walk_any(dtype, g, true, st);
+  rc = walk_any(dtype, g, true, learn ? kDk : kNone, st);
   if (rc) return rc;
   // forward: that of q
   g.rev = false;
@@ -377,9 +375,8 @@ extern "C" int smat_head_decay_scan_backward(
   g.start = start;
   g.o = group > 1 ? (void*)sc.dq : dq;
   g.x = Q;
-  g.learn = learn ? kDq : kNone;
   g.part = sc.part[2];
-  rc = walk_any(dtype, g, true, st);
+  rc = walk_any(dtype, g, true, learn ? kDq : kNone, st);
   if (rc) return rc;
   if (group > 1 && nch > 0) {
     const int64_t n = (int64_t)T * r;

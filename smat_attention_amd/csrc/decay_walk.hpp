@@ -77,7 +77,6 @@ struct Walk {
   float* save_s;           // states entering chunks in the kernel's layout; or null
   const float* load_s;     // LEARN kDv: what save_s received
   Side x;                  // LEARN kDq: Q; kDk: K
-  int learn;
   float* part;             // LEARN: (nruns, nb, W)
 };
 
@@ -278,14 +277,14 @@ __device__ __forceinline__ Frag<Terms<In>::in> value_rows(const bf16* tile, int 
 // The column tiles of a wave and the waves of a workgroup, by the columns of all (64 or 128):
 // two tiles a wave share the reads of K, Q and P.  With LEARN they would not fit the registers,
 // and inputs of several terms leave LDS for one workgroup a CU, which eight waves fill better.
-template <typename In, int P, bool LEARN> constexpr int tiles() {
+template <typename In, int P, int LEARN> constexpr int tiles() {
 #ifdef V8
   return 1;
 #else
   return P == 64 || LEARN || Terms<In>::in > 1 ? 1 : 2;
 #endif
 }
-template <typename In, int P, bool LEARN> constexpr int waves() {
+template <typename In, int P, int LEARN> constexpr int waves() {
   return P / 16 / tiles<In, P, LEARN>();
 }
 constexpr int kMaxWaves = 8;
@@ -304,35 +303,57 @@ template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets)
   return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) + tab_floats<In>() * 4;
 }
 // Waves a SIMD: as many as registers and LDS have room for.
-template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_occ() {
+template <typename In, int RB, int P, bool OUT, int LEARN> constexpr int walk_occ() {
   const int fit = dl::kMaxLds / walk_lds<In, RB, P, OUT>(1) * waves<In, P, LEARN>() / 4;
   const int most = LEARN ? 2 : !OUT ? (P == 64 ? 4 : RB > 2 ? 2 : 3) : P == 64 && RB < 3 ? 3 : 2;
   return fit < most ? fit : most;
 }
 // Two sets, so that the next chunk's rows are written beside this one's use, where that many
 // still fit.
-template <typename In, int RB, int P, bool OUT, bool LEARN> constexpr int walk_sets() {
+template <typename In, int RB, int P, bool OUT, int LEARN> constexpr int walk_sets() {
   return walk_lds<In, RB, P, OUT>(2) * walk_occ<In, RB, P, OUT, LEARN>() * 4 /
                      waves<In, P, LEARN>() <= dl::kMaxLds ? 2 : 1;
 }
 
-// A rows fragment from the caller's rows: row tile mt of the chunk (in the walk's order),
-// 32-column block kb.
-template <typename In>
-__device__ __forceinline__ Frag<Terms<In>::in> global_frag(const In* base, int64_t st, int len,
-                                                           int cols, int mt, int kb) {
-  const int t = 16 * mt + (lane_id() & 15), g = lane_id() >> 4;
-  const In* row = base + min(t, len - 1) * st;
-  f32x4 h[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = 32 * kb + 16 * i + 4 * g + j;
-      const float x = to_f32(row[min(c, cols - 1)]);
-      h[i][j] = t < len && c < cols ? x : 0.f;
+// Four consecutive values of a row as they come, at the element's own alignment: of columns
+// col .. col + 3 of `cols` (a multiple of four; those past the last read as zero).
+template <typename In> struct Quad {
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u2h __attribute__((ext_vector_type(2), aligned(2)));
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  typename std::conditional<sizeof(In) == 2, u2, f32x4>::type x;
+  __device__ __forceinline__ void load(const In* row, int col, int cols) {
+    const In* p = row + min(col, cols - 4);
+    if constexpr (sizeof(In) == 2)
+      x = *reinterpret_cast<const u2h*>(p);
+    else
+      x = *reinterpret_cast<const f32x4u*>(p);
+  }
+  __device__ __forceinline__ f32x4 get(bool live) const {
+    f32x4 y;
+    if constexpr (__is_same(In, bf16)) {
+      y = f32x4{__uint_as_float(x[0] << 16), __uint_as_float(x[0] & 0xffff0000u),
+                __uint_as_float(x[1] << 16), __uint_as_float(x[1] & 0xffff0000u)};
+    } else if constexpr (__is_same(In, f16)) {
+      const f16x4 h = __builtin_bit_cast(f16x4, x);
+      y = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+    } else {
+      y = x;
     }
-  return dl::split<Terms<In>::in>(h[0], h[1]);
+    return live ? y : zero4();
+  }
+};
+// The same one by one, for any number of columns.
+template <typename In>
+__device__ __forceinline__ f32x4 four_of(const In* row, int col, int cols, bool live) {
+  f32x4 y;
+  col = fresh(col);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = to_f32(row[min(col + i, cols - 1)]);
+    y[i] = live && col + i < cols ? x : 0.f;
+  }
+  return y;
 }
 
 // A product rounded here, not fused into what reads it: results keep their bits whichever
@@ -363,12 +384,13 @@ __device__ __forceinline__ void steps(Load load, Use use) {
   }
 }
 
-template <typename In, int RB, int P, bool OUT, bool LEARN>
+template <typename In, int RB, int P, bool OUT, int LEARN>
 __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void decay_walk_kernel(
     Walk g) {
   constexpr int W = waves<In, P, LEARN>(), CT = tiles<In, P, LEARN>(), NT = Terms<In>::in, NI = kMid, VB = P / 32;
   constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>(), SET = set_elems<In, RB, P, OUT>();
   constexpr int KD = walk_sets<In, RB, P, OUT, LEARN>(), TP = (kTiles + W - 1) / W;
+  constexpr bool AHEAD = NT == 1;                  // (two terms: as fast without)
   extern __shared__ __align__(1024) bf16 lds[];
   bf16* pl = lds + KD * SET;
   float* tab = reinterpret_cast<float*>(pl + (OUT ? NI * kLow * kFrag : 0));   // a^0 .. a^64
@@ -492,6 +514,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
   float acc = 0.f;                                 // LEARN: this lane's part of the gradient
   const In* xs = LEARN ? (const In*)g.x.p + s / g.x.div * g.x.sb : nullptr;
   const int64_t x_st = g.rev ? -g.x.st : g.x.st;
+  const bool quads = g.p % 4 == 0;
 
   for (int c = 0; c < chunks; ++c) {
     bf16* set = lds + (KD == 2 ? (c & 1) * SET : 0);
@@ -504,6 +527,31 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
     if (more) load(c + 1);
     const float aC = tab[len];
     const In* xrow = LEARN ? xs + (int64_t)(g.rev ? t0 + len - 1 : t0) * g.x.st : nullptr;
+    // LEARN: what meets the products below from memory, read here, well before
+    constexpr bool EARLY = LEARN && sizeof(In) == 2;
+    Quad<In> xq[LEARN && LEARN != kDv ? 4 : 1], xz[EARLY && LEARN == kDq ? TP * VB * 2 : 1];
+    f32x4 xS[LEARN == kDv ? 2 * RB : 1];
+    auto row_of = [&](int mt) { return xrow + min(16 * mt + m, len - 1) * x_st; };
+    if constexpr (LEARN) {
+      static_assert(CT == 1, "");
+      if constexpr (LEARN == kDv) {
+        const f32x4* from = reinterpret_cast<const f32x4*>(g.load_s) +
+                            (((int64_t)s * g.nch + c1 - 1 - c) * W + w) * (2 * RB * 64) + lane_id();
+#pragma unroll
+        for (int mt = 0; mt < 2 * RB; ++mt) xS[mt] = from[mt * 64];
+      } else if (quads) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) xq[mt].load(row_of(mt), 16 * tile0 + 4 * gq, g.p);
+        if constexpr (EARLY && LEARN == kDq) {
+#pragma unroll
+          for (int i = 0; i < TP * VB * 2; ++i) {
+            int mt, jt;
+            tile_of(min(w + i / (VB * 2) * W, kTiles - 1), mt, jt);
+            xz[i].load(row_of(mt), 16 * (i % (VB * 2)) + 4 * gq, g.p);
+          }
+        }
+      }
+    }
     f32x4 ot[OUT ? CT : 1][OUT ? 4 : 1];
     if constexpr (OUT) {
       if (g.save_s) {
@@ -517,7 +565,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
         Frag<NT> k[RB], q[RB];
         f32x4 d;
       };
-      steps<TP, NT == 1, Pair>(
+      steps<TP, AHEAD, Pair>(
           [&](int u, Pair& b) {
             int mt, jt;
             tile_of(min(w + u * W, kTiles - 1), mt, jt);
@@ -535,12 +583,29 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
 #pragma unroll
             for (int kb = 0; kb < RB; ++kb) x = dl::mul_inputs(x, b.k[kb], b.q[kb]);
             x = rounded(x * b.d);
-            if constexpr (LEARN) {
-              if (g.learn == kDq && w + u * W < kTiles) {   // here i: dO, j: V; K in V's place
+            if constexpr (LEARN == kDq) {
+              if (w + u * W < kTiles) {   // here i: dO, j: V; K in V's place
                 f32x4 z = zero4();
-                for (int kb = 0; kb < VB; ++kb)
+                const bool live = 16 * mt + m < len;
+#pragma unroll
+                for (int kb = 0; kb < VB; ++kb) {
+                  f32x4 h[2];
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) {
+                    const int col = 32 * kb + 16 * j + 4 * gq;
+                    if (EARLY && quads) {
+                      h[j] = xz[EARLY ? (u * VB + kb) * 2 + j : 0].get(live && col < g.p);
+                    } else if (quads) {
+                      Quad<In> q;
+                      q.load(row_of(mt), col, g.p);
+                      h[j] = q.get(live && col < g.p);
+                    } else {
+                      h[j] = four_of(row_of(mt), col, g.p, live);
+                    }
+                  }
                   z = dl::mul_inputs(z, value_rows<In, VB>(vt, jt, kb),
-                                     global_frag(xrow, x_st, len, g.p, mt, kb));
+                                     dl::split<NT>(h[0], h[1]));
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                   acc += (float)(16 * (mt - jt) + m - 4 * gq - i) * (x[i] * z[i]);
@@ -559,7 +624,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
       struct Four {
         Frag<NT> q[4];
       };
-      steps<RB, NT == 1, Four>(
+      steps<RB, AHEAD, Four>(
           [&](int kb, Four& b) {
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) b.q[mt] = rows_of<RB, NT>(qt, mt, kb);
@@ -579,32 +644,25 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
 #pragma unroll
       for (int i = 0; i < CT * 4; ++i) ot[i / 4][i % 4] = rounded(ot[i / 4][i % 4] * e[i % 4]);
       if constexpr (LEARN) {
-        if (g.learn == kDq || g.learn == kDk) {    // (i + 1) q . dq, and i k . dk in turned order
+        if constexpr (LEARN == kDv) {              // n a^n <S, Y>
+          float dot = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < 2 * RB; ++mt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dot += xS[mt][i] * S[0][mt][i];
+          acc += (float)len * aC * dot;
+        } else {                                   // (i + 1) q . dq, and i k . dk in turned order
+          const int col = 16 * tile0 + 4 * gq;
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) {
             const int t = 16 * mt + m;
-            const In* row = xrow + min(t, len - 1) * x_st;
+            const f32x4 x = quads ? xq[mt].get(t < len && col < g.p)
+                                  : four_of(row_of(mt), col, g.p, t < len);
             float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < CT * 4; ++i) {
-              const int cc = 16 * (tile0 + i / 4) + 4 * gq + i % 4;
-              const float x = to_f32(row[min(cc, g.p - 1)]);
-              dot += cc < g.p ? x * ot[i / 4][mt][i % 4] : 0.f;
-            }
-            if (t < len) acc += (float)(t + (g.rev ? 0 : 1)) * dot;
+            for (int i = 0; i < 4; ++i) dot += x[i] * ot[0][mt][i];
+            acc += (float)(t + (g.rev ? 0 : 1)) * dot;
           }
-        } else if (g.learn == kDv) {               // n a^n <S, Y>
-          const f32x4* from = reinterpret_cast<const f32x4*>(g.load_s) +
-                              (((int64_t)s * g.nch + c1 - 1 - c) * W + w) * (CT * 2 * RB * 64) +
-                              lane_id();
-          float dot = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < CT * 2 * RB; ++mt) {
-            const f32x4 x = from[mt * 64];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dot += x[i] * S[mt / (2 * RB)][mt % (2 * RB)][i];
-          }
-          acc += (float)len * aC * dot;
         }
       }
     }
@@ -629,7 +687,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
       struct One {
         Frag<NI> p;
       };
-      steps<6, NT == 1, One>(
+      steps<6, AHEAD, One>(
           [&](int st, One& b) {
             const int mt = st < 2 ? st : st < 4 ? 2 : 3, kb = st < 2 ? 0 : st & 1;
             const bf16* at = pl + dl::tri(mt, kb) * kFrag + lane_id() * 8;
@@ -728,7 +786,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
       struct Some {
         Frag<NT> k[U];
       };
-      steps<2 * RB / U, NT == 1, Some>(
+      steps<2 * RB / U, AHEAD, Some>(
           [&](int st, Some& b) {
 #pragma unroll
             for (int u = 0; u < U; ++u) b.k[u] = cols_of<RB, NT>(kt, st * U + u, kb);
@@ -754,7 +812,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
       put(c + 1);
     }
   }
-  if (LEARN && g.learn) {
+  if (LEARN) {
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) acc += __shfl_xor(acc, d);
     if (lane_id() == 0) g.part[sn * W + w] = acc;
@@ -776,7 +834,7 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
 
 inline int learn_waves(int p) { return p <= 64 ? 4 : 8; }
 
-template <typename In, int RB, int P, bool OUT, bool LEARN>
+template <typename In, int RB, int P, bool OUT, int LEARN>
 static void walk(const Walk& g, hipStream_t st) {
   constexpr int lds = walk_lds<In, RB, P, OUT>(walk_sets<In, RB, P, OUT, LEARN>());
   static_assert(lds <= dl::kMaxLds, "");
@@ -787,15 +845,19 @@ static void walk(const Walk& g, hipStream_t st) {
 }
 
 // One file a type instantiates it.
-template <typename In> int launch_walk(const Walk& g, bool out, hipStream_t st) {
+template <typename In> int launch_walk(const Walk& g, bool out, int learn, hipStream_t st) {
   auto go = [&](auto rb, auto cols) {
     constexpr int RB = decltype(rb)::value, P = decltype(cols)::value;
     if (!out)
-      walk<In, RB, P, false, false>(g, st);
-    else if (g.learn)
-      walk<In, RB, P, true, true>(g, st);
+      walk<In, RB, P, false, kNone>(g, st);
+    else if (learn == kDq)
+      walk<In, RB, P, true, kDq>(g, st);
+    else if (learn == kDk)
+      walk<In, RB, P, true, kDk>(g, st);
+    else if (learn == kDv)
+      walk<In, RB, P, true, kDv>(g, st);
     else
-      walk<In, RB, P, true, false>(g, st);
+      walk<In, RB, P, true, kNone>(g, st);
     return launch_status("smat_head_decay_scan");
   };
   auto rows = [&](auto cols) {
@@ -809,9 +871,9 @@ template <typename In> int launch_walk(const Walk& g, bool out, hipStream_t st) 
   return g.p <= 64 ? rows(std::integral_constant<int, 64>())
                    : rows(std::integral_constant<int, 128>());
 }
-extern template int launch_walk<bf16>(const Walk&, bool, hipStream_t);
-extern template int launch_walk<f16>(const Walk&, bool, hipStream_t);
-extern template int launch_walk<float>(const Walk&, bool, hipStream_t);
+extern template int launch_walk<bf16>(const Walk&, bool, int, hipStream_t);
+extern template int launch_walk<f16>(const Walk&, bool, int, hipStream_t);
+extern template int launch_walk<float>(const Walk&, bool, int, hipStream_t);
 
 }  // namespace hd
 }  // namespace smat
