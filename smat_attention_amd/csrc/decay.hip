@@ -34,8 +34,9 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* _
       int tokens;
       if (g.runs) {
         const int first = g.runs[4 * i], last = g.runs[4 * i + 1];
-        tokens = last > first ? g.chunks[2 * last - 2] + g.chunks[2 * last - 1] - g.chunks[2 * first]
-                              : 0;
+        tokens = 0;
+        if (last > first)
+          tokens = g.chunks[2 * last - 2] + g.chunks[2 * last - 1] - g.chunks[2 * first];
       } else {
         tokens = (int)min((int64_t)(i + 1) * g.K * C, (int64_t)g.T) - i * g.K * C;
       }
@@ -97,10 +98,14 @@ __global__ __launch_bounds__(256) void decay_grad_kernel(const float* p0, const 
   if (threadIdx.x == 0) dlogA[h] = (float)sum[0];
 }
 
-static int walk_any(int dtype, const Walk& g, bool out, int learn, hipStream_t st) {
+static int walk_all(int dtype, const Walks& g, bool out, int learn, hipStream_t st) {
   if (dtype == SMAT_BF16) return launch_walk<bf16>(g, out, learn, st);
   if (dtype == SMAT_F16) return launch_walk<f16>(g, out, learn, st);
   return launch_walk<float>(g, out, learn, st);
+}
+
+static int walk_any(int dtype, const Walk& g, bool out, int learn, hipStream_t st) {
+  return walk_all(dtype, {{g}, 1}, out, learn, st);
 }
 
 // First pass and carry of a walk (k, v, rev and upd set): start from init.
@@ -143,8 +148,9 @@ static int check(const char* who, int dtype, const Walk& g, int nbk, int r, int 
   }
   // a grid has less than 2^32 threads along its first axis and 65535 workgroups along others
   SMAT_REQUIRE(g.nb < (1 << 23) && g.nruns <= dl::kMaxGrid && g.nseg <= dl::kMaxGrid,
-               SMAT_EUNSUPPORTED, "%s: nb=%d must stay below 2^23, %d segments and %d runs within %d",
-               who, g.nb, g.nseg, g.nruns, dl::kMaxGrid);
+               SMAT_EUNSUPPORTED,
+               "%s: nb=%d must stay below 2^23, %d segments and %d runs within %d", who, g.nb,
+               g.nseg, g.nruns, dl::kMaxGrid);
   return SMAT_OK;
 }
 
@@ -349,8 +355,7 @@ extern "C" int smat_head_decay_scan_backward(
   g.o = dv;
   g.load_s = save_s;
   g.part = sc.part[0];
-  rc = walk_any(dtype, g, true, learn ? kDv : kNone, st);
-  if (rc) return rc;
+  Walks all = {{g}, 3};
   g.q = V;
   g.k = dO;
   g.v = Q;
@@ -363,8 +368,7 @@ extern "C" int smat_head_decay_scan_backward(
   g.wide = group > 1;
   g.x = Kk;
   g.part = sc.part[1];
-  rc = walk_any(dtype, g, true, learn ? kDk : kNone, st);
-  if (rc) return rc;
+  all.w[1] = g;
   // forward: that of q
   g.rev = false;
   g.q = dO;
@@ -376,8 +380,19 @@ extern "C" int smat_head_decay_scan_backward(
   g.o = group > 1 ? (void*)sc.dq : dq;
   g.x = Q;
   g.part = sc.part[2];
-  rc = walk_any(dtype, g, true, learn ? kDq : kNone, st);
-  if (rc) return rc;
+  all.w[2] = g;
+  // in one launch where one kernel serves all three (96 sequences of 4096, 64 x 64: 149 us, one
+  // after the other 174), and its grid has less than 2^32 threads along the axis
+  if (!learn && dl::rblocks(r) == dl::rblocks(p) && (r <= 64) == (p <= 64) && nb < (1 << 21)) {
+    rc = walk_all(dtype, all, true, kNone, st);
+    if (rc) return rc;
+  } else {
+    const int roles[] = {kDv, kDk, kDq};
+    for (int i = 0; i < 3; ++i) {
+      rc = walk_any(dtype, all.w[i], true, learn ? roles[i] : kNone, st);
+      if (rc) return rc;
+    }
+  }
   if (group > 1 && nch > 0) {
     const int64_t n = (int64_t)T * r;
     const int blocks = (int)((n + 1023) / 1024 < 4096 ? (n + 1023) / 1024 : 4096);

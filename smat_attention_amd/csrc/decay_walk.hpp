@@ -79,6 +79,11 @@ struct Walk {
   Side x;                  // LEARN kDq: Q; kDk: K
   float* part;             // LEARN: (nruns, nb, W)
 };
+// Up to three walks of the same sequences in one launch (their widths in the same blocks).
+struct Walks {
+  Walk w[3];
+  int n;
+};
 
 // fp32 values as three bf16 terms, exactly: each term takes the next eight bits, so none is
 // rounded up past the type's end.
@@ -300,7 +305,8 @@ template <typename In> constexpr int tab_floats() {
   return C + 4 + 2 * C + (Terms<In>::in == 1 ? 4 * 256 : 0);
 }
 template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets) {
-  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) + tab_floats<In>() * 4;
+  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) +
+         tab_floats<In>() * 4;
 }
 // Waves a SIMD: as many as registers and LDS have room for.
 template <typename In, int RB, int P, bool OUT, int LEARN> constexpr int walk_occ() {
@@ -385,17 +391,26 @@ __device__ __forceinline__ void steps(Load load, Use use) {
 }
 
 template <typename In, int RB, int P, bool OUT, int LEARN>
-__global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void decay_walk_kernel(
-    Walk g) {
-  constexpr int W = waves<In, P, LEARN>(), CT = tiles<In, P, LEARN>(), NT = Terms<In>::in, NI = kMid, VB = P / 32;
-  constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>(), SET = set_elems<In, RB, P, OUT>();
+__global__
+__launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void
+decay_walk_kernel(Walks all) {
+  // with several, workgroups of one sequence and run lie eight apart: on one XCD, whose L2 they
+  // share the rows in
+  const int role = all.n == 1 ? 0 : (int)blockIdx.x / 8 % 3;
+  const int s = all.n == 1 ? (int)blockIdx.x : (int)blockIdx.x / 24 * 8 + (int)blockIdx.x % 8;
+  const Walk& g = all.w[role];
+  if (s >= g.nb) return;
+  constexpr int W = waves<In, P, LEARN>(), CT = tiles<In, P, LEARN>(), VB = P / 32;
+  constexpr int NT = Terms<In>::in, NI = kMid;
+  constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>();
+  constexpr int SET = set_elems<In, RB, P, OUT>();
   constexpr int KD = walk_sets<In, RB, P, OUT, LEARN>(), TP = (kTiles + W - 1) / W;
   constexpr bool AHEAD = NT == 1;                  // (two terms: as fast without)
   extern __shared__ __align__(1024) bf16 lds[];
   bf16* pl = lds + KD * SET;
   float* tab = reinterpret_cast<float*>(pl + (OUT ? NI * kLow * kFrag : 0));   // a^0 .. a^64
   float* wt = tab + C + 4;                         // wt[64 - n + j] = w_j of a chunk of n
-  const int w = dl::uniform_wave(), s = blockIdx.x;
+  const int w = dl::uniform_wave();
   const int m = lane_id() & 15, gq = lane_id() >> 4;
   int run, c0, c1, seg;
   bool head, tail;
@@ -422,7 +437,8 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
   Rows<In, RB, W, false> rq, rk;
   Rows<In, VB, W, true> rv;
   constexpr uint32_t EB = sizeof(In);
-  const uint32_t qb = (uint32_t)g.q.st * EB, kb_ = (uint32_t)g.k.st * EB, vb_ = (uint32_t)g.v.st * EB;
+  const uint32_t qb = (uint32_t)g.q.st * EB, kb_ = (uint32_t)g.k.st * EB,
+                 vb_ = (uint32_t)g.v.st * EB;
   auto rows_at = [&](const Side& x, int t) {
     return (const char*)x.p + (s / x.div * x.sb + (int64_t)t * x.st) * EB;
   };
@@ -835,17 +851,18 @@ __global__ __launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, 
 inline int learn_waves(int p) { return p <= 64 ? 4 : 8; }
 
 template <typename In, int RB, int P, bool OUT, int LEARN>
-static void walk(const Walk& g, hipStream_t st) {
+static void walk(const Walks& a, hipStream_t st) {
   constexpr int lds = walk_lds<In, RB, P, OUT>(walk_sets<In, RB, P, OUT, LEARN>());
   static_assert(lds <= dl::kMaxLds, "");
   auto kern = decay_walk_kernel<In, RB, P, OUT, LEARN>;
   static uint64_t done;
   dl::allow_lds(kern, lds, done);
-  hipLaunchKernelGGL(kern, dim3(g.nb, g.nruns), dim3(64 * waves<In, P, LEARN>()), lds, st, g);
+  const int nb = a.w[0].nb, x = a.n == 1 ? nb : (nb + 7) / 8 * 24;
+  hipLaunchKernelGGL(kern, dim3(x, a.w[0].nruns), dim3(64 * waves<In, P, LEARN>()), lds, st, a);
 }
 
 // One file a type instantiates it.
-template <typename In> int launch_walk(const Walk& g, bool out, int learn, hipStream_t st) {
+template <typename In> int launch_walk(const Walks& g, bool out, int learn, hipStream_t st) {
   auto go = [&](auto rb, auto cols) {
     constexpr int RB = decltype(rb)::value, P = decltype(cols)::value;
     if (!out)
@@ -861,19 +878,19 @@ template <typename In> int launch_walk(const Walk& g, bool out, int learn, hipSt
     return launch_status("smat_head_decay_scan");
   };
   auto rows = [&](auto cols) {
-    switch (dl::rblocks(g.r)) {
+    switch (dl::rblocks(g.w[0].r)) {
       case 1: return go(std::integral_constant<int, 1>(), cols);
       case 2: return go(std::integral_constant<int, 2>(), cols);
       case 3: return go(std::integral_constant<int, 3>(), cols);
       default: return go(std::integral_constant<int, 4>(), cols);
     }
   };
-  return g.p <= 64 ? rows(std::integral_constant<int, 64>())
+  return g.w[0].p <= 64 ? rows(std::integral_constant<int, 64>())
                    : rows(std::integral_constant<int, 128>());
 }
-extern template int launch_walk<bf16>(const Walk&, bool, int, hipStream_t);
-extern template int launch_walk<f16>(const Walk&, bool, int, hipStream_t);
-extern template int launch_walk<float>(const Walk&, bool, int, hipStream_t);
+extern template int launch_walk<bf16>(const Walks&, bool, int, hipStream_t);
+extern template int launch_walk<f16>(const Walks&, bool, int, hipStream_t);
+extern template int launch_walk<float>(const Walks&, bool, int, hipStream_t);
 
 }  // namespace hd
 }  // namespace smat

@@ -3,6 +3,6 @@
 
 namespace smat {
 namespace hd {
-template int launch_walk<f16>(const Walk&, bool, int, hipStream_t);
+template int launch_walk<f16>(const Walks&, bool, int, hipStream_t);
 }  // namespace hd
 }  // namespace smat

@@ -3,6 +3,6 @@
 
 namespace smat {
 namespace hd {
-template int launch_walk<float>(const Walk&, bool, int, hipStream_t);
+template int launch_walk<float>(const Walks&, bool, int, hipStream_t);
 }  // namespace hd
 }  // namespace smat

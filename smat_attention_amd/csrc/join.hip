@@ -508,7 +508,8 @@ extern "C" int smat_block_join_backward(
   const int rc = check(who, dtype, h_dtype, g, (float)p);
   if (rc) return rc;
   if (rows == 0) return SMAT_OK;
-  SMAT_REQUIRE(f && h && factors && ((uintptr_t)factors & 7) == 0 && df && dh_out && (!gate || (z && dz)) && (!dx || pre),
+  SMAT_REQUIRE(f && h && factors && ((uintptr_t)factors & 7) == 0 && df && dh_out &&
+                   (!gate || (z && dz)) && (!dx || pre),
                SMAT_EINVAL, "%s: null pointer, or factors not 8-byte aligned", who);
   const bool sums = dpost || ds || dpre;
   const int64_t need = sums ? smat_block_join_workspace_bytes(rows, D) : 0;

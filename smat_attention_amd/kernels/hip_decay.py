@@ -70,7 +70,8 @@ def check_scan(who, Q, K, V, logA, state, segments):
     _shape(who, "K", K, (nbk, T, r))
     _shape(who, "V", V, (nb, T, p))
     if T > 2 ** 31 - CHUNK or nb >= 2 ** 23:
-        raise ValueError(f"{who}: {T} tokens of {nb} sequences, at most 2^31 - {CHUNK} and 2^23 - 1")
+        raise ValueError(f"{who}: {T} tokens of {nb} sequences, at most 2^31 - {CHUNK} and "
+                         f"2^23 - 1")
     check_sizes(who, nbk, nb, logA, r, p)
     check_types(who, Q, K, V, logA, state)
     if state is not None:
