@@ -13,7 +13,8 @@ namespace smat {
 namespace hd {
 
 // The states entering the runs of a segment, from init or from zero; `rev`: the runs in
-// turned order.  Every element on its own, sixteen runs' E in flight.
+// turned order.  Every element on its own, sixteen runs' E in flight; bound by E in and the
+// states out (8 x 64 runs of 128 x 128: 16 us, 4.2 TB/s).
 __global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* __restrict__ init,
                                                           const float* __restrict__ E,
                                                           float* __restrict__ start) {
@@ -58,7 +59,8 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* _
   }
 }
 
-// out = the sum over a key head's value heads of fp32 rows, rounded once.
+// out = the sum over a key head's value heads of fp32 rows, rounded once.  Bound by HBM: 16
+// value heads of 8192 x 128 to 8 of bf16: 14 us, 6.0 TB/s (the rows partly lie in the last cache).
 template <typename In>
 __global__ __launch_bounds__(256) void decay_heads_kernel(const float* __restrict__ part,
                                                           In* __restrict__ out, int group,
@@ -191,10 +193,10 @@ static Scratch take(dl::Arena& ar, int64_t nb, int64_t nbk, int64_t T, int nseg,
 // times that where inputs have two and three terms, and 0.42 of it in the first pass.  Two
 // workgroups on a CU take 1.45 times as long each, three (bf16, 64 columns) 1.9; more than fit
 // follow one another.  The carry moves its states at 4 TB/s, and two launches more
-// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 8511 whole, 606 in 32 runs, 474 in
-// 64, 508 in 128; 32 of 128 chunks, 64 x 64: 341 whole, 80 in 8, 64 in 16, 67 in 22; 96 of 64
-// chunks with gradients: 714 whole, 313 in 4, 262 in 8; fp16, 12 of 157 chunks, 96 x 96: 131 in
-// 16, 113 in 20, 123 in 40.)
+// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 8008 in two runs, 586 in 32, 455 in
+// 64, 506 in 128; 32 of 128 chunks, 64 x 64: 323 whole, 80 in 8, 64 in 16, 67 in 22; 96 of 64
+// chunks with gradients: 393 whole, 266 in 4, 241 in 8, 275 in 16; fp16, 12 of 157 chunks,
+// 96 x 96: 131 in 16, 113 in 20, 125 in 40.)
 extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
                                           const int32_t* times, int n, int r, int p) {
   using namespace smat;
@@ -381,8 +383,8 @@ extern "C" int smat_head_decay_scan_backward(
   g.x = Q;
   g.part = sc.part[2];
   all.w[2] = g;
-  // in one launch where one kernel serves all three (96 sequences of 4096, 64 x 64: 149 us, one
-  // after the other 174), and its grid has less than 2^32 threads along the axis
+  // in one launch where one kernel serves all three (96 sequences of 4096, 64 x 64, three
+  // terms everywhere: 149 us, one after the other 174; now 136), and its grid has less than 2^32 threads along the axis
   if (!learn && dl::rblocks(r) == dl::rblocks(p) && (r <= 64) == (p <= 64) && nb < (1 << 21)) {
     rc = walk_all(dtype, all, true, kNone, st);
     if (rc) return rc;

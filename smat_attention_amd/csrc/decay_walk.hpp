@@ -20,13 +20,22 @@
 // one's, and its factors are e_i = a^i, w_j = a^(n-j).
 //
 // The columns of the state do not mix, so a wave takes 16 or 32 of them with all key rows in
-// registers (fp32).  A workgroup has all columns of a sequence: its four waves share the
-// chunk's rows in LDS and one P = (Q K^T) o D, of which each forms a few tiles.
+// registers (fp32).  A workgroup has all columns of a sequence: its four or eight waves share
+// the chunk's rows in LDS and one P = (Q K^T) o D, of which each forms a few tiles.
 //
 // Operands: every product runs on v_mfma_f32_16x16x32_bf16, values held in fewer than
 // their own bits as sums of bf16 terms (delta_common.hpp): bf16 inputs one term, fp16 two,
-// fp32 and what is computed in fp32 (P, the state, w V) three, 24 bits.  Results are
-// rounded once, where they are stored.
+// fp32 and what is computed in fp32 three, 24 bits; the state and P where they meet rows
+// to a 16-bit output two, 17 bits.  Results are rounded once, where they are stored.
+//
+// Per chunk, bf16, r = p = 128: 196 MFMA and some 850 vector instructions a wave (the splits
+// most of them), two waves a SIMD; 8 sequences of 131072 take 298 us with outputs (3.6 TB/s;
+// every row in L2 takes a fifth less) and 150 in the first pass (3.6); 32 of 8192, 64 x 64, 39
+// and 20.  So it is bound by how well two or three waves a SIMD cover a chunk's chain of LDS
+// reads, products, splits and barriers, and next by HBM.  fp16 has twice the tiles and products
+// and one workgroup of eight waves a CU: 12 of 10007, 96 x 96, 83 and 37 (2.2 TB/s in the two).
+// Tried and slower or no faster: volatile LDS reads, products and splits interleaved by hand,
+// two column tiles a wave with LEARN (spills), splits in registers ahead of fp16's products.
 #pragma once
 
 #include "delta_common.hpp"

@@ -176,4 +176,14 @@ constexpr int kMaxR = 128;
 constexpr int kMaxP = 144;
 constexpr int kMaxC = 256;
 
+// hipFuncSetAttribute for a kernel's LDS, once a device.
+template <typename K> inline void allow_lds(K kern, int bytes, uint64_t& done) {
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit) return;
+  (void)hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+}
+
 }  // namespace smat

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._lib import ptr
+from ._lib import DTYPE_CODE, ptr
 from .hip_delta import CHUNK, _near_rows, same_device
 from .hip_fwd import _call_on, _code, _shape
 
@@ -55,13 +55,27 @@ class _Plan:
                 self.nruns, self.K, self.r, self.p, float(scale))
 
     def workspace(self, backward, learn, device):
+        if not backward and self.nruns == self.nseg:   # a forward without cuts needs none
+            return None, 0
         n = _lib.query("smat_head_decay_workspace_bytes", self.nb, max(self.nbk, 1), self.T,
                        self.nseg, self.nruns, self.r, self.p, backward, learn)
         return (torch.empty(n, device=device, dtype=torch.uint8) if n else None), n
 
 
 def check_scan(who, Q, K, V, logA, state, segments):
-    """The argument checks of the whole-sequence form."""
+    """The argument checks of the whole-sequence form (those that word the errors are called
+    only when one fails: a short call is a launch of some ten microseconds)."""
+    dt, dev = Q.dtype, Q.device
+    if (segments is None and Q.is_cuda and dev == K.device and dev == V.device
+            and dev == logA.device and K.dtype == dt and V.dtype == dt and dt in DTYPE_CODE
+            and logA.dtype == torch.float32 and Q.dim() == 3 and V.dim() == 3 and logA.dim() == 1
+            and K.shape == Q.shape):
+        (nbk, T, r), (nb, Tv, p), heads = Q.shape, V.shape, logA.shape[0]
+        if (T == Tv and T < 2 ** 30 and 0 < nbk <= nb < 2 ** 23 and nb % nbk == 0 and heads > 0
+                and nb % heads == 0 and 1 <= r <= MAX_D and 1 <= p <= MAX_D
+                and (state is None or state.device == dev and state.dtype == torch.float32
+                     and state.shape == (nb, r, p))):
+            return
     if Q.dim() != 3 or V.dim() != 3:
         raise ValueError(f"{who}: Q, K and V must be (sequences, T, columns)")
     same_device(who, Q, K, V, logA, state)
@@ -82,7 +96,7 @@ def check_scan(who, Q, K, V, logA, state, segments):
 def check_sizes(who, nbk, nb, logA, r, p):
     if (nbk == 0) != (nb == 0) or (nbk and nb % nbk):
         raise ValueError(f"{who}: {nbk} key sequences do not divide {nb} value sequences")
-    if logA.dim() != 1 or not len(logA) or nb % len(logA):
+    if logA.dim() != 1 or not logA.shape[0] or nb % logA.shape[0]:
         raise ValueError(f"{who}: logA must be (heads,) with heads dividing the {nb} value "
                          f"sequences, got {tuple(logA.shape)}")
     if not (1 <= r <= MAX_D and 1 <= p <= MAX_D):
@@ -104,7 +118,7 @@ def scan(Q, K, V, logA, state, scale, segments, want_state: bool, save: bool, le
     """``(o, state_out or None, kept, inputs)``: the forward over checked arguments; ``kept`` is
     what the backward takes from it (the states entering the runs and, to learn the decays,
     those entering the chunks), ``inputs`` are the tensors that the kernels read."""
-    plan = _Plan("head_decay_scan", Q, V, len(logA), segments)
+    plan = _Plan("head_decay_scan", Q, V, logA.shape[0], segments)
     code, dev = _code(Q, "head_decay_scan"), Q.device
     (Q, q_sb, q_st), (K, k_sb, k_st), (V, v_sb, v_st) = map(_near_rows, (Q, K, V))
     logA = logA.float().contiguous()
@@ -132,7 +146,7 @@ def scan_backward(inputs, kept, dO, dS, scale, segments, want_dstate: bool, lear
     """``(dQ, dK, dV, dlogA or None, dstate or None)`` of one forward."""
     Q, K, V, logA = inputs
     start, chunk_states = kept
-    plan = _Plan("head_decay_scan", Q, V, len(logA), segments)
+    plan = _Plan("head_decay_scan", Q, V, logA.shape[0], segments)
     code, dev = _code(Q, "head_decay_scan"), Q.device
     (_, q_sb, q_st), (_, k_sb, k_st), (_, v_sb, v_st) = map(_near_rows, (Q, K, V))
     dO, d_sb, d_st = _near_rows(dO)
@@ -144,7 +158,7 @@ def scan_backward(inputs, kept, dO, dS, scale, segments, want_dstate: bool, lear
               if want_dstate else None)
     dlogA = None
     if learn:
-        dlogA = (torch.empty if plan.nb else torch.zeros)(len(logA), device=dev,
+        dlogA = (torch.empty if plan.nb else torch.zeros)(logA.shape[0], device=dev,
                                                           dtype=torch.float32)
     ws, n = plan.workspace(1, int(learn), dev)
     if dS is not None:

@@ -96,6 +96,9 @@ CASES = [
     (2, 8191, "linear", True, True, True, 0.0),
     (2, 8192, "silu", True, True, True, 0.1),
     (5000, 40, "sigmoid", True, True, True, 0.1),
+    # more rows than workgroups at a time, sixteen waves a row
+    (515, 4100, "sigmoid", True, True, True, 0.1),
+    (600, 8192, None, True, False, True, 0.0),
 ]
 
 
