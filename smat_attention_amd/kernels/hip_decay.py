@@ -180,9 +180,8 @@ class HeadDecayFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, Q, K, V, logA, state, scale, segments, want_state):
         learn = ctx.needs_input_grad[3]
-        o, s_out, kept, inputs = scan(
-            Q.detach(), K.detach(), V.detach(), logA.detach(),
-            None if state is None else state.detach(), scale, segments, want_state, True, learn)
+        o, s_out, kept, inputs = scan(Q, K, V, logA, state, scale, segments, want_state, True,
+                                      learn)
         ctx.save_for_backward(*inputs, *kept)
         ctx.meta = (scale, segments, logA.dtype, learn)
         ctx.set_materialize_grads(False)
@@ -191,7 +190,8 @@ class HeadDecayFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dO, dS):
-        inputs, kept = ctx.saved_tensors[:4], ctx.saved_tensors[4:]
+        saved = ctx.saved_tensors
+        inputs, kept = saved[:4], saved[4:]
         scale, segments, a_type, learn = ctx.meta
         if dO is None and dS is None:
             return (None,) * 8

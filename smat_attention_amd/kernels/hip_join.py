@@ -105,9 +105,8 @@ class BlockJoinFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, f, h, gate, post, vector, pre, seed, opt):
-        d = [None if t is None else t.detach() for t in (f, h, gate, post, vector, pre)]
-        out, x, factors = forward(*d, seed, opt, True)
-        ctx.save_for_backward(*d, factors)
+        out, x, factors = forward(f, h, gate, post, vector, pre, seed, opt, True)
+        ctx.save_for_backward(f, h, gate, post, vector, pre, factors)
         ctx.opt = opt
         ctx.set_materialize_grads(False)
         return out, x
@@ -127,8 +126,8 @@ class BlockJoinFunction(torch.autograd.Function):
         dho = torch.empty(shape, device=dev, dtype=h.dtype)
         rows = f2.shape[0]
         make = torch.empty if rows else torch.zeros
-        sums = [make(D, device=dev, dtype=torch.float32)
-                if w is not None and ctx.needs_input_grad[i] else None
+        need = ctx.needs_input_grad
+        sums = [make(D, device=dev, dtype=torch.float32) if w is not None and need[i] else None
                 for i, w in ((3, post), (4, vector), (5, pre))]
         n = (_lib.query("smat_block_join_workspace_bytes", rows, D)
              if any(s is not None for s in sums) else 0)
