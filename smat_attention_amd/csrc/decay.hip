@@ -384,7 +384,8 @@ extern "C" int smat_head_decay_scan_backward(
   g.part = sc.part[2];
   all.w[2] = g;
   // in one launch where one kernel serves all three (96 sequences of 4096, 64 x 64, three
-  // terms everywhere: 149 us, one after the other 174; now 136), and its grid has less than 2^32 threads along the axis
+  // terms everywhere: 149 us, one after the other 174; now 130), and its grid has less than
+  // 2^32 threads along the axis
   if (!learn && dl::rblocks(r) == dl::rblocks(p) && (r <= 64) == (p <= 64) && nb < (1 << 21)) {
     rc = walk_all(dtype, all, true, kNone, st);
     if (rc) return rc;

@@ -6,6 +6,8 @@ the arithmetic before it: fp32 sums of products whose operands carry 24 bits.  E
 sum of terms; ``big`` is the same sum over the terms' magnitudes (the oracle on absolute values),
 and each term has passed at most r + p + 128 roundings of 2^-24 of what it was added to in its own
 chunk, and 72 (64 tokens, the decay, the splits) in each of the chunks the state took it through.
+(The products of an output of 16 bits take the state and P to 17 bits, 2^-17 = 128 * 2^-24 of each
+term: as much as the count has beyond the r + p + 72 roundings of a chunk's own sums.)
 """
 import math
 
