@@ -451,7 +451,7 @@ static int launch_join(int dtype, int h_dtype, Args& g, hipStream_t st) {
   return go(float(), float());
 }
 
-static int check(const char* who, int dtype, int h_dtype, const Args& g, float p) {
+static int check(const char* who, int dtype, int h_dtype, const Args& g, double p) {
   SMAT_REQUIRE(dtype == SMAT_BF16 || dtype == SMAT_F16 || dtype == SMAT_F32, SMAT_EINVAL,
                "%s: unknown dtype %d", who, dtype);
   SMAT_REQUIRE(h_dtype == dtype || h_dtype == SMAT_F32, SMAT_EINVAL,
@@ -465,7 +465,7 @@ static int check(const char* who, int dtype, int h_dtype, const Args& g, float p
   for (int t : g.wt)
     SMAT_REQUIRE(t == SMAT_BF16 || t == SMAT_F16 || t == SMAT_F32, SMAT_EINVAL,
                  "%s: unknown weight dtype %d", who, t);
-  SMAT_REQUIRE(g.eps >= 0.f && p >= 0.f && p < 1.f && (p == 0.f || g.seed), SMAT_EINVAL,
+  SMAT_REQUIRE(g.eps >= 0.f && p >= 0 && p < 1 && (p == 0 || g.seed), SMAT_EINVAL,
                "%s: eps=%g, dropout=%g (needs a seed)", who, g.eps, p);
   return SMAT_OK;
 }
@@ -515,7 +515,7 @@ extern "C" int smat_block_join(int dtype, int h_dtype, const void* f, const void
   const char* who = "smat_block_join";
   Args g = make(f, h, z, post, s, pre, post_t, s_t, pre_t, seed, rows, D, gate, eps, scale, p, salt,
                 f_st, h_st, z_st);
-  const int rc = check(who, dtype, h_dtype, g, (float)p);
+  const int rc = check(who, dtype, h_dtype, g, p);
   if (rc) return rc;
   if (rows == 0) return SMAT_OK;
   SMAT_REQUIRE(f && h && h2 && (!gate || z) && (!pre || x), SMAT_EINVAL, "%s: null pointer", who);
@@ -545,7 +545,7 @@ extern "C" int smat_block_join_backward(
   const int64_t* seed = (const int64_t*)(factors ? factors + 2 * rows : nullptr);
   Args g = make(f, h, z, post, s, pre, post_t, s_t, pre_t, seed, rows, D, gate, eps, scale, p, salt,
                 f_st, h_st, z_st);
-  const int rc = check(who, dtype, h_dtype, g, (float)p);
+  const int rc = check(who, dtype, h_dtype, g, p);
   if (rc) return rc;
   if (rows == 0) return SMAT_OK;
   SMAT_REQUIRE(f && h && factors && ((uintptr_t)factors & 7) == 0 && df && dh_out &&

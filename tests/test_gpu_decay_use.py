@@ -250,6 +250,45 @@ def test_past_31_bits():
     assert torch.equal(h[-T:], a) and torch.equal(x[-T:], b)
 
 
+def test_the_same_tensor_twice():
+    """One tensor as queries, keys and values, and as a block's output and its residual: the
+    gradients are the sums of the separate ones'."""
+    q, _, _, logA, _ = inputs(2, 2, 200, 64, 64, 2, FP32, seed=40)
+    dO = torch.randn(2, 200, 64, device=DEV)
+    one = q.clone().requires_grad_(True)
+    three = [q.clone().requires_grad_(True) for _ in range(3)]
+    a, b = A.head_decay_scan(one, one, one, logA), A.head_decay_scan(*three, logA)
+    assert torch.equal(a, b)
+    got, = torch.autograd.grad(a, one, dO)
+    dq, dk, dv = (t.double() for t in torch.autograd.grad(b, three, dO))
+    # two fp32 additions, in whichever order
+    lim = 2 * 2.0 ** -24 * (dq.abs() + dk.abs() + dv.abs())
+    assert ((got.double() - (dq + dk + dv)).abs() <= lim).all()
+    w = torch.rand(64, device=DEV)
+    two = [q.clone().requires_grad_(True) for _ in range(2)]
+    (h, x), (h2, x2) = (A.block_join(f, r, post_weight=w, pre_weight=w)
+                        for f, r in ((one, one), two))
+    assert torch.equal(h, h2) and torch.equal(x, x2)
+    got, = torch.autograd.grad((h, x), one, (dO, dO))
+    df, dh = (t.double() for t in torch.autograd.grad((h2, x2), two, (dO, dO)))
+    assert ((got.double() - (df + dh)).abs() <= 2.0 ** -24 * (df.abs() + dh.abs())).all()
+
+
+def test_an_input_changed_after_the_forward_is_refused():
+    q, k, v, logA, _ = inputs(1, 1, 70, 16, 16, 1, FP32, seed=41)
+    f = v.clone()
+    x = [t.requires_grad_(True) for t in (q, k, v, logA)]
+    o = A.head_decay_scan(*x)
+    r = f.clone().requires_grad_(True)
+    h, _ = A.block_join(f, r, gate=f)
+    with torch.no_grad():
+        x[2].zero_()
+        f.zero_()
+    for y in (o, h):
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad(y.sum(), x if y is o else r)
+
+
 def _layer(P, x, h, scan, join, mask):
     """One block over (B, T, D): projections, the scan over heads, the output's projection, and
     the block's end."""

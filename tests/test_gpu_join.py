@@ -265,6 +265,17 @@ def test_zero_rows_and_far_gates():
             check(name, a, b, big[name], 136)
 
 
+def test_rates_at_the_ends():
+    """A rate whose threshold is the generator's last word, and one below half a step, which
+    keeps everything: both within the documented range."""
+    f, h = torch.ones(64, 512, device=DEV), torch.zeros(64, 512, device=DEV)
+    seed = torch.tensor([5], device=DEV)
+    y, _ = A.block_join(f, h, dropout=1 - 2.0 ** -40, seed=seed)
+    assert ((y == 0) | (y == 2.0 ** 40)).all()
+    y, _ = A.block_join(f, h, dropout=2.0 ** -40, seed=seed)
+    assert torch.equal(y, f)
+
+
 def test_seed_steps_before_the_backward():
     """The gradient belongs to the forward's mask, whatever the seed holds by then."""
     f, h = (torch.randn(9, 50, device=DEV) for _ in range(2))
