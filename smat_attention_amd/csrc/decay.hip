@@ -210,8 +210,8 @@ extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int3
   dl::dispatch(dtype, r, [&](auto in, auto rb) {
     typedef decltype(in) In;
     constexpr int RB = decltype(rb)::value;
-    on = p <= 64 ? hd::walk_occ<In, RB, 64, true, 0>() * 4 / hd::waves<In, 64, 0>()
-                 : hd::walk_occ<In, RB, 128, true, 0>() * 4 / hd::waves<In, 128, 0>();
+    on = p <= 64 ? hd::walk_occ<In, RB, 64, true, 0>() * 4 / hd::waves<In, 64, true, 0>()
+                 : hd::walk_occ<In, RB, 128, true, 0>() * 4 / hd::waves<In, 128, true, 0>();
     return 0;
   });
   static const double terms[] = {1.0, 1.35, 1.7}, share[] = {0.0, 1.0, 1.45, 1.9};

@@ -29,11 +29,11 @@
 // to a 16-bit output two, 17 bits.  Results are rounded once, where they are stored.
 //
 // Per chunk, bf16, r = p = 128: 196 MFMA and some 850 vector instructions a wave (the splits
-// most of them), two waves a SIMD; 8 sequences of 131072 take 298 us with outputs (3.6 TB/s;
-// every row in L2 takes a fifth less) and 150 in the first pass (3.6); 32 of 8192, 64 x 64, 39
+// most of them), two waves a SIMD; 8 sequences of 131072 take 294 us with outputs (3.6 TB/s;
+// every row in L2 takes a fifth less) and 127 in the first pass (4.2); 32 of 8192, 64 x 64, 39
 // and 20.  So it is bound by how well two or three waves a SIMD cover a chunk's chain of LDS
 // reads, products, splits and barriers, and next by HBM.  fp16 has twice the tiles and products
-// and one workgroup of eight waves a CU: 12 of 10007, 96 x 96, 83 and 37 (2.2 TB/s in the two).
+// and one workgroup of eight waves a CU: 12 of 10007, 96 x 96, 83 and 29.
 // Tried and slower or no faster: volatile LDS reads, products and splits interleaved by hand,
 // two column tiles a wave with LEARN (spills), splits in registers ahead of fp16's products.
 #pragma once
@@ -315,13 +315,15 @@ __device__ __forceinline__ Frag<Terms<In>::in> value_rows(const bf16* tile, int 
 }
 
 // The column tiles of a wave and the waves of a workgroup, by the columns of all (64 or 128):
-// two tiles a wave share the reads of K, Q and P.  With LEARN they would not fit the registers,
-// and inputs of several terms leave LDS for one workgroup a CU, which eight waves fill better.
-template <typename In, int P, int LEARN> constexpr int tiles() {
-  return P == 64 || LEARN || Terms<In>::in > 1 ? 1 : 2;
+// two tiles a wave share the reads of K, Q and P (8 sequences of 131072, 128 x 128: 294 us, with
+// one 385, at four waves a SIMD and registers spilt).  With LEARN they would not fit the registers,
+// inputs of several terms leave LDS for one workgroup a CU, which eight waves fill better, and the
+// first pass reads K alone: four waves a SIMD there (127 us, two of two tiles 152).
+template <typename In, int P, bool OUT, int LEARN> constexpr int tiles() {
+  return P == 64 || !OUT || LEARN || Terms<In>::in > 1 ? 1 : 2;
 }
-template <typename In, int P, int LEARN> constexpr int waves() {
-  return P / 16 / tiles<In, P, LEARN>();
+template <typename In, int P, bool OUT, int LEARN> constexpr int waves() {
+  return P / 16 / tiles<In, P, OUT, LEARN>();
 }
 constexpr int kMaxWaves = 8;
 template <typename In, int P> constexpr int value_elems() {
@@ -341,15 +343,16 @@ template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets)
 }
 // Waves a SIMD: as many as registers and LDS have room for.
 template <typename In, int RB, int P, bool OUT, int LEARN> constexpr int walk_occ() {
-  const int fit = dl::kMaxLds / walk_lds<In, RB, P, OUT>(1) * waves<In, P, LEARN>() / 4;
-  const int most = LEARN ? 2 : !OUT ? (P == 64 ? 4 : RB > 2 ? 2 : 3) : P == 64 && RB < 3 ? 3 : 2;
+  const int fit = dl::kMaxLds / walk_lds<In, RB, P, OUT>(1) * waves<In, P, OUT, LEARN>() / 4;
+  const bool few = P == 128 && RB * Terms<In>::in > (Terms<In>::in == 3 ? 3 : 6);
+  const int most = LEARN ? 2 : !OUT ? (few ? 2 : 4) : P == 64 && RB < 3 ? 3 : 2;
   return fit < most ? fit : most;
 }
 // Two sets, so that the next chunk's rows are written beside this one's use, where that many
 // still fit.
 template <typename In, int RB, int P, bool OUT, int LEARN> constexpr int walk_sets() {
   return walk_lds<In, RB, P, OUT>(2) * walk_occ<In, RB, P, OUT, LEARN>() * 4 /
-                     waves<In, P, LEARN>() <= dl::kMaxLds ? 2 : 1;
+                     waves<In, P, OUT, LEARN>() <= dl::kMaxLds ? 2 : 1;
 }
 
 // Four consecutive values of a row as they come, at the element's own alignment: of columns
@@ -423,7 +426,7 @@ __device__ __forceinline__ void steps(Load load, Use use) {
 
 template <typename In, int RB, int P, bool OUT, int LEARN>
 __global__
-__launch_bounds__((64 * waves<In, P, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void
+__launch_bounds__((64 * waves<In, P, OUT, LEARN>()), (walk_occ<In, RB, P, OUT, LEARN>())) void
 decay_walk_kernel(Walks all) {
   // with several, workgroups of one sequence and run lie eight apart: on one XCD, whose L2 they
   // share the rows in
@@ -431,7 +434,7 @@ decay_walk_kernel(Walks all) {
   const int s = all.n == 1 ? (int)blockIdx.x : (int)blockIdx.x / 24 * 8 + (int)blockIdx.x % 8;
   const Walk& g = all.w[role];
   if (s >= g.nb) return;
-  constexpr int W = waves<In, P, LEARN>(), CT = tiles<In, P, LEARN>(), VB = P / 32;
+  constexpr int W = waves<In, P, OUT, LEARN>(), CT = tiles<In, P, OUT, LEARN>(), VB = P / 32;
   constexpr int NT = Terms<In>::in, NI = kMid, NO = out_terms<In>();
   constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>();
   constexpr int SET = set_elems<In, RB, P, OUT>();
@@ -904,7 +907,7 @@ static void walk(const Walks& a, hipStream_t st) {
   static uint64_t done;
   dl::allow_lds(kern, lds, done);
   const int nb = a.w[0].nb, x = a.n == 1 ? nb : (nb + 7) / 8 * 24;
-  hipLaunchKernelGGL(kern, dim3(x, a.w[0].nruns), dim3(64 * waves<In, P, LEARN>()), lds, st, a);
+  hipLaunchKernelGGL(kern, dim3(x, a.w[0].nruns), dim3(64 * waves<In, P, OUT, LEARN>()), lds, st, a);
 }
 
 // One file a type instantiates it.
