@@ -634,7 +634,7 @@ int smat_delta_step(int dtype, const void* q, const void* k, const void* v, cons
  * it (may be NULL; not state itself).
  * Training: save_start (nruns, nb, r, p) fp32 receives the states entering runs (only where
  * nruns > nseg; may be NULL), save_s (nb, nch, P, R) fp32 those entering chunks, R being r
- * rounded up to 32 and P 64 or 128 (may be NULL: needed for dlogA).
+ * rounded up to 32 and P 64 or 128, 16-byte aligned (may be NULL: needed for dlogA).
  * workspace: smat_head_decay_workspace_bytes(..., backward, learn) bytes, 256-byte aligned.
  */
 int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,

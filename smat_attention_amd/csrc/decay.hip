@@ -14,20 +14,25 @@ namespace hd {
 
 // The states entering the runs of a segment, from init or from zero; `rev`: the runs in
 // turned order.  Every element on its own, sixteen runs' E in flight; bound by E in and the
-// states out (8 x 64 runs of 128 x 128: 16 us, 4.2 TB/s).
-__global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* __restrict__ init,
-                                                          const float* __restrict__ E,
-                                                          float* __restrict__ start) {
-  constexpr int U = 16, BLOCK = 256;
+// states out: 16 sequences of 32 runs of 128 x 128 in 6 segments 11.6 us, 5.5 TB/s (one element a
+// thread 20), and where runs are many and elements few by a batch's latency: 8 of 64 runs 16.
+// T: one element, or four (a wave then reads 1 KB of a run).
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void decay_carry_kernel(Walk g, const T* __restrict__ init,
+                                                            const T* __restrict__ E,
+                                                            T* __restrict__ start) {
+  constexpr int U = 16;
   __shared__ float decay[BLOCK];                   // of the tokens of a block of runs
   const int s = blockIdx.x, seg = blockIdx.z;
-  const int64_t rp = (int64_t)g.r * g.p, e = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  const int64_t rp = (int64_t)g.r * g.p / (sizeof(T) / 4);
+  const int64_t e = (int64_t)blockIdx.y * BLOCK + threadIdx.x;
   const int r0 = g.segrun ? g.segrun[seg] : 0, r1 = g.segrun ? g.segrun[seg + 1] : g.nruns;
   auto run_at = [&](int n) { return g.rev ? r0 + r1 - 1 - n : n; };
   const int64_t step = g.nb * rp;                  // between a sequence's runs
-  const float* E0 = E + s * rp + min(e, rp - 1);
-  float* start0 = start + s * rp + e;
-  float S = init && e < rp ? init[((int64_t)seg * g.nb + s) * rp + e] : 0.f;
+  const T* E0 = E + s * rp + min(e, rp - 1);
+  T* start0 = start + s * rp + e;
+  T S = {};
+  if (init && e < rp) S = init[((int64_t)seg * g.nb + s) * rp + e];
   for (int b = r0; b < r1; b += BLOCK) {
     __syncthreads();
     if (b + (int)threadIdx.x < r1) {
@@ -45,10 +50,12 @@ __global__ __launch_bounds__(256) void decay_carry_kernel(Walk g, const float* _
     }
     __syncthreads();
     for (int n = b; n < min(b + BLOCK, r1); n += U) {
-      float x[U];
+      T x[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)                  // a segment's last run has no E: another's
-        x[u] = r1 - r0 > 1 ? E0[run_at(min(n + u, r1 - 2)) * step] : 0.f;
+      for (int u = 0; u < U; ++u) {                // a segment's last run has no E: another's
+        x[u] = T{};
+        if (r1 - r0 > 1) x[u] = E0[run_at(min(n + u, r1 - 2)) * step];
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (n + u < r1) {
@@ -119,8 +126,12 @@ static int carry(int dtype, const Walk& base, const float* init, float* E, float
   int rc = walk_any(dtype, g, false, kNone, st);
   if (rc) return rc;
   const int64_t rp = (int64_t)g.r * g.p;
-  hipLaunchKernelGGL(decay_carry_kernel, dim3(g.nb, (rp + 255) / 256, g.nseg), dim3(256), 0, st, g,
-                     init, E, start);
+  if (rp % 4 == 0 && aligned16(init) && aligned16(E) && aligned16(start))
+    hipLaunchKernelGGL((decay_carry_kernel<f32x4, 64>), dim3(g.nb, (rp + 255) / 256, g.nseg),
+                       dim3(64), 0, st, g, (const f32x4*)init, (const f32x4*)E, (f32x4*)start);
+  else
+    hipLaunchKernelGGL((decay_carry_kernel<float, 256>), dim3(g.nb, (rp + 255) / 256, g.nseg),
+                       dim3(256), 0, st, g, init, E, start);
   return launch_status("smat_head_decay_scan: carry");
 }
 
@@ -193,10 +204,10 @@ static Scratch take(dl::Arena& ar, int64_t nb, int64_t nbk, int64_t T, int nseg,
 // times that where inputs have two and three terms, and 0.42 of it in the first pass.  Two
 // workgroups on a CU take 1.45 times as long each, three (bf16, 64 columns) 1.9; more than fit
 // follow one another.  The carry moves its states at 4 TB/s, and two launches more
-// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 8008 in two runs, 586 in 32, 455 in
-// 64, 506 in 128; 32 of 128 chunks, 64 x 64: 323 whole, 80 in 8, 64 in 16, 67 in 22; 96 of 64
-// chunks with gradients: 393 whole, 266 in 4, 241 in 8, 275 in 16; fp16, 12 of 157 chunks,
-// 96 x 96: 131 in 16, 113 in 20, 125 in 40.)
+// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 7391 in two runs, 538 in 32, 436 in
+// 64, 481 in 128; 32 of 128 chunks, 64 x 64: 323 whole, 80 in 8, 64 in 16, 67 in 22; 96 of 64
+// chunks with gradients: 393 whole, 270 in 4, 236 in 8, 273 in 16; fp16, 12 of 157 chunks,
+// 96 x 96: 135 in 16, 116 in 20, 116 in 40.)
 extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
                                           const int32_t* times, int n, int r, int p) {
   using namespace smat;
@@ -276,6 +287,7 @@ extern "C" int smat_head_decay_scan(int dtype, const void* q, const void* k, con
   if (nb == 0) return SMAT_OK;
   SMAT_REQUIRE(logA && (nch == 0 || (q && k && v && out)), SMAT_EINVAL, "%s: null pointer", who);
   SMAT_REQUIRE(state_out != state || !state, SMAT_EINVAL, "%s: state_out must not be state", who);
+  SMAT_REQUIRE(aligned16(save_s), SMAT_EINVAL, "%s: save_s is not 16-byte aligned", who);
   rc = check_workspace(who, workspace, workspace_bytes,
                        smat_head_decay_workspace_bytes(nb, nbk, T, nseg, nruns, r, p, 0, 0));
   if (rc) return rc;
@@ -325,6 +337,7 @@ extern "C" int smat_head_decay_scan_backward(
                "%s: null pointer", who);
   SMAT_REQUIRE((nruns == nseg || start) && (!learn || save_s || nch == 0), SMAT_EINVAL,
                "%s: the states that the forward kept are missing", who);
+  SMAT_REQUIRE(aligned16(save_s), SMAT_EINVAL, "%s: save_s is not 16-byte aligned", who);
   rc = check_workspace(
       who, workspace, workspace_bytes,
       smat_head_decay_workspace_bytes(nb, nbk, T, nseg, nruns, r, p, 1, learn));

@@ -115,9 +115,9 @@ def test_step_refusals(anywhere):
 def test_entry_refusals():
     """What the C entries themselves refuse, before any launch."""
     def scan(nb=1, nbk=1, heads=1, T=17, nch=1, r=8, p=8, st=8, ws=FAKE << 8, dtype=0, nseg=1,
-             nruns=1, tables=(None,) * 3):
-        _lib.call("smat_head_decay_scan", dtype, FAKE, FAKE, FAKE, FAKE, None, FAKE, None, None, None,
-                  *tables, nb, nbk, heads, T, nseg, nch, nruns, 1, r, p, 1.0, 64, st, 64, 8, 64, 8,
+             nruns=1, tables=(None,) * 3, save_s=None):
+        _lib.call("smat_head_decay_scan", dtype, FAKE, FAKE, FAKE, FAKE, None, FAKE, None, None,
+                  save_s, *tables, nb, nbk, heads, T, nseg, nch, nruns, 1, r, p, 1.0, 64, st, 64, 8, 64, 8,
                   ws, 1 << 50, None)
     for kw, match in ((dict(r=7), "must lie in 8..128"), (dict(p=129), "must lie in 8..128"),
                       (dict(nb=3, nbk=2), "must divide"), (dict(nb=3, heads=2), "must divide"),
@@ -125,6 +125,7 @@ def test_entry_refusals():
                       (dict(st=-8), "elements apart"), (dict(T=65), "1 chunks for T=65"),
                       (dict(T=65, nch=2), "runs of 1 chunks"), (dict(dtype=3), "unknown dtype"),
                       (dict(tables=(FAKE, None, None)), "need the chunk"),
+                      (dict(save_s=FAKE + 4), "16-byte aligned"),
                       (dict(T=2 ** 31 - 1, nch=2 ** 25), "bad sizes")):
         with pytest.raises(HipKernelError, match=match):
             scan(**kw)

@@ -145,6 +145,7 @@ def test_fp32_results_have_fp32_accuracy(dtype):
     (2, 2, 64 * 40 + 5, 64, 64, None, True),
     (2, 1, 64 * 33, 128, 48, None, False),
     (1, 1, 64 * 70 + 1, 40, 99, [0, 64 * 50 + 3, 64 * 50 + 3, 64 * 70 + 1], True),
+    (1, 1, 64 * 40, 41, 99, None, True),
 ])
 def test_split_along_the_sequence(dtype, nb, nbk, T, r, p, off, st):
     """Few long sequences are cut into runs joined through their decays."""
@@ -167,6 +168,16 @@ def test_split_along_the_sequence(dtype, nb, nbk, T, r, p, off, st):
     check("S", So.detach(), rS, bS, ch, r, p)
     for name, a, b, big in zip(("dq", "dk", "dv", "dlogA", "dS0"), got, rg, bg):
         check(name, a, b, big, ch, r, p)
+
+
+def test_a_state_at_any_address():
+    """A state that does not begin at 16 bytes enters the runs as another does: every element goes
+    the same way."""
+    q, k, v, logA, S = inputs(2, 2, 64 * 40, 64, 64, 2, BF16, seed=23, lead=(), slow=2.0 ** -12)
+    off = torch.empty(S.numel() + 1, device=DEV)[1:].view_as(S).copy_(S)
+    assert off.data_ptr() % 16
+    a, b = (A.head_decay_scan(q, k, v, logA, state=s, return_state=True) for s in (S, off))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
 @pytest.mark.parametrize("la", [0.0, -1e-7, -30.0, -200.0, -math.inf])
