@@ -25,8 +25,9 @@
 //
 // Operands: every product runs on v_mfma_f32_16x16x32_bf16, values held in fewer than
 // their own bits as sums of bf16 terms (delta_common.hpp): bf16 inputs one term, fp16 two,
-// fp32 and what is computed in fp32 three, 24 bits; the state and P where they meet rows
-// to a 16-bit output two, 17 bits.  Results are rounded once, where they are stored.
+// fp32 and what is computed in fp32, the state and P, three, 24 bits, whatever the output's
+// type: with two, outputs that are small differences of large sums are off by many of their own
+// steps.  Results are rounded once, where they are stored.
 //
 // Per chunk, bf16, r = p = 128: 196 MFMA and some 850 vector instructions a wave (the splits
 // most of them), two waves a SIMD; 8 sequences of 131072 take 294 us with outputs (3.6 TB/s;
@@ -124,32 +125,6 @@ template <int NT> __device__ __forceinline__ Frag<kMid> terms(const f32x4& a, co
     return cut(a, b);
   else
     return dl::split<kMid>(a, b);
-}
-
-// The state and P where they meet rows to an output of 16 bits: two terms, 17 bits, off by at
-// most 2^-17 of the value, where storing rounds by 2^-9 (bf16) or 2^-12 (fp16); an fp32 output
-// takes three.  Nothing of it enters the state.  The first terms of a value are the same
-// however many follow.
-template <typename In> constexpr int out_terms() { return sizeof(In) == 2 ? 2 : kMid; }
-template <int N> __device__ __forceinline__ Frag<N> first_terms(const f32x4& a, const f32x4& b) {
-  const Frag<kMid> all = dl::split<kMid>(a, b);
-  Frag<N> f;
-#pragma unroll
-  for (int n = 0; n < N; ++n) f.t[n] = all.t[n];
-  return f;
-}
-// Their products: of two and two terms all, of three and three those of order below three.
-template <int U, int NA, int NB>
-__device__ __forceinline__ void mul_out(f32x4 (&c)[U], const Frag<NA> (&a)[U],
-                                        const Frag<NB> (&b)[U]) {
-  constexpr int M = NA + NB < 4 ? NA + NB - 1 : 3;
-#pragma unroll
-  for (int o = M - 1; o >= 0; --o)
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-      if (o - i >= 0 && o - i < NB)
-#pragma unroll
-        for (int u = 0; u < U; ++u) c[u] = mma(c[u], a[u].t[i], b[u].t[o - i]);
 }
 
 // A chunk's rows in LDS, 32 B columns of 16 bits: row t at t (64 B + 32) bytes, and 16 more in
@@ -338,7 +313,7 @@ template <typename In> constexpr int tab_floats() {
   return C + 4 + 2 * C + (Terms<In>::in == 1 ? 4 * 256 : 0);
 }
 template <typename In, int RB, int P, bool OUT> constexpr int walk_lds(int sets) {
-  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? out_terms<In>() * kLow * kFrag * 2 : 0) +
+  return sets * set_elems<In, RB, P, OUT>() * 2 + (OUT ? kMid * kLow * kFrag * 2 : 0) +
          tab_floats<In>() * 4;
 }
 // Waves a SIMD: as many as registers and LDS have room for.
@@ -435,14 +410,14 @@ decay_walk_kernel(Walks all) {
   const Walk& g = all.w[role];
   if (s >= g.nb) return;
   constexpr int W = waves<In, P, OUT, LEARN>(), CT = tiles<In, P, OUT, LEARN>(), VB = P / 32;
-  constexpr int NT = Terms<In>::in, NI = kMid, NO = out_terms<In>();
+  constexpr int NT = Terms<In>::in, NI = kMid;
   constexpr int KT = NT * tile_elems(RB), VT = value_elems<In, P>();
   constexpr int SET = set_elems<In, RB, P, OUT>();
   constexpr int KD = walk_sets<In, RB, P, OUT, LEARN>(), TP = (kTiles + W - 1) / W;
   constexpr bool AHEAD = NT == 1;                  // (two terms: as fast without)
   extern __shared__ __align__(1024) bf16 lds[];
   bf16* pl = lds + KD * SET;
-  float* tab = reinterpret_cast<float*>(pl + (OUT ? NO * kLow * kFrag : 0));   // a^0 .. a^64
+  float* tab = reinterpret_cast<float*>(pl + (OUT ? NI * kLow * kFrag : 0));   // a^0 .. a^64
   float* wt = tab + C + 4;                         // wt[64 - n + j] = w_j of a chunk of n
   const int w = dl::uniform_wave();
   const int m = lane_id() & 15, gq = lane_id() >> 4;
@@ -661,21 +636,16 @@ decay_walk_kernel(Walks all) {
                   acc += (float)(16 * (mt - jt) + m - 4 * gq - i) * (x[i] * z[i]);
               }
             }
-            const Frag<NO> f = first_terms<NO>(x, zero4());
+            const Frag<NI> f = terms<NT>(x, zero4());
             const int half = mt == 2 && jt == 2 ? 1 : jt & 1;
             bf16* at = pl + dl::tri(mt, jt >> 1) * kFrag + lane_id() * 8 + 4 * half;
 #pragma unroll
-            for (int n = 0; n < NO; ++n)
+            for (int n = 0; n < NI; ++n)
               *reinterpret_cast<bf16x4*>(at + n * kLow * kFrag) = dl::low_half(f.t[n]);
           });
       // (Q S)^T: columns in registers, the token in the lane
 #pragma unroll
       for (int i = 0; i < CT * 4; ++i) ot[i / 4][i % 4] = zero4();
-      // the decays' gradient is fp32: it takes the state's third term too
-      constexpr int NS = LEARN == kDq || LEARN == kDk ? NI : NO;
-      f32x4 low[NS > NO ? 4 : 1];
-#pragma unroll
-      for (f32x4& x : low) x = zero4();
       struct Four {
         Frag<NT> q[4];
       };
@@ -685,23 +655,15 @@ decay_walk_kernel(Walks all) {
             for (int mt = 0; mt < 4; ++mt) b.q[mt] = rows_of<RB, NT>(qt, mt, kb);
           },
           [&](int kb, Four& b) {
-            Frag<NS> sb[CT];
+            Frag<NI> sb[CT];
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct)
-              sb[ct] = first_terms<NS>(S[ct][2 * kb], S[ct][2 * kb + 1]);
+            for (int ct = 0; ct < CT; ++ct) sb[ct] = terms<NT>(S[ct][2 * kb], S[ct][2 * kb + 1]);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
-              Frag<NO> all[4];
+              Frag<NI> all[4];
 #pragma unroll
-              for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-                for (int n = 0; n < NO; ++n) all[mt].t[n] = sb[ct].t[n];
-              mul_out(ot[ct], all, b.q);
-              if constexpr (NS > NO) {
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt)
-                  low[mt] = mma(low[mt], sb[ct].t[NS - 1], b.q[mt].t[0]);
-              }
+              for (int mt = 0; mt < 4; ++mt) all[mt] = sb[ct];
+              dl::mul_each(ot[ct], all, b.q);
             }
           });
 #pragma unroll
@@ -723,9 +685,7 @@ decay_walk_kernel(Walks all) {
                                   : four_of(row_of(mt), col, g.p, t < len);
             float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              dot += x[i] * (NS > NO ? ot[0][mt][i] + e[mt] * low[NS > NO ? mt : 0][i]
-                                     : ot[0][mt][i]);
+            for (int i = 0; i < 4; ++i) dot += x[i] * ot[0][mt][i];
             acc += (float)(t + (g.rev ? 0 : 1)) * dot;
           }
         }
@@ -750,14 +710,14 @@ decay_walk_kernel(Walks all) {
       // ---- P is in LDS
       __builtin_amdgcn_s_setprio(1);
       struct One {
-        Frag<NO> p;
+        Frag<NI> p;
       };
       steps<6, AHEAD, One>(
           [&](int st, One& b) {
             const int mt = st < 2 ? st : st < 4 ? 2 : 3, kb = st < 2 ? 0 : st & 1;
             const bf16* at = pl + dl::tri(mt, kb) * kFrag + lane_id() * 8;
 #pragma unroll
-            for (int n = 0; n < NO; ++n) {
+            for (int n = 0; n < NI; ++n) {
               if (dl::half_tri(mt, kb)) {
                 const bf16x4 h =
                     *reinterpret_cast<const bf16x4*>(at + n * kLow * kFrag + (mt == 2 ? 4 : 0));
@@ -772,14 +732,14 @@ decay_walk_kernel(Walks all) {
             const int mt = st < 2 ? st : st < 4 ? 2 : 3, kb = st < 2 ? 0 : st & 1;
             f32x4 x[CT];
             Frag<NT> v[CT];
-            Frag<NO> all[CT];
+            Frag<NI> all[CT];
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
               x[ct] = ot[ct][mt];
               v[ct] = vf[ct][kb];
               all[ct] = b.p;
             }
-            mul_out(x, v, all);
+            dl::mul_each(x, v, all);
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) ot[ct][mt] = x[ct];
           });
