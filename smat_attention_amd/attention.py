@@ -363,7 +363,7 @@ def block_join(f, h, *, post_weight=None, gate=None, gate_kind: str = "sigmoid",
 
     ``f (..., D)`` is the block's output, ``h`` the residual stream, of f's type or fp32, and
     ``gate`` = z, of f's type; 8 <= D <= 8192.  ``gate_kind`` is ``"sigmoid"``, ``"silu"``
-    (``z sigmoid(z)``) or ``"linear"`` (z itself).  ``post_weight, pre_weight (D,)`` and ``scale``,
+    (``z sigmoid(z)``) or ``"linear"`` (z itself); a gate of -inf is closed under the first two.  ``post_weight, pre_weight (D,)`` and ``scale``,
     a number or ``(D,)``, in any of the three types.  Without ``post_weight`` y is f, without
     ``gate`` u is y, and without ``pre_weight`` there is no x.  Returns ``(h', x)`` in h's and f's
     types, x None if there is none; computed in fp32 and rounded once.

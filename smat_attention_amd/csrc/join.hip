@@ -114,13 +114,17 @@ __device__ __forceinline__ f8 weights(const void* w, int type, float absent, int
   return y;
 }
 
-// gate(z), and its slope.  The exp is of -|z|, and 1 - sigmoid(z) is sigmoid(-z): neither
-// overflows, and nothing cancels at either end.  exp(x) is 2^(x log2 e) with the product's
+// gate(z), and its slope.  The exp is of x = -|z|, and 1 - sigmoid(z) is sigmoid(-z), so nothing
+// cancels at either end.  x ends at -200, where exp(x) has long been zero in fp32: beyond 2.3e38
+// and at infinity the products below would overflow, and then cancel to no number.  (A comparison,
+// not a minimum: what is not a number stays so.)  exp(x) is 2^(x log2 e) with the product's
 // rounding error put back, since the hardware's exponential takes it as it is, and as the square
 // of 2^(x log2 e / 2), since that instruction gives no subnormal results.
-__device__ __forceinline__ void sigmoid(float z, float& s, float& t) {
+__device__ __forceinline__ void sigmoid(float z, float& s, float& t, float& x) {
   constexpr float high = 0x1.715476p+0f, low = 0x1.4ae0cp-26f;     // log2 e
-  const float x = -fabsf(z), y = x * high;
+  x = -fabsf(z);
+  x = x < -200.f ? -200.f : x;
+  const float y = x * high;
   const float off = fmaf(x, low, fmaf(x, high, -y));
   const float root = __builtin_amdgcn_exp2f(0.5f * y);
   const float e = root * fmaf(off, 0x1.62e43p-1f, 1.f) * root;
@@ -137,18 +141,19 @@ __device__ __forceinline__ void gate_of(int kind, const f8& z, f8& a, f8& slope)
   } else if (kind == kSigmoid) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float s, t;
-      sigmoid(z[i], s, t);
+      float s, t, x;
+      sigmoid(z[i], s, t, x);
       a[i] = s;
       if (SLOPE) slope[i] = s * t;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float s, t;
-      sigmoid(z[i], s, t);
-      a[i] = z[i] * s;
-      if (SLOPE) slope[i] = s * (1.f + z[i] * t);
+      // at an infinite z the factor that is zero meets a finite one
+      float s, t, x;
+      sigmoid(z[i], s, t, x);
+      a[i] = (z[i] >= 0.f ? z[i] : x) * s;
+      if (SLOPE) slope[i] = s * (1.f + (z[i] >= 0.f ? -x : x) * t);
     }
   }
 }
