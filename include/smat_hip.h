@@ -683,10 +683,11 @@ int smat_head_decay_step(int dtype, const void* q, const void* k, const void* v,
  * f, z, x: (rows, D) of dtype; h, h2: of h_dtype (dtype or fp32); f, h, z with row strides and
  * unit column stride, outputs contiguous.  gate: 0 none (z NULL), 1 z itself, 2 sigmoid, 3 silu.
  * post, s, pre: (D) of types post_t, s_t, pre_t, or NULL: no norm after the block, `scale` for
- * every column, no x.  p: dropout in [0, 1); place (row, column) is kept, times 1 / (1 - p),
- * where its word of Philox 4x32 (ten rounds; key = *seed's low and high halves, counter =
- * column / 4, row, salt, 0; word column % 4) is at least p 2^32.  seed: one int64 on the device,
- * or NULL where p = 0.
+ * every column, no x.  p: dropout in [0, 1); place (row, column) is kept where its word of
+ * Philox 4x32 (ten rounds; key = *seed's low and high halves, counter = column / 4, row, salt, 0;
+ * word column % 4) is at least t = p 2^32, rounded to even and at most 2^32 - 1, and is then times
+ * 2^32 / (2^32 - t); a dropped place counts for nothing, finite or not.  seed: one int64 on the
+ * device, or NULL where p = 0.
  * factors: (rows + 1, 2) fp32, 8-byte aligned, receive 1 / rms(f) and 1 / rms(h2) of every row
  * and the seed's eight bytes for the gradient, or NULL.
  * 8 <= D <= 8192, rows < 2^31.

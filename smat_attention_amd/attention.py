@@ -368,8 +368,9 @@ def block_join(f, h, *, post_weight=None, gate=None, gate_kind: str = "sigmoid",
     ``gate`` u is y, and without ``pre_weight`` there is no x.  Returns ``(h', x)`` in h's and f's
     types, x None if there is none; computed in fp32 and rounded once.
 
-    ``dropout`` keeps a place with probability ``1 - dropout`` and scales it by its inverse.
-    Which ones is a function of ``seed`` (an int64 tensor of one element on the GPU: a captured
+    ``dropout`` keeps a place with probability ``1 - dropout`` and scales it by its inverse, the
+    rate rounded to a multiple of 2^-32 and at most ``1 - 2^-32``.  What is dropped counts for
+    nothing, there and in the gradient, finite or not.  Which ones is a function of ``seed`` (an int64 tensor of one element on the GPU: a captured
     graph reads it at every replay), ``salt`` (a number below 2^32, one a layer), the row and the
     column, from a counter-based generator; no mask is stored, and the gradient forms it again.
 

@@ -28,7 +28,7 @@
 //
 // Dropout's mask is never stored: place (row, column) is kept where its word of Philox 4x32,
 // ten rounds (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC 2011),
-// is at least p 2^32; key = the seed's halves, counter = (column / 4, row, salt, 0), the word
+// is at least p 2^32 (rounded to even, at most 2^32 - 1); key = the seed's halves, counter = (column / 4, row, salt, 0), the word
 // column % 4 of the four.
 #include "row_groups.hpp"
 #include "smat_host.hpp"
@@ -45,7 +45,7 @@ struct Args {
   int wt[3];
   const int64_t* seed;                     // or null: no dropout; the backward's is the kept one
   uint32_t salt, threshold;
-  float scale, keep, eps;                  // scale: where s is null; keep: 1 / (1 - p)
+  float scale, keep, eps;                  // scale: where s is null; keep: a kept place's factor
   int gate;
   int64_t rows, f_st, h_st, z_st;
   int D, group;                            // threads a row
@@ -512,7 +512,8 @@ static Args make(const void* f, const void* h, const void* z, const void* post, 
   g.scale = scale;
   const double t = rint(p * 4294967296.0);         // ties to even
   g.threshold = t >= 4294967295.0 ? 4294967295u : (uint32_t)t;
-  g.keep = (float)(1.0 / (1.0 - p));
+  // the inverse of the rate that the threshold keeps, not of 1 - p: near one they differ
+  g.keep = (float)(4294967296.0 / (4294967296.0 - g.threshold));
   g.salt = salt;
   g.f_st = f_st;
   g.h_st = h_st;
