@@ -1111,8 +1111,10 @@ class HeadDecayDecoder:
     token.
 
     ``state`` fp32 ``(nb, r, p)`` is taken over and updated in place (zero it for a new
-    sequence, copy it to branch); ``logA (heads,)`` is the layer's.  The arguments of the calls
-    are :func:`head_decay_scan`'s and :func:`head_decay_step`'s."""
+    sequence, copy it to branch); ``logA (heads,)`` is the layer's, read at every call, so that
+    an update in place is seen (fp32 and contiguous as it is; another through a copy, a launch of
+    4 us more a call).  The arguments of the calls are :func:`head_decay_scan`'s and :func:`head_decay_step`'s.  ``prefill``
+    writes the new state apart and copies it over."""
 
     def __init__(self, state: torch.Tensor, logA: torch.Tensor, *, scale: float = 1.0):
         who = "HeadDecayDecoder"
@@ -1120,19 +1122,23 @@ class HeadDecayDecoder:
         if state.dim() != 3 or state.dtype != torch.float32 or not state.is_contiguous():
             raise ValueError(f"{who}: the state must be contiguous fp32 (nb, r, p)")
         _decay.check_sizes(who, state.shape[0], state.shape[0], logA, *state.shape[1:])
-        self.S, self.logA, self.scale = state, logA.detach().float().contiguous(), float(scale)
+        self.S, self.logA, self.scale = state, logA.detach(), float(scale)
+        self._as_it_is = logA.dtype == torch.float32 and logA.is_contiguous()
+
+    def _decays(self) -> torch.Tensor:
+        return self.logA if self._as_it_is else self.logA.float().contiguous()
 
     @torch.no_grad()
     def prefill(self, Q, K, V) -> torch.Tensor:
         """Any number of tokens at once; returns ``o (nb, T, p)``."""
-        o, S = head_decay_scan(Q, K, V, self.logA, scale=self.scale, state=self.S,
+        o, S = head_decay_scan(Q, K, V, self._decays(), scale=self.scale, state=self.S,
                                return_state=True)
         self.S.copy_(S)
         return o
 
     def step(self, q, k, v, *, out=None) -> torch.Tensor:
         """One token; returns ``o (nb, p)``."""
-        return head_decay_step(q, k, v, self.logA, self.S, scale=self.scale, out=out)
+        return head_decay_step(q, k, v, self._decays(), self.S, scale=self.scale, out=out)
 
     def cache_words(self) -> int:
         return int(self.S.numel())
