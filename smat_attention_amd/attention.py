@@ -33,6 +33,7 @@ from typing import Callable, Dict, Optional
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from .kernels import hip_decay as _decay
 from .kernels import hip_delta as _delta
@@ -91,6 +92,12 @@ def _acc(x: torch.Tensor, acc_dtype, who: str) -> torch.dtype:
 # ---------------------------------------------------------------------------
 
 def _wants_grad(*ts) -> bool:
+    """Whether autograd needs this call's node.  A tangent of forward-mode differentiation is
+    refused: the kernels have none, and a result without one would read as a constant."""
+    if _forward_ad._current_level >= 0 and any(
+            t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise NotImplementedError("forward-mode derivatives are not implemented: the inputs have "
+                                  "tangents")
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
@@ -1113,8 +1120,8 @@ class HeadDecayDecoder:
     ``state`` fp32 ``(nb, r, p)`` is taken over and updated in place (zero it for a new
     sequence, copy it to branch); ``logA (heads,)`` is the layer's, read at every call, so that
     an update in place is seen (fp32 and contiguous as it is; another through a copy, a launch of
-    4 us more a call).  The arguments of the calls are :func:`head_decay_scan`'s and :func:`head_decay_step`'s.  ``prefill``
-    writes the new state apart and copies it over."""
+    4 us more a call).  The arguments of the calls are :func:`head_decay_scan`'s and
+    :func:`head_decay_step`'s.  ``prefill`` writes the new state apart and copies it over."""
 
     def __init__(self, state: torch.Tensor, logA: torch.Tensor, *, scale: float = 1.0):
         who = "HeadDecayDecoder"
