@@ -370,16 +370,19 @@ def block_join(f, h, *, post_weight=None, gate=None, gate_kind: str = "sigmoid",
 
     ``f (..., D)`` is the block's output, ``h`` the residual stream, of f's type or fp32, and
     ``gate`` = z, of f's type; 8 <= D <= 8192.  ``gate_kind`` is ``"sigmoid"``, ``"silu"``
-    (``z sigmoid(z)``) or ``"linear"`` (z itself); a gate of -inf is closed under the first two.  ``post_weight, pre_weight (D,)`` and ``scale``,
-    a number or ``(D,)``, in any of the three types.  Without ``post_weight`` y is f, without
-    ``gate`` u is y, and without ``pre_weight`` there is no x.  Returns ``(h', x)`` in h's and f's
-    types, x None if there is none; computed in fp32 and rounded once.
+    (``z sigmoid(z)``) or ``"linear"`` (z itself); a gate of -inf is closed under the first two.
+    ``post_weight, pre_weight (D,)`` and ``scale``, a number or ``(D,)``, in any of the three
+    types.  Without ``post_weight`` y is f, without ``gate`` u is y, and without ``pre_weight``
+    there is no x.  Returns ``(h', x)`` in h's and f's
+    types, x None if there is none; computed in fp32, a row's squares too (whose sum ends at values
+    of some 1e17), and rounded once.
 
     ``dropout`` keeps a place with probability ``1 - dropout`` and scales it by its inverse, the
     rate rounded to a multiple of 2^-32 and at most ``1 - 2^-32``.  What is dropped counts for
-    nothing, there and in the gradient, finite or not.  Which ones is a function of ``seed`` (an int64 tensor of one element on the GPU: a captured
-    graph reads it at every replay), ``salt`` (a number below 2^32, one a layer), the row and the
-    column, from a counter-based generator; no mask is stored, and the gradient forms it again.
+    nothing, there and in the gradient, finite or not (rms(f) is of the whole row).  Which ones
+    is a function of ``seed`` (an int64 tensor of one element on the GPU: a captured graph reads it
+    at every replay), ``salt`` (a number below 2^32, one a layer), the row and the column, from a
+    counter-based generator; no mask is stored, and the gradient forms it again.
 
     Differentiable in f, h, gate, the weights and a tensor ``scale``.  The rows of a tensor with
     one stride between them are read in place; others (a gate expanded over tokens) are copied.

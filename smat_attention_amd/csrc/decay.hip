@@ -204,10 +204,11 @@ static Scratch take(dl::Arena& ar, int64_t nb, int64_t nbk, int64_t T, int nseg,
 // times that where inputs have two and three terms, and 0.42 of it in the first pass.  Two
 // workgroups on a CU take 1.45 times as long each, three (bf16, 64 columns) 1.9; more than fit
 // follow one another.  The carry moves its states at 4 TB/s, and two launches more
-// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 7391 in two runs, 538 in 32, 436 in
-// 64, 481 in 128; 32 of 128 chunks, 64 x 64: 323 whole, 80 in 8, 64 in 16, 67 in 22; 96 of 64
-// chunks with gradients: 393 whole, 270 in 4, 236 in 8, 273 in 16; fp16, 12 of 157 chunks,
-// 96 x 96: 135 in 16, 116 in 20, 116 in 40.)
+// take 9.  (bf16, 8 sequences of 2048 chunks, r = p = 128: 7823 in two runs, 575 in 32, 466 in
+// 64, 506 in 128; 32 of 128 chunks, 64 x 64: 350 whole, 84 in 8, 66 in 16, 67 in 22; 96 of 64
+// chunks with gradients: 415 whole, 275 in 4, 244 in 8, 279 in 16; fp16, 12 of 157 chunks,
+// 96 x 96: 141 in 16, 120 in 20, 120 in 40; fp32, 8 of 64 chunks, 128 x 128: 140 in 8, 88 in 16,
+// 66 in 32; 4 of 16, 64 x 64: 90 whole, 46 in 4, 31 in 8.)
 extern "C" int smat_head_decay_run_chunks(int dtype, int nb, int nch, const int32_t* lengths,
                                           const int32_t* times, int n, int r, int p) {
   using namespace smat;
@@ -396,8 +397,8 @@ extern "C" int smat_head_decay_scan_backward(
   g.x = Q;
   g.part = sc.part[2];
   all.w[2] = g;
-  // in one launch where one kernel serves all three (96 sequences of 4096, 64 x 64, three
-  // terms everywhere: 149 us, one after the other 174; now 130), and its grid has less than
+  // in one launch where one kernel serves all three (96 sequences of 4096, 64 x 64:
+  // 149 us, one after the other 174; now 140), and its grid has less than
   // 2^32 threads along the axis
   if (!learn && dl::rblocks(r) == dl::rblocks(p) && (r <= 64) == (p <= 64) && nb < (1 << 21)) {
     rc = walk_all(dtype, all, true, kNone, st);

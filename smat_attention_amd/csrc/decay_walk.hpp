@@ -29,12 +29,17 @@
 // type: with two, outputs that are small differences of large sums are off by many of their own
 // steps.  Results are rounded once, where they are stored.
 //
-// Per chunk, bf16, r = p = 128: 196 MFMA and some 850 vector instructions a wave (the splits
-// most of them), two waves a SIMD; 8 sequences of 131072 take 294 us with outputs (3.6 TB/s;
-// every row in L2 takes a fifth less) and 127 in the first pass (4.2); 32 of 8192, 64 x 64, 39
+// Per chunk, bf16, r = p = 128: 240 MFMA and some 870 vector instructions a wave (the splits
+// most of them), two waves a SIMD; 8 sequences of 131072 take 313 us with outputs (3.4 TB/s;
+// every row in L2 takes a fifth less) and 125 in the first pass (4.3); 32 of 8192, 64 x 64, 40
 // and 20.  So it is bound by how well two or three waves a SIMD cover a chunk's chain of LDS
 // reads, products, splits and barriers, and next by HBM.  fp16 has twice the tiles and products
-// and one workgroup of eight waves a CU: 12 of 10007, 96 x 96, 83 and 29.
+// and one workgroup of eight waves a CU: 12 of 10007, 96 x 96, 86 and 29.  Widths between the
+// blocks (96 of 128) run the larger block's products, and every chunk takes the path with bounds.
+// Kernels that spill (registers a lane; none in 16 bits without learned decays): the walk for q
+// with learned decays, bf16 96 x 64: 4, fp16 64 x 64, 96 and 128 x 128: 10, fp32 up to 32; those
+// for k and v in fp16 at 128: 10 and 2, in fp32 at 128 columns up to 12 and 20; fp32's outputs
+// without, 96 and 128 x 128: 4 and 10.
 // Tried and slower or no faster: volatile LDS reads, products and splits interleaved by hand,
 // two column tiles a wave with LEARN (spills), splits in registers ahead of fp16's products.
 #pragma once
@@ -290,10 +295,10 @@ __device__ __forceinline__ Frag<Terms<In>::in> value_rows(const bf16* tile, int 
 }
 
 // The column tiles of a wave and the waves of a workgroup, by the columns of all (64 or 128):
-// two tiles a wave share the reads of K, Q and P (8 sequences of 131072, 128 x 128: 294 us, with
-// one 385, at four waves a SIMD and registers spilt).  With LEARN they would not fit the registers,
+// two tiles a wave share the reads of K, Q and P (8 sequences of 131072, 128 x 128: with one tile
+// 352 us where two took 297).  With LEARN they would not fit the registers,
 // inputs of several terms leave LDS for one workgroup a CU, which eight waves fill better, and the
-// first pass reads K alone: four waves a SIMD there (127 us, two of two tiles 152).
+// first pass reads K alone: four waves a SIMD there (125 us, two of two tiles 152).
 template <typename In, int P, bool OUT, int LEARN> constexpr int tiles() {
   return P == 64 || !OUT || LEARN || Terms<In>::in > 1 ? 1 : 2;
 }

@@ -19,17 +19,23 @@
 // of its columns; rows are walked with the weights, and in the backward the columns' sums, in
 // registers.  The sums leave through the workgroups' parts, added in a fixed order.
 //
-// Measured: without dropout at 131072 x 1024 (bf16, h fp32) the forward takes 352 us, 5.3 TB/s,
-// above a copy's rate, and the gradient runs at 5.0.  With it the generator is nearly half the
-// time: a block of four columns takes 40 32-bit products at a quarter rate; 32768 x 768 bf16:
-// forward 72 us (3.5 TB/s), gradient 118 (3.4), sums 4.  Beyond 4096 columns a row is sixteen
-// waves' and a lane has 128 registers: the gradient's sums go to LDS there, and no row is loaded
-// ahead (4104 columns, bf16: 181 us, 2.2 TB/s; sums in registers 344, and rows ahead 600, spilt).
+// Measured: without dropout at 131072 x 1024 (bf16, h fp32) the forward takes 351 us, 5.3 TB/s,
+// above a copy's rate, and the gradient 526, 5.6.  32768 x 768, all bf16, has half the bytes a
+// value and is bound by instructions: forward 71 us (3.5 TB/s; 56 without dropout, 41 without a
+// gate too), gradient 124 (3.4; 105 without dropout), sums 4.  The generator is a lane's 36 wide
+// multiply-adds a row at a quarter rate and their exclusive ors, the gate eight exponentials and
+// reciprocals; a quarter of the lanes have no columns there (as many values at 1024 columns: 46
+// us for 55); and one kernel for every gate and absent tensor spills 16 to 18 scalars (gradient
+// 24 to 27), read back in the rows' loop.  A row is a wave's at least: at 64 columns, 8 lanes of
+// 64, the forward runs at 0.8 TB/s.
+// Beyond 4096 columns a row is nine to sixteen waves' and a lane has 128 registers: the gradient's
+// sums go to LDS there, and no row is loaded ahead (6144 x 4104, bf16: 188 us, 2.1 TB/s; sums in
+// registers 344, and rows ahead 600); 5 to 8 registers are spilt still, in fp32 39 (330 us, 2.4).
 //
 // Dropout's mask is never stored: place (row, column) is kept where its word of Philox 4x32,
 // ten rounds (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC 2011),
-// is at least p 2^32 (rounded to even, at most 2^32 - 1); key = the seed's halves, counter = (column / 4, row, salt, 0), the word
-// column % 4 of the four.
+// is at least p 2^32 (rounded to even, at most 2^32 - 1); key = the seed's halves, counter =
+// (column / 4, row, salt, 0), the word column % 4 of the four.
 #include "row_groups.hpp"
 #include "smat_host.hpp"
 
@@ -297,7 +303,7 @@ template <typename In, typename H, int MOST>
 __global__ __launch_bounds__(MOST) void join_backward_kernel(Args g) {
   __shared__ float sums[2][16];
   extern __shared__ __align__(16) float part[];    // the columns' sums of the groups: 3 D
-  // Sixteen waves a row leave a lane 128 registers: the next row is not loaded ahead, and the
+  // Nine waves a row and more leave a lane 128 registers: the next row is not loaded ahead, and the
   // sums are in LDS, every lane's own, (3, 8, threads).
   constexpr bool MANY = MOST <= 512;
   Walk l(g.group, sums);
